@@ -13,6 +13,7 @@ from cuda_force_amd.ops import (
     QUANT_BLOCK_SIZE,
     BackendReport,
     ExtensionMissingError,
+    TokenLogprobs,
     backend_report,
     dequantize_int8,
     fake_quantize_int8,
@@ -30,6 +31,7 @@ from cuda_force_amd.ops import (
     softmax_scaled,
     sum_reduce,
     swiglu,
+    token_logprobs,
 )
 
 __version__ = "0.1.0"
@@ -40,6 +42,7 @@ __all__ = [
     "QUANT_BLOCK_SIZE",
     "BackendReport",
     "ExtensionMissingError",
+    "TokenLogprobs",
     "backend_report",
     "dequantize_int8",
     "fake_quantize_int8",
@@ -57,4 +60,5 @@ __all__ = [
     "softmax_scaled",
     "sum_reduce",
     "swiglu",
+    "token_logprobs",
 ]

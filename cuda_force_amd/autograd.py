@@ -1,4 +1,7 @@
-"""LoRA training path: an autograd function whose adapter gradients are HIP kernels.
+"""Autograd functions whose gradients are HIP kernels: the LoRA linear's adapter
+gradients, and the token log probabilities' gradient of the logits.
+
+LoRA training path.
 
 The reference has no backward kernels: it guards the operator
 (cpp/src/bindings.cpp:369-377) and sends any grad-requiring call to the ATen
@@ -17,6 +20,10 @@ that the adapter gradients need anyway. The gradient of w (the base weight is
 usually frozen) is a plain GEMM too. When the backward itself is recorded
 (create_graph) the gradient of x is composed from torch operators, which can
 be differentiated again.
+
+token_logprobs keeps its logits, two statistics per row and the entropy, and
+writes the gradient of the logits in one pass (cf_token_logprobs_backward); it
+is differentiable once.
 """
 
 from __future__ import annotations
@@ -57,3 +64,36 @@ def lora_linear_autograd(
 ) -> torch.Tensor:
     """Differentiable fused LoRA linear (op layout, 2-D contiguous operands)."""
     return _LoRALinearFunction.apply(x, weight, lora_a, lora_b, scale)
+
+
+class _TokenLogprobsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, scale, entropy, top):  # type: ignore[override]
+        picked, stats, h, top_logprobs, top_tokens = torch.ops.cudaforge.token_logprobs(
+            logits, tokens, scale, entropy, top)
+        ctx.save_for_backward(logits, tokens, stats, h)
+        ctx.scale = scale
+        ctx.mark_non_differentiable(top_logprobs, top_tokens)
+        if not entropy:
+            ctx.mark_non_differentiable(h)
+        ctx.set_materialize_grads(False)
+        return picked, h, top_logprobs, top_tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logprobs, grad_entropy, *_):  # type: ignore[override]
+        logits, tokens, stats, h = ctx.saved_tensors
+        if h.numel() == 0:
+            grad_entropy = None
+        grad = torch.ops.cudaforge.token_logprobs_backward(
+            logits, tokens, ctx.scale, stats, h, grad_logprobs, grad_entropy)
+        return grad, None, None, None, None
+
+
+def token_logprobs_autograd(
+    logits: torch.Tensor, tokens: torch.Tensor, scale: float, entropy: bool, top: int
+) -> tuple[torch.Tensor, ...]:
+    """Differentiable token log probabilities: 2-D logits dense along the
+    vocabulary, 2-D int64 tokens; (logprobs, entropy, top_logprobs, top_tokens),
+    empty tensors for what was not asked for."""
+    return _TokenLogprobsFunction.apply(logits, tokens, scale, entropy, top)

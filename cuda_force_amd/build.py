@@ -8,8 +8,8 @@
 
 Run ``python -m cuda_force_amd.build`` (or ``__graft_entry__.build()``). The
 reference builds its extension through setup.py + CMake with nvcc
-(setup.py:25-93, cuda/CMakeLists.txt:46-102); this tree needs neither: two
-compiler invocations per artefact, run in parallel.
+(setup.py:25-93, cuda/CMakeLists.txt:46-102); this tree needs neither: one
+compiler invocation per source, run in parallel, and one to link each artefact.
 """
 
 from __future__ import annotations
@@ -46,7 +46,10 @@ HIP_SOURCES = (
     "cf_tensor_core.hip",
     "cf_matmul_fp8.hip",
     "cf_attention.hip",
+    "cf_logprobs.hip",
 )
+
+TORCH_SOURCES = ("torch_ops.cpp", "torch_ops_generation.cpp")
 
 # Per-source additions. The fused LoRA kernel accumulates in VGPRs: the
 # compiler's AGPR accumulator allocation rotates registers every K-step.
@@ -132,12 +135,11 @@ def build_torch_extension() -> Path:
     out = torch_extension_path()
     tmp = out.with_name(out.name + ".tmp")
     abi = int(getattr(__import__("torch")._C, "_GLIBCXX_USE_CXX11_ABI", True))
-    cmd = [
+    flags = [
         "g++",
         "-O2",
         "-std=c++17",
         "-fPIC",
-        "-shared",
         "-Wall",
         "-Wno-unused-parameter",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
@@ -148,7 +150,19 @@ def build_torch_extension() -> Path:
         f"-I{python_include}",
         f"-I{REPO_ROOT / 'include'}",
         *[f"-I{p}" for p in includes],
-        str(CSRC / "torch_ops.cpp"),
+    ]
+
+    def compile_one(name: str) -> Path:
+        obj = BUILD_DIR / (Path(name).stem + ".o")
+        _run([*flags, "-c", str(CSRC / name), "-o", str(obj)])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(TORCH_SOURCES)) as pool:
+        objects = list(pool.map(compile_one, TORCH_SOURCES))
+    cmd = [
+        "g++",
+        "-shared",
+        *map(str, objects),
         "-o",
         str(tmp),
         f"-L{PACKAGE_DIR}",

@@ -1,0 +1,215 @@
+// Dispatcher registration of the operators of token generation: log
+// probabilities of tokens with their gradient. Same conventions as
+// torch_ops.cpp: ATen on the CPU, the C ABI of libcudaforge_hip.so on
+// PyTorch's current HIP stream on the GPU, never synchronising; workspaces
+// from torch's caching allocator.
+#include "torch_ops_common.hpp"
+
+namespace cudaforge_amd {
+namespace {
+
+// ---- token log probabilities -------------------------------------------------
+
+using LogprobsResult = std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>;
+
+void check_logits(const torch::Tensor& logits, const torch::Tensor& tokens, double scale) {
+    check_2d(logits, "logits");
+    TORCH_CHECK(logits.size(1) <= 1 || logits.stride(1) == 1, "logits must be dense along the vocabulary");
+    TORCH_CHECK(logits.size(0) <= 1 || logits.stride(0) >= logits.size(1),
+                "logits' rows overlap: call .contiguous() first");
+    check_2d(tokens, "tokens");
+    check_contiguous(tokens, "tokens");
+    check_same_device(logits, tokens, "tokens");
+    TORCH_CHECK(tokens.scalar_type() == torch::kInt64, "tokens must be int64, got ", tokens.scalar_type());
+    TORCH_CHECK(tokens.size(0) == logits.size(0), "tokens has ", tokens.size(0), " rows but logits has ",
+                logits.size(0));
+    TORCH_CHECK(tokens.size(1) >= 1, "tokens must name at least one token per row");
+    TORCH_CHECK(scale > 0, "scale must be positive, got ", scale);
+}
+
+int64_t row_stride(const torch::Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+LogprobsResult token_logprobs_hip(const torch::Tensor& logits, const torch::Tensor& tokens, double scale,
+                                  bool entropy, int64_t top) {
+    check_logits(logits, tokens, scale);
+    const at::DeviceGuard guard(logits.device());
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    TORCH_CHECK(top >= 0 && top <= vocab, "top ", top, " is not in 0 .. ", vocab, " (the vocabulary)");
+    const auto f32 = logits.options().dtype(torch::kFloat32);
+    torch::Tensor logprobs = torch::empty(tokens.sizes(), f32);
+    torch::Tensor stats = torch::empty({rows, 2}, f32);
+    torch::Tensor h = torch::empty({entropy ? rows : 0}, f32);
+    torch::Tensor top_logprobs = torch::empty({top > 0 ? rows : 0, top}, f32);
+    torch::Tensor top_tokens = torch::empty({top > 0 ? rows : 0, top}, tokens.options());
+    const cf_dtype dtype = to_cf(logits, "logits");
+    const size_t bytes = cf_token_logprobs_workspace_bytes(dtype, rows, vocab, top);
+    torch::Tensor workspace;
+    if (bytes > 0) workspace = torch::empty({static_cast<int64_t>(bytes)}, logits.options().dtype(torch::kUInt8));
+    check_status(cf_token_logprobs(logits.data_ptr(), dtype, rows, vocab, row_stride(logits),
+                                   tokens.data_ptr<int64_t>(), tokens.size(1), static_cast<float>(scale),
+                                   logprobs.data_ptr<float>(), stats.data_ptr<float>(),
+                                   entropy ? h.data_ptr<float>() : nullptr, top,
+                                   top > 0 ? top_logprobs.data_ptr<float>() : nullptr,
+                                   top > 0 ? top_tokens.data_ptr<int64_t>() : nullptr,
+                                   bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_for(logits)));
+    return {logprobs, stats, h, top_logprobs, top_tokens};
+}
+
+/// Contiguous fp32 gradient of the expected shape, or null where it is absent.
+const float* gradient(const std::optional<torch::Tensor>& g, const torch::Tensor& like, torch::IntArrayRef sizes,
+                      const char* name, torch::Tensor& held) {
+    if (!g.has_value() || !g->defined()) return nullptr;
+    check_same_device(like, *g, name);
+    TORCH_CHECK(g->sizes() == sizes, name, " has shape ", g->sizes(), ", expected ", sizes);
+    TORCH_CHECK(g->scalar_type() == torch::kFloat32, name, " must be float32, got ", g->scalar_type());
+    held = g->contiguous();
+    return held.data_ptr<float>();
+}
+
+torch::Tensor token_logprobs_backward_hip(const torch::Tensor& logits, const torch::Tensor& tokens, double scale,
+                                          const torch::Tensor& stats, const torch::Tensor& entropy,
+                                          const std::optional<torch::Tensor>& grad_logprobs,
+                                          const std::optional<torch::Tensor>& grad_entropy) {
+    check_logits(logits, tokens, scale);
+    const at::DeviceGuard guard(logits.device());
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    check_same_device(logits, stats, "stats");
+    check_contiguous(stats, "stats");
+    TORCH_CHECK(stats.scalar_type() == torch::kFloat32 && stats.numel() == 2 * rows, "stats must be float32 [", rows,
+                ", 2]");
+    torch::Tensor held_lp, held_h;
+    const float* g = gradient(grad_logprobs, logits, tokens.sizes(), "grad_logprobs", held_lp);
+    const float* h = gradient(grad_entropy, logits, {rows}, "grad_entropy", held_h);
+    if (h != nullptr) {
+        check_same_device(logits, entropy, "entropy");
+        check_contiguous(entropy, "entropy");
+        TORCH_CHECK(entropy.scalar_type() == torch::kFloat32 && entropy.numel() == rows, "entropy must be float32 [",
+                    rows, "]");
+    }
+    // Laid out as the logits: rows padded to an aligned pitch stay aligned.
+    torch::Tensor grad = torch::empty_strided(logits.sizes(), {row_stride(logits), 1}, logits.options());
+    check_status(cf_token_logprobs_backward(logits.data_ptr(), to_cf(logits, "logits"), rows, vocab,
+                                            row_stride(logits), tokens.data_ptr<int64_t>(), tokens.size(1),
+                                            static_cast<float>(scale), stats.data_ptr<float>(),
+                                            h != nullptr ? entropy.data_ptr<float>() : nullptr, g, h, grad.data_ptr(),
+                                            row_stride(grad), stream_for(logits)));
+    return grad;
+}
+
+LogprobsResult token_logprobs_cpu(const torch::Tensor& logits, const torch::Tensor& tokens, double scale,
+                                  bool entropy, int64_t top) {
+    check_logits(logits, tokens, scale);
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    TORCH_CHECK(top >= 0 && top <= vocab, "top ", top, " is not in 0 .. ", vocab, " (the vocabulary)");
+    const torch::Tensor wide = logits.to(torch::kFloat32);
+    const torch::Tensor shift = vocab > 0 ? std::get<0>(wide.max(1, true)) : torch::zeros({rows, 1}, wide.options());
+    const torch::Tensor x = (wide - shift) * scale;
+    const torch::Tensor log_sum = x.exp().sum(1, true).log();
+    const torch::Tensor logp = x - log_sum;
+    const torch::Tensor stats = torch::cat({shift, log_sum / std::log(2.0)}, 1);
+    torch::Tensor picked = logp.gather(1, tokens.clamp(0, vocab - 1));
+    picked = picked.masked_fill(tokens < 0, 0.0).masked_fill(tokens >= vocab, std::numeric_limits<float>::quiet_NaN());
+    const torch::Tensor p = logp.exp();
+    const torch::Tensor h = entropy ? -torch::where(p == 0, torch::zeros_like(p), p * logp).sum(1)
+                                    : torch::empty({0}, wide.options());
+    if (top == 0) {
+        return {picked, stats, h, torch::empty({0, 0}, wide.options()), torch::empty({0, 0}, tokens.options())};
+    }
+    const torch::Tensor order = std::get<1>(wide.sort(/*stable=*/true, 1, /*descending=*/true)).slice(1, 0, top);
+    return {picked, stats, h, logp.gather(1, order), order.contiguous()};
+}
+
+torch::Tensor token_logprobs_backward_cpu(const torch::Tensor& logits, const torch::Tensor& tokens, double scale,
+                                          const torch::Tensor& stats, const torch::Tensor& entropy,
+                                          const std::optional<torch::Tensor>& grad_logprobs,
+                                          const std::optional<torch::Tensor>& grad_entropy) {
+    check_logits(logits, tokens, scale);
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    const torch::Tensor wide = logits.to(torch::kFloat32);
+    const torch::Tensor logp = (wide - stats.slice(1, 0, 1)) * scale - stats.slice(1, 1, 2) * std::log(2.0);
+    const torch::Tensor p = logp.exp();
+    torch::Tensor held;
+    torch::Tensor grad = torch::zeros_like(p);
+    const bool has_h = gradient(grad_entropy, logits, {rows}, "grad_entropy", held) != nullptr;
+    if (has_h) {
+        const torch::Tensor kept = torch::where(p == 0, torch::zeros_like(p), logp);
+        grad -= held.unsqueeze(1) * p * (kept + entropy.unsqueeze(1));
+    }
+    if (gradient(grad_logprobs, logits, tokens.sizes(), "grad_logprobs", held) != nullptr) {
+        torch::Tensor g = held.masked_fill(tokens < 0, 0.0);
+        g = g.masked_fill(tokens >= vocab, std::numeric_limits<float>::quiet_NaN());
+        grad -= g.sum(1, true) * p;
+        grad.scatter_add_(1, tokens.clamp(0, vocab - 1), g);
+        if (!has_h) grad.masked_fill_((tokens < 0).all(1, true), 0.0);
+    }
+    return (scale * grad).to(logits.scalar_type());
+}
+
+}  // namespace
+
+// ---- direct entry for ordinary GPU calls (the rules: torch_ops_common.hpp) ------
+
+py::object try_token_logprobs(py::handle logits_, py::handle tokens_, py::handle scale_, py::handle entropy_,
+                              py::handle top_) {
+    if (!THPVariable_CheckTypeExact(Py_TYPE(logits_.ptr()))) return py::none();
+    const at::Tensor& logits = THPVariable_Unpack(logits_.ptr());
+    const at::Tensor* tokens = ordinary(tokens_);
+    const std::optional<double> scale = plain_double(scale_);
+    const std::optional<int64_t> top = plain_int(top_);
+    if (!plain_gpu(logits) || tokens == nullptr || !scale || !top || !PyBool_Check(entropy_.ptr()) ||
+        !ordinary_context()) {
+        return py::none();
+    }
+    const bool entropy = entropy_.ptr() == Py_True;
+    if (!kernel_dtype(logits.scalar_type()) || tokens->scalar_type() != torch::kInt64 ||
+        tokens->device() != logits.device() || grad_needed({&logits}) || logits.dim() != 2 || logits.numel() == 0 ||
+        logits.stride(1) != 1 || (logits.size(0) > 1 && logits.stride(0) < logits.size(1)) ||
+        tokens->size(0) != logits.size(0) || tokens->dim() > 2 || *scale <= 0 || *top < 0 || *top > logits.size(1)) {
+        return py::none();
+    }
+    LogprobsResult out;
+    {
+        py::gil_scoped_release no_gil;
+        const bool one = tokens->dim() == 1;
+        out = token_logprobs_hip(logits, one ? tokens->unsqueeze(1) : *tokens, *scale, entropy, *top);
+        if (one) std::get<0>(out) = std::get<0>(out).squeeze(1);
+    }
+    const auto& [logprobs, stats, h, top_logprobs, top_tokens] = out;
+    return py::make_tuple(wrap(logprobs), entropy ? wrap(h) : py::none(), *top > 0 ? wrap(top_logprobs) : py::none(),
+                          *top > 0 ? wrap(top_tokens) : py::none());
+}
+
+void bind_generation(py::module_& m) {
+    m.def("try_token_logprobs", torch::wrap_pybind_function(&try_token_logprobs));
+}
+
+}  // namespace cudaforge_amd
+
+TORCH_LIBRARY_FRAGMENT(cudaforge, m) {
+    m.def(
+        "token_logprobs(Tensor logits, Tensor tokens, float scale, bool entropy, int top) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def(
+        "token_logprobs_backward(Tensor logits, Tensor tokens, float scale, Tensor stats, Tensor entropy, "
+        "Tensor? grad_logprobs, Tensor? grad_entropy) -> Tensor");
+}
+
+// As in torch_ops.cpp: differentiating the operators themselves raises;
+// the Python layer has the differentiable form.
+TORCH_LIBRARY_IMPL(cudaforge, Autograd, m) {
+    for (const char* name : {"token_logprobs", "token_logprobs_backward"}) {
+        m.impl(name, torch::autograd::autogradNotImplementedFallback());
+    }
+}
+
+TORCH_LIBRARY_IMPL(cudaforge, CPU, m) {
+    using namespace cudaforge_amd;
+    m.impl("token_logprobs", &token_logprobs_cpu);
+    m.impl("token_logprobs_backward", &token_logprobs_backward_cpu);
+}
+
+TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
+    using namespace cudaforge_amd;
+    m.impl("token_logprobs", &token_logprobs_hip);
+    m.impl("token_logprobs_backward", &token_logprobs_backward_hip);
+}

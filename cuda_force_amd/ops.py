@@ -18,8 +18,8 @@ Dispatch rules (reference ops.py:125-153, widened):
   plain PyTorch, as the reference does.
 * When a backward pass is expected, rmsnorm/softmax/sum/activations/quant take
   the differentiable PyTorch composition, as the reference does; lora_linear
-  takes its own autograd function whose adapter gradients are HIP kernels
-  (``cuda_force_amd.autograd``).
+  and token_logprobs take their own autograd functions, whose gradients are HIP
+  kernels (``cuda_force_amd.autograd``).
 """
 
 from __future__ import annotations
@@ -29,6 +29,7 @@ import logging
 import os
 import warnings
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -324,6 +325,115 @@ def softmax_scaled(
         return torch.ops.cudaforge.softmax_scaled(rows, float(scale), int(causal_period), dtype).view(x.shape)
     _refuse_gpu_fallback("softmax_scaled", x)
     return _softmax_scaled_reference(x, scale, causal_period).to(dtype)
+
+
+#: Most alternatives, and most given tokens, per row of token_logprobs.
+LOGPROBS_TOP_MAX = 64
+LOGPROBS_TOKENS_MAX = 1024
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns; None in the place of what was not asked for."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor | None = None
+    top_logprobs: torch.Tensor | None = None
+    top_tokens: torch.Tensor | None = None
+
+
+def _token_logprobs_reference(
+    logits: torch.Tensor, tokens: torch.Tensor, scale: float, entropy: bool, top: int
+) -> tuple[torch.Tensor | None, ...]:
+    """2-D logits and tokens; differentiable. Arithmetic in fp32, or in fp64
+    where the logits are."""
+    vocab = logits.shape[1]
+    wide = logits if logits.dtype == torch.float64 else logits.float()
+    logp = torch.log_softmax(wide * scale, dim=-1)
+    picked = logp.gather(1, tokens.clamp(0, vocab - 1))
+    picked = picked.masked_fill(tokens < 0, 0.0).masked_fill(tokens >= vocab, float("nan"))
+    h = None
+    if entropy:
+        p = logp.exp()
+        h = -torch.where(p == 0, torch.zeros_like(p), p * logp.masked_fill(p == 0, 0.0)).sum(-1)
+    if top == 0:
+        return picked, h, None, None
+    order = torch.sort(wide.detach(), dim=-1, descending=True, stable=True).indices[:, :top].contiguous()
+    return picked, h, logp.detach().gather(1, order), order
+
+
+def token_logprobs(
+    logits: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, entropy: bool = False, top: int = 0
+) -> TokenLogprobs:
+    """Log probabilities of given tokens under ``softmax(scale * logits)``, with
+    the distribution's entropy and its likeliest tokens, in one pass over the
+    logits.
+
+    ``logits`` is ``[..., vocab]`` (rows may be padded: only the last dimension
+    has to be dense); ``tokens`` is ``[...]`` for one token per row or ``[...,
+    n]`` for several (n <= 1024). Results are fp32: ``logprobs`` shaped like
+    ``tokens``; ``entropy`` ``[...]`` in nats if asked for; ``top_logprobs``
+    and ``top_tokens`` ``[..., top]`` (top <= 64) in descending order, equal
+    logits by ascending token. A negative token is padding: log probability 0
+    and no gradient; a token past the vocabulary gives NaN. ``scale`` is an
+    inverse temperature and must be positive.
+
+    ``logprobs`` and ``entropy`` are differentiable once with respect to the
+    logits (HIP kernels on the GPU); the top alternatives are not. Not in the
+    reference's API.
+
+    Raises:
+        ValueError: for shapes that do not match, a scale that is not positive
+            and finite, or a ``top`` out of range.
+        TypeError: if ``tokens`` are not integers.
+    """
+    if _DIRECT is not None and not _compiling():
+        direct = _DIRECT.try_token_logprobs(logits, tokens, scale, entropy, top)
+        if direct is not None:
+            return TokenLogprobs(*direct)
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"tokens must be int64 or int32, got {tokens.dtype}")
+    if logits.ndim < 1 or logits.shape[-1] == 0:
+        raise ValueError(f"logits must be [..., vocab], got shape {tuple(logits.shape)}")
+    one = tokens.shape == logits.shape[:-1]
+    if not one and (tokens.ndim != logits.ndim or tokens.shape[:-1] != logits.shape[:-1]):
+        raise ValueError(
+            f"tokens must be {tuple(logits.shape[:-1])} or that with a last dimension of tokens per row, "
+            f"got {tuple(tokens.shape)}"
+        )
+    if not one and not 1 <= tokens.shape[-1] <= LOGPROBS_TOKENS_MAX:
+        raise ValueError(f"tokens per row must be 1 .. {LOGPROBS_TOKENS_MAX}, got {tokens.shape[-1]}")
+    if not 0 < scale < 1e29:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    vocab = logits.shape[-1]
+    if not 0 <= top <= min(LOGPROBS_TOP_MAX, vocab):
+        raise ValueError(f"top must be 0 .. {min(LOGPROBS_TOP_MAX, vocab)}, got {top}")
+    if tokens.device != logits.device:
+        raise ValueError(f"tokens are on {tokens.device} but logits on {logits.device}")
+    lead = logits.shape[:-1]
+    rows = logits.reshape(-1, vocab)
+    if rows.shape[0] > 1 and (rows.stride(1) != 1 or rows.stride(0) < vocab) or rows.shape[0] == 1 and rows.stride(1) != 1:
+        rows = rows.contiguous()
+    count = 1 if one else tokens.shape[-1]
+    given = tokens.to(torch.int64).reshape(-1, count).contiguous()
+    arguments = (rows, given, float(scale), bool(entropy), int(top))
+    if rows.dtype in KERNEL_DTYPES and _needs_autograd(logits) and logits.is_cuda and _EXTENSION_LOADED:
+        _require_extension("token_logprobs", (logits,))
+        from cuda_force_amd.autograd import token_logprobs_autograd
+
+        got = token_logprobs_autograd(*arguments)
+    elif rows.dtype in KERNEL_DTYPES and _dispatch_available("token_logprobs", rows):
+        picked, _, h, *best = torch.ops.cudaforge.token_logprobs(*arguments)
+        got = (picked, h, *best)
+    else:
+        _refuse_gpu_fallback("token_logprobs", logits)
+        got = _token_logprobs_reference(*arguments)
+    picked, h, top_logprobs, top_tokens = got
+    return TokenLogprobs(
+        picked.view(tokens.shape),
+        h.view(lead) if entropy else None,
+        top_logprobs.view(*lead, top) if top else None,
+        top_tokens.view(*lead, top) if top else None,
+    )
 
 
 #: Head sizes the causal attention kernels take (sequence lengths: multiples of 8).

@@ -191,6 +191,56 @@ cf_status cf_softmax_scaled(const void* x, cf_dtype x_dtype, void* y, cf_dtype y
                             int64_t rows, int64_t cols, float scale, int64_t causal_period,
                             void* stream);
 
+/* ---- token log probabilities --------------------------------------------- */
+
+/* Most likeliest tokens, and most given tokens, per row below. */
+#define CF_LOGPROBS_TOP_MAX 64
+#define CF_LOGPROBS_TOKENS_MAX 1024
+
+/* Workspace bytes cf_token_logprobs needs: partial results of rows that
+ * several workgroups share (0: none). It has no counterpart in the reference,
+ * which samples from torch tensors. */
+size_t cf_token_logprobs_workspace_bytes(cf_dtype dtype, int64_t rows, int64_t vocab, int64_t top);
+
+/* For every row of logits [rows, vocab] (row_stride elements apart, dense
+ * along the vocabulary; fp32, fp16 or bf16, fp32 arithmetic), with x = scale *
+ * logits and L = ln sum_j exp(x_j), in one pass:
+ *   logprobs[row, i] = x[tokens[row, i]] - L   (token_count tokens per row;
+ *       a negative token is padding and gives 0, one >= vocab gives NaN);
+ *   row_stats[row, 2] (may be NULL) = the largest logit and log2 of
+ *       sum_j exp(x_j - scale * largest): what the backward needs;
+ *   entropy[row] (NULL: not wanted) = -sum_j p_j ln p_j in nats, p = exp(x - L);
+ *   top_logprobs / top_tokens [row, top] (top 0: not wanted) = the largest
+ *       x_j - L in descending order; equal logits by ascending token; NaN
+ *       logits first, -0 equal to 0.
+ * scale (an inverse temperature) is positive; 1 <= token_count <=
+ * CF_LOGPROBS_TOKENS_MAX; top <= CF_LOGPROBS_TOP_MAX and <= vocab; vocab <=
+ * 2^27. Logits of -inf have probability 0; a row with nothing above -inf, a
+ * +inf or a NaN gives NaN, as a softmax does. Deterministic. It has no
+ * counterpart in the reference. */
+cf_status cf_token_logprobs(const void* logits, cf_dtype dtype, int64_t rows, int64_t vocab,
+                            int64_t row_stride, const int64_t* tokens, int64_t token_count,
+                            float scale, float* logprobs, float* row_stats, float* entropy,
+                            int64_t top, float* top_logprobs, int64_t* top_tokens, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* The gradient of cf_token_logprobs's logprobs and entropy: with g =
+ * grad_logprobs [rows, token_count] and h = grad_entropy [rows] (NULL: zeros),
+ * G = sum of g over the row's tokens that are not padding, H = entropy,
+ *   grad_logits_j = scale * (sum_{i: tokens_i = j} g_i - p_j (G + h (ln p_j + H)))
+ * in the logits' dtype, rounded once; grad_row_stride elements between rows
+ * (what lies between them is left alone). A row whose tokens are all padding
+ * and whose h is 0 gets zeros. row_stats and entropy are the forward's
+ * (entropy is read only with grad_entropy). grad_logits must not overlap
+ * logits. No atomics: deterministic, a token given twice gets its gradients'
+ * sum. It has no counterpart in the reference. */
+cf_status cf_token_logprobs_backward(const void* logits, cf_dtype dtype, int64_t rows,
+                                     int64_t vocab, int64_t row_stride, const int64_t* tokens,
+                                     int64_t token_count, float scale, const float* row_stats,
+                                     const float* entropy, const float* grad_logprobs,
+                                     const float* grad_entropy, void* grad_logits,
+                                     int64_t grad_row_stride, void* stream);
+
 /* ---- reductions --------------------------------------------------------- */
 
 /* Bytes of workspace cf_reduce_sum needs for `count` elements (the stage-1
