@@ -33,6 +33,7 @@ from cuda_force_amd.ops import (
     swiglu,
     token_logprobs,
 )
+from cuda_force_amd.paged_cache import paged_attention_shared
 
 __version__ = "0.1.0"
 
@@ -50,6 +51,7 @@ __all__ = [
     "gelu",
     "kernel_supports",
     "lora_linear",
+    "paged_attention_shared",
     "quantization_error",
     "quantize_int8",
     "rmsnorm",

@@ -86,6 +86,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I32,
         [_P, _I32, _I64, _I64, _I64, _P, _I64, _F, _P, _P, _P, _P, _P, _I64, _P],
     ),
+    "cf_paged_attention_shared_workspace_bytes": (
+        _SZ,
+        [_I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    ),
+    "cf_paged_attention_shared": (
+        _I32,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P, _SZ, _P],
+    ),
     "cf_reduce_sum_workspace_bytes": (_SZ, [_I64]),
     "cf_reduce_sum": (_I32, [_P, _I32, _P, _I64, _P, _SZ, _I32, _P]),
     "cf_reduce_sum_noalloc": (_I32, [_P, _I32, _P, _I64, _I32, _P]),

@@ -1,0 +1,1044 @@
+// Attention for one decode step over a paged cache whose sequences share
+// prompts: what cf_paged_attention computes, with the keys and values of a
+// shared prompt read once for all the sequences behind it.
+//
+// For sequence s, head h, KV head h / (H / KVH) and context c:
+//   out[s, h] = sum_{t < c} softmax_t(scale q[s, h] . k[t]) v[t].
+// Sequences group_starts[g] .. group_starts[g + 1] - 1 hold the same K and V
+// in their first prefix_lens[g] tokens. A sequence's context is cut in two:
+// its group's prefix, which it attends to together with the other sequences
+// of the group, and the rest, alone; the parts are joined by the rescaling
+// rule of a softmax (running maximum, sum, weighted values). A sequence whose
+// context is shorter than its group's prefix goes alone from its first token.
+//
+// Reading each prefix once makes it a matrix product: the query rows of a
+// group (sequences x heads of a KV head) against the prefix, on the matrix
+// cores. The rests stay bound by HBM.
+//   * A work item is (row tile, KV head, token range) of a prefix or (sequence,
+//     KV head, token range) of a rest, one workgroup of four waves each, both
+//     kinds in one launch. Long ranges are split over workgroups from the
+//     lengths found on the device; a second kernel joins the pieces.
+//   * Scores are formed transposed, S^T = K Q^T: a lane then holds one query
+//     row and several tokens, so a row's maximum and sum are lane-local but for
+//     one exchange, and the probabilities are in place as the B operand of
+//     O^T += V^T P^T without moving between lanes.
+//   * K and V tiles go from the cache straight to LDS (no registers), in 16-byte
+//     pieces whose order inside a row is changed so that the fragment reads hit
+//     all banks. Tiles with many query rows are shared by four waves of
+//     different rows through a ring of stages; tiles with few rows belong to
+//     one wave, the four waves taking different tokens.
+//   * 16-bit caches run 32 x 32 x 16 MFMA over 32 rows and 32 tokens, fp32
+//     caches 16 x 16 x 4 fp32 MFMA over 16 rows and 16 tokens (fp32 products).
+//     Probabilities are rounded to the cache's type for the second product
+//     (relative error half an ulp each, of either sign); sums stay in fp32.
+// Tokens behind a range's end, and tokens whose page is not in the cache, get
+// no weight: their scores are replaced and their V rows are cleared in LDS, so
+// that whatever lies there (NaN, infinities) stays out.
+#include <type_traits>
+
+#include "cf_common.hpp"
+#include "cf_lds_dma.hpp"
+
+namespace cf {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWaveSize;
+constexpr int kStages = 4;       // ring of tiles shared by four waves
+constexpr int kMaxSplits = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct SharedArgs {
+    const void* query;
+    const void* k_cache;
+    const void* v_cache;
+    const int32_t* starts;  // [groups + 1]
+    const int32_t* prefix;  // [groups]
+    const uint32_t* tables;
+    const int32_t* context;
+    void* out;
+    float* ml;   // [slots][sequences * heads][2]: maximum (base 2), sum
+    float* acc;  // [slots][sequences * heads][head_dim]
+    uint32_t pages;
+    uint32_t block_size;
+    int block_shift;  // log2(block_size), or -1
+    int sequences;
+    int heads;
+    int kv_heads;
+    int per;          // query heads per KV head
+    int head_dim;
+    int groups;
+    int max_blocks;
+    int capacity;     // tokens a table row reaches
+    int prefix_splits;
+    int rest_splits;
+    int prefix_tiles;  // row tiles over all groups, at most
+    int rest_tiles;    // row tiles per sequence and KV head
+    int prefix_items;  // workgroups of the first kind
+    float c;           // scale * log2(e)
+};
+
+// ---- groups, ranges -----------------------------------------------------------
+
+struct Group {
+    int first;   // sequences first .. end - 1
+    int end;
+    int prefix;  // tokens
+};
+
+__device__ __forceinline__ int clamp_to(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
+
+__device__ __forceinline__ int wave_max_int(int v) {
+#pragma unroll
+    for (int d = 1; d < kWaveSize; d <<= 1) v = max(v, __shfl_xor(v, d));
+    return v;
+}
+
+/// The group of sequence s (uniform), or end = 0. Starts are taken as the
+/// largest so far, so that groups never overlap whatever is stored.
+__device__ Group group_of(const SharedArgs& a, int s) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    int first = 0;
+    for (int base = 0; base <= a.groups; base += kWaveSize) {
+        const int g = base + lane;
+        const int start = g <= a.groups ? clamp_to(a.starts[g], a.sequences) : 0;
+        const uint64_t above = __builtin_amdgcn_ballot_w64(g <= a.groups && start > s);
+        if (above != 0) {
+            const int at = __builtin_ctzll(above);
+            const int g_end = base + at;  // the first start past s
+            first = max(first, wave_max_int(lane < at ? start : 0));
+            if (g_end == 0) return Group{0, 0, 0};
+            return Group{first, __builtin_amdgcn_readlane(start, at), clamp_to(a.prefix[g_end - 1], a.capacity)};
+        }
+        first = max(first, wave_max_int(start));
+    }
+    return Group{0, 0, 0};
+}
+
+/// The group of row tile `tile` (uniform) of kRows rows; `tile` becomes the
+/// tile within the group. end = 0: no such tile.
+__device__ Group group_of_tile(const SharedArgs& a, int rows, int& tile) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    int before = 0;  // largest start so far
+    for (int base = 0; base < a.groups; base += kWaveSize) {
+        const int g = base + lane;
+        int start = g < a.groups ? clamp_to(a.starts[g], a.sequences) : 0;
+        if (lane == 0) start = max(start, before);
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) {
+            const int o = __shfl_up(start, d);
+            if (lane >= d) start = max(start, o);
+        }
+        const int end = g < a.groups ? max(start, clamp_to(a.starts[g + 1], a.sequences)) : start;
+        int tiles = ((end - start) * a.per + rows - 1) / rows;
+        int total = tiles;
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) {
+            const int o = __shfl_up(total, d);
+            if (lane >= d) total += o;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(total > tile);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            tile -= __builtin_amdgcn_readlane(total - tiles, at);
+            return Group{__builtin_amdgcn_readlane(start, at), __builtin_amdgcn_readlane(end, at),
+                         clamp_to(a.prefix[base + at], a.capacity)};
+        }
+        tile -= __builtin_amdgcn_readlane(total, kWaveSize - 1);
+        before = __builtin_amdgcn_readlane(start, kWaveSize - 1);
+    }
+    return Group{0, 0, 0};
+}
+
+__device__ __forceinline__ int context_of(const SharedArgs& a, int s) { return clamp_to(a.context[s], a.capacity); }
+
+/// Tokens of each of at most `splits` ranges of `length` tokens: whole steps.
+__device__ __forceinline__ int split_length(int length, int splits, int step) {
+    const int each = (length + splits - 1) / splits;
+    return (each + step - 1) / step * step;
+}
+
+// ---- fragments ------------------------------------------------------------------
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
+
+/// LDS byte address of a pointer into shared memory.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8_t*)(const_cast<void*>(p))));
+}
+
+/// 16 bytes per lane from `from` (a lane's own address) to LDS bytes
+/// dst + 16 lane. In inline assembly for the reason given at dma16_m0; it has no
+/// register output.
+__device__ __forceinline__ void copy16_to_lds(const void* from, uint32_t dst) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(from), "{m0}"(__builtin_amdgcn_readfirstlane(dst))
+                 : "memory");
+}
+
+/// Waits until at most n vector-memory operations of the wave are in flight.
+template <int n>
+__device__ __forceinline__ void wait_vm() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(n));
+    asm volatile("" ::: "memory");
+}
+
+/// Waits for the wave's LDS operations.
+__device__ __forceinline__ void wait_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xF | (7 << 4) | (0 << 8) | (3 << 14));
+    asm volatile("" ::: "memory");
+}
+
+/// What depends on the cache's type: rows and tokens of a tile, fragments,
+/// products. kD: head size rounded up to 64, 128 or 256.
+template <typename T, int kD>
+struct Tile {
+    static constexpr bool kWide = sizeof(T) == 4;
+    static constexpr int kRows = kWide ? 16 : 32;    // query rows per wave
+    static constexpr int kTokens = kWide ? 16 : 32;  // tokens per tile
+    static constexpr int kPerVec = 16 / static_cast<int>(sizeof(T));
+    static constexpr int kRowBytes = kD * static_cast<int>(sizeof(T));
+    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kBytes = kTokens * kRowBytes;            // K or V of one tile
+    static constexpr int kCopies = kBytes / (16 * kWaveSize);     // wave-wide copies of it
+    static constexpr int kScores = kRows * kTokens / kWaveSize;   // scores per lane
+    static constexpr int kAcc = kRows * kD / kWaveSize;           // output values per lane
+    static constexpr int kOutPitch = kD + 4;                      // floats per row of the output area
+
+    /// Order of the 16-byte pieces of a K row: a fragment read takes the same
+    /// piece of 16 rows.
+    __device__ __forceinline__ static int k_swizzle(int row) {
+        return kChunks >= 16 ? (row & 15) : ((row >> 1) & 7);
+    }
+    /// And of a V row: a transposed (fp32: plain) read takes 64 bytes of four
+    /// rows, neighbours (fp32: four apart).
+    __device__ __forceinline__ static int v_swizzle(int row) {
+        if constexpr (kWide) return row & 12;
+        return kChunks >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+    }
+
+    using Query = std::conditional_t<kWide, f32x4_t, u32x4_t>;
+    static constexpr int kQueries = kWide ? kD / 16 : kD / 16;  // 16-byte query pieces per lane
+    using Score = std::conditional_t<kWide, f32x4_t, f32x16_t>;
+
+    /// Query row of a lane, and its half or quarter.
+    __device__ __forceinline__ static int row_of(int lane) { return lane & (kRows - 1); }
+    __device__ __forceinline__ static int part_of(int lane) { return lane / kRows; }
+    /// First dim of a lane's query piece u.
+    __device__ __forceinline__ static int query_dim(int u, int lane) {
+        return 16 * u + kPerVec * part_of(lane);
+    }
+    /// Token (in the tile) of a lane's score i.
+    __device__ __forceinline__ static int token_of(int i, int lane) {
+        if constexpr (kWide) return 4 * part_of(lane) + i;
+        return 8 * (i >> 2) + 4 * part_of(lane) + (i & 3);
+    }
+    /// Dim of a lane's output value i: four neighbours from each i % 4 == 0.
+    __device__ __forceinline__ static int dim_of(int i, int lane) {
+        if constexpr (kWide) return 16 * (i >> 2) + 4 * part_of(lane) + (i & 3);
+        return 32 * (i >> 4) + 8 * ((i >> 2) & 3) + 4 * part_of(lane) + (i & 3);
+    }
+
+    __device__ __forceinline__ static Score scores(const uint8_t* k, const Query (&q)[kQueries], int lane) {
+        Score s;
+#pragma unroll
+        for (int i = 0; i < kScores; ++i) s[i] = 0.0f;
+        const int row = lane & (kTokens - 1);
+        const int sw = k_swizzle(row);
+#pragma unroll
+        for (int u = 0; u < kQueries; ++u) {
+            // 16-bit: 16 dims a step, 8 per half; fp32: 16 dims, 4 per quarter.
+            const int piece = (kWide ? 4 : 2) * u + part_of(lane);
+            const u32x4_t raw = *reinterpret_cast<const u32x4_t*>(k + row * kRowBytes + ((piece ^ sw) << 4));
+            if constexpr (kWide) {
+                const f32x4_t kk = __builtin_bit_cast(f32x4_t, raw);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], q[u][e], s, 0, 0, 0);
+            } else if constexpr (std::is_same<T, bf16_t>::value) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, raw),
+                                                            __builtin_bit_cast(bf16x8_t, q[u]), s, 0, 0, 0);
+            } else {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, raw),
+                                                           __builtin_bit_cast(f16x8_t, q[u]), s, 0, 0, 0);
+            }
+        }
+        return s;
+    }
+
+    /// acc += V^T P^T for the tile's probabilities p.
+    __device__ __forceinline__ static void values(const uint8_t* v, const Score& p, Score (&acc)[kAcc / kScores],
+                                                  int lane) {
+        if constexpr (kWide) {
+            const int g = lane >> 4;
+            const int j = lane & 15;
+#pragma unroll
+            for (int b = 0; b < kD / 16; ++b) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 4 * g + e;
+                    const int piece = (4 * b + (j >> 2)) ^ v_swizzle(row);
+                    const float x = *reinterpret_cast<const float*>(v + row * kRowBytes + (piece << 4) + (j & 3) * 4);
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, p[e], acc[b], 0, 0, 0);
+                }
+            }
+        } else {
+            const int half = lane >> 5;
+            const int quad = (lane >> 4) & 1;
+            const int j = lane & 15;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t bits[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (std::is_same<T, bf16_t>::value) {
+                        bits[e] = f32x2_to_bf16x2_bits(p[8 * u + 2 * e], p[8 * u + 2 * e + 1]);
+                    } else {
+                        bits[e] = Storage<T>::to_bits2(p[8 * u + 2 * e], p[8 * u + 2 * e + 1]);
+                    }
+                }
+                const u32x4_t pb = {bits[0], bits[1], bits[2], bits[3]};
+                // Tokens 16 u + 4 half .. + 3, then the same 8 further on.
+                const int row = 16 * u + 4 * half + (j >> 2);
+                const int sw = v_swizzle(row);
+#pragma unroll
+                for (int b = 0; b < kD / 32; ++b) {
+                    const int piece = (4 * b + 2 * quad + ((j & 3) >> 1)) ^ sw;
+                    const uint8_t* at = v + row * kRowBytes + (piece << 4) + (j & 1) * 8;
+                    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4_t*)(lds_u8_t*)(const_cast<uint8_t*>(at)));
+                    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4_t*)(lds_u8_t*)(const_cast<uint8_t*>(at + 8 * kRowBytes)));
+                    const auto vv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (std::is_same<T, bf16_t>::value) {
+                        acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vv),
+                                                                         __builtin_bit_cast(bf16x8_t, pb), acc[b], 0,
+                                                                         0, 0);
+                    } else {
+                        acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vv),
+                                                                        __builtin_bit_cast(f16x8_t, pb), acc[b], 0, 0,
+                                                                        0);
+                    }
+                }
+            }
+        }
+    }
+};
+
+/// LDS of a workgroup: four waves' tiles (K and V each) or a ring of four
+/// shared ones; afterwards the waves' outputs.
+template <typename T, int kD>
+constexpr int lds_bytes() {
+    using L = Tile<T, kD>;
+    constexpr int tiles = kStages * 2 * L::kBytes;
+    constexpr int outputs = kWaves * L::kRows * L::kOutPitch * 4;
+    return tiles > outputs ? tiles : outputs;
+}
+static_assert(kStages == kWaves, "the ring and the waves' own tiles take the same space");
+
+// ---- one work item ----------------------------------------------------------------
+
+/// One workgroup's part: tokens lo .. hi - 1 of the cache behind `table`, for
+/// query rows first_row .. of a set of sequences x heads of one KV head.
+struct Item {
+    const uint32_t* table;
+    int lo, hi;
+    int kv_head;
+    int first_sequence;
+    int sequences;   // rows are (sequence, head of the KV head)
+    int first_row;
+    int least;       // sequences with fewer tokens do not take part
+    int slot;
+};
+
+/// Four waves of different rows (kRowWaves 4) or of different tokens (1).
+template <typename T, int kD, int kRowWaves>
+__device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32]) {
+    using L = Tile<T, kD>;
+    constexpr int kTokenWaves = kWaves / kRowWaves;
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & (kWaveSize - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
+    const int row_wave = kRowWaves == 1 ? 0 : wave;
+    const int token_wave = kRowWaves == 1 ? wave : 0;
+    const int total_rows = w.sequences * a.per;
+
+    // Query rows of this wave; rows past the end are zeros.
+    typename L::Query q[L::kQueries];
+    const int row = w.first_row + row_wave * L::kRows + L::row_of(lane);
+    {
+        const bool inside = row < total_rows;
+        const int seq = w.first_sequence + (inside ? row / a.per : 0);
+        const int head = w.kv_head * a.per + (inside ? row % a.per : 0);
+        const T* from = static_cast<const T*>(a.query) + (static_cast<int64_t>(seq) * a.heads + head) * a.head_dim;
+#pragma unroll
+        for (int u = 0; u < L::kQueries; ++u) {
+            const int dim = L::query_dim(u, lane);
+            u32x4_t raw = {0u, 0u, 0u, 0u};
+            if (inside && dim < a.head_dim) raw = *reinterpret_cast<const u32x4_t*>(from + dim);
+            q[u] = __builtin_bit_cast(typename L::Query, raw);
+        }
+    }
+    if (a.head_dim < kD) {  // the copies leave the end of every row as it is
+        for (int i = tid; i < kStages * 2 * L::kBytes / 16; i += kThreads) {
+            reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0u, 0u, 0u, 0u};
+        }
+        __syncthreads();
+    }
+
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    const int64_t token_bytes = static_cast<int64_t>(a.kv_heads) * a.head_dim * sizeof(T);
+    const int64_t head_bytes = static_cast<int64_t>(w.kv_head) * a.head_dim * sizeof(T);
+    const int row_pieces = a.head_dim * static_cast<int>(sizeof(T)) / 16;
+
+    // 64 entries of the block table in lane registers: a token's page is a lane
+    // shuffle, not a load that would have to wait behind the copies.
+    int window_base = 0;
+    uint32_t window = 0;
+    bool loaded = false;
+    auto block_of = [&](int t) {
+        const uint32_t ut = static_cast<uint32_t>(t);
+        return static_cast<int>(a.block_shift >= 0 ? ut >> a.block_shift : ut / a.block_size);
+    };
+    // Where this wave's copies of the tile at token `first` read: the cache row
+    // of each copy's token (0 for one that is not there), and which of the
+    // tile's tokens are there.
+    constexpr int kCopies = L::kCopies / kRowWaves;
+    static_assert(L::kCopies % kRowWaves == 0, "copies per wave");
+    const int first_copy = row_wave * kCopies;
+    struct Rows {
+        uint32_t row[kCopies];
+        uint64_t valid;
+    };
+    auto look_up = [&](int first) {
+        const int begin = block_of(first);
+        const int end = block_of(first + L::kTokens - 1);  // at most kTokens - 1 further
+        if (!loaded || end >= window_base + kWaveSize) {   // tiles are taken in ascending order
+            window_base = begin;
+            window = w.table[min(begin + lane, a.max_blocks - 1)];
+            loaded = true;
+        }
+        const int t = first + (lane & (L::kTokens - 1));
+        const int block = block_of(t);
+        const uint32_t at = static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size;
+        const uint32_t page = static_cast<uint32_t>(__shfl(static_cast<int>(window), block - window_base));
+        const bool there = t < w.hi && page < a.pages;
+        const uint32_t row = there ? page * a.block_size + at : 0u;
+        Rows r;
+        r.valid = __builtin_amdgcn_ballot_w64(there) & ((uint64_t{1} << L::kTokens) - 1);
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) {
+            r.row[n] = static_cast<uint32_t>(
+                __shfl(static_cast<int>(row), ((first_copy + n) * kWaveSize + lane) / L::kChunks));
+        }
+        return r;
+    };
+    // This wave's copies of a K or V tile to LDS.
+    auto fetch = [&](const void* cache, const Rows& rows, uint32_t dst, bool is_k) {
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) {
+            const int piece_index = (first_copy + n) * kWaveSize + lane;
+            const int r = piece_index / L::kChunks;
+            const int piece = (piece_index % L::kChunks) ^ (is_k ? L::k_swizzle(r) : L::v_swizzle(r));
+            const uint8_t* from = static_cast<const uint8_t*>(cache) + rows.row[n] * token_bytes + head_bytes + piece * 16;
+            if (piece < row_pieces) copy16_to_lds(from, dst + static_cast<uint32_t>(first_copy + n) * 16 * kWaveSize);
+        }
+    };
+
+    float m = -INFINITY;  // the row's running maximum
+    float l = 0.0f;       // this lane's share of the running sum
+    typename L::Score acc[L::kAcc / L::kScores];
+#pragma unroll
+    for (int b = 0; b < L::kAcc / L::kScores; ++b) {
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) acc[b][i] = 0.0f;
+    }
+
+    constexpr uint64_t kAll = (uint64_t{1} << L::kTokens) - 1;
+    // Scores to probabilities, and the running values.
+    auto soften = [&](typename L::Score& s, uint64_t valid) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) {
+            s[i] *= a.c;
+            if (valid != kAll) s[i] = (valid >> L::token_of(i, lane)) & 1 ? s[i] : -INFINITY;
+            top = fmaxf(top, s[i]);
+        }
+#pragma unroll
+        for (int d = L::kRows; d < kWaveSize; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float m_new = fmaxf(m, top);
+        const float shift = m_new == -INFINITY ? 0.0f : m_new;
+        if (__builtin_amdgcn_ballot_w64(m_new > m) != 0) {
+            const float f = exp2f(m - shift);
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < L::kAcc / L::kScores; ++b) {
+#pragma unroll
+                for (int i = 0; i < L::kScores; ++i) acc[b][i] *= f;
+            }
+            m = m_new;
+        }
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] - shift);
+            l += s[i];
+        }
+    };
+    // Clear the V rows of tokens that are not there (waves' lanes in turn).
+    auto clear = [&](uint8_t* v, uint64_t valid, int start, int step) {
+        for (int i = start; i < L::kTokens * L::kChunks; i += step) {
+            if (((valid >> (i / L::kChunks)) & 1) == 0) {
+                reinterpret_cast<u32x4_t*>(v)[i] = u32x4_t{0u, 0u, 0u, 0u};
+            }
+        }
+    };
+
+    if constexpr (kRowWaves == 1) {
+        // The wave's own K and V tile, one copied while the other is used.
+        uint8_t* k = lds + wave * 2 * L::kBytes;
+        uint8_t* v = k + L::kBytes;
+        const uint32_t k_dst = lds_base + static_cast<uint32_t>(wave) * 2 * L::kBytes;
+        const uint32_t v_dst = k_dst + L::kBytes;
+        int t = w.lo + token_wave * L::kTokens;
+        constexpr int kStep = kTokenWaves * L::kTokens;
+        if (t < w.hi) {
+            Rows rows = look_up(t);
+            fetch(a.k_cache, rows, k_dst, true);
+            fetch(a.v_cache, rows, v_dst, false);
+            for (; t < w.hi; t += kStep) {
+                const bool more = t + kStep < w.hi;
+                const uint64_t now = rows.valid;
+                // K has landed: only V's copies may be in flight. (Copies that
+                // no lane takes part in are not issued, so a head narrower than
+                // kD waits for all.)
+                if (a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
+                typename L::Score s = L::scores(k, q, lane);
+                wait_lds();
+                if (more) {
+                    rows = look_up(t + kStep);
+                    fetch(a.k_cache, rows, k_dst, true);
+                }
+                soften(s, now);
+                if (more && a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
+                if (now != kAll) {
+                    clear(v, now, lane, kWaveSize);
+                    wait_lds();
+                }
+                L::values(v, s, acc, lane);
+                wait_lds();
+                if (more) fetch(a.v_cache, rows, v_dst, false);
+            }
+        }
+    } else {
+        // A ring of tiles; every wave copies a quarter of each.
+        const int tiles = (w.hi - w.lo + L::kTokens - 1) / L::kTokens;
+        auto issue = [&](int tile) {
+            const Rows rows = look_up(w.lo + tile * L::kTokens);
+            const uint32_t dst = lds_base + static_cast<uint32_t>(tile % kStages) * 2 * L::kBytes;
+            fetch(a.k_cache, rows, dst, true);
+            fetch(a.v_cache, rows, dst + L::kBytes, false);
+            return rows.valid;
+        };
+        uint64_t valid[kStages];  // of tiles i .. i + kStages - 1
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) valid[i] = i < tiles ? issue(i) : 0;
+        for (int i = 0; i < tiles; ++i) {
+            // This wave's copies of tile i have landed; behind it two tiles
+            // (fewer at the end) are in flight.
+            if (i + kStages - 2 < tiles && a.head_dim == kD) {
+                wait_vm<(kStages - 2) * 2 * kCopies>();
+            } else {
+                wait_vm<0>();
+            }
+            bare_barrier();
+            // Into tile i - 1's place, which every wave is past.
+            valid[kStages - 1] = i + kStages - 1 < tiles ? issue(i + kStages - 1) : 0;
+            uint8_t* k = lds + (i % kStages) * 2 * L::kBytes;
+            uint8_t* v = k + L::kBytes;
+            const uint64_t now = valid[0];
+            typename L::Score s = L::scores(k, q, lane);
+            soften(s, now);
+            if (now != kAll) {
+                clear(v, now, tid, kThreads);
+                __syncthreads();
+            }
+            L::values(v, s, acc, lane);
+            wait_lds();  // before the barrier that lets the tile be overwritten
+#pragma unroll
+            for (int j = 0; j + 1 < kStages; ++j) valid[j] = valid[j + 1];
+        }
+    }
+
+#pragma unroll
+    for (int d = L::kRows; d < kWaveSize; d <<= 1) l += __shfl_xor(l, d);
+    wait_vm<0>();
+    __syncthreads();  // all tiles are done with: their space takes the outputs
+    float* mine = reinterpret_cast<float*>(lds) + wave * L::kRows * L::kOutPitch;
+#pragma unroll
+    for (int i = 0; i < L::kAcc; i += 4) {
+        f32x4_t four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = acc[(i + e) / L::kScores][(i + e) % L::kScores];
+        *reinterpret_cast<f32x4_t*>(mine + L::row_of(lane) * L::kOutPitch + L::dim_of(i, lane)) = four;
+    }
+    if (L::part_of(lane) == 0) {
+        lds_m[wave][L::row_of(lane)] = m;
+        lds_l[wave][L::row_of(lane)] = l;
+    }
+    __syncthreads();
+    // Rows x groups of four dims, over the workgroup; token waves are joined.
+    constexpr int kOutRows = kRowWaves * L::kRows;
+    constexpr int kFours = kD / 4;
+    for (int i = tid; i < kOutRows * kFours; i += kThreads) {
+        const int r = i / kFours;
+        const int dim = (i % kFours) * 4;
+        const int grow = w.first_row + r;
+        if (grow >= total_rows || dim >= a.head_dim) continue;
+        const int seq = w.first_sequence + grow / a.per;
+        if (context_of(a, seq) < w.least) continue;
+        const int64_t out_row = static_cast<int64_t>(seq) * a.heads + w.kv_head * a.per + grow % a.per;
+        const int64_t at = static_cast<int64_t>(w.slot) * a.sequences * a.heads + out_row;
+        const int owner = kRowWaves == 1 ? 0 : r / L::kRows;
+        const int lr = r % L::kRows;
+        float mm = lds_m[owner][lr];
+#pragma unroll
+        for (int t = 1; t < kTokenWaves; ++t) mm = fmaxf(mm, lds_m[t][lr]);
+        float ll = 0.0f;
+        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < kTokenWaves; ++t) {
+            const int src = owner + t;
+            const float f = kTokenWaves == 1 ? 1.0f : lds_m[src][lr] == -INFINITY ? 0.0f : exp2f(lds_m[src][lr] - mm);
+            // A wave without a finite score still passes its NaN on.
+            ll += kTokenWaves > 1 && lds_m[src][lr] == -INFINITY ? lds_l[src][lr] : lds_l[src][lr] * f;
+            const f32x4_t four = *reinterpret_cast<const f32x4_t*>(
+                reinterpret_cast<const float*>(lds) + (src * L::kRows + lr) * L::kOutPitch + dim);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(four[e], f, sum[e]);
+        }
+        if (dim == 0) {
+            a.ml[2 * at] = mm;
+            a.ml[2 * at + 1] = ll;
+        }
+        float* to = a.acc + at * a.head_dim + dim;
+        *reinterpret_cast<f32x4_t*>(to) = sum;
+    }
+}
+
+/// Tokens of a range are a multiple of this (but for the last).
+template <typename T, int kD, int kRowWaves>
+constexpr int range_step() { return kWaves / kRowWaves * Tile<T, kD>::kTokens; }
+
+template <typename T, int kD, int kRowWaves>
+__global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedArgs a) {
+    using L = Tile<T, kD>;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[lds_bytes<T, kD>()];
+    __shared__ float lds_m[kWaves][32];
+    __shared__ float lds_l[kWaves][32];
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    Item w{};
+    int id = static_cast<int>(blockIdx.x);
+    if (id < a.prefix_items) {
+        // Row tile outermost: with a multiple of eight (KV head, range) pairs
+        // all row tiles of a pair run on one XCD, whose L2 then reads it once.
+        const int pairs = a.kv_heads * a.prefix_splits;
+        int tile = id / pairs;
+        id %= pairs;
+        const int split = id % a.prefix_splits;
+        w.kv_head = id / a.prefix_splits;
+        constexpr int kRows = kRowWaves * L::kRows;
+        const Group g = group_of_tile(a, kRows, tile);
+        if (g.end == 0 || g.prefix == 0) return;
+        const int each = split_length(g.prefix, a.prefix_splits, range_step<T, kD, kRowWaves>());
+        w.lo = split * each;
+        w.hi = min(g.prefix, w.lo + each);
+        if (w.lo >= w.hi) return;
+        // The pages of the first sequence that holds the whole prefix.
+        int holder = -1;
+        for (int s = g.first; s < g.end; s += kWaveSize) {
+            const bool holds = s + lane < g.end && context_of(a, s + lane) >= g.prefix;
+            const uint64_t any = __builtin_amdgcn_ballot_w64(holds);
+            if (any != 0) {
+                holder = s + __builtin_ctzll(any);
+                break;
+            }
+        }
+        if (holder < 0) return;
+        w.table = a.tables + static_cast<int64_t>(holder) * a.max_blocks;
+        w.first_sequence = g.first;
+        w.sequences = g.end - g.first;
+        w.first_row = tile * kRows;
+        w.least = g.prefix;
+        w.slot = split;
+        attend<T, kD, kRowWaves>(a, w, lds, lds_m, lds_l);
+    } else {
+        id -= a.prefix_items;
+        const int split = id % a.rest_splits;
+        id /= a.rest_splits;
+        const int tile = id % a.rest_tiles;
+        id /= a.rest_tiles;
+        w.kv_head = id % a.kv_heads;
+        const int s = id / a.kv_heads;
+        const int context = context_of(a, s);
+        const Group g = a.groups > 0 ? group_of(a, s) : Group{0, 0, 0};
+        const int first = g.end > 0 && g.prefix <= context ? g.prefix : 0;
+        const int each = split_length(context - first, a.rest_splits, range_step<T, kD, 1>());
+        w.lo = first + split * each;
+        w.hi = min(context, w.lo + each);
+        if (w.lo >= w.hi) return;
+        w.table = a.tables + static_cast<int64_t>(s) * a.max_blocks;
+        w.first_sequence = s;
+        w.sequences = 1;
+        w.first_row = tile * L::kRows;
+        w.least = 0;
+        w.slot = a.prefix_splits + split;
+        attend<T, kD, 1>(a, w, lds, lds_m, lds_l);
+    }
+}
+
+/// Any head size and alignment: a wave per (sequence, head, range of the whole
+/// context), a token at a time, dims over the lanes. No prefix is shared.
+template <typename T, int kPer>
+__global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedArgs a) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWaveSize;
+    if (id >= static_cast<int64_t>(a.sequences) * a.heads * a.rest_splits) return;
+    const int split = static_cast<int>(id % a.rest_splits);
+    const int64_t out_row = id / a.rest_splits;
+    const int head = static_cast<int>(out_row % a.heads);
+    const int s = static_cast<int>(out_row / a.heads);
+    const int context = context_of(a, s);
+    const int each = split_length(context, a.rest_splits, 32);
+    const int lo = split * each;
+    const int hi = min(context, lo + each);
+    if (lo >= hi) return;
+    const T* q = static_cast<const T*>(a.query) + out_row * a.head_dim;
+    float qv[kPer];
+    float acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int d = lane + i * kWaveSize;
+        qv[i] = d < a.head_dim ? Storage<T>::load(q + d) : 0.0f;
+        acc[i] = 0.0f;
+    }
+    float m = -INFINITY;
+    float l = 0.0f;
+    for (int t = lo; t < hi; ++t) {
+        const uint32_t page = a.tables[static_cast<int64_t>(s) * a.max_blocks + t / a.block_size];
+        if (page >= a.pages) continue;
+        const int64_t row = static_cast<int64_t>(page) * a.block_size + t % a.block_size;
+        const int64_t at = (row * a.kv_heads + head / a.per) * a.head_dim;
+        const T* k = static_cast<const T*>(a.k_cache) + at;
+        const T* v = static_cast<const T*>(a.v_cache) + at;
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int d = lane + i * kWaveSize;
+            if (d < a.head_dim) dot = fmaf(qv[i], Storage<T>::load(k + d), dot);
+        }
+        const float y = wave_reduce_f32<AddF32>(dot) * a.c;
+        const float m_new = fmaxf(m, y);
+        const float shift = m_new == -INFINITY ? 0.0f : m_new;
+        const float f = exp2f(m - shift);
+        const float p = exp2f(y - shift);
+        m = m_new;
+        l = fmaf(l, f, p);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int d = lane + i * kWaveSize;
+            if (d < a.head_dim) acc[i] = fmaf(acc[i], f, p * Storage<T>::load(v + d));
+        }
+    }
+    const int64_t slot_row = static_cast<int64_t>(split) * a.sequences * a.heads + out_row;
+    if (lane == 0) {
+        a.ml[2 * slot_row] = m;
+        a.ml[2 * slot_row + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int d = lane + i * kWaveSize;
+        if (d < a.head_dim) a.acc[slot_row * a.head_dim + d] = acc[i];
+    }
+}
+
+/// Joins the pieces of one (sequence, head): a wave each. prefix_step and
+/// rest_step are the first kernel's range steps (prefix_step 0: nothing was
+/// shared).
+template <typename T>
+__global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedArgs a, int prefix_step,
+                                                                         int rest_step) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    const int64_t rows = static_cast<int64_t>(a.sequences) * a.heads;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWaveSize;
+    if (row >= rows) return;
+    const int s = __builtin_amdgcn_readfirstlane(static_cast<int>(row / a.heads));
+    const int context = context_of(a, s);
+    int first = 0;
+    int prefix_pieces = 0;
+    if (prefix_step > 0) {
+        const Group g = group_of(a, s);
+        if (g.end > 0 && g.prefix <= context && g.prefix > 0) {
+            first = g.prefix;
+            const int each = split_length(first, a.prefix_splits, prefix_step);
+            prefix_pieces = (first + each - 1) / each;
+        }
+    }
+    int rest_pieces = 0;
+    if (context > first) {
+        const int each = split_length(context - first, a.rest_splits, rest_step);
+        rest_pieces = (context - first + each - 1) / each;
+    }
+    const int pieces = prefix_pieces + rest_pieces;
+    auto slot_of = [&](int i) { return i < prefix_pieces ? i : a.prefix_splits + i - prefix_pieces; };
+    // Lane i weighs piece i (at most 2 x 64 pieces).
+    static_assert(kMaxSplits <= kWaveSize, "two pieces per lane");
+    float pm[2], pl[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int i = lane + n * kWaveSize;
+        pm[n] = -INFINITY;
+        pl[n] = 0.0f;
+        if (i < pieces) {
+            const int64_t at = slot_of(i) * rows + row;
+            pm[n] = a.ml[2 * at];
+            pl[n] = a.ml[2 * at + 1];
+        }
+    }
+    const float m = wave_reduce_f32<MaxF32>(fmaxf(pm[0], pm[1]));
+    float weight[2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        weight[n] = pm[n] == -INFINITY ? 0.0f : exp2f(pm[n] - m);
+        sum += pm[n] == -INFINITY ? pl[n] : pl[n] * weight[n];
+    }
+    const float l = wave_reduce_f32<AddF32>(sum);
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + row * a.head_dim;
+    for (int d0 = 0; d0 < a.head_dim; d0 += kWaveSize) {
+        const int d = d0 + lane;
+        float o = 0.0f;
+        for (int i = 0; i < pieces; ++i) {
+            const float f = __shfl(i < kWaveSize ? weight[0] : weight[1], i & (kWaveSize - 1));
+            if (d < a.head_dim) o = fmaf(a.acc[(slot_of(i) * rows + row) * a.head_dim + d], f, o);
+        }
+        if (d < a.head_dim) Storage<T>::store(out + d, l == 0.0f ? 0.0f : o * inverse);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------
+
+struct Plan {
+    int dim;        // head size of the matrix kernel, or 0: the general kernel
+    int row_waves;  // 4: prefix tiles of four waves' rows
+    int prefix_splits;
+    int rest_splits;
+    int prefix_tiles;
+    int rest_tiles;
+};
+
+Plan plan_of(cf_dtype dtype, int64_t sequences, int64_t groups, int64_t heads, int64_t kv_heads, int64_t head_dim,
+             int64_t capacity) {
+    Plan p{};
+    const int64_t per = heads / kv_heads;
+    const bool wide = dtype == CF_F32;
+    const int64_t vec = wide ? 4 : 8;
+    if (head_dim % vec == 0 && head_dim <= (wide ? 128 : 256)) p.dim = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    auto splits = [&](int64_t items, int64_t target, int64_t least) {
+        int64_t n = items > 0 ? target / items : 1;
+        const int64_t most = ceil_div<int64_t>(capacity, least);
+        if (n > most) n = most;
+        if (n > kMaxSplits) n = kMaxSplits;
+        return static_cast<int>(n < 1 ? 1 : n);
+    };
+    if (p.dim == 0) {
+        p.rest_splits = splits(sequences * heads, 4096, 64);
+        return p;
+    }
+    const int64_t wave_rows = wide ? 16 : 32;
+    const int64_t rows = sequences * per;
+    if (groups > 0) {
+        // Four waves of rows where the groups fill more than one wave's.
+        p.row_waves = rows > wave_rows * groups ? 4 : 1;
+        const int64_t tile = p.row_waves * wave_rows;
+        p.prefix_tiles = static_cast<int>(rows / tile + groups);
+        const int64_t likely = ceil_div<int64_t>(rows, tile * groups) * groups;
+        p.prefix_splits = splits(likely * kv_heads, 512, 64);
+    } else {
+        p.row_waves = 1;
+    }
+    p.rest_tiles = static_cast<int>(ceil_div<int64_t>(per, wave_rows));
+    p.rest_splits = splits(sequences * kv_heads * p.rest_tiles, 512, 128);
+    return p;
+}
+
+int64_t capacity_of(int64_t max_blocks, int64_t block_size) {
+    const int64_t most = (int64_t{1} << 31) - 4096;  // token positions and the steps behind them stay in 32 bits
+    return max_blocks > most / block_size ? most : max_blocks * block_size;
+}
+
+size_t workspace_of(const Plan& p, int64_t sequences, int64_t heads, int64_t head_dim) {
+    const size_t slots = static_cast<size_t>(p.prefix_splits) + p.rest_splits;
+    const size_t rows = static_cast<size_t>(sequences) * heads;
+    return (slots * rows * 8 + 15) / 16 * 16 + slots * rows * head_dim * 4;
+}
+
+bool sizes_ok(int64_t sequences, int64_t groups, int64_t heads, int64_t kv_heads, int64_t head_dim,
+              int64_t block_size, int64_t max_blocks) {
+    return sequences > 0 && groups >= 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && head_dim <= 1024 &&
+           block_size > 0 && max_blocks > 0 && heads % kv_heads == 0;
+}
+
+template <typename T, int kD>
+void run_matrix(const SharedArgs& a, const Plan& p, dim3 grid, hipStream_t stream) {
+    if (p.row_waves == 4) {
+        launch(shared_attention_kernel<T, kD, 4>, grid, dim3(kThreads), 0, stream, a);
+    } else {
+        launch(shared_attention_kernel<T, kD, 1>, grid, dim3(kThreads), 0, stream, a);
+    }
+}
+
+template <typename T>
+void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
+    constexpr int tokens = sizeof(T) == 4 ? 16 : 32;
+    const int64_t rows = static_cast<int64_t>(a.sequences) * a.heads;
+    int prefix_step = 0;
+    int rest_step = 32;
+    if (p.dim == 0) {
+        const dim3 grid(static_cast<unsigned>(ceil_div<int64_t>(rows * a.rest_splits, kWaves)));
+        if (a.head_dim <= 128) {
+            launch(shared_attention_any_kernel<T, 2>, grid, dim3(kThreads), 0, stream, a);
+        } else {
+            launch(shared_attention_any_kernel<T, 16>, grid, dim3(kThreads), 0, stream, a);
+        }
+    } else {
+        prefix_step = a.groups > 0 ? kWaves / p.row_waves * tokens : 0;
+        rest_step = kWaves * tokens;
+        const int64_t rest = static_cast<int64_t>(a.sequences) * a.kv_heads * a.rest_tiles * a.rest_splits;
+        const dim3 grid(static_cast<unsigned>(a.prefix_items + rest));
+        if (p.dim == 64) {
+            run_matrix<T, 64>(a, p, grid, stream);
+        } else if (p.dim == 128) {
+            run_matrix<T, 128>(a, p, grid, stream);
+        } else if constexpr (sizeof(T) == 2) {
+            run_matrix<T, 256>(a, p, grid, stream);
+        }
+    }
+    launch(shared_attention_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div<int64_t>(rows, kWaves))),
+           dim3(kThreads), 0, stream, a, prefix_step, rest_step);
+}
+
+}  // namespace
+}  // namespace cf
+
+extern "C" {
+
+size_t cf_paged_attention_shared_workspace_bytes(cf_dtype dtype, int64_t num_sequences, int64_t num_groups,
+                                                 int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                                 int64_t block_size, int64_t max_blocks_per_sequence) {
+    if (!cf::valid_dtype(dtype) || !cf::sizes_ok(num_sequences, num_groups, num_heads, num_kv_heads, head_dim,
+                                                 block_size, max_blocks_per_sequence)) {
+        return 0;
+    }
+    const cf::Plan p = cf::plan_of(dtype, num_sequences, num_groups, num_heads, num_kv_heads, head_dim,
+                                   cf::capacity_of(max_blocks_per_sequence, block_size));
+    return cf::workspace_of(p, num_sequences, num_heads, head_dim);
+}
+
+cf_status cf_paged_attention_shared(const void* query, const void* k_cache, const void* v_cache,
+                                    const int32_t* group_starts, const int32_t* prefix_lens,
+                                    const uint32_t* block_tables, const int32_t* context_lens, void* out,
+                                    cf_dtype dtype, int64_t num_pages, int64_t num_sequences, int64_t num_groups,
+                                    int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                    int64_t max_blocks_per_sequence, float scale, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    CF_ENTRY();
+    const char* who = "cf_paged_attention_shared";
+    if (num_sequences <= 0 || num_heads <= 0 || head_dim <= 0) return CF_OK;
+    CF_REQUIRE(cf::valid_dtype(dtype), "%s: unknown dtype %d", who, static_cast<int>(dtype));
+    CF_REQUIRE(cf::sizes_ok(num_sequences, num_groups, num_heads, num_kv_heads, head_dim, block_size,
+                            max_blocks_per_sequence) && num_pages > 0,
+               "%s: %lld heads over %lld KV heads of %lld (at most 1024), blocks of %lld, %lld per sequence, %lld "
+               "pages, %lld groups",
+               who, static_cast<long long>(num_heads), static_cast<long long>(num_kv_heads),
+               static_cast<long long>(head_dim), static_cast<long long>(block_size),
+               static_cast<long long>(max_blocks_per_sequence), static_cast<long long>(num_pages),
+               static_cast<long long>(num_groups));
+    CF_REQUIRE(query != nullptr && k_cache != nullptr && v_cache != nullptr && block_tables != nullptr &&
+                   context_lens != nullptr && out != nullptr,
+               "%s: null pointer", who);
+    CF_REQUIRE(num_groups == 0 || (group_starts != nullptr && prefix_lens != nullptr), "%s: null pointer", who);
+    const size_t size = cf::dtype_size(dtype);
+    CF_REQUIRE(cf::host_aligned(query, size) && cf::host_aligned(k_cache, size) && cf::host_aligned(v_cache, size) &&
+                   cf::host_aligned(out, size),
+               "%s: misaligned pointer", who);
+    // Cache rows, token positions and work items are counted in 32 bits.
+    constexpr int64_t kMost = (int64_t{1} << 31) - 4096;
+    CF_REQUIRE(num_pages <= kMost / block_size && max_blocks_per_sequence <= kMost && num_groups <= (1 << 20) &&
+                   num_sequences <= kMost / num_heads,
+               "%s: %lld pages of %lld tokens, %lld sequences of %lld heads or %lld groups exceed 32-bit counts", who,
+               static_cast<long long>(num_pages), static_cast<long long>(block_size),
+               static_cast<long long>(num_sequences), static_cast<long long>(num_heads),
+               static_cast<long long>(num_groups));
+    cf::Plan p = cf::plan_of(dtype, num_sequences, num_groups, num_heads, num_kv_heads, head_dim,
+                             cf::capacity_of(max_blocks_per_sequence, block_size));
+    const size_t needed = cf::workspace_of(p, num_sequences, num_heads, head_dim);
+    CF_REQUIRE(workspace != nullptr && workspace_bytes >= needed && cf::host_aligned(workspace, 16),
+               "%s: needs %zu bytes of 16-byte aligned workspace", who, needed);
+    if (p.dim != 0 && !(cf::host_aligned(query, 16) && cf::host_aligned(k_cache, 16) && cf::host_aligned(v_cache, 16))) {
+        p.dim = 0;  // same workspace, read as ranges of whole contexts
+        p.prefix_splits = 0;
+    }
+    cf::SharedArgs a{};
+    a.query = query;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.starts = group_starts;
+    a.prefix = prefix_lens;
+    a.tables = block_tables;
+    a.context = context_lens;
+    a.out = out;
+    a.pages = static_cast<uint32_t>(num_pages);
+    a.block_size = static_cast<uint32_t>(block_size);
+    a.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll(static_cast<uint64_t>(block_size)) : -1;
+    a.sequences = static_cast<int>(num_sequences);
+    a.heads = static_cast<int>(num_heads);
+    a.kv_heads = static_cast<int>(num_kv_heads);
+    a.per = static_cast<int>(num_heads / num_kv_heads);
+    a.head_dim = static_cast<int>(head_dim);
+    a.groups = p.dim != 0 ? static_cast<int>(num_groups) : 0;
+    a.max_blocks = static_cast<int>(max_blocks_per_sequence);
+    a.capacity = static_cast<int>(cf::capacity_of(max_blocks_per_sequence, block_size));
+    a.prefix_splits = p.prefix_splits;
+    a.rest_splits = p.rest_splits;
+    a.prefix_tiles = p.prefix_tiles;
+    a.rest_tiles = p.rest_tiles;
+    const int64_t prefix_items =
+        a.groups > 0 ? static_cast<int64_t>(p.prefix_tiles) * num_kv_heads * p.prefix_splits : 0;
+    const int64_t rest_items = num_sequences * num_kv_heads * (p.rest_tiles > 0 ? p.rest_tiles : 1) * p.rest_splits;
+    CF_REQUIRE(prefix_items + rest_items < kMost && num_sequences * num_heads * p.rest_splits < kMost,
+               "%s: too many work items", who);
+    a.prefix_items = static_cast<int>(prefix_items);
+    a.c = scale * cf::kLog2e;
+    const size_t rows = static_cast<size_t>(num_sequences) * num_heads;
+    const size_t slots = static_cast<size_t>(p.prefix_splits) + p.rest_splits;
+    a.ml = static_cast<float*>(workspace);
+    a.acc = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (slots * rows * 8 + 15) / 16 * 16);
+    auto s = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case CF_F32: cf::run<float>(a, p, s); break;
+        case CF_F16: cf::run<cf::f16_t>(a, p, s); break;
+        case CF_BF16: cf::run<cf::bf16_t>(a, p, s); break;
+    }
+    return cf::check_launch("launching shared-prefix paged attention", s);
+}
+
+}  // extern "C"

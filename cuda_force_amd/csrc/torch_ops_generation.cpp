@@ -1,9 +1,12 @@
-// Dispatcher registration of the operators of token generation: log
-// probabilities of tokens with their gradient. Same conventions as
+// Dispatcher registration of the operators of token generation: attention over
+// a paged cache behind shared prompts, and log probabilities of tokens with
+// their gradient. Same conventions as
 // torch_ops.cpp: ATen on the CPU, the C ABI of libcudaforge_hip.so on
 // PyTorch's current HIP stream on the GPU, never synchronising; workspaces
 // from torch's caching allocator.
 #include "torch_ops_common.hpp"
+
+#include <algorithm>
 
 namespace cudaforge_amd {
 namespace {
@@ -145,6 +148,98 @@ torch::Tensor token_logprobs_backward_cpu(const torch::Tensor& logits, const tor
     return (scale * grad).to(logits.scalar_type());
 }
 
+// ---- paged attention behind shared prompts -----------------------------------
+
+void check_ints(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, const char* name) {
+    TORCH_CHECK(t.dim() == dim, name, " must have ", dim, " dimensions, got ", t.dim());
+    TORCH_CHECK(t.scalar_type() == torch::kInt32, name, " must be int32, got ", t.scalar_type());
+    check_contiguous(t, name);
+    check_same_device(like, t, name);
+}
+
+void check_shared(const torch::Tensor& query, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                  const torch::Tensor& starts, const torch::Tensor& prefix, const torch::Tensor& tables,
+                  const torch::Tensor& context) {
+    TORCH_CHECK(query.dim() == 3, "query must be [sequences, heads, head_dim], got ", query.dim(), " dimensions");
+    TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [pages, block, kv_heads, head_dim], got ", k_cache.dim(),
+                " dimensions");
+    TORCH_CHECK(v_cache.sizes() == k_cache.sizes(), "v_cache has shape ", v_cache.sizes(), " but k_cache ",
+                k_cache.sizes());
+    for (const auto& [t, name] : {std::pair<const torch::Tensor*, const char*>{&k_cache, "k_cache"},
+                                  {&v_cache, "v_cache"}}) {
+        check_contiguous(*t, name);
+        check_same_device(query, *t, name);
+        TORCH_CHECK(t->scalar_type() == query.scalar_type(), name, " has dtype ", t->scalar_type(),
+                    " but query has ", query.scalar_type());
+    }
+    check_contiguous(query, "query");
+    TORCH_CHECK(k_cache.size(3) == query.size(2), "the cache's head size is ", k_cache.size(3), " but the query's ",
+                query.size(2));
+    TORCH_CHECK(k_cache.size(2) > 0 && query.size(1) % k_cache.size(2) == 0, query.size(1),
+                " heads are not a multiple of ", k_cache.size(2), " KV heads");
+    check_ints(tables, 2, query, "block_tables");
+    check_ints(context, 1, query, "context_lens");
+    check_ints(starts, 1, query, "group_starts");
+    check_ints(prefix, 1, query, "prefix_lens");
+    TORCH_CHECK(tables.size(0) == query.size(0) && context.size(0) == query.size(0),
+                "block_tables and context_lens must have a row for each of ", query.size(0), " sequences");
+    TORCH_CHECK(starts.size(0) == prefix.size(0) + 1, "group_starts must have one entry more than prefix_lens");
+}
+
+torch::Tensor paged_attention_shared_hip(const torch::Tensor& query, const torch::Tensor& k_cache,
+                                         const torch::Tensor& v_cache, const torch::Tensor& starts,
+                                         const torch::Tensor& prefix, const torch::Tensor& tables,
+                                         const torch::Tensor& context, double scale) {
+    check_shared(query, k_cache, v_cache, starts, prefix, tables, context);
+    const at::DeviceGuard guard(query.device());
+    torch::Tensor out = torch::empty_like(query);
+    if (query.numel() == 0) return out;
+    if (k_cache.size(0) == 0 || k_cache.size(1) == 0 || tables.size(1) == 0) return out.zero_();
+    const cf_dtype dtype = to_cf(query, "query");
+    const int64_t sequences = query.size(0), heads = query.size(1), dim = query.size(2);
+    const int64_t groups = prefix.size(0), kv_heads = k_cache.size(2), block = k_cache.size(1);
+    const size_t bytes = cf_paged_attention_shared_workspace_bytes(dtype, sequences, groups, heads, kv_heads, dim,
+                                                                   block, tables.size(1));
+    const torch::Tensor workspace =
+        torch::empty({static_cast<int64_t>(bytes)}, query.options().dtype(torch::kUInt8));
+    check_status(cf_paged_attention_shared(
+        query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), starts.data_ptr<int32_t>(),
+        prefix.data_ptr<int32_t>(), reinterpret_cast<const uint32_t*>(tables.data_ptr<int32_t>()),
+        context.data_ptr<int32_t>(), out.data_ptr(), dtype, k_cache.size(0), sequences, groups, heads, kv_heads, dim,
+        block, tables.size(1), static_cast<float>(scale), workspace.data_ptr(), bytes, stream_for(query)));
+    return out;
+}
+
+/// Sequence by sequence over its own table: sharing changes no result.
+torch::Tensor paged_attention_shared_cpu(const torch::Tensor& query, const torch::Tensor& k_cache,
+                                         const torch::Tensor& v_cache, const torch::Tensor& starts,
+                                         const torch::Tensor& prefix, const torch::Tensor& tables,
+                                         const torch::Tensor& context, double scale) {
+    check_shared(query, k_cache, v_cache, starts, prefix, tables, context);
+    torch::Tensor out = torch::zeros_like(query);
+    const int64_t pages = k_cache.size(0), block = k_cache.size(1), kv_heads = k_cache.size(2), dim = k_cache.size(3);
+    if (query.numel() == 0 || pages == 0 || block == 0 || tables.size(1) == 0) return out;
+    const torch::Tensor keys = k_cache.reshape({pages * block, kv_heads, dim});
+    const torch::Tensor vals = v_cache.reshape({pages * block, kv_heads, dim});
+    for (int64_t s = 0; s < query.size(0); ++s) {
+        const int64_t length = std::min<int64_t>(std::max(context[s].item<int32_t>(), 0), tables.size(1) * block);
+        const torch::Tensor token = torch::arange(length);
+        const torch::Tensor page = tables[s].to(torch::kInt64).index({token.floor_divide(block)});
+        const torch::Tensor there = (page >= 0) & (page < pages);
+        const torch::Tensor slot = (page * block + token.remainder(block)).index({there});
+        if (slot.numel() == 0) continue;
+        const torch::Tensor k = keys.index({slot}).to(torch::kFloat32).permute({1, 2, 0});
+        const torch::Tensor v = vals.index({slot}).to(torch::kFloat32).permute({1, 0, 2});
+        const torch::Tensor q = query[s].to(torch::kFloat32).view({kv_heads, -1, dim});
+        const torch::Tensor scores = torch::matmul(q, k) * scale;
+        torch::Tensor o = torch::matmul(torch::softmax(scores, -1), v);
+        const torch::Tensor none = (scores == -std::numeric_limits<float>::infinity()).all(-1, true);
+        o = o.masked_fill(none, 0.0);
+        out[s].copy_(o.view({query.size(1), dim}));
+    }
+    return out;
+}
+
 }  // namespace
 
 // ---- direct entry for ordinary GPU calls (the rules: torch_ops_common.hpp) ------
@@ -179,13 +274,49 @@ py::object try_token_logprobs(py::handle logits_, py::handle tokens_, py::handle
                           *top > 0 ? wrap(top_tokens) : py::none());
 }
 
+py::object try_paged_attention_shared(py::handle query_, py::handle k_, py::handle v_, py::handle starts_,
+                                      py::handle prefix_, py::handle tables_, py::handle context_,
+                                      py::handle scale_) {
+    const at::Tensor* query = ordinary(query_);
+    const at::Tensor* k = ordinary(k_);
+    const at::Tensor* v = ordinary(v_);
+    const at::Tensor* starts = ordinary(starts_);
+    const at::Tensor* prefix = ordinary(prefix_);
+    const at::Tensor* tables = ordinary(tables_);
+    const at::Tensor* context = ordinary(context_);
+    const std::optional<double> scale = plain_double(scale_);
+    if (starts == nullptr || prefix == nullptr || tables == nullptr || context == nullptr || !scale ||
+        !ordinary_context() || !ordinary_set({query, k, v})) {
+        return py::none();
+    }
+    if (query->dim() != 3 || k->dim() != 4 || v->sizes() != k->sizes() || k->size(3) != query->size(2) ||
+        query->size(2) > 1024 || query->size(1) % k->size(2) != 0 || starts->dim() != 1 || prefix->dim() != 1 ||
+        tables->dim() != 2 || context->dim() != 1 || starts->size(0) != prefix->size(0) + 1 ||
+        tables->size(0) != query->size(0) || context->size(0) != query->size(0)) {
+        return py::none();
+    }
+    for (const at::Tensor* t : {starts, prefix, tables, context}) {
+        if (t->scalar_type() != torch::kInt32 || t->device() != query->device()) return py::none();
+    }
+    at::Tensor out;
+    {
+        py::gil_scoped_release no_gil;
+        out = paged_attention_shared_hip(*query, *k, *v, *starts, *prefix, *tables, *context, *scale);
+    }
+    return wrap(out);
+}
+
 void bind_generation(py::module_& m) {
+    m.def("try_paged_attention_shared", torch::wrap_pybind_function(&try_paged_attention_shared));
     m.def("try_token_logprobs", torch::wrap_pybind_function(&try_token_logprobs));
 }
 
 }  // namespace cudaforge_amd
 
 TORCH_LIBRARY_FRAGMENT(cudaforge, m) {
+    m.def(
+        "paged_attention_shared(Tensor query, Tensor k_cache, Tensor v_cache, Tensor group_starts, "
+        "Tensor prefix_lens, Tensor block_tables, Tensor context_lens, float scale) -> Tensor");
     m.def(
         "token_logprobs(Tensor logits, Tensor tokens, float scale, bool entropy, int top) "
         "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
@@ -197,19 +328,21 @@ TORCH_LIBRARY_FRAGMENT(cudaforge, m) {
 // As in torch_ops.cpp: differentiating the operators themselves raises;
 // the Python layer has the differentiable form.
 TORCH_LIBRARY_IMPL(cudaforge, Autograd, m) {
-    for (const char* name : {"token_logprobs", "token_logprobs_backward"}) {
+    for (const char* name : {"paged_attention_shared", "token_logprobs", "token_logprobs_backward"}) {
         m.impl(name, torch::autograd::autogradNotImplementedFallback());
     }
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, CPU, m) {
     using namespace cudaforge_amd;
+    m.impl("paged_attention_shared", &paged_attention_shared_cpu);
     m.impl("token_logprobs", &token_logprobs_cpu);
     m.impl("token_logprobs_backward", &token_logprobs_backward_cpu);
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
     using namespace cudaforge_amd;
+    m.impl("paged_attention_shared", &paged_attention_shared_hip);
     m.impl("token_logprobs", &token_logprobs_hip);
     m.impl("token_logprobs_backward", &token_logprobs_backward_hip);
 }

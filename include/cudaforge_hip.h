@@ -524,6 +524,47 @@ cf_status cf_paged_attention(const void* query, const void* k_cache, const void*
                              int64_t max_blocks_per_sequence, float scale, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ---- paged attention behind shared prompts ------------------------------- */
+
+/* Workspace bytes cf_paged_attention_shared needs: the pieces of split
+ * contexts. It has no counterpart in the reference. */
+size_t cf_paged_attention_shared_workspace_bytes(cf_dtype dtype, int64_t num_sequences,
+                                                 int64_t num_groups, int64_t num_heads,
+                                                 int64_t num_kv_heads, int64_t head_dim,
+                                                 int64_t block_size,
+                                                 int64_t max_blocks_per_sequence);
+
+/* What cf_paged_attention computes (same layouts; fp32, fp16 or bf16), for a
+ * batch in which groups of neighbouring sequences begin with the same tokens:
+ * sequences group_starts[g] .. group_starts[g + 1] - 1 (g < num_groups) hold
+ * equal K and V in their first prefix_lens[g] tokens, which are read once for
+ * all of them, from the first of these sequences whose context holds the whole
+ * prefix. A prefix need not end with a block, and the sequences' tables may name
+ * the same pages or copies. A sequence whose context is shorter than its
+ * group's prefix, and one that no group holds, is served from its own table
+ * alone. group_starts [num_groups + 1] and prefix_lens [num_groups] are int32
+ * on the device; starts are taken in ascending order (one below an earlier one
+ * counts as that one) and within 0 .. num_sequences, prefixes within the
+ * tables' reach. num_groups 0: nothing is shared, both may be NULL.
+ * k_cache and v_cache hold num_pages blocks: a token whose table entry is not
+ * below num_pages is left out, as are contexts' tokens past the table. Sequences
+ * without tokens get zeros, and so does a row all of whose scores are -inf.
+ * Cache rows behind a context's end are never used, whatever they hold.
+ * Matrix-core kernels take head sizes that are multiples of 8 up to 256 (fp32:
+ * multiples of 4 up to 128) with 16-byte aligned query and caches; every other
+ * head size up to 1024 runs a general kernel, which shares nothing.
+ * Deterministic. The workspace is 16-byte aligned, in any state; overlapping
+ * calls need their own. It has no counterpart in the reference, whose operator
+ * reads every sequence's own table (cuda/include/cudaforge/paged_attention.cuh:61-65). */
+cf_status cf_paged_attention_shared(const void* query, const void* k_cache, const void* v_cache,
+                                    const int32_t* group_starts, const int32_t* prefix_lens,
+                                    const uint32_t* block_tables, const int32_t* context_lens,
+                                    void* out, cf_dtype dtype, int64_t num_pages,
+                                    int64_t num_sequences, int64_t num_groups, int64_t num_heads,
+                                    int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                    int64_t max_blocks_per_sequence, float scale, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /* ---- causal attention products ------------------------------------------ */
 
 /* scores[b, h, s, t] = sum_d q[b, s, h, d] * k[b, t, h, d] for t <= s: the
