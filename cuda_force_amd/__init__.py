@@ -33,7 +33,14 @@ from cuda_force_amd.ops import (
     swiglu,
     token_logprobs,
 )
-from cuda_force_amd.paged_cache import paged_attention_shared
+from cuda_force_amd.paged_cache import (
+    cache_compact,
+    cache_copy,
+    cache_extend,
+    cache_fork,
+    cache_release,
+    paged_attention_shared,
+)
 
 __version__ = "0.1.0"
 
@@ -45,6 +52,11 @@ __all__ = [
     "ExtensionMissingError",
     "TokenLogprobs",
     "backend_report",
+    "cache_compact",
+    "cache_copy",
+    "cache_extend",
+    "cache_fork",
+    "cache_release",
     "dequantize_int8",
     "fake_quantize_int8",
     "fused_residual_rmsnorm",

@@ -86,6 +86,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I32,
         [_P, _I32, _I64, _I64, _I64, _P, _I64, _F, _P, _P, _P, _P, _P, _I64, _P],
     ),
+    "cf_cache_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "cf_cache_copy": (_I32, [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _SZ, _P]),
+    "cf_cache_fork": (
+        _I32,
+        [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _SZ, _P],
+    ),
+    "cf_cache_extend": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _SZ, _P]),
+    "cf_cache_release": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P]),
+    "cf_cache_compact": (
+        _I32,
+        [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ, _P],
+    ),
     "cf_paged_attention_shared_workspace_bytes": (
         _SZ,
         [_I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64],

@@ -47,6 +47,7 @@ HIP_SOURCES = (
     "cf_matmul_fp8.hip",
     "cf_attention.hip",
     "cf_logprobs.hip",
+    "cf_pages.hip",
     "cf_shared_attention.hip",
 )
 

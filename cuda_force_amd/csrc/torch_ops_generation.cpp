@@ -1,6 +1,6 @@
-// Dispatcher registration of the operators of token generation: attention over
-// a paged cache behind shared prompts, and log probabilities of tokens with
-// their gradient. Same conventions as
+// Dispatcher registration of the operators of token generation: pages of a
+// paged cache, attention over it behind shared prompts, and log probabilities
+// of tokens with their gradient. Same conventions as
 // torch_ops.cpp: ATen on the CPU, the C ABI of libcudaforge_hip.so on
 // PyTorch's current HIP stream on the GPU, never synchronising; workspaces
 // from torch's caching allocator.
@@ -148,7 +148,7 @@ torch::Tensor token_logprobs_backward_cpu(const torch::Tensor& logits, const tor
     return (scale * grad).to(logits.scalar_type());
 }
 
-// ---- paged attention behind shared prompts -----------------------------------
+// ---- pages of a paged cache ------------------------------------------------
 
 void check_ints(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, const char* name) {
     TORCH_CHECK(t.dim() == dim, name, " must have ", dim, " dimensions, got ", t.dim());
@@ -156,6 +156,157 @@ void check_ints(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, 
     check_contiguous(t, name);
     check_same_device(like, t, name);
 }
+
+/// Caches as the C ABI takes them: pointers, and the bytes of a page.
+struct CacheList {
+    std::vector<void*> pointers;
+    int64_t page_bytes = 0;
+    int64_t pages = 0;
+    int64_t block = 0;
+};
+
+CacheList cache_list(at::TensorList caches, bool by_token) {
+    TORCH_CHECK(!caches.empty(), "caches must name at least one tensor");
+    const torch::Tensor& first = caches[0];
+    TORCH_CHECK(first.dim() >= (by_token ? 2 : 1), "caches must be [pages, block, ...], got ", first.sizes());
+    CacheList list;
+    list.pages = first.size(0);
+    list.block = first.dim() > 1 ? first.size(1) : 1;
+    for (const torch::Tensor& t : caches) {
+        check_contiguous(t, "a cache");
+        check_same_device(first, t, "a cache");
+        TORCH_CHECK(t.sizes() == first.sizes() && t.scalar_type() == first.scalar_type(),
+                    "caches differ in shape or dtype: ", t.sizes(), " and ", first.sizes());
+        list.pointers.push_back(t.data_ptr());
+    }
+    list.page_bytes = list.pages > 0 ? first.numel() / list.pages * first.element_size() : 0;
+    return list;
+}
+
+/// Counts a write for autograd's saved-tensor checks, as the mutating
+/// operators of torch do.
+void mark_written(const torch::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+torch::Tensor page_workspace(const torch::Tensor& like, int64_t pages, int64_t sequences, int64_t count) {
+    const size_t bytes = cf_cache_workspace_bytes(pages, sequences, count);
+    return torch::empty({static_cast<int64_t>(bytes)}, like.options().dtype(torch::kUInt8));
+}
+
+void check_state(const torch::Tensor& counts, const torch::Tensor& tables, const torch::Tensor& context) {
+    check_ints(counts, 1, counts, "ref_counts");
+    check_ints(tables, 2, counts, "block_tables");
+    check_ints(context, 1, counts, "context_lens");
+    TORCH_CHECK(tables.size(0) == context.size(0), "block_tables has ", tables.size(0), " rows but context_lens ",
+                context.size(0));
+}
+
+uint32_t* entries(const torch::Tensor& tables) { return reinterpret_cast<uint32_t*>(tables.data_ptr<int32_t>()); }
+
+torch::Tensor cache_copy_hip(at::TensorList caches, const torch::Tensor& src, const torch::Tensor& dst) {
+    const CacheList list = cache_list(caches, false);
+    check_ints(src, 1, caches[0], "src");
+    check_ints(dst, 1, caches[0], "dst");
+    TORCH_CHECK(src.size(0) == dst.size(0), "src and dst differ in length: ", src.size(0), " and ", dst.size(0));
+    const at::DeviceGuard guard(src.device());
+    torch::Tensor status = torch::empty_like(src);
+    if (src.numel() == 0) return status;
+    if (list.page_bytes == 0) return status.fill_(list.pages == 0 ? 1 : 0);
+    const torch::Tensor workspace = page_workspace(src, list.pages, 0, src.size(0));
+    check_status(cf_cache_copy(list.pointers.data(), list.pointers.size(), list.page_bytes, list.pages,
+                               src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), src.size(0),
+                               status.data_ptr<int32_t>(), workspace.data_ptr(), workspace.numel(), stream_for(src)));
+    for (const torch::Tensor& t : caches) mark_written(t);
+    return status;
+}
+
+torch::Tensor cache_fork_hip(at::TensorList caches, const torch::Tensor& counts, const torch::Tensor& tables,
+                             const torch::Tensor& context, const torch::Tensor& parents,
+                             const torch::Tensor& children) {
+    const CacheList list = cache_list(caches, true);
+    check_state(counts, tables, context);
+    check_same_device(counts, caches[0], "a cache");
+    check_ints(parents, 1, counts, "parents");
+    check_ints(children, 1, counts, "children");
+    TORCH_CHECK(counts.size(0) == list.pages, "ref_counts counts ", counts.size(0), " pages, the caches hold ",
+                list.pages);
+    TORCH_CHECK(parents.size(0) == children.size(0), "parents and children differ in length: ", parents.size(0),
+                " and ", children.size(0));
+    const at::DeviceGuard guard(counts.device());
+    torch::Tensor status = torch::empty_like(parents);
+    if (parents.numel() == 0) return status;
+    if (list.page_bytes == 0 || tables.numel() == 0) return status.fill_(1);
+    const torch::Tensor workspace = page_workspace(counts, list.pages, tables.size(0), parents.size(0));
+    check_status(cf_cache_fork(list.pointers.data(), list.pointers.size(), list.page_bytes,
+                               counts.data_ptr<int32_t>(), entries(tables), context.data_ptr<int32_t>(), list.pages,
+                               list.block, tables.size(0), tables.size(1), parents.data_ptr<int32_t>(),
+                               children.data_ptr<int32_t>(), parents.size(0), status.data_ptr<int32_t>(),
+                               workspace.data_ptr(), workspace.numel(), stream_for(counts)));
+    for (const torch::Tensor& t : caches) mark_written(t);
+    for (const torch::Tensor* t : {&counts, &tables, &context}) mark_written(*t);
+    return status;
+}
+
+torch::Tensor cache_extend_hip(const torch::Tensor& counts, const torch::Tensor& tables, const torch::Tensor& context,
+                               const torch::Tensor& sequences, int64_t block, int64_t tokens) {
+    check_state(counts, tables, context);
+    check_ints(sequences, 1, counts, "sequences");
+    TORCH_CHECK(block > 0 && tokens > 0, "block_size and tokens must be positive, got ", block, " and ", tokens);
+    const at::DeviceGuard guard(counts.device());
+    torch::Tensor slots = torch::empty({sequences.size(0), tokens}, sequences.options().dtype(torch::kInt64));
+    if (sequences.numel() == 0) return slots;
+    if (tables.numel() == 0 || counts.numel() == 0) return slots.fill_(-1);
+    const torch::Tensor workspace = page_workspace(counts, counts.size(0), tables.size(0), sequences.size(0));
+    check_status(cf_cache_extend(counts.data_ptr<int32_t>(), entries(tables), context.data_ptr<int32_t>(),
+                                 counts.size(0), block, tables.size(0), tables.size(1), sequences.data_ptr<int32_t>(),
+                                 sequences.size(0), tokens, slots.data_ptr<int64_t>(), workspace.data_ptr(),
+                                 workspace.numel(), stream_for(counts)));
+    for (const torch::Tensor* t : {&counts, &tables, &context}) mark_written(*t);
+    return slots;
+}
+
+void cache_release_hip(const torch::Tensor& counts, const torch::Tensor& tables, const torch::Tensor& context,
+                       const torch::Tensor& sequences, int64_t block) {
+    check_state(counts, tables, context);
+    check_ints(sequences, 1, counts, "sequences");
+    TORCH_CHECK(block > 0, "block_size must be positive, got ", block);
+    const at::DeviceGuard guard(counts.device());
+    if (sequences.numel() == 0 || tables.numel() == 0 || counts.numel() == 0) return;
+    check_status(cf_cache_release(counts.data_ptr<int32_t>(), entries(tables), context.data_ptr<int32_t>(),
+                                  counts.size(0), block, tables.size(0), tables.size(1),
+                                  sequences.data_ptr<int32_t>(), sequences.size(0), stream_for(counts)));
+    for (const torch::Tensor* t : {&counts, &context}) mark_written(*t);
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> cache_compact_hip(at::TensorList caches,
+                                                                          const torch::Tensor& counts,
+                                                                          const torch::Tensor& tables,
+                                                                          const torch::Tensor& context) {
+    const CacheList list = cache_list(caches, true);
+    check_state(counts, tables, context);
+    check_same_device(counts, caches[0], "a cache");
+    TORCH_CHECK(counts.size(0) == list.pages, "ref_counts counts ", counts.size(0), " pages, the caches hold ",
+                list.pages);
+    const at::DeviceGuard guard(counts.device());
+    torch::Tensor new_counts = torch::empty_like(counts);
+    torch::Tensor new_tables = torch::empty_like(tables);
+    torch::Tensor live = torch::empty({1}, counts.options());
+    if (list.pages == 0 || list.block == 0) {
+        new_tables.copy_(tables);
+        return {new_counts.copy_(counts), new_tables, live.fill_(0)};
+    }
+    const torch::Tensor workspace = page_workspace(counts, list.pages, tables.size(0), 0);
+    check_status(cf_cache_compact(list.pointers.data(), list.page_bytes > 0 ? list.pointers.size() : 0,
+                                  list.page_bytes, counts.data_ptr<int32_t>(), entries(tables),
+                                  context.data_ptr<int32_t>(), list.pages, list.block, tables.size(0), tables.size(1),
+                                  new_counts.data_ptr<int32_t>(), entries(new_tables), live.data_ptr<int32_t>(),
+                                  workspace.data_ptr(), workspace.numel(), stream_for(counts)));
+    for (const torch::Tensor& t : caches) mark_written(t);
+    return {new_counts, new_tables, live};
+}
+
+// ---- paged attention behind shared prompts -----------------------------------
 
 void check_shared(const torch::Tensor& query, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
                   const torch::Tensor& starts, const torch::Tensor& prefix, const torch::Tensor& tables,
@@ -274,6 +425,130 @@ py::object try_token_logprobs(py::handle logits_, py::handle tokens_, py::handle
                           *top > 0 ? wrap(top_tokens) : py::none());
 }
 
+/// A list or tuple of ordinary tensors without gradients, or nothing.
+std::optional<std::vector<at::Tensor>> ordinary_list(py::handle object) {
+    if (!PyList_CheckExact(object.ptr()) && !PyTuple_CheckExact(object.ptr())) return std::nullopt;
+    std::vector<at::Tensor> list;
+    for (const py::handle item : py::reinterpret_borrow<py::sequence>(object)) {
+        const at::Tensor* t = ordinary(item);
+        if (t == nullptr || t->requires_grad()) return std::nullopt;
+        if (!list.empty() && (t->sizes() != list[0].sizes() || t->scalar_type() != list[0].scalar_type() ||
+                              t->device() != list[0].device())) {
+            return std::nullopt;
+        }
+        list.push_back(*t);
+    }
+    return list.empty() ? std::nullopt : std::make_optional(std::move(list));
+}
+
+/// Ordinary int32 tensors of the given dimensions, all on one device.
+bool ordinary_ints(std::initializer_list<std::pair<const at::Tensor*, int64_t>> tensors) {
+    const at::Tensor* first = tensors.begin()->first;
+    for (const auto& [t, dim] : tensors) {
+        if (t == nullptr || t->scalar_type() != torch::kInt32 || t->dim() != dim || t->device() != first->device()) {
+            return false;
+        }
+    }
+    return true;
+}
+
+py::object try_cache_copy(py::handle caches_, py::handle src_, py::handle dst_) {
+    const at::Tensor* src = ordinary(src_);
+    const at::Tensor* dst = ordinary(dst_);
+    if (!ordinary_context() || !ordinary_ints({{src, 1}, {dst, 1}}) || src->size(0) != dst->size(0)) return py::none();
+    const auto caches = ordinary_list(caches_);
+    if (!caches || (*caches)[0].device() != src->device() || (*caches)[0].dim() < 1) return py::none();
+    at::Tensor status;
+    {
+        py::gil_scoped_release no_gil;
+        status = cache_copy_hip(*caches, *src, *dst);
+    }
+    return wrap(status);
+}
+
+py::object try_cache_fork(py::handle caches_, py::handle counts_, py::handle tables_, py::handle context_,
+                          py::handle parents_, py::handle children_) {
+    const at::Tensor* counts = ordinary(counts_);
+    const at::Tensor* tables = ordinary(tables_);
+    const at::Tensor* context = ordinary(context_);
+    const at::Tensor* parents = ordinary(parents_);
+    const at::Tensor* children = ordinary(children_);
+    if (!ordinary_context() ||
+        !ordinary_ints({{counts, 1}, {tables, 2}, {context, 1}, {parents, 1}, {children, 1}}) ||
+        tables->size(0) != context->size(0) || parents->size(0) != children->size(0)) {
+        return py::none();
+    }
+    const auto caches = ordinary_list(caches_);
+    if (!caches || (*caches)[0].device() != counts->device() || (*caches)[0].dim() < 2 ||
+        (*caches)[0].size(0) != counts->size(0)) {
+        return py::none();
+    }
+    at::Tensor status;
+    {
+        py::gil_scoped_release no_gil;
+        status = cache_fork_hip(*caches, *counts, *tables, *context, *parents, *children);
+    }
+    return wrap(status);
+}
+
+py::object try_cache_extend(py::handle counts_, py::handle tables_, py::handle context_, py::handle sequences_,
+                            py::handle block_, py::handle tokens_) {
+    const at::Tensor* counts = ordinary(counts_);
+    const at::Tensor* tables = ordinary(tables_);
+    const at::Tensor* context = ordinary(context_);
+    const at::Tensor* sequences = ordinary(sequences_);
+    const std::optional<int64_t> block = plain_int(block_);
+    const std::optional<int64_t> tokens = plain_int(tokens_);
+    if (!ordinary_context() || !ordinary_ints({{counts, 1}, {tables, 2}, {context, 1}, {sequences, 1}}) ||
+        tables->size(0) != context->size(0) || !block || !tokens || *block <= 0 || *tokens <= 0) {
+        return py::none();
+    }
+    at::Tensor slots;
+    {
+        py::gil_scoped_release no_gil;
+        slots = cache_extend_hip(*counts, *tables, *context, *sequences, *block, *tokens);
+    }
+    return wrap(slots);
+}
+
+/// True when the call was taken.
+bool try_cache_release(py::handle counts_, py::handle tables_, py::handle context_, py::handle sequences_,
+                       py::handle block_) {
+    const at::Tensor* counts = ordinary(counts_);
+    const at::Tensor* tables = ordinary(tables_);
+    const at::Tensor* context = ordinary(context_);
+    const at::Tensor* sequences = ordinary(sequences_);
+    const std::optional<int64_t> block = plain_int(block_);
+    if (!ordinary_context() || !ordinary_ints({{counts, 1}, {tables, 2}, {context, 1}, {sequences, 1}}) ||
+        tables->size(0) != context->size(0) || !block || *block <= 0) {
+        return false;
+    }
+    py::gil_scoped_release no_gil;
+    cache_release_hip(*counts, *tables, *context, *sequences, *block);
+    return true;
+}
+
+py::object try_cache_compact(py::handle caches_, py::handle counts_, py::handle tables_, py::handle context_) {
+    const at::Tensor* counts = ordinary(counts_);
+    const at::Tensor* tables = ordinary(tables_);
+    const at::Tensor* context = ordinary(context_);
+    if (!ordinary_context() || !ordinary_ints({{counts, 1}, {tables, 2}, {context, 1}}) ||
+        tables->size(0) != context->size(0)) {
+        return py::none();
+    }
+    const auto caches = ordinary_list(caches_);
+    if (!caches || (*caches)[0].device() != counts->device() || (*caches)[0].dim() < 2 ||
+        (*caches)[0].size(0) != counts->size(0)) {
+        return py::none();
+    }
+    std::tuple<at::Tensor, at::Tensor, at::Tensor> out;
+    {
+        py::gil_scoped_release no_gil;
+        out = cache_compact_hip(*caches, *counts, *tables, *context);
+    }
+    return py::make_tuple(wrap(std::get<0>(out)), wrap(std::get<1>(out)), wrap(std::get<2>(out)));
+}
+
 py::object try_paged_attention_shared(py::handle query_, py::handle k_, py::handle v_, py::handle starts_,
                                       py::handle prefix_, py::handle tables_, py::handle context_,
                                       py::handle scale_) {
@@ -307,6 +582,11 @@ py::object try_paged_attention_shared(py::handle query_, py::handle k_, py::hand
 }
 
 void bind_generation(py::module_& m) {
+    m.def("try_cache_copy", torch::wrap_pybind_function(&try_cache_copy));
+    m.def("try_cache_fork", torch::wrap_pybind_function(&try_cache_fork));
+    m.def("try_cache_extend", torch::wrap_pybind_function(&try_cache_extend));
+    m.def("try_cache_release", torch::wrap_pybind_function(&try_cache_release));
+    m.def("try_cache_compact", torch::wrap_pybind_function(&try_cache_compact));
     m.def("try_paged_attention_shared", torch::wrap_pybind_function(&try_paged_attention_shared));
     m.def("try_token_logprobs", torch::wrap_pybind_function(&try_token_logprobs));
 }
@@ -314,6 +594,19 @@ void bind_generation(py::module_& m) {
 }  // namespace cudaforge_amd
 
 TORCH_LIBRARY_FRAGMENT(cudaforge, m) {
+    m.def("cache_copy(Tensor(a!)[] caches, Tensor src, Tensor dst) -> Tensor");
+    m.def(
+        "cache_fork(Tensor(a!)[] caches, Tensor(b!) ref_counts, Tensor(c!) block_tables, Tensor(d!) context_lens, "
+        "Tensor parents, Tensor children) -> Tensor");
+    m.def(
+        "cache_extend(Tensor(a!) ref_counts, Tensor(b!) block_tables, Tensor(c!) context_lens, Tensor sequences, "
+        "int block_size, int tokens) -> Tensor");
+    m.def(
+        "cache_release(Tensor(a!) ref_counts, Tensor block_tables, Tensor(b!) context_lens, Tensor sequences, "
+        "int block_size) -> ()");
+    m.def(
+        "cache_compact(Tensor(a!)[] caches, Tensor ref_counts, Tensor block_tables, Tensor context_lens) "
+        "-> (Tensor, Tensor, Tensor)");
     m.def(
         "paged_attention_shared(Tensor query, Tensor k_cache, Tensor v_cache, Tensor group_starts, "
         "Tensor prefix_lens, Tensor block_tables, Tensor context_lens, float scale) -> Tensor");
@@ -333,6 +626,8 @@ TORCH_LIBRARY_IMPL(cudaforge, Autograd, m) {
     }
 }
 
+// The page operators' CPU implementations are the Python layer's
+// (paged_cache.py): plain loops over the tables.
 TORCH_LIBRARY_IMPL(cudaforge, CPU, m) {
     using namespace cudaforge_amd;
     m.impl("paged_attention_shared", &paged_attention_shared_cpu);
@@ -342,6 +637,11 @@ TORCH_LIBRARY_IMPL(cudaforge, CPU, m) {
 
 TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
     using namespace cudaforge_amd;
+    m.impl("cache_copy", &cache_copy_hip);
+    m.impl("cache_fork", &cache_fork_hip);
+    m.impl("cache_extend", &cache_extend_hip);
+    m.impl("cache_release", &cache_release_hip);
+    m.impl("cache_compact", &cache_compact_hip);
     m.impl("paged_attention_shared", &paged_attention_shared_hip);
     m.impl("token_logprobs", &token_logprobs_hip);
     m.impl("token_logprobs_backward", &token_logprobs_backward_hip);

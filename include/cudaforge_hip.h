@@ -524,6 +524,95 @@ cf_status cf_paged_attention(const void* query, const void* k_cache, const void*
                              int64_t max_blocks_per_sequence, float scale, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ---- pages of a paged KV cache ------------------------------------------- */
+
+/* The operators below work on a cache's state on the device:
+ *   ref_counts [num_pages] int32: table rows that name the page; <= 0: free;
+ *   block_tables [num_sequences, max_blocks_per_sequence] uint32 and
+ *   context_lens [num_sequences] int32, as cf_paged_attention reads them (a
+ *   sequence with a length <= 0 is empty; entries behind a length mean nothing);
+ *   caches: a host array of num_caches device pointers (K and V of every
+ *   layer), each num_pages pages of page_bytes bytes of any type; it is read
+ *   before the call returns. 16-byte aligned caches whose pages (fork: tokens)
+ *   are multiples of 16 bytes move fastest.
+ * Lists (sequences, pages) are int32 on the device too: nothing is read back by
+ * the host. An entry that cannot be served is left out and says so in its
+ * status; what it names is not touched. Free pages are handed out lowest first,
+ * in the order of the list. Results depend on the inputs alone. Calls on one
+ * state must not overlap. */
+
+/* Cache tensors per launch; more take further launches. */
+#define CF_CACHE_TENSORS_MAX 64
+
+/* Workspace bytes (16-byte aligned, in any state) that the operators below need
+ * for lists of `count` entries; num_sequences 0 for cf_cache_copy, count 0 for
+ * cf_cache_compact. It has no counterpart in the reference. */
+size_t cf_cache_workspace_bytes(int64_t num_pages, int64_t num_sequences, int64_t count);
+
+/* Copies page src[i] of every cache to page dst[i], i < count, all as they were
+ * before the call. status[i]: 0 copied; 1 left out: a page out of range, a dst
+ * that an earlier in-range entry names, or a src that any entry names as its
+ * dst (the order of such copies would matter). Needs
+ * cf_cache_workspace_bytes(num_pages, 0, count). It has no counterpart in the
+ * reference. */
+cf_status cf_cache_copy(void* const* caches, int64_t num_caches, int64_t page_bytes,
+                        int64_t num_pages, const int32_t* src, const int32_t* dst, int64_t count,
+                        int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Makes row children[i] continue from row parents[i]: it gets the parent's
+ * length; whole pages are shared (their counts go up), a partial last page is
+ * copied to a free one (its used tokens only), so both rows may grow.
+ * status[i]: 0 done; 1 left out: a row out of range, an empty parent or one
+ * whose length passes the table, a child that is not empty or that an earlier
+ * such entry names; 2: no page was free for it (nor for any later entry that
+ * needs one). A page entry out of range is copied as it stands and counted
+ * nowhere. Needs cf_cache_workspace_bytes(num_pages, num_sequences, count). It
+ * has no counterpart in the reference. */
+cf_status cf_cache_fork(void* const* caches, int64_t num_caches, int64_t page_bytes,
+                        int32_t* ref_counts, uint32_t* block_tables, int32_t* context_lens,
+                        int64_t num_pages, int64_t block_size, int64_t num_sequences,
+                        int64_t max_blocks_per_sequence, const int32_t* parents,
+                        const int32_t* children, int64_t count, int32_t* status, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Makes row sequences[i] `tokens` longer (>= 1; an empty row starts anew) and
+ * takes the pages that this needs. slots [count, tokens] int64: where the new
+ * tokens go, page * block_size + offset; all -1 for an entry left out: a row out
+ * of range, named by an earlier entry, or whose table would overflow, or for
+ * which not all pages were free (nor then for any later entry that needs one).
+ * Slots in a last page that the table names wrongly are -1 alone. Needs
+ * cf_cache_workspace_bytes(num_pages, num_sequences, count). It has no
+ * counterpart in the reference. */
+cf_status cf_cache_extend(int32_t* ref_counts, uint32_t* block_tables, int32_t* context_lens,
+                          int64_t num_pages, int64_t block_size, int64_t num_sequences,
+                          int64_t max_blocks_per_sequence, const int32_t* sequences, int64_t count,
+                          int64_t tokens, int64_t* slots, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* Empties row sequences[i]: its length becomes 0, the counts of its pages go
+ * down by one each (not below 0). Rows out of range are left out, a row named
+ * twice is released once; table entries stay as they are. No workspace. It has
+ * no counterpart in the reference. */
+cf_status cf_cache_release(int32_t* ref_counts, uint32_t* block_tables, int32_t* context_lens,
+                           int64_t num_pages, int64_t block_size, int64_t num_sequences,
+                           int64_t max_blocks_per_sequence, const int32_t* sequences, int64_t count,
+                           void* stream);
+
+/* Moves live pages (count > 0) to the front: with L of them, live page number
+ * j at or past L goes to free page number j below L (both in ascending order).
+ * new_ref_counts and new_block_tables describe the cache afterwards (each may
+ * be the old array itself), *live_pages = L: pages L and up may be given up.
+ * Moved pages' old copies stay until their pages are used again, so the old
+ * tables remain readable till then. Needs
+ * cf_cache_workspace_bytes(num_pages, num_sequences, 0). It has no counterpart
+ * in the reference. */
+cf_status cf_cache_compact(void* const* caches, int64_t num_caches, int64_t page_bytes,
+                           const int32_t* ref_counts, const uint32_t* block_tables,
+                           const int32_t* context_lens, int64_t num_pages, int64_t block_size,
+                           int64_t num_sequences, int64_t max_blocks_per_sequence,
+                           int32_t* new_ref_counts, uint32_t* new_block_tables, int32_t* live_pages,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- paged attention behind shared prompts ------------------------------- */
 
 /* Workspace bytes cf_paged_attention_shared needs: the pieces of split
