@@ -58,15 +58,17 @@ struct SharedArgs {
     const int32_t* context;
     void* out;
     float* ml;   // [slots][sequences * heads][2]: maximum (base 2), sum
-    float* acc;  // [slots][sequences * heads][head_dim]
+    float* acc;  // [slots][sequences * heads][pitch]
     uint32_t pages;
     uint32_t block_size;
-    int block_shift;  // log2(block_size), or -1
+    int block_shift;      // log2(block_size), or -1
+    uint32_t page_bytes;  // 0: 2^32 or more
     int sequences;
     int heads;
     int kv_heads;
     int per;          // query heads per KV head
     int head_dim;
+    int pitch;        // head_dim rounded up to 4
     int groups;
     int max_blocks;
     int capacity;     // tokens a table row reaches
@@ -75,7 +77,8 @@ struct SharedArgs {
     int prefix_tiles;  // row tiles over all groups, at most
     int rest_tiles;    // row tiles per sequence and KV head
     int prefix_items;  // workgroups of the first kind
-    float c;           // scale * log2(e)
+    float c;           // |scale| log2(e), above 0
+    uint32_t query_sign;  // flips the query's signs for a negative scale
 };
 
 // ---- groups, ranges -----------------------------------------------------------
@@ -99,50 +102,58 @@ __device__ __forceinline__ int wave_max_int(int v) {
 __device__ Group group_of(const SharedArgs& a, int s) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     int first = 0;
-    for (int base = 0; base <= a.groups; base += kWaveSize) {
+    for (int base = 0; base <= a.groups; base += kWaveSize - 1) {  // one start is looked at twice
         const int g = base + lane;
-        const int start = g <= a.groups ? clamp_to(a.starts[g], a.sequences) : 0;
-        const uint64_t above = __builtin_amdgcn_ballot_w64(g <= a.groups && start > s);
+        const bool there = g <= a.groups;
+        const int start = there ? clamp_to(a.starts[g], a.sequences) : 0;
+        const int prefix = g < a.groups ? clamp_to(a.prefix[g], a.capacity) : 0;
+        const uint64_t above = __builtin_amdgcn_ballot_w64(there && start > s);
         if (above != 0) {
-            const int at = __builtin_ctzll(above);
-            const int g_end = base + at;  // the first start past s
+            const int at = __builtin_ctzll(above);  // the first start past s ends the group
+            if (base + at == 0) return Group{0, 0, 0};
             first = max(first, wave_max_int(lane < at ? start : 0));
-            if (g_end == 0) return Group{0, 0, 0};
-            return Group{first, __builtin_amdgcn_readlane(start, at), clamp_to(a.prefix[g_end - 1], a.capacity)};
+            return Group{first, __builtin_amdgcn_readlane(start, at), __builtin_amdgcn_readlane(prefix, at - 1)};
         }
         first = max(first, wave_max_int(start));
     }
     return Group{0, 0, 0};
 }
 
-/// The group of row tile `tile` (uniform) of kRows rows; `tile` becomes the
+/// The group of row tile `tile` (uniform) of `rows` rows; `tile` becomes the
 /// tile within the group. end = 0: no such tile.
 __device__ Group group_of_tile(const SharedArgs& a, int rows, int& tile) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     int before = 0;  // largest start so far
     for (int base = 0; base < a.groups; base += kWaveSize) {
         const int g = base + lane;
-        int start = g < a.groups ? clamp_to(a.starts[g], a.sequences) : 0;
+        const bool there = g < a.groups;
+        int start = there ? clamp_to(a.starts[g], a.sequences) : 0;
+        int end = there ? clamp_to(a.starts[g + 1], a.sequences) : 0;
+        const int prefix = there ? clamp_to(a.prefix[g], a.capacity) : 0;
         if (lane == 0) start = max(start, before);
+        if (a.groups > 1) {
 #pragma unroll
-        for (int d = 1; d < kWaveSize; d <<= 1) {
-            const int o = __shfl_up(start, d);
-            if (lane >= d) start = max(start, o);
+            for (int d = 1; d < kWaveSize; d <<= 1) {
+                const int o = __shfl_up(start, d);
+                if (lane >= d) start = max(start, o);
+            }
         }
-        const int end = g < a.groups ? max(start, clamp_to(a.starts[g + 1], a.sequences)) : start;
-        int tiles = ((end - start) * a.per + rows - 1) / rows;
+        end = there ? max(start, end) : start;
+        const int tiles = ((end - start) * a.per + rows - 1) / rows;
         int total = tiles;
+        if (a.groups > 1) {
 #pragma unroll
-        for (int d = 1; d < kWaveSize; d <<= 1) {
-            const int o = __shfl_up(total, d);
-            if (lane >= d) total += o;
+            for (int d = 1; d < kWaveSize; d <<= 1) {
+                const int o = __shfl_up(total, d);
+                if (lane >= d) total += o;
+            }
         }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(total > tile);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(there && total > tile);
         if (past != 0) {
             const int at = __builtin_ctzll(past);
             tile -= __builtin_amdgcn_readlane(total - tiles, at);
             return Group{__builtin_amdgcn_readlane(start, at), __builtin_amdgcn_readlane(end, at),
-                         clamp_to(a.prefix[base + at], a.capacity)};
+                         __builtin_amdgcn_readlane(prefix, at)};
         }
         tile -= __builtin_amdgcn_readlane(total, kWaveSize - 1);
         before = __builtin_amdgcn_readlane(start, kWaveSize - 1);
@@ -183,6 +194,14 @@ __device__ __forceinline__ void copy16_to_lds(const void* from, uint32_t dst) {
                  : "memory");
 }
 
+/// The same from a base that all lanes share, and each lane's offset from it.
+__device__ __forceinline__ void copy16_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(dst))
+                 : "memory");
+}
+
 /// Waits until at most n vector-memory operations of the wave are in flight.
 template <int n>
 __device__ __forceinline__ void wait_vm() {
@@ -196,6 +215,18 @@ __device__ __forceinline__ void wait_lds() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xF | (7 << 4) | (0 << 8) | (3 << 14));
     asm volatile("" ::: "memory");
+}
+
+/// The larger of each lane's value and that of the lanes with the same place
+/// in the other groups of kGroup (32 or 16) lanes, exchanged in registers.
+template <int kGroup>
+__device__ __forceinline__ float groups_max(float v) {
+    if constexpr (kGroup == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 /// What depends on the cache's type: rows and tokens of a tile, fragments,
@@ -237,11 +268,8 @@ struct Tile {
     __device__ __forceinline__ static int query_dim(int u, int lane) {
         return 16 * u + kPerVec * part_of(lane);
     }
-    /// Token (in the tile) of a lane's score i.
-    __device__ __forceinline__ static int token_of(int i, int lane) {
-        if constexpr (kWide) return 4 * part_of(lane) + i;
-        return 8 * (i >> 2) + 4 * part_of(lane) + (i & 3);
-    }
+    /// A lane's score i is token 4 part + token_of(i) of the tile.
+    __device__ __forceinline__ static constexpr int token_of(int i) { return kWide ? i : 8 * (i >> 2) + (i & 3); }
     /// Dim of a lane's output value i: four neighbours from each i % 4 == 0.
     __device__ __forceinline__ static int dim_of(int i, int lane) {
         if constexpr (kWide) return 16 * (i >> 2) + 4 * part_of(lane) + (i & 3);
@@ -356,6 +384,7 @@ struct Item {
     int sequences;   // rows are (sequence, head of the KV head)
     int first_row;
     int least;       // sequences with fewer tokens do not take part
+    int last_block;  // of the range
     int slot;
 };
 
@@ -383,7 +412,7 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         for (int u = 0; u < L::kQueries; ++u) {
             const int dim = L::query_dim(u, lane);
             u32x4_t raw = {0u, 0u, 0u, 0u};
-            if (inside && dim < a.head_dim) raw = *reinterpret_cast<const u32x4_t*>(from + dim);
+            if (inside && dim < a.head_dim) raw = *reinterpret_cast<const u32x4_t*>(from + dim) ^ a.query_sign;
             q[u] = __builtin_bit_cast(typename L::Query, raw);
         }
     }
@@ -395,63 +424,68 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
     }
 
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    const int64_t token_bytes = static_cast<int64_t>(a.kv_heads) * a.head_dim * sizeof(T);
-    const int64_t head_bytes = static_cast<int64_t>(w.kv_head) * a.head_dim * sizeof(T);
+    const uint32_t token_bytes = static_cast<uint32_t>(a.kv_heads) * a.head_dim * sizeof(T);
+    const uint32_t head_bytes = static_cast<uint32_t>(w.kv_head) * a.head_dim * sizeof(T);
+    const uint8_t* k_head = static_cast<const uint8_t*>(a.k_cache) + head_bytes;
+    const uint8_t* v_head = static_cast<const uint8_t*>(a.v_cache) + head_bytes;
     const int row_pieces = a.head_dim * static_cast<int>(sizeof(T)) / 16;
+    // Tiles begin at multiples of kTokens; tokens before lo are masked.
+    const int begin = w.lo / L::kTokens * L::kTokens;
+    const int tiles = (w.hi - begin + L::kTokens - 1) / L::kTokens;
 
-    // 64 entries of the block table in lane registers: a token's page is a lane
-    // shuffle, not a load that would have to wait behind the copies.
-    int window_base = 0;
-    uint32_t window = 0;
-    bool loaded = false;
-    auto block_of = [&](int t) {
-        const uint32_t ut = static_cast<uint32_t>(t);
-        return static_cast<int>(a.block_shift >= 0 ? ut >> a.block_shift : ut / a.block_size);
-    };
-    // Where this wave's copies of the tile at token `first` read: the cache row
-    // of each copy's token (0 for one that is not there), and which of the
-    // tile's tokens are there.
+    // A copy takes kPerCopy neighbouring tokens; kSpan tokens of this wave's
+    // share of a tile lie in one page (blocks of a power of two from 16 on).
     constexpr int kCopies = L::kCopies / kRowWaves;
     static_assert(L::kCopies % kRowWaves == 0, "copies per wave");
+    constexpr int kPerCopy = kWaveSize / L::kChunks;
+    static_assert(kPerCopy >= 1, "a row within a copy");
+    constexpr int kSpan = kCopies * kPerCopy < 16 ? kCopies * kPerCopy : 16;
+    constexpr int kSpanCopies = kSpan / kPerCopy;
     const int first_copy = row_wave * kCopies;
-    struct Rows {
-        uint32_t row[kCopies];
-        uint64_t valid;
-    };
-    auto look_up = [&](int first) {
-        const int begin = block_of(first);
-        const int end = block_of(first + L::kTokens - 1);  // at most kTokens - 1 further
-        if (!loaded || end >= window_base + kWaveSize) {   // tiles are taken in ascending order
-            window_base = begin;
-            window = w.table[min(begin + lane, a.max_blocks - 1)];
-            loaded = true;
+
+    // 64 entries of the block table in lane registers: a token's page is a lane
+    // read, not a load that would have to wait behind the copies. `sound`: all
+    // entries of the range name pages.
+    int window_base = static_cast<int>(static_cast<uint32_t>(begin) / a.block_size);
+    auto load_window = [&]() { return w.table[min(window_base + lane, w.last_block)]; };
+    uint32_t window = load_window();
+    bool sound = __builtin_amdgcn_ballot_w64(window >= a.pages) == 0;
+    for (int b = window_base + kWaveSize; b <= w.last_block && sound; b += kWaveSize) {
+        sound = __builtin_amdgcn_ballot_w64(w.table[min(b + lane, w.last_block)] >= a.pages) == 0;
+    }
+    const bool fast = sound && a.block_shift >= 4 && a.page_bytes != 0;
+    // Byte offset in the cache of token t, rounded to its span; tokens behind
+    // the range's last page take that page.
+    auto place_of = [&](int t) {
+        const int block = min(t >> a.block_shift, w.last_block);
+        if (block >= window_base + kWaveSize) {  // tiles are taken in ascending order
+            window_base = block;
+            window = load_window();
         }
-        const int t = first + (lane & (L::kTokens - 1));
-        const int block = block_of(t);
-        const uint32_t at = static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size;
-        const uint32_t page = static_cast<uint32_t>(__shfl(static_cast<int>(window), block - window_base));
-        const bool there = t < w.hi && page < a.pages;
-        const uint32_t row = there ? page * a.block_size + at : 0u;
-        Rows r;
-        r.valid = __builtin_amdgcn_ballot_w64(there) & ((uint64_t{1} << L::kTokens) - 1);
+        const uint32_t page = __builtin_amdgcn_readlane(window, block - window_base);
+        return static_cast<uint64_t>(page) * a.page_bytes +
+               (static_cast<uint32_t>(t) & (a.block_size - 1)) * token_bytes;
+    };
+    // This wave's copies of K (0) or V (1) of the tile at token `first` to LDS.
+    auto fetch = [&](int first, uint32_t dst, auto which) {
+        constexpr bool is_k = decltype(which)::value == 0;
 #pragma unroll
-        for (int n = 0; n < kCopies; ++n) {
-            r.row[n] = static_cast<uint32_t>(
-                __shfl(static_cast<int>(row), ((first_copy + n) * kWaveSize + lane) / L::kChunks));
-        }
-        return r;
-    };
-    // This wave's copies of a K or V tile to LDS.
-    auto fetch = [&](const void* cache, const Rows& rows, uint32_t dst, bool is_k) {
+        for (int n0 = 0; n0 < kCopies; n0 += kSpanCopies) {
+            const uint8_t* base = (is_k ? k_head : v_head) + place_of(first + (first_copy + n0) * kPerCopy);
 #pragma unroll
-        for (int n = 0; n < kCopies; ++n) {
-            const int piece_index = (first_copy + n) * kWaveSize + lane;
-            const int r = piece_index / L::kChunks;
-            const int piece = (piece_index % L::kChunks) ^ (is_k ? L::k_swizzle(r) : L::v_swizzle(r));
-            const uint8_t* from = static_cast<const uint8_t*>(cache) + rows.row[n] * token_bytes + head_bytes + piece * 16;
-            if (piece < row_pieces) copy16_to_lds(from, dst + static_cast<uint32_t>(first_copy + n) * 16 * kWaveSize);
+            for (int n = n0; n < n0 + kSpanCopies; ++n) {
+                const int r = (first_copy + n) * kPerCopy + lane / L::kChunks;
+                const int piece = (lane % L::kChunks) ^ (is_k ? L::k_swizzle(r) : L::v_swizzle(r));
+                const uint32_t offset = static_cast<uint32_t>((n - n0) * kPerCopy + lane / L::kChunks) * token_bytes +
+                                        static_cast<uint32_t>(piece) * 16;
+                if (piece < row_pieces) {
+                    copy16_to_lds(base, offset, dst + static_cast<uint32_t>(first_copy + n) * 16 * kWaveSize);
+                }
+            }
         }
     };
+    using K = std::integral_constant<int, 0>;
+    using V = std::integral_constant<int, 1>;
 
     float m = -INFINITY;  // the row's running maximum
     float l = 0.0f;       // this lane's share of the running sum
@@ -462,22 +496,38 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         for (int i = 0; i < L::kScores; ++i) acc[b][i] = 0.0f;
     }
 
-    constexpr uint64_t kAll = (uint64_t{1} << L::kTokens) - 1;
-    // Scores to probabilities, and the running values.
-    auto soften = [&](typename L::Score& s, uint64_t valid) {
-        float top = -INFINITY;
+    // The tokens of the tile at `first` that lie in the range, a bit each.
+    constexpr uint32_t kAll = 0xFFFFFFFFu >> (32 - L::kTokens);
+    auto in_range = [&](int first) {
+        const int ahead = w.lo - first;
+        const int count = w.hi - first;
+        return (ahead > 0 ? kAll << ahead : kAll) & (count < L::kTokens ? (1u << count) - 1u : kAll);
+    };
+    auto mask = [&](typename L::Score& s, uint32_t valid) {
+        const uint32_t mine = valid >> (4 * L::part_of(lane));
 #pragma unroll
-        for (int i = 0; i < L::kScores; ++i) {
-            s[i] *= a.c;
-            if (valid != kAll) s[i] = (valid >> L::token_of(i, lane)) & 1 ? s[i] : -INFINITY;
-            top = fmaxf(top, s[i]);
+        for (int i = 0; i < L::kScores; ++i) s[i] = (mine & (1u << L::token_of(i))) != 0 ? s[i] : -INFINITY;
+    };
+    // Clear the V rows of tokens that are not there.
+    auto clear = [&](uint8_t* v, uint32_t valid, int start, int step) {
+        for (int i = start; i < L::kTokens * L::kChunks; i += step) {
+            if (((valid >> (i / L::kChunks)) & 1) == 0) {
+                reinterpret_cast<u32x4_t*>(v)[i] = u32x4_t{0u, 0u, 0u, 0u};
+            }
         }
+    };
+    // Scores to probabilities, and the running values. m may lag the true
+    // maximum by up to kLag (base 2): sums and outputs are rescaled only when it
+    // would lag more (fp32 holds the factor, and so does fp16: 2^8 at most).
+    constexpr float kLag = 8.0f;
+    auto soften = [&](typename L::Score& s) {
+        float top = s[0];
 #pragma unroll
-        for (int d = L::kRows; d < kWaveSize; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        const float m_new = fmaxf(m, top);
-        const float shift = m_new == -INFINITY ? 0.0f : m_new;
-        if (__builtin_amdgcn_ballot_w64(m_new > m) != 0) {
-            const float f = exp2f(m - shift);
+        for (int i = 1; i < L::kScores; ++i) top = fmaxf(top, s[i]);
+        top = groups_max<L::kRows>(top);
+        const float m_new = fmaxf(m, top * a.c);
+        if (__builtin_amdgcn_ballot_w64(m_new > m + kLag) != 0) {
+            const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
             l *= f;
 #pragma unroll
             for (int b = 0; b < L::kAcc / L::kScores; ++b) {
@@ -486,71 +536,98 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             }
             m = m_new;
         }
+        const float shift = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int i = 0; i < L::kScores; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - shift);
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -shift));
             l += s[i];
         }
     };
-    // Clear the V rows of tokens that are not there (waves' lanes in turn).
-    auto clear = [&](uint8_t* v, uint64_t valid, int start, int step) {
-        for (int i = start; i < L::kTokens * L::kChunks; i += step) {
-            if (((valid >> (i / L::kChunks)) & 1) == 0) {
-                reinterpret_cast<u32x4_t*>(v)[i] = u32x4_t{0u, 0u, 0u, 0u};
-            }
-        }
-    };
+    auto edge = [&](int first) { return first < w.lo || first + L::kTokens > w.hi; };
 
-    if constexpr (kRowWaves == 1) {
+    if (!fast) {
+        // Any block size, and tables with entries that name no page: every token
+        // looked up by itself, a tile at a time.
+        uint8_t* k = lds + (kRowWaves == 1 ? wave * 2 * L::kBytes : 0);
+        uint8_t* v = k + L::kBytes;
+        const uint32_t k_dst = lds_base + (kRowWaves == 1 ? static_cast<uint32_t>(wave) * 2 * L::kBytes : 0u);
+        for (int i = token_wave; i < tiles; i += kTokenWaves) {
+            const int t = begin + i * L::kTokens + (lane & (L::kTokens - 1));
+            const uint32_t block = static_cast<uint32_t>(t) / a.block_size;
+            const bool inside = t >= w.lo && t < w.hi;
+            const uint32_t page = inside ? w.table[block] : a.pages;
+            const uint32_t cache_row = page < a.pages ? page * a.block_size + static_cast<uint32_t>(t) - block * a.block_size : 0u;
+            const uint32_t valid = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(page < a.pages)) & kAll;
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) {
+                const int r = (first_copy + n) * kPerCopy + lane / L::kChunks;
+                const uint64_t from = static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(cache_row), r))) * token_bytes;
+                const uint32_t dst = k_dst + static_cast<uint32_t>(first_copy + n) * 16 * kWaveSize;
+                const int k_piece = (lane % L::kChunks) ^ L::k_swizzle(r);
+                const int v_piece = (lane % L::kChunks) ^ L::v_swizzle(r);
+                if (k_piece < row_pieces) copy16_to_lds(k_head + from + k_piece * 16, dst);
+                if (v_piece < row_pieces) copy16_to_lds(v_head + from + v_piece * 16, dst + L::kBytes);
+            }
+            wait_vm<0>();
+            if constexpr (kRowWaves > 1) __syncthreads();
+            typename L::Score s = L::scores(k, q, lane);
+            if (valid != kAll) mask(s, valid);
+            soften(s);
+            if (valid != kAll) {
+                clear(v, valid, kRowWaves == 1 ? lane : tid, kRowWaves == 1 ? kWaveSize : kThreads);
+                wait_lds();
+                if constexpr (kRowWaves > 1) __syncthreads();
+            }
+            L::values(v, s, acc, lane);
+            wait_lds();
+            if constexpr (kRowWaves > 1) __syncthreads();
+        }
+    } else if constexpr (kRowWaves == 1) {
         // The wave's own K and V tile, one copied while the other is used.
         uint8_t* k = lds + wave * 2 * L::kBytes;
         uint8_t* v = k + L::kBytes;
         const uint32_t k_dst = lds_base + static_cast<uint32_t>(wave) * 2 * L::kBytes;
         const uint32_t v_dst = k_dst + L::kBytes;
-        int t = w.lo + token_wave * L::kTokens;
+        int t = begin + token_wave * L::kTokens;
         constexpr int kStep = kTokenWaves * L::kTokens;
         if (t < w.hi) {
-            Rows rows = look_up(t);
-            fetch(a.k_cache, rows, k_dst, true);
-            fetch(a.v_cache, rows, v_dst, false);
-            for (; t < w.hi; t += kStep) {
-                const bool more = t + kStep < w.hi;
-                const uint64_t now = rows.valid;
-                // K has landed: only V's copies may be in flight. (Copies that
-                // no lane takes part in are not issued, so a head narrower than
-                // kD waits for all.)
-                if (a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
-                typename L::Score s = L::scores(k, q, lane);
+            fetch(t, k_dst, K{});
+            fetch(t, v_dst, V{});
+        }
+        for (; t < w.hi; t += kStep) {
+            const bool more = t + kStep < w.hi;
+            // K has landed: only V's copies may be in flight. (Copies that no
+            // lane takes part in are not issued, so a head narrower than kD
+            // waits for all.)
+            if (a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
+            typename L::Score s = L::scores(k, q, lane);
+            wait_lds();
+            if (more) fetch(t + kStep, k_dst, K{});
+            const bool partial = edge(t);
+            if (partial) mask(s, in_range(t));
+            soften(s);
+            if (more && a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
+            if (partial) {
+                clear(v, in_range(t), lane, kWaveSize);
                 wait_lds();
-                if (more) {
-                    rows = look_up(t + kStep);
-                    fetch(a.k_cache, rows, k_dst, true);
-                }
-                soften(s, now);
-                if (more && a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
-                if (now != kAll) {
-                    clear(v, now, lane, kWaveSize);
-                    wait_lds();
-                }
-                L::values(v, s, acc, lane);
-                wait_lds();
-                if (more) fetch(a.v_cache, rows, v_dst, false);
             }
+            L::values(v, s, acc, lane);
+            wait_lds();
+            if (more) fetch(t + kStep, v_dst, V{});
         }
     } else {
         // A ring of tiles; every wave copies a quarter of each.
-        const int tiles = (w.hi - w.lo + L::kTokens - 1) / L::kTokens;
-        auto issue = [&](int tile) {
-            const Rows rows = look_up(w.lo + tile * L::kTokens);
-            const uint32_t dst = lds_base + static_cast<uint32_t>(tile % kStages) * 2 * L::kBytes;
-            fetch(a.k_cache, rows, dst, true);
-            fetch(a.v_cache, rows, dst + L::kBytes, false);
-            return rows.valid;
+        auto issue = [&](int tile, uint32_t stage) {
+            const uint32_t dst = lds_base + stage * 2 * L::kBytes;
+            fetch(begin + tile * L::kTokens, dst, K{});
+            fetch(begin + tile * L::kTokens, dst + L::kBytes, V{});
         };
-        uint64_t valid[kStages];  // of tiles i .. i + kStages - 1
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) valid[i] = i < tiles ? issue(i) : 0;
-        for (int i = 0; i < tiles; ++i) {
+        for (int i = 0; i < kStages - 1; ++i) {
+            if (i < tiles) issue(i, i);
+        }
+        auto step = [&](auto stage, int i) {
+            constexpr int kAt = decltype(stage)::value;
             // This wave's copies of tile i have landed; behind it two tiles
             // (fewer at the end) are in flight.
             if (i + kStages - 2 < tiles && a.head_dim == kD) {
@@ -558,22 +635,27 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             } else {
                 wait_vm<0>();
             }
-            bare_barrier();
-            // Into tile i - 1's place, which every wave is past.
-            valid[kStages - 1] = i + kStages - 1 < tiles ? issue(i + kStages - 1) : 0;
-            uint8_t* k = lds + (i % kStages) * 2 * L::kBytes;
-            uint8_t* v = k + L::kBytes;
-            const uint64_t now = valid[0];
-            typename L::Score s = L::scores(k, q, lane);
-            soften(s, now);
-            if (now != kAll) {
-                clear(v, now, tid, kThreads);
+            bare_barrier();  // and every wave is past tile i - 1, whose place is filled next
+            if (i + kStages - 1 < tiles) issue(i + kStages - 1, (kAt + kStages - 1) % kStages);
+            typename L::Score s = L::scores(lds + kAt * 2 * L::kBytes, q, lane);
+            const int first = begin + i * L::kTokens;
+            uint8_t* v = lds + kAt * 2 * L::kBytes + L::kBytes;
+            const bool partial = edge(first);
+            if (partial) mask(s, in_range(first));
+            soften(s);
+            if (partial) {
+                clear(v, in_range(first), tid, kThreads);
                 __syncthreads();
             }
             L::values(v, s, acc, lane);
             wait_lds();  // before the barrier that lets the tile be overwritten
-#pragma unroll
-            for (int j = 0; j + 1 < kStages; ++j) valid[j] = valid[j + 1];
+        };
+        static_assert(kStages == 4, "steps written out below");
+        for (int i = 0; i < tiles; i += kStages) {
+            step(std::integral_constant<int, 0>{}, i);
+            if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
+            if (i + 2 < tiles) step(std::integral_constant<int, 2>{}, i + 2);
+            if (i + 3 < tiles) step(std::integral_constant<int, 3>{}, i + 3);
         }
     }
 
@@ -628,7 +710,7 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             a.ml[2 * at] = mm;
             a.ml[2 * at + 1] = ll;
         }
-        float* to = a.acc + at * a.head_dim + dim;
+        float* to = a.acc + at * a.pitch + dim;
         *reinterpret_cast<f32x4_t*>(to) = sum;
     }
 }
@@ -638,7 +720,7 @@ template <typename T, int kD, int kRowWaves>
 constexpr int range_step() { return kWaves / kRowWaves * Tile<T, kD>::kTokens; }
 
 template <typename T, int kD, int kRowWaves>
-__global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void shared_attention_kernel(SharedArgs a) {
     using L = Tile<T, kD>;
     __shared__ __attribute__((aligned(16))) uint8_t lds[lds_bytes<T, kD>()];
     __shared__ float lds_m[kWaves][32];
@@ -673,6 +755,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedArgs a
         }
         if (holder < 0) return;
         w.table = a.tables + static_cast<int64_t>(holder) * a.max_blocks;
+        w.last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
         w.first_sequence = g.first;
         w.sequences = g.end - g.first;
         w.first_row = tile * kRows;
@@ -695,6 +778,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedArgs a
         w.hi = min(context, w.lo + each);
         if (w.lo >= w.hi) return;
         w.table = a.tables + static_cast<int64_t>(s) * a.max_blocks;
+        w.last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
         w.first_sequence = s;
         w.sequences = 1;
         w.first_row = tile * L::kRows;
@@ -744,7 +828,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedAr
             const int d = lane + i * kWaveSize;
             if (d < a.head_dim) dot = fmaf(qv[i], Storage<T>::load(k + d), dot);
         }
-        const float y = wave_reduce_f32<AddF32>(dot) * a.c;
+        const float y = wave_reduce_f32<AddF32>(dot) * (a.query_sign != 0 ? -a.c : a.c);
         const float m_new = fmaxf(m, y);
         const float shift = m_new == -INFINITY ? 0.0f : m_new;
         const float f = exp2f(m - shift);
@@ -765,21 +849,20 @@ __global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedAr
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int d = lane + i * kWaveSize;
-        if (d < a.head_dim) a.acc[slot_row * a.head_dim + d] = acc[i];
+        if (d < a.head_dim) a.acc[slot_row * a.pitch + d] = acc[i];
     }
 }
 
-/// Joins the pieces of one (sequence, head): a wave each. prefix_step and
+/// Joins the pieces of one (sequence, head), a workgroup each. prefix_step and
 /// rest_step are the first kernel's range steps (prefix_step 0: nothing was
 /// shared).
-template <typename T>
+template <typename T, int kD>
 __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedArgs a, int prefix_step,
                                                                          int rest_step) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     const int64_t rows = static_cast<int64_t>(a.sequences) * a.heads;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWaveSize;
-    if (row >= rows) return;
-    const int s = __builtin_amdgcn_readfirstlane(static_cast<int>(row / a.heads));
+    const int64_t row = blockIdx.x;
+    const int s = static_cast<int>(blockIdx.x) / a.heads;
     const int context = context_of(a, s);
     int first = 0;
     int prefix_pieces = 0;
@@ -798,7 +881,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
     }
     const int pieces = prefix_pieces + rest_pieces;
     auto slot_of = [&](int i) { return i < prefix_pieces ? i : a.prefix_splits + i - prefix_pieces; };
-    // Lane i weighs piece i (at most 2 x 64 pieces).
+    // Every wave weighs all pieces: lane i piece i (at most 2 x 64).
     static_assert(kMaxSplits <= kWaveSize, "two pieces per lane");
     float pm[2], pl[2];
 #pragma unroll
@@ -812,6 +895,24 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
             pl[n] = a.ml[2 * at + 1];
         }
     }
+    // Threads: groups of kLanes lanes take the pieces in turn, four dims a lane.
+    constexpr int kLanes = kD / 4;
+    constexpr int kTeams = kThreads / kLanes;
+    constexpr int kAhead = 4;
+    const int team = static_cast<int>(threadIdx.x) / kLanes;
+    const int dim = (static_cast<int>(threadIdx.x) % kLanes) * 4;
+    f32x4_t part[kAhead];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const int i = i0 + n * kTeams + team;
+            part[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (i < pieces && dim < a.head_dim) {
+                part[n] = *reinterpret_cast<const f32x4_t*>(a.acc + (slot_of(i) * rows + row) * a.pitch + dim);
+            }
+        }
+    };
+    load(0);  // in flight while the weights are found
     const float m = wave_reduce_f32<MaxF32>(fmaxf(pm[0], pm[1]));
     float weight[2];
     float sum = 0.0f;
@@ -821,16 +922,31 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
         sum += pm[n] == -INFINITY ? pl[n] : pl[n] * weight[n];
     }
     const float l = wave_reduce_f32<AddF32>(sum);
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = 0; i0 < pieces; i0 += kAhead * kTeams) {
+        if (i0 > 0) load(i0);
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const int i = i0 + n * kTeams + team;
+            const float low = __shfl(weight[0], i & (kWaveSize - 1));
+            const float high = __shfl(weight[1], i & (kWaveSize - 1));
+            const float f = i < kWaveSize ? low : high;
+            if (i < pieces) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(part[n][e], f, o[e]);
+            }
+        }
+    }
+    __shared__ __attribute__((aligned(16))) float teams[kTeams][kD];
+    *reinterpret_cast<f32x4_t*>(&teams[team][dim]) = o;
+    __syncthreads();
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = static_cast<T*>(a.out) + row * a.head_dim;
-    for (int d0 = 0; d0 < a.head_dim; d0 += kWaveSize) {
-        const int d = d0 + lane;
-        float o = 0.0f;
-        for (int i = 0; i < pieces; ++i) {
-            const float f = __shfl(i < kWaveSize ? weight[0] : weight[1], i & (kWaveSize - 1));
-            if (d < a.head_dim) o = fmaf(a.acc[(slot_of(i) * rows + row) * a.head_dim + d], f, o);
-        }
-        if (d < a.head_dim) Storage<T>::store(out + d, l == 0.0f ? 0.0f : o * inverse);
+    for (int d = static_cast<int>(threadIdx.x); d < a.head_dim; d += kThreads) {
+        float v = teams[0][d];
+#pragma unroll
+        for (int t = 1; t < kTeams; ++t) v += teams[t][d];
+        Storage<T>::store(out + d, l == 0.0f ? 0.0f : v * inverse);
     }
 }
 
@@ -888,7 +1004,7 @@ int64_t capacity_of(int64_t max_blocks, int64_t block_size) {
 size_t workspace_of(const Plan& p, int64_t sequences, int64_t heads, int64_t head_dim) {
     const size_t slots = static_cast<size_t>(p.prefix_splits) + p.rest_splits;
     const size_t rows = static_cast<size_t>(sequences) * heads;
-    return (slots * rows * 8 + 15) / 16 * 16 + slots * rows * head_dim * 4;
+    return (slots * rows * 8 + 15) / 16 * 16 + slots * rows * ((head_dim + 3) / 4 * 4) * 4;
 }
 
 bool sizes_ok(int64_t sequences, int64_t groups, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -932,8 +1048,11 @@ void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
             run_matrix<T, 256>(a, p, grid, stream);
         }
     }
-    launch(shared_attention_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div<int64_t>(rows, kWaves))),
-           dim3(kThreads), 0, stream, a, prefix_step, rest_step);
+    auto* join = a.head_dim <= 64    ? shared_attention_join_kernel<T, 64>
+                 : a.head_dim <= 128 ? shared_attention_join_kernel<T, 128>
+                 : a.head_dim <= 256 ? shared_attention_join_kernel<T, 256>
+                                     : shared_attention_join_kernel<T, 1024>;
+    launch(join, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, stream, a, prefix_step, rest_step);
 }
 
 }  // namespace
@@ -982,12 +1101,12 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
                "%s: misaligned pointer", who);
     // Cache rows, token positions and work items are counted in 32 bits.
     constexpr int64_t kMost = (int64_t{1} << 31) - 4096;
-    CF_REQUIRE(num_pages <= kMost / block_size && max_blocks_per_sequence <= kMost && num_groups <= (1 << 20) &&
+    CF_REQUIRE(num_pages <= kMost / block_size && max_blocks_per_sequence <= kMost && num_kv_heads <= (1 << 14) && num_groups <= (1 << 20) &&
                    num_sequences <= kMost / num_heads,
-               "%s: %lld pages of %lld tokens, %lld sequences of %lld heads or %lld groups exceed 32-bit counts", who,
+               "%s: %lld pages of %lld tokens, %lld sequences of %lld heads, %lld KV heads or %lld groups exceed 32-bit counts", who,
                static_cast<long long>(num_pages), static_cast<long long>(block_size),
                static_cast<long long>(num_sequences), static_cast<long long>(num_heads),
-               static_cast<long long>(num_groups));
+               static_cast<long long>(num_kv_heads), static_cast<long long>(num_groups));
     cf::Plan p = cf::plan_of(dtype, num_sequences, num_groups, num_heads, num_kv_heads, head_dim,
                              cf::capacity_of(max_blocks_per_sequence, block_size));
     const size_t needed = cf::workspace_of(p, num_sequences, num_heads, head_dim);
@@ -1009,11 +1128,14 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
     a.pages = static_cast<uint32_t>(num_pages);
     a.block_size = static_cast<uint32_t>(block_size);
     a.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll(static_cast<uint64_t>(block_size)) : -1;
+    const uint64_t page_bytes = static_cast<uint64_t>(block_size) * num_kv_heads * head_dim * size;
+    a.page_bytes = page_bytes < (uint64_t{1} << 32) ? static_cast<uint32_t>(page_bytes) : 0;
     a.sequences = static_cast<int>(num_sequences);
     a.heads = static_cast<int>(num_heads);
     a.kv_heads = static_cast<int>(num_kv_heads);
     a.per = static_cast<int>(num_heads / num_kv_heads);
     a.head_dim = static_cast<int>(head_dim);
+    a.pitch = (a.head_dim + 3) / 4 * 4;
     a.groups = p.dim != 0 ? static_cast<int>(num_groups) : 0;
     a.max_blocks = static_cast<int>(max_blocks_per_sequence);
     a.capacity = static_cast<int>(cf::capacity_of(max_blocks_per_sequence, block_size));
@@ -1027,7 +1149,11 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
     CF_REQUIRE(prefix_items + rest_items < kMost && num_sequences * num_heads * p.rest_splits < kMost,
                "%s: too many work items", who);
     a.prefix_items = static_cast<int>(prefix_items);
-    a.c = scale * cf::kLog2e;
+    // The kernels take maxima of unscaled scores, so the factor must not be
+    // negative, nor 0 (which times a masked score is NaN).
+    const float c = scale * cf::kLog2e;
+    a.c = c == 0.0f ? 1.0e-37f : c < 0.0f ? -c : c;
+    a.query_sign = c < 0.0f ? (dtype == CF_F32 ? 0x80000000u : 0x80008000u) : 0u;
     const size_t rows = static_cast<size_t>(num_sequences) * num_heads;
     const size_t slots = static_cast<size_t>(p.prefix_splits) + p.rest_splits;
     a.ml = static_cast<float*>(workspace);
