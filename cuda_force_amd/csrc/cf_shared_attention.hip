@@ -76,6 +76,8 @@ struct SharedArgs {
     int rest_splits;
     int prefix_tiles;  // row tiles over all groups, at most
     int rest_tiles;    // row tiles per sequence and KV head
+    int rest_step;     // tokens of a rest's range are a multiple of this
+    bool rest_solo;    // a wave per rest item
     int prefix_items;  // workgroups of the first kind
     float c;           // |scale| log2(e), above 0
     uint32_t query_sign;  // flips the query's signs for a negative scale
@@ -163,9 +165,12 @@ __device__ Group group_of_tile(const SharedArgs& a, int rows, int& tile) {
 
 __device__ __forceinline__ int context_of(const SharedArgs& a, int s) { return clamp_to(a.context[s], a.capacity); }
 
-/// Tokens of each of at most `splits` ranges of `length` tokens: whole steps.
-__device__ __forceinline__ int split_length(int length, int splits, int step) {
-    const int each = (length + splits - 1) / splits;
+/// Tokens of each of at most `splits` ranges of `length` tokens: whole steps,
+/// and about `least` or more (a range has fixed costs, its piece of the result
+/// among them).
+__device__ __forceinline__ int split_length(int length, int splits, int step, int least) {
+    const int wanted = min(splits, max(1, length / least));
+    const int each = (length + wanted - 1) / wanted;
     return (each + step - 1) / step * step;
 }
 
@@ -196,9 +201,12 @@ __device__ __forceinline__ void copy16_to_lds(const void* from, uint32_t dst) {
 
 /// The same from a base that all lanes share, and each lane's offset from it.
 __device__ __forceinline__ void copy16_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
+    const uint64_t address = reinterpret_cast<uint64_t>(base);
+    const uint64_t low = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address)));
+    const uint64_t high = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32)));
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                  :
-                 : "v"(offset), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(dst))
+                 : "v"(offset), "s"(high << 32 | low), "{m0}"(__builtin_amdgcn_readfirstlane(dst))
                  : "memory");
 }
 
@@ -388,16 +396,22 @@ struct Item {
     int slot;
 };
 
-/// Four waves of different rows (kRowWaves 4) or of different tokens (1).
-template <typename T, int kD, int kRowWaves>
-__device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32]) {
+/// The waves of a workgroup take different rows (kRows), different tokens of the
+/// same rows (kTokens), or items of their own (kSolo: no barrier).
+enum class Waves { kRows, kTokens, kSolo };
+
+template <typename T, int kD, Waves kWork>
+__device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
+                       int (*lds_row)[32]) {
     using L = Tile<T, kD>;
-    constexpr int kTokenWaves = kWaves / kRowWaves;
+    constexpr int kRowWaves = kWork == Waves::kRows ? kWaves : 1;
+    constexpr int kTokenWaves = kWork == Waves::kTokens ? kWaves : 1;
+    constexpr bool kSolo = kWork == Waves::kSolo;
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & (kWaveSize - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
     const int row_wave = kRowWaves == 1 ? 0 : wave;
-    const int token_wave = kRowWaves == 1 ? wave : 0;
+    const int token_wave = kWork == Waves::kTokens ? wave : 0;
     const int total_rows = w.sequences * a.per;
 
     // Query rows of this wave; rows past the end are zeros.
@@ -407,7 +421,12 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         const bool inside = row < total_rows;
         const int seq = w.first_sequence + (inside ? row / a.per : 0);
         const int head = w.kv_head * a.per + (inside ? row % a.per : 0);
-        const T* from = static_cast<const T*>(a.query) + (static_cast<int64_t>(seq) * a.heads + head) * a.head_dim;
+        const int out_row = seq * a.heads + head;
+        const T* from = static_cast<const T*>(a.query) + static_cast<int64_t>(out_row) * a.head_dim;
+        // Where the row's piece goes; nowhere for a sequence that takes no part.
+        if (!kSolo && L::part_of(lane) == 0) {
+            lds_row[wave][L::row_of(lane)] = inside && context_of(a, seq) >= w.least ? out_row : -1;
+        }
 #pragma unroll
         for (int u = 0; u < L::kQueries; ++u) {
             const int dim = L::query_dim(u, lane);
@@ -417,10 +436,18 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         }
     }
     if (a.head_dim < kD) {  // the copies leave the end of every row as it is
-        for (int i = tid; i < kStages * 2 * L::kBytes / 16; i += kThreads) {
-            reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0u, 0u, 0u, 0u};
+        constexpr int kPieces = 2 * L::kBytes / 16;  // of one stage, or of a wave's own tiles
+        if constexpr (kSolo) {
+            for (int i = lane; i < kPieces; i += kWaveSize) {
+                reinterpret_cast<u32x4_t*>(lds)[wave * kPieces + i] = u32x4_t{0u, 0u, 0u, 0u};
+            }
+            wait_lds();
+        } else {
+            for (int i = tid; i < kStages * kPieces; i += kThreads) {
+                reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0u, 0u, 0u, 0u};
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
@@ -626,22 +653,24 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         for (int i = 0; i < kStages - 1; ++i) {
             if (i < tiles) issue(i, i);
         }
+        // The scores of tile i + 1 are formed beside the probabilities of tile
+        // i, so that the matrix cores and the vector ALU overlap within a wave.
+        // This wave's copies of a tile have landed when at most those of the
+        // tiles behind it are in flight; fewer are at the end.
+        if (tiles > 2 && a.head_dim == kD) wait_vm<2 * 2 * kCopies>(); else wait_vm<0>();
+        bare_barrier();
+        typename L::Score s = L::scores(lds, q, lane);
         auto step = [&](auto stage, int i) {
             constexpr int kAt = decltype(stage)::value;
-            // This wave's copies of tile i have landed; behind it two tiles
-            // (fewer at the end) are in flight.
-            if (i + kStages - 2 < tiles && a.head_dim == kD) {
-                wait_vm<(kStages - 2) * 2 * kCopies>();
-            } else {
-                wait_vm<0>();
-            }
+            if (i + 2 < tiles && a.head_dim == kD) wait_vm<2 * kCopies>(); else wait_vm<0>();
             bare_barrier();  // and every wave is past tile i - 1, whose place is filled next
             if (i + kStages - 1 < tiles) issue(i + kStages - 1, (kAt + kStages - 1) % kStages);
-            typename L::Score s = L::scores(lds + kAt * 2 * L::kBytes, q, lane);
             const int first = begin + i * L::kTokens;
             uint8_t* v = lds + kAt * 2 * L::kBytes + L::kBytes;
             const bool partial = edge(first);
             if (partial) mask(s, in_range(first));
+            // Past the last tile this reads a stage that nothing uses.
+            const typename L::Score ahead = L::scores(lds + (kAt + 1) % kStages * 2 * L::kBytes, q, lane);
             soften(s);
             if (partial) {
                 clear(v, in_range(first), tid, kThreads);
@@ -649,6 +678,7 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             }
             L::values(v, s, acc, lane);
             wait_lds();  // before the barrier that lets the tile be overwritten
+            s = ahead;
         };
         static_assert(kStages == 4, "steps written out below");
         for (int i = 0; i < tiles; i += kStages) {
@@ -659,6 +689,26 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         }
     }
 
+    const int64_t slot_rows = static_cast<int64_t>(w.slot) * a.sequences * a.heads;
+    if constexpr (kSolo) {
+#pragma unroll
+        for (int d = L::kRows; d < kWaveSize; d <<= 1) l += __shfl_xor(l, d);
+        if (row >= total_rows) return;
+        const int64_t at = slot_rows + static_cast<int64_t>(w.first_sequence) * a.heads + w.kv_head * a.per + row;
+        if (L::part_of(lane) == 0) {
+            a.ml[2 * at] = m;
+            a.ml[2 * at + 1] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < L::kAcc; i += 4) {
+            f32x4_t four;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) four[e] = acc[(i + e) / L::kScores][(i + e) % L::kScores];
+            const int dim = L::dim_of(i, lane);
+            if (dim < a.head_dim) *reinterpret_cast<f32x4_t*>(a.acc + at * a.pitch + dim) = four;
+        }
+        return;
+    }
 #pragma unroll
     for (int d = L::kRows; d < kWaveSize; d <<= 1) l += __shfl_xor(l, d);
     wait_vm<0>();
@@ -679,17 +729,18 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
     // Rows x groups of four dims, over the workgroup; token waves are joined.
     constexpr int kOutRows = kRowWaves * L::kRows;
     constexpr int kFours = kD / 4;
-    for (int i = tid; i < kOutRows * kFours; i += kThreads) {
+    constexpr int kRounds = kOutRows * kFours / kThreads;
+    static_assert(kOutRows * kFours % kThreads == 0, "whole rounds");
+#pragma unroll 4
+    for (int n = 0; n < kRounds; ++n) {
+        const int i = n * kThreads + tid;
         const int r = i / kFours;
         const int dim = (i % kFours) * 4;
-        const int grow = w.first_row + r;
-        if (grow >= total_rows || dim >= a.head_dim) continue;
-        const int seq = w.first_sequence + grow / a.per;
-        if (context_of(a, seq) < w.least) continue;
-        const int64_t out_row = static_cast<int64_t>(seq) * a.heads + w.kv_head * a.per + grow % a.per;
-        const int64_t at = static_cast<int64_t>(w.slot) * a.sequences * a.heads + out_row;
         const int owner = kRowWaves == 1 ? 0 : r / L::kRows;
         const int lr = r % L::kRows;
+        const int out_row = lds_row[owner][lr];
+        if (out_row < 0 || dim >= a.head_dim) continue;
+        const int64_t at = slot_rows + out_row;
         float mm = lds_m[owner][lr];
 #pragma unroll
         for (int t = 1; t < kTokenWaves; ++t) mm = fmaxf(mm, lds_m[t][lr]);
@@ -710,14 +761,17 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             a.ml[2 * at] = mm;
             a.ml[2 * at + 1] = ll;
         }
-        float* to = a.acc + at * a.pitch + dim;
-        *reinterpret_cast<f32x4_t*>(to) = sum;
+        *reinterpret_cast<f32x4_t*>(a.acc + at * a.pitch + dim) = sum;
     }
 }
 
 /// Tokens of a range are a multiple of this (but for the last).
 template <typename T, int kD, int kRowWaves>
 constexpr int range_step() { return kWaves / kRowWaves * Tile<T, kD>::kTokens; }
+/// And about this long at least: four waves of rows leave a large piece each.
+template <int kRowWaves>
+constexpr int range_least() { return kRowWaves == 1 ? 128 : 256; }
+constexpr int kRestLeast = 128;
 
 template <typename T, int kD, int kRowWaves>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void shared_attention_kernel(SharedArgs a) {
@@ -725,21 +779,25 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 1
     __shared__ __attribute__((aligned(16))) uint8_t lds[lds_bytes<T, kD>()];
     __shared__ float lds_m[kWaves][32];
     __shared__ float lds_l[kWaves][32];
+    __shared__ int lds_row[kWaves][32];
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     Item w{};
     int id = static_cast<int>(blockIdx.x);
     if (id < a.prefix_items) {
-        // Row tile outermost: with a multiple of eight (KV head, range) pairs
-        // all row tiles of a pair run on one XCD, whose L2 then reads it once.
-        const int pairs = a.kv_heads * a.prefix_splits;
-        int tile = id / pairs;
-        id %= pairs;
-        const int split = id % a.prefix_splits;
-        w.kv_head = id / a.prefix_splits;
+        // (Range, KV head) pairs in eights, the row tiles of an eight in a row:
+        // all tiles of a pair run on one XCD, whose L2 then reads it once. Ranges
+        // that are there come first.
+        const int block = id / (8 * a.prefix_tiles);
+        id -= block * 8 * a.prefix_tiles;
+        int tile = id / 8;
+        const int pair = block * 8 + id % 8;
+        const int split = pair / a.kv_heads;
+        if (split >= a.prefix_splits) return;
+        w.kv_head = pair % a.kv_heads;
         constexpr int kRows = kRowWaves * L::kRows;
         const Group g = group_of_tile(a, kRows, tile);
         if (g.end == 0 || g.prefix == 0) return;
-        const int each = split_length(g.prefix, a.prefix_splits, range_step<T, kD, kRowWaves>());
+        const int each = split_length(g.prefix, a.prefix_splits, range_step<T, kD, kRowWaves>(), range_least<kRowWaves>());
         w.lo = split * each;
         w.hi = min(g.prefix, w.lo + each);
         if (w.lo >= w.hi) return;
@@ -761,19 +819,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 1
         w.first_row = tile * kRows;
         w.least = g.prefix;
         w.slot = split;
-        attend<T, kD, kRowWaves>(a, w, lds, lds_m, lds_l);
+        attend<T, kD, kRowWaves == 4 ? Waves::kRows : Waves::kTokens>(a, w, lds, lds_m, lds_l, lds_row);
     } else {
+        // Where there are items enough, each wave has its own; else a workgroup.
         id -= a.prefix_items;
-        const int split = id % a.rest_splits;
-        id /= a.rest_splits;
-        const int tile = id % a.rest_tiles;
-        id /= a.rest_tiles;
+        if (a.rest_solo) id = id * kWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWaveSize);
+        const int items = a.sequences * a.kv_heads * a.rest_tiles;
+        const int split = id / items;
+        if (split >= a.rest_splits) return;
+        id %= items;
         w.kv_head = id % a.kv_heads;
-        const int s = id / a.kv_heads;
+        id /= a.kv_heads;
+        const int tile = id % a.rest_tiles;
+        const int s = id / a.rest_tiles;
         const int context = context_of(a, s);
         const Group g = a.groups > 0 ? group_of(a, s) : Group{0, 0, 0};
         const int first = g.end > 0 && g.prefix <= context ? g.prefix : 0;
-        const int each = split_length(context - first, a.rest_splits, range_step<T, kD, 1>());
+        const int each = split_length(context - first, a.rest_splits, a.rest_step, kRestLeast);
         w.lo = first + split * each;
         w.hi = min(context, w.lo + each);
         if (w.lo >= w.hi) return;
@@ -784,7 +846,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 1
         w.first_row = tile * L::kRows;
         w.least = 0;
         w.slot = a.prefix_splits + split;
-        attend<T, kD, 1>(a, w, lds, lds_m, lds_l);
+        if (a.rest_solo) {
+            attend<T, kD, Waves::kSolo>(a, w, lds, lds_m, lds_l, lds_row);
+        } else {
+            attend<T, kD, Waves::kTokens>(a, w, lds, lds_m, lds_l, lds_row);
+        }
     }
 }
 
@@ -800,7 +866,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedAr
     const int head = static_cast<int>(out_row % a.heads);
     const int s = static_cast<int>(out_row / a.heads);
     const int context = context_of(a, s);
-    const int each = split_length(context, a.rest_splits, 32);
+    const int each = split_length(context, a.rest_splits, 32, 32);
     const int lo = split * each;
     const int hi = min(context, lo + each);
     if (lo >= hi) return;
@@ -853,30 +919,36 @@ __global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedAr
     }
 }
 
-/// Joins the pieces of one (sequence, head), a workgroup each. prefix_step and
-/// rest_step are the first kernel's range steps (prefix_step 0: nothing was
-/// shared).
-template <typename T, int kD>
-__global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedArgs a, int prefix_step,
-                                                                         int rest_step) {
+/// How the first kernel cut the contexts: its steps and least lengths. prefix
+/// step 0: nothing was shared.
+struct Cuts {
+    int prefix_step, prefix_least, rest_least;
+};
+
+/// Joins the pieces of one (sequence, head): four waves each, or one where there
+/// are rows enough to fill the GPU with that.
+template <typename T, int kD, int kRowWaves>
+__global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedArgs a, Cuts cuts) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     const int64_t rows = static_cast<int64_t>(a.sequences) * a.heads;
-    const int64_t row = blockIdx.x;
-    const int s = static_cast<int>(blockIdx.x) / a.heads;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWaveSize);
+    const int row = static_cast<int>(blockIdx.x) * (kWaves / kRowWaves) + (kRowWaves == 1 ? wave : 0);
+    if (row >= rows) return;
+    const int s = row / a.heads;
     const int context = context_of(a, s);
     int first = 0;
     int prefix_pieces = 0;
-    if (prefix_step > 0) {
+    if (cuts.prefix_step > 0) {
         const Group g = group_of(a, s);
         if (g.end > 0 && g.prefix <= context && g.prefix > 0) {
             first = g.prefix;
-            const int each = split_length(first, a.prefix_splits, prefix_step);
+            const int each = split_length(first, a.prefix_splits, cuts.prefix_step, cuts.prefix_least);
             prefix_pieces = (first + each - 1) / each;
         }
     }
     int rest_pieces = 0;
     if (context > first) {
-        const int each = split_length(context - first, a.rest_splits, rest_step);
+        const int each = split_length(context - first, a.rest_splits, a.rest_step, cuts.rest_least);
         rest_pieces = (context - first + each - 1) / each;
     }
     const int pieces = prefix_pieces + rest_pieces;
@@ -897,10 +969,11 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
     }
     // Threads: groups of kLanes lanes take the pieces in turn, four dims a lane.
     constexpr int kLanes = kD / 4;
-    constexpr int kTeams = kThreads / kLanes;
+    constexpr int kTeams = kRowWaves * kWaveSize / kLanes;
     constexpr int kAhead = 4;
-    const int team = static_cast<int>(threadIdx.x) / kLanes;
-    const int dim = (static_cast<int>(threadIdx.x) % kLanes) * 4;
+    const int thread = kRowWaves == 1 ? lane : static_cast<int>(threadIdx.x);
+    const int team = thread / kLanes;
+    const int dim = (thread % kLanes) * 4;
     f32x4_t part[kAhead];
     auto load = [&](int i0) {
 #pragma unroll
@@ -937,12 +1010,13 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
             }
         }
     }
-    __shared__ __attribute__((aligned(16))) float teams[kTeams][kD];
+    __shared__ __attribute__((aligned(16))) float all_teams[kWaves / kRowWaves][kTeams][kD];
+    auto& teams = all_teams[kRowWaves == 1 ? wave : 0];
     *reinterpret_cast<f32x4_t*>(&teams[team][dim]) = o;
-    __syncthreads();
+    if constexpr (kRowWaves == 1) wait_lds(); else __syncthreads();
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = static_cast<T*>(a.out) + row * a.head_dim;
-    for (int d = static_cast<int>(threadIdx.x); d < a.head_dim; d += kThreads) {
+    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.head_dim;
+    for (int d = thread; d < a.head_dim; d += kRowWaves * kWaveSize) {
         float v = teams[0][d];
 #pragma unroll
         for (int t = 1; t < kTeams; ++t) v += teams[t][d];
@@ -959,6 +1033,8 @@ struct Plan {
     int rest_splits;
     int prefix_tiles;
     int rest_tiles;
+    int rest_step;
+    bool rest_solo;
 };
 
 Plan plan_of(cf_dtype dtype, int64_t sequences, int64_t groups, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -977,6 +1053,7 @@ Plan plan_of(cf_dtype dtype, int64_t sequences, int64_t groups, int64_t heads, i
     };
     if (p.dim == 0) {
         p.rest_splits = splits(sequences * heads, 4096, 64);
+        p.rest_step = 32;
         return p;
     }
     const int64_t wave_rows = wide ? 16 : 32;
@@ -992,7 +1069,12 @@ Plan plan_of(cf_dtype dtype, int64_t sequences, int64_t groups, int64_t heads, i
         p.row_waves = 1;
     }
     p.rest_tiles = static_cast<int>(ceil_div<int64_t>(per, wave_rows));
-    p.rest_splits = splits(sequences * kv_heads * p.rest_tiles, 512, 128);
+    // A wave for every rest where that fills the GPU (2048 waves at two per
+    // SIMD) well enough; its ranges are then whole tiles.
+    const int64_t rests = sequences * kv_heads * p.rest_tiles;
+    p.rest_solo = rests >= 256;
+    p.rest_splits = splits(rests, p.rest_solo ? 2048 : 512, 128);
+    p.rest_step = static_cast<int>(wave_rows) * (p.rest_solo ? 1 : kWaves);  // a tile has as many tokens as rows
     return p;
 }
 
@@ -1026,8 +1108,7 @@ template <typename T>
 void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
     constexpr int tokens = sizeof(T) == 4 ? 16 : 32;
     const int64_t rows = static_cast<int64_t>(a.sequences) * a.heads;
-    int prefix_step = 0;
-    int rest_step = 32;
+    Cuts cuts{0, 1, 32};
     if (p.dim == 0) {
         const dim3 grid(static_cast<unsigned>(ceil_div<int64_t>(rows * a.rest_splits, kWaves)));
         if (a.head_dim <= 128) {
@@ -1036,9 +1117,11 @@ void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
             launch(shared_attention_any_kernel<T, 16>, grid, dim3(kThreads), 0, stream, a);
         }
     } else {
-        prefix_step = a.groups > 0 ? kWaves / p.row_waves * tokens : 0;
-        rest_step = kWaves * tokens;
-        const int64_t rest = static_cast<int64_t>(a.sequences) * a.kv_heads * a.rest_tiles * a.rest_splits;
+        cuts.prefix_step = a.groups > 0 ? kWaves / p.row_waves * tokens : 0;
+        cuts.prefix_least = p.row_waves == 4 ? range_least<4>() : range_least<1>();
+        cuts.rest_least = kRestLeast;
+        int64_t rest = static_cast<int64_t>(a.sequences) * a.kv_heads * a.rest_tiles * a.rest_splits;
+        if (a.rest_solo) rest = ceil_div<int64_t>(rest, kWaves);
         const dim3 grid(static_cast<unsigned>(a.prefix_items + rest));
         if (p.dim == 64) {
             run_matrix<T, 64>(a, p, grid, stream);
@@ -1048,11 +1131,17 @@ void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
             run_matrix<T, 256>(a, p, grid, stream);
         }
     }
-    auto* join = a.head_dim <= 64    ? shared_attention_join_kernel<T, 64>
-                 : a.head_dim <= 128 ? shared_attention_join_kernel<T, 128>
-                 : a.head_dim <= 256 ? shared_attention_join_kernel<T, 256>
-                                     : shared_attention_join_kernel<T, 1024>;
-    launch(join, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, stream, a, prefix_step, rest_step);
+    // A wave per row from a round of the GPU's waves on (2048 rows: 5.9 -> 4.6 us).
+    const bool one_wave = rows >= 1024 && a.head_dim <= 256;
+    auto* join = one_wave ? (a.head_dim <= 64    ? shared_attention_join_kernel<T, 64, 1>
+                             : a.head_dim <= 128 ? shared_attention_join_kernel<T, 128, 1>
+                                                 : shared_attention_join_kernel<T, 256, 1>)
+                          : (a.head_dim <= 64    ? shared_attention_join_kernel<T, 64, 4>
+                             : a.head_dim <= 128 ? shared_attention_join_kernel<T, 128, 4>
+                             : a.head_dim <= 256 ? shared_attention_join_kernel<T, 256, 4>
+                                                 : shared_attention_join_kernel<T, 1024, 4>);
+    launch(join, dim3(static_cast<unsigned>(one_wave ? ceil_div<int64_t>(rows, kWaves) : rows)), dim3(kThreads), 0,
+           stream, a, cuts);
 }
 
 }  // namespace
@@ -1115,6 +1204,7 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
     if (p.dim != 0 && !(cf::host_aligned(query, 16) && cf::host_aligned(k_cache, 16) && cf::host_aligned(v_cache, 16))) {
         p.dim = 0;  // same workspace, read as ranges of whole contexts
         p.prefix_splits = 0;
+        p.rest_step = 32;
     }
     cf::SharedArgs a{};
     a.query = query;
@@ -1143,8 +1233,10 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
     a.rest_splits = p.rest_splits;
     a.prefix_tiles = p.prefix_tiles;
     a.rest_tiles = p.rest_tiles;
+    a.rest_step = p.rest_step;
+    a.rest_solo = p.rest_solo;
     const int64_t prefix_items =
-        a.groups > 0 ? static_cast<int64_t>(p.prefix_tiles) * num_kv_heads * p.prefix_splits : 0;
+        a.groups > 0 ? (num_kv_heads * p.prefix_splits + 7) / 8 * 8 * p.prefix_tiles : 0;
     const int64_t rest_items = num_sequences * num_kv_heads * (p.rest_tiles > 0 ? p.rest_tiles : 1) * p.rest_splits;
     CF_REQUIRE(prefix_items + rest_items < kMost && num_sequences * num_heads * p.rest_splits < kMost,
                "%s: too many work items", who);
