@@ -42,9 +42,8 @@
 namespace cf {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;  // per workgroup where nothing else is said
 constexpr int kThreads = kWaves * kWaveSize;
-constexpr int kStages = 4;       // ring of tiles shared by four waves
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -76,7 +75,10 @@ struct SharedArgs {
     int rest_splits;
     int prefix_tiles;  // row tiles over all groups, at most
     int rest_tiles;    // row tiles per sequence and KV head
-    int rest_step;     // tokens of a rest's range are a multiple of this
+    int prefix_step;   // tokens of a prefix's range are a multiple of this; 0: nothing is shared
+    int prefix_least;  // and at least about this
+    int rest_step;     // the same for rests
+    int rest_least;
     bool rest_solo;    // a wave per rest item
     int prefix_items;  // workgroups of the first kind
     float c;           // |scale| log2(e), above 0
@@ -121,9 +123,32 @@ __device__ Group group_of(const SharedArgs& a, int s) {
     return Group{0, 0, 0};
 }
 
-/// The group of row tile `tile` (uniform) of `rows` rows; `tile` becomes the
-/// tile within the group. end = 0: no such tile.
-__device__ Group group_of_tile(const SharedArgs& a, int rows, int& tile) {
+__device__ __forceinline__ int context_of(const SharedArgs& a, int s) { return clamp_to(a.context[s], a.capacity); }
+
+/// Tokens of each of at most `splits` ranges of `length` tokens: whole steps,
+/// and about `least` or more (a range has fixed costs, its piece of the result
+/// among them).
+__device__ __forceinline__ int split_length(int length, int splits, int step, int least) {
+    const int wanted = min(splits, max(1, (length + least - 1) / least));
+    const int each = (length + wanted - 1) / wanted;
+    return (each + step - 1) / step * step;
+}
+
+/// One XCD's share of the prefixes' work: a group, its row tile, and the place
+/// of a (range, KV head) pair in the XCD's run of them.
+struct PrefixItem {
+    Group group;  // end = 0: no such item
+    int tile;
+    int place;
+    int run;   // pairs per XCD
+    int each;  // tokens per range
+};
+
+/// Item `index` (uniform) of an XCD, over all groups in turn: the groups' items
+/// lie end to end, so the first workgroups have all the work. (Workgroups without
+/// work among the others cost half of the GPU: they are dealt to the shader
+/// engines in turn, and every second one was empty.)
+__device__ PrefixItem prefix_item(const SharedArgs& a, int rows, int step, int least, int index) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     int before = 0;  // largest start so far
     for (int base = 0; base < a.groups; base += kWaveSize) {
@@ -141,8 +166,11 @@ __device__ Group group_of_tile(const SharedArgs& a, int rows, int& tile) {
             }
         }
         end = there ? max(start, end) : start;
-        const int tiles = ((end - start) * a.per + rows - 1) / rows;
-        int total = tiles;
+        const int tiles = prefix > 0 ? ((end - start) * a.per + rows - 1) / rows : 0;
+        const int each = split_length(max(prefix, 1), a.prefix_splits, step, least);
+        const int run = ((prefix + each - 1) / each * a.kv_heads + 7) / 8;
+        const int items = tiles * run;
+        int total = items;
         if (a.groups > 1) {
 #pragma unroll
             for (int d = 1; d < kWaveSize; d <<= 1) {
@@ -150,28 +178,20 @@ __device__ Group group_of_tile(const SharedArgs& a, int rows, int& tile) {
                 if (lane >= d) total += o;
             }
         }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(there && total > tile);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(total > index);
         if (past != 0) {
             const int at = __builtin_ctzll(past);
-            tile -= __builtin_amdgcn_readlane(total - tiles, at);
-            return Group{__builtin_amdgcn_readlane(start, at), __builtin_amdgcn_readlane(end, at),
-                         __builtin_amdgcn_readlane(prefix, at)};
+            index -= __builtin_amdgcn_readlane(total - items, at);
+            const int n = __builtin_amdgcn_readlane(tiles, at);
+            return PrefixItem{Group{__builtin_amdgcn_readlane(start, at), __builtin_amdgcn_readlane(end, at),
+                                    __builtin_amdgcn_readlane(prefix, at)},
+                              index % n, index / n, __builtin_amdgcn_readlane(run, at),
+                              __builtin_amdgcn_readlane(each, at)};
         }
-        tile -= __builtin_amdgcn_readlane(total, kWaveSize - 1);
+        index -= __builtin_amdgcn_readlane(total, kWaveSize - 1);
         before = __builtin_amdgcn_readlane(start, kWaveSize - 1);
     }
-    return Group{0, 0, 0};
-}
-
-__device__ __forceinline__ int context_of(const SharedArgs& a, int s) { return clamp_to(a.context[s], a.capacity); }
-
-/// Tokens of each of at most `splits` ranges of `length` tokens: whole steps,
-/// and about `least` or more (a range has fixed costs, its piece of the result
-/// among them).
-__device__ __forceinline__ int split_length(int length, int splits, int step, int least) {
-    const int wanted = min(splits, max(1, length / least));
-    const int each = (length + wanted - 1) / wanted;
-    return (each + step - 1) / step * step;
+    return PrefixItem{Group{0, 0, 0}, 0, 0, 0, 0};
 }
 
 // ---- fragments ------------------------------------------------------------------
@@ -369,16 +389,15 @@ struct Tile {
     }
 };
 
-/// LDS of a workgroup: four waves' tiles (K and V each) or a ring of four
+/// LDS of a workgroup: its waves' own tiles (K and V each), or a ring of as many
 /// shared ones; afterwards the waves' outputs.
 template <typename T, int kD>
 constexpr int lds_bytes() {
     using L = Tile<T, kD>;
-    constexpr int tiles = kStages * 2 * L::kBytes;
+    constexpr int tiles = kWaves * 2 * L::kBytes;
     constexpr int outputs = kWaves * L::kRows * L::kOutPitch * 4;
     return tiles > outputs ? tiles : outputs;
 }
-static_assert(kStages == kWaves, "the ring and the waves' own tiles take the same space");
 
 // ---- one work item ----------------------------------------------------------------
 
@@ -400,12 +419,14 @@ struct Item {
 /// same rows (kTokens), or items of their own (kSolo: no barrier).
 enum class Waves { kRows, kTokens, kSolo };
 
+/// kRows: through a ring of kWaves tiles.
 template <typename T, int kD, Waves kWork>
 __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
                        int (*lds_row)[32]) {
     using L = Tile<T, kD>;
     constexpr int kRowWaves = kWork == Waves::kRows ? kWaves : 1;
     constexpr int kTokenWaves = kWork == Waves::kTokens ? kWaves : 1;
+    constexpr int kStages = kWaves;
     constexpr bool kSolo = kWork == Waves::kSolo;
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & (kWaveSize - 1);
@@ -460,15 +481,18 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
     const int begin = w.lo / L::kTokens * L::kTokens;
     const int tiles = (w.hi - begin + L::kTokens - 1) / L::kTokens;
 
-    // A copy takes kPerCopy neighbouring tokens; kSpan tokens of this wave's
-    // share of a tile lie in one page (blocks of a power of two from 16 on).
-    constexpr int kCopies = L::kCopies / kRowWaves;
-    static_assert(L::kCopies % kRowWaves == 0, "copies per wave");
+    // A copy takes kPerCopy neighbouring tokens. A wave's own tiles are copied
+    // whole, K and V; of a ring's tile each wave copies a share of K or of V.
+    // kSpan neighbouring tokens lie in one page (blocks of a power of two from 16
+    // on).
     constexpr int kPerCopy = kWaveSize / L::kChunks;
     static_assert(kPerCopy >= 1, "a row within a copy");
+    constexpr int kCopies = kRowWaves == 1 ? L::kCopies : 2 * L::kCopies / kWaves;
+    static_assert(kRowWaves == 1 || 2 * L::kCopies % kWaves == 0, "copies per wave");
     constexpr int kSpan = kCopies * kPerCopy < 16 ? kCopies * kPerCopy : 16;
     constexpr int kSpanCopies = kSpan / kPerCopy;
-    const int first_copy = row_wave * kCopies;
+    const bool ring_v = kRowWaves > 1 && wave >= kWaves / 2;
+    const int first_copy = kRowWaves == 1 ? 0 : wave % (kWaves / 2) * kCopies;
 
     // 64 entries of the block table in lane registers: a token's page is a lane
     // read, not a load that would have to wait behind the copies. `sound`: all
@@ -488,21 +512,23 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         if (block >= window_base + kWaveSize) {  // tiles are taken in ascending order
             window_base = block;
             window = load_window();
+            // Waited for here: after the branch the compiler would wait for every
+            // copy in flight, whether or not this ran.
+            asm volatile("" : "+v"(window));
         }
         const uint32_t page = __builtin_amdgcn_readlane(window, block - window_base);
         return static_cast<uint64_t>(page) * a.page_bytes +
                (static_cast<uint32_t>(t) & (a.block_size - 1)) * token_bytes;
     };
-    // This wave's copies of K (0) or V (1) of the tile at token `first` to LDS.
-    auto fetch = [&](int first, uint32_t dst, auto which) {
-        constexpr bool is_k = decltype(which)::value == 0;
+    // This wave's copies of K or V of the tile at token `first` to LDS.
+    auto fetch = [&](int first, uint32_t dst, bool is_v) {
 #pragma unroll
         for (int n0 = 0; n0 < kCopies; n0 += kSpanCopies) {
-            const uint8_t* base = (is_k ? k_head : v_head) + place_of(first + (first_copy + n0) * kPerCopy);
+            const uint8_t* base = (is_v ? v_head : k_head) + place_of(first + (first_copy + n0) * kPerCopy);
 #pragma unroll
             for (int n = n0; n < n0 + kSpanCopies; ++n) {
                 const int r = (first_copy + n) * kPerCopy + lane / L::kChunks;
-                const int piece = (lane % L::kChunks) ^ (is_k ? L::k_swizzle(r) : L::v_swizzle(r));
+                const int piece = (lane % L::kChunks) ^ (is_v ? L::v_swizzle(r) : L::k_swizzle(r));
                 const uint32_t offset = static_cast<uint32_t>((n - n0) * kPerCopy + lane / L::kChunks) * token_bytes +
                                         static_cast<uint32_t>(piece) * 16;
                 if (piece < row_pieces) {
@@ -511,8 +537,6 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             }
         }
     };
-    using K = std::integral_constant<int, 0>;
-    using V = std::integral_constant<int, 1>;
 
     float m = -INFINITY;  // the row's running maximum
     float l = 0.0f;       // this lane's share of the running sum
@@ -585,11 +609,10 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             const uint32_t page = inside ? w.table[block] : a.pages;
             const uint32_t cache_row = page < a.pages ? page * a.block_size + static_cast<uint32_t>(t) - block * a.block_size : 0u;
             const uint32_t valid = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(page < a.pages)) & kAll;
-#pragma unroll
-            for (int n = 0; n < kCopies; ++n) {
-                const int r = (first_copy + n) * kPerCopy + lane / L::kChunks;
+            for (int n = kRowWaves == 1 ? 0 : wave; n < L::kCopies; n += kRowWaves) {
+                const int r = n * kPerCopy + lane / L::kChunks;
                 const uint64_t from = static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(cache_row), r))) * token_bytes;
-                const uint32_t dst = k_dst + static_cast<uint32_t>(first_copy + n) * 16 * kWaveSize;
+                const uint32_t dst = k_dst + static_cast<uint32_t>(n) * 16 * kWaveSize;
                 const int k_piece = (lane % L::kChunks) ^ L::k_swizzle(r);
                 const int v_piece = (lane % L::kChunks) ^ L::v_swizzle(r);
                 if (k_piece < row_pieces) copy16_to_lds(k_head + from + k_piece * 16, dst);
@@ -618,8 +641,8 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
         int t = begin + token_wave * L::kTokens;
         constexpr int kStep = kTokenWaves * L::kTokens;
         if (t < w.hi) {
-            fetch(t, k_dst, K{});
-            fetch(t, v_dst, V{});
+            fetch(t, k_dst, false);
+            fetch(t, v_dst, true);
         }
         for (; t < w.hi; t += kStep) {
             const bool more = t + kStep < w.hi;
@@ -629,7 +652,7 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             if (a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
             typename L::Score s = L::scores(k, q, lane);
             wait_lds();
-            if (more) fetch(t + kStep, k_dst, K{});
+            if (more) fetch(t + kStep, k_dst, false);
             const bool partial = edge(t);
             if (partial) mask(s, in_range(t));
             soften(s);
@@ -640,37 +663,30 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             }
             L::values(v, s, acc, lane);
             wait_lds();
-            if (more) fetch(t + kStep, v_dst, V{});
+            if (more) fetch(t + kStep, v_dst, true);
         }
     } else {
-        // A ring of tiles; every wave copies a quarter of each.
-        auto issue = [&](int tile, uint32_t stage) {
-            const uint32_t dst = lds_base + stage * 2 * L::kBytes;
-            fetch(begin + tile * L::kTokens, dst, K{});
-            fetch(begin + tile * L::kTokens, dst + L::kBytes, V{});
+        // A ring of tiles, all but one of them in flight.
+        constexpr int kStageBytes = 2 * L::kBytes;
+        auto issue = [&](int tile) {
+            const uint32_t dst = lds_base + static_cast<uint32_t>(tile % kStages) * kStageBytes;
+            fetch(begin + tile * L::kTokens, ring_v ? dst + L::kBytes : dst, ring_v);
         };
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) {
-            if (i < tiles) issue(i, i);
-        }
-        // The scores of tile i + 1 are formed beside the probabilities of tile
-        // i, so that the matrix cores and the vector ALU overlap within a wave.
-        // This wave's copies of a tile have landed when at most those of the
-        // tiles behind it are in flight; fewer are at the end.
-        if (tiles > 2 && a.head_dim == kD) wait_vm<2 * 2 * kCopies>(); else wait_vm<0>();
-        bare_barrier();
-        typename L::Score s = L::scores(lds, q, lane);
-        auto step = [&](auto stage, int i) {
-            constexpr int kAt = decltype(stage)::value;
-            if (i + 2 < tiles && a.head_dim == kD) wait_vm<2 * kCopies>(); else wait_vm<0>();
+        for (int i = 0; i < kStages - 1 && i < tiles; ++i) issue(i);
+        // The ring's steps written out, so that LDS addresses are constants.
+        auto step = [&](auto at, int i) {
+            constexpr int kAt = decltype(at)::value;
+            // This wave's copies of tile i have landed; those of the tiles behind
+            // it (fewer at the end) are in flight.
+            if (i + kStages - 2 < tiles && a.head_dim == kD) wait_vm<(kStages - 2) * kCopies>(); else wait_vm<0>();
             bare_barrier();  // and every wave is past tile i - 1, whose place is filled next
-            if (i + kStages - 1 < tiles) issue(i + kStages - 1, (kAt + kStages - 1) % kStages);
+            if (i + kStages - 1 < tiles) issue(i + kStages - 1);
+            uint8_t* k = lds + kAt * kStageBytes;
+            uint8_t* v = k + L::kBytes;
+            typename L::Score s = L::scores(k, q, lane);
             const int first = begin + i * L::kTokens;
-            uint8_t* v = lds + kAt * 2 * L::kBytes + L::kBytes;
             const bool partial = edge(first);
             if (partial) mask(s, in_range(first));
-            // Past the last tile this reads a stage that nothing uses.
-            const typename L::Score ahead = L::scores(lds + (kAt + 1) % kStages * 2 * L::kBytes, q, lane);
             soften(s);
             if (partial) {
                 clear(v, in_range(first), tid, kThreads);
@@ -678,9 +694,8 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             }
             L::values(v, s, acc, lane);
             wait_lds();  // before the barrier that lets the tile be overwritten
-            s = ahead;
         };
-        static_assert(kStages == 4, "steps written out below");
+        static_assert(kStages == 4, "four steps");
         for (int i = 0; i < tiles; i += kStages) {
             step(std::integral_constant<int, 0>{}, i);
             if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
@@ -729,13 +744,13 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
     // Rows x groups of four dims, over the workgroup; token waves are joined.
     constexpr int kOutRows = kRowWaves * L::kRows;
     constexpr int kFours = kD / 4;
-    constexpr int kRounds = kOutRows * kFours / kThreads;
-    static_assert(kOutRows * kFours % kThreads == 0, "whole rounds");
+    constexpr int kRounds = (kOutRows * kFours + kThreads - 1) / kThreads;
 #pragma unroll 4
     for (int n = 0; n < kRounds; ++n) {
         const int i = n * kThreads + tid;
         const int r = i / kFours;
         const int dim = (i % kFours) * 4;
+        if (r >= kOutRows) break;
         const int owner = kRowWaves == 1 ? 0 : r / L::kRows;
         const int lr = r % L::kRows;
         const int out_row = lds_row[owner][lr];
@@ -765,16 +780,11 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
     }
 }
 
-/// Tokens of a range are a multiple of this (but for the last).
+/// Prefix tiles of four waves' rows, or of one's (kRowWaves 1: the four take
+/// different tokens).
 template <typename T, int kD, int kRowWaves>
-constexpr int range_step() { return kWaves / kRowWaves * Tile<T, kD>::kTokens; }
-/// And about this long at least: four waves of rows leave a large piece each.
-template <int kRowWaves>
-constexpr int range_least() { return kRowWaves == 1 ? 128 : 256; }
-constexpr int kRestLeast = 128;
-
-template <typename T, int kD, int kRowWaves>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void shared_attention_kernel(SharedArgs a) {
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void shared_attention_kernel(SharedArgs a) {
     using L = Tile<T, kD>;
     __shared__ __attribute__((aligned(16))) uint8_t lds[lds_bytes<T, kD>()];
     __shared__ float lds_m[kWaves][32];
@@ -784,22 +794,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 1
     Item w{};
     int id = static_cast<int>(blockIdx.x);
     if (id < a.prefix_items) {
-        // (Range, KV head) pairs in eights, the row tiles of an eight in a row:
-        // all tiles of a pair run on one XCD, whose L2 then reads it once. Ranges
-        // that are there come first.
-        const int block = id / (8 * a.prefix_tiles);
-        id -= block * 8 * a.prefix_tiles;
-        int tile = id / 8;
-        const int pair = block * 8 + id % 8;
-        const int split = pair / a.kv_heads;
-        if (split >= a.prefix_splits) return;
-        w.kv_head = pair % a.kv_heads;
+        // Workgroup i runs on XCD i % 8. The (range, KV head) pairs of a prefix are
+        // cut into eight runs, one per XCD, heads varying fastest: an XCD then
+        // reads neighbouring tokens with all their heads, and all row tiles of a
+        // pair, whose L2 serves them from one read.
         constexpr int kRows = kRowWaves * L::kRows;
-        const Group g = group_of_tile(a, kRows, tile);
-        if (g.end == 0 || g.prefix == 0) return;
-        const int each = split_length(g.prefix, a.prefix_splits, range_step<T, kD, kRowWaves>(), range_least<kRowWaves>());
-        w.lo = split * each;
-        w.hi = min(g.prefix, w.lo + each);
+        const PrefixItem p = prefix_item(a, kRows, a.prefix_step, a.prefix_least, id / 8);
+        const Group& g = p.group;
+        if (g.end == 0) return;
+        const int pair = id % 8 * p.run + p.place;
+        const int split = pair / a.kv_heads;
+        w.kv_head = pair % a.kv_heads;
+        w.lo = split * p.each;
+        w.hi = min(g.prefix, w.lo + p.each);
         if (w.lo >= w.hi) return;
         // The pages of the first sequence that holds the whole prefix.
         int holder = -1;
@@ -816,18 +823,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 1
         w.last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
         w.first_sequence = g.first;
         w.sequences = g.end - g.first;
-        w.first_row = tile * kRows;
+        w.first_row = p.tile * kRows;
         w.least = g.prefix;
         w.slot = split;
-        attend<T, kD, kRowWaves == 4 ? Waves::kRows : Waves::kTokens>(a, w, lds, lds_m, lds_l, lds_row);
+        attend<T, kD, kRowWaves == 1 ? Waves::kTokens : Waves::kRows>(a, w, lds, lds_m, lds_l, lds_row);
     } else {
         // Where there are items enough, each wave has its own; else a workgroup.
         id -= a.prefix_items;
+        const int rests = a.sequences * a.kv_heads * a.rest_tiles;
+        const int per_layer = a.rest_solo ? (rests + kWaves - 1) / kWaves : rests;  // workgroups of one range index
+        const int split = id / per_layer;
+        id %= per_layer;
+        if (per_layer % 8 == 0) id = id % 8 * (per_layer / 8) + id / 8;  // neighbours on one XCD, as above
         if (a.rest_solo) id = id * kWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWaveSize);
-        const int items = a.sequences * a.kv_heads * a.rest_tiles;
-        const int split = id / items;
-        if (split >= a.rest_splits) return;
-        id %= items;
+        if (id >= rests) return;
         w.kv_head = id % a.kv_heads;
         id /= a.kv_heads;
         const int tile = id % a.rest_tiles;
@@ -835,7 +844,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kD > 1
         const int context = context_of(a, s);
         const Group g = a.groups > 0 ? group_of(a, s) : Group{0, 0, 0};
         const int first = g.end > 0 && g.prefix <= context ? g.prefix : 0;
-        const int each = split_length(context - first, a.rest_splits, a.rest_step, kRestLeast);
+        const int each = split_length(context - first, a.rest_splits, a.rest_step, a.rest_least);
         w.lo = first + split * each;
         w.hi = min(context, w.lo + each);
         if (w.lo >= w.hi) return;
@@ -866,7 +875,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedAr
     const int head = static_cast<int>(out_row % a.heads);
     const int s = static_cast<int>(out_row / a.heads);
     const int context = context_of(a, s);
-    const int each = split_length(context, a.rest_splits, 32, 32);
+    const int each = split_length(context, a.rest_splits, a.rest_step, a.rest_least);
     const int lo = split * each;
     const int hi = min(context, lo + each);
     if (lo >= hi) return;
@@ -919,16 +928,10 @@ __global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedAr
     }
 }
 
-/// How the first kernel cut the contexts: its steps and least lengths. prefix
-/// step 0: nothing was shared.
-struct Cuts {
-    int prefix_step, prefix_least, rest_least;
-};
-
 /// Joins the pieces of one (sequence, head): four waves each, or one where there
 /// are rows enough to fill the GPU with that.
 template <typename T, int kD, int kRowWaves>
-__global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedArgs a, Cuts cuts) {
+__global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedArgs a) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     const int64_t rows = static_cast<int64_t>(a.sequences) * a.heads;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWaveSize);
@@ -938,17 +941,17 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
     const int context = context_of(a, s);
     int first = 0;
     int prefix_pieces = 0;
-    if (cuts.prefix_step > 0) {
+    if (a.prefix_step > 0) {
         const Group g = group_of(a, s);
         if (g.end > 0 && g.prefix <= context && g.prefix > 0) {
             first = g.prefix;
-            const int each = split_length(first, a.prefix_splits, cuts.prefix_step, cuts.prefix_least);
+            const int each = split_length(first, a.prefix_splits, a.prefix_step, a.prefix_least);
             prefix_pieces = (first + each - 1) / each;
         }
     }
     int rest_pieces = 0;
     if (context > first) {
-        const int each = split_length(context - first, a.rest_splits, a.rest_step, cuts.rest_least);
+        const int each = split_length(context - first, a.rest_splits, a.rest_step, a.rest_least);
         rest_pieces = (context - first + each - 1) / each;
     }
     const int pieces = prefix_pieces + rest_pieces;
@@ -1028,12 +1031,15 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
 
 struct Plan {
     int dim;        // head size of the matrix kernel, or 0: the general kernel
-    int row_waves;  // 4: prefix tiles of four waves' rows
+    int row_waves;  // prefix tiles of 1 or 4 waves' rows
+    int prefix_least;
     int prefix_splits;
     int rest_splits;
     int prefix_tiles;
     int rest_tiles;
+    int prefix_step;
     int rest_step;
+    int rest_least;
     bool rest_solo;
 };
 
@@ -1053,28 +1059,37 @@ Plan plan_of(cf_dtype dtype, int64_t sequences, int64_t groups, int64_t heads, i
     };
     if (p.dim == 0) {
         p.rest_splits = splits(sequences * heads, 4096, 64);
-        p.rest_step = 32;
+        p.rest_step = p.rest_least = 32;
         return p;
     }
     const int64_t wave_rows = wide ? 16 : 32;
     const int64_t rows = sequences * per;
+    constexpr int64_t slots = 512;  // workgroups at two per CU
+    p.row_waves = 1;
     if (groups > 0) {
-        // Four waves of rows where the groups fill more than one wave's.
-        p.row_waves = rows > wave_rows * groups ? 4 : 1;
+        // Four waves of rows where the groups fill more than two waves' on
+        // average; below, two tiles of one wave's rows, four waves over their
+        // tokens (64 rows behind 2048 tokens, 8 KV heads of 128 in bf16: 14.4 ->
+        // 10.1 us, 32 rows in fp32 14.0 -> 11.9). Eight waves of rows, a workgroup
+        // per CU, were within 3% from 16384 shared tokens on and up to 16% slower
+        // below.
+        p.row_waves = rows > 2 * wave_rows * groups ? 4 : 1;
+        // A tile has as many tokens as a wave has rows.
+        p.prefix_step = static_cast<int>(p.row_waves == 4 ? wave_rows : kWaves * wave_rows);
+        p.prefix_least = p.row_waves == 1 ? 128 : wide ? 64 : 256;
         const int64_t tile = p.row_waves * wave_rows;
-        p.prefix_tiles = static_cast<int>(rows / tile + groups);
+        p.prefix_tiles = static_cast<int>((rows + groups * (tile - 1)) / tile);  // at most, however the groups lie
         const int64_t likely = ceil_div<int64_t>(rows, tile * groups) * groups;
-        p.prefix_splits = splits(likely * kv_heads, 512, 64);
-    } else {
-        p.row_waves = 1;
+        p.prefix_splits = splits(likely * kv_heads, slots, p.prefix_least);
     }
     p.rest_tiles = static_cast<int>(ceil_div<int64_t>(per, wave_rows));
     // A wave for every rest where that fills the GPU (2048 waves at two per
     // SIMD) well enough; its ranges are then whole tiles.
     const int64_t rests = sequences * kv_heads * p.rest_tiles;
     p.rest_solo = rests >= 256;
-    p.rest_splits = splits(rests, p.rest_solo ? 2048 : 512, 128);
-    p.rest_step = static_cast<int>(wave_rows) * (p.rest_solo ? 1 : kWaves);  // a tile has as many tokens as rows
+    p.rest_least = p.rest_solo ? 256 : 128;
+    p.rest_splits = splits(rests, p.rest_solo ? slots * kWaves : slots, p.rest_least);
+    p.rest_step = static_cast<int>(wave_rows) * (p.rest_solo ? 1 : kWaves);
     return p;
 }
 
@@ -1106,9 +1121,7 @@ void run_matrix(const SharedArgs& a, const Plan& p, dim3 grid, hipStream_t strea
 
 template <typename T>
 void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
-    constexpr int tokens = sizeof(T) == 4 ? 16 : 32;
     const int64_t rows = static_cast<int64_t>(a.sequences) * a.heads;
-    Cuts cuts{0, 1, 32};
     if (p.dim == 0) {
         const dim3 grid(static_cast<unsigned>(ceil_div<int64_t>(rows * a.rest_splits, kWaves)));
         if (a.head_dim <= 128) {
@@ -1117,11 +1130,9 @@ void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
             launch(shared_attention_any_kernel<T, 16>, grid, dim3(kThreads), 0, stream, a);
         }
     } else {
-        cuts.prefix_step = a.groups > 0 ? kWaves / p.row_waves * tokens : 0;
-        cuts.prefix_least = p.row_waves == 4 ? range_least<4>() : range_least<1>();
-        cuts.rest_least = kRestLeast;
-        int64_t rest = static_cast<int64_t>(a.sequences) * a.kv_heads * a.rest_tiles * a.rest_splits;
+        int64_t rest = static_cast<int64_t>(a.sequences) * a.kv_heads * a.rest_tiles;
         if (a.rest_solo) rest = ceil_div<int64_t>(rest, kWaves);
+        rest *= a.rest_splits;
         const dim3 grid(static_cast<unsigned>(a.prefix_items + rest));
         if (p.dim == 64) {
             run_matrix<T, 64>(a, p, grid, stream);
@@ -1141,7 +1152,7 @@ void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
                              : a.head_dim <= 256 ? shared_attention_join_kernel<T, 256, 4>
                                                  : shared_attention_join_kernel<T, 1024, 4>);
     launch(join, dim3(static_cast<unsigned>(one_wave ? ceil_div<int64_t>(rows, kWaves) : rows)), dim3(kThreads), 0,
-           stream, a, cuts);
+           stream, a);
 }
 
 }  // namespace
@@ -1203,8 +1214,8 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
                "%s: needs %zu bytes of 16-byte aligned workspace", who, needed);
     if (p.dim != 0 && !(cf::host_aligned(query, 16) && cf::host_aligned(k_cache, 16) && cf::host_aligned(v_cache, 16))) {
         p.dim = 0;  // same workspace, read as ranges of whole contexts
-        p.prefix_splits = 0;
-        p.rest_step = 32;
+        p.prefix_splits = p.prefix_step = 0;
+        p.rest_step = p.rest_least = 32;
     }
     cf::SharedArgs a{};
     a.query = query;
@@ -1233,7 +1244,10 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
     a.rest_splits = p.rest_splits;
     a.prefix_tiles = p.prefix_tiles;
     a.rest_tiles = p.rest_tiles;
+    a.prefix_step = p.prefix_step;
+    a.prefix_least = p.prefix_least;
     a.rest_step = p.rest_step;
+    a.rest_least = p.rest_least;
     a.rest_solo = p.rest_solo;
     const int64_t prefix_items =
         a.groups > 0 ? (num_kv_heads * p.prefix_splits + 7) / 8 * 8 * p.prefix_tiles : 0;
