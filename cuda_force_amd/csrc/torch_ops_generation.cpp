@@ -32,14 +32,15 @@ void check_logits(const torch::Tensor& logits, const torch::Tensor& tokens, doub
 
 int64_t row_stride(const torch::Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
 
-LogprobsResult token_logprobs_hip(const torch::Tensor& logits, const torch::Tensor& tokens, double scale,
-                                  bool entropy, int64_t top) {
+/// The results for tokens [rows, n], the first of them as `shape` has it.
+LogprobsResult logprobs_of(const torch::Tensor& logits, const torch::Tensor& tokens, torch::IntArrayRef shape,
+                           double scale, bool entropy, int64_t top) {
     check_logits(logits, tokens, scale);
     const at::DeviceGuard guard(logits.device());
     const int64_t rows = logits.size(0), vocab = logits.size(1);
     TORCH_CHECK(top >= 0 && top <= vocab, "top ", top, " is not in 0 .. ", vocab, " (the vocabulary)");
     const auto f32 = logits.options().dtype(torch::kFloat32);
-    torch::Tensor logprobs = torch::empty(tokens.sizes(), f32);
+    torch::Tensor logprobs = torch::empty(shape, f32);
     torch::Tensor stats = torch::empty({rows, 2}, f32);
     torch::Tensor h = torch::empty({entropy ? rows : 0}, f32);
     torch::Tensor top_logprobs = torch::empty({top > 0 ? rows : 0, top}, f32);
@@ -56,6 +57,11 @@ LogprobsResult token_logprobs_hip(const torch::Tensor& logits, const torch::Tens
                                    top > 0 ? top_tokens.data_ptr<int64_t>() : nullptr,
                                    bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_for(logits)));
     return {logprobs, stats, h, top_logprobs, top_tokens};
+}
+
+LogprobsResult token_logprobs_hip(const torch::Tensor& logits, const torch::Tensor& tokens, double scale,
+                                  bool entropy, int64_t top) {
+    return logprobs_of(logits, tokens, tokens.sizes(), scale, entropy, top);
 }
 
 /// Contiguous fp32 gradient of the expected shape, or null where it is absent.
@@ -395,6 +401,67 @@ torch::Tensor paged_attention_shared_cpu(const torch::Tensor& query, const torch
 
 // ---- direct entry for ordinary GPU calls (the rules: torch_ops_common.hpp) ------
 
+/// The autograd function of cuda_force_amd/autograd.py as a native node: the
+/// same saved tensors and kernels, without the interpreter in either direction.
+/// Outputs: log probabilities shaped as the tokens, then the entropy, then the
+/// likeliest tokens' two, where asked for.
+struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits,
+                                                  const at::Tensor& tokens, double scale, bool entropy, int64_t top) {
+        const at::Tensor given = tokens.dim() == 1 ? tokens.unsqueeze(1) : tokens;
+        auto [logprobs, stats, h, top_logprobs, top_tokens] =
+            logprobs_of(logits, given, tokens.sizes(), scale, entropy, top);
+        torch::autograd::variable_list out{logprobs};
+        if (entropy) out.push_back(h);
+        if (top > 0) {
+            out.push_back(top_logprobs);
+            out.push_back(top_tokens);
+            ctx->mark_non_differentiable({top_logprobs, top_tokens});
+        }
+        ctx->save_for_backward({logits, given, stats, h});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["entropy"] = entropy;
+        ctx->set_materialize_grads(false);
+        return out;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2], &h = saved[3];
+        const double scale = ctx->saved_data["scale"].toDouble();
+        std::optional<at::Tensor> g, gh;
+        if (grads[0].defined()) g = grads[0].dim() == 1 ? grads[0].unsqueeze(1) : grads[0];
+        if (ctx->saved_data["entropy"].toBool() && grads[1].defined()) gh = grads[1];
+        at::Tensor grad;
+        if (g || gh) {
+            // What saved-tensor hooks return, a batched gradient, a mode
+            // entered since, and a recorded backward (whose result the
+            // dispatcher's entry refuses to differentiate) go through the
+            // dispatcher.
+            const bool direct = !at::GradMode::is_enabled() && ordinary_context() && plain_gpu(logits) &&
+                                plain_gpu(tokens) && plain_gpu(stats) && plain_gpu(h) && (!g || plain_gpu(*g)) &&
+                                (!gh || plain_gpu(*gh));
+            if (direct) {
+                grad = token_logprobs_backward_hip(logits, tokens, scale, stats, h, g, gh);
+            } else {
+                static const auto op = c10::Dispatcher::singleton()
+                                           .findSchemaOrThrow("cudaforge::token_logprobs_backward", "")
+                                           .typed<at::Tensor(const at::Tensor&, const at::Tensor&, double,
+                                                             const at::Tensor&, const at::Tensor&,
+                                                             const std::optional<at::Tensor>&,
+                                                             const std::optional<at::Tensor>&)>();
+                grad = op.call(logits, tokens, scale, stats, h, g, gh);
+            }
+        }
+        return {grad, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+/// Calls above these go the general way, which names the limit.
+constexpr int64_t kLogprobsTokens = 1024;
+constexpr int64_t kLogprobsTop = 64;
+
 py::object try_token_logprobs(py::handle logits_, py::handle tokens_, py::handle scale_, py::handle entropy_,
                               py::handle top_) {
     if (!THPVariable_CheckTypeExact(Py_TYPE(logits_.ptr()))) return py::none();
@@ -408,19 +475,29 @@ py::object try_token_logprobs(py::handle logits_, py::handle tokens_, py::handle
     }
     const bool entropy = entropy_.ptr() == Py_True;
     if (!kernel_dtype(logits.scalar_type()) || tokens->scalar_type() != torch::kInt64 ||
-        tokens->device() != logits.device() || grad_needed({&logits}) || logits.dim() != 2 || logits.numel() == 0 ||
-        logits.stride(1) != 1 || (logits.size(0) > 1 && logits.stride(0) < logits.size(1)) ||
-        tokens->size(0) != logits.size(0) || tokens->dim() > 2 || *scale <= 0 || *top < 0 || *top > logits.size(1)) {
+        tokens->device() != logits.device() || logits.dim() != 2 || logits.numel() == 0 || logits.stride(1) != 1 ||
+        (logits.size(0) > 1 && logits.stride(0) < logits.size(1)) || tokens->size(0) != logits.size(0) ||
+        tokens->dim() > 2 || (tokens->dim() == 2 && tokens->size(1) > kLogprobsTokens) ||
+        !(*scale > 0 && *scale < 1e29) || *top < 0 || *top > std::min(kLogprobsTop, logits.size(1))) {
         return py::none();
     }
-    LogprobsResult out;
+    const bool grad = grad_needed({&logits});
+    at::Tensor logprobs, h, top_logprobs, top_tokens;
     {
         py::gil_scoped_release no_gil;
-        const bool one = tokens->dim() == 1;
-        out = token_logprobs_hip(logits, one ? tokens->unsqueeze(1) : *tokens, *scale, entropy, *top);
-        if (one) std::get<0>(out) = std::get<0>(out).squeeze(1);
+        if (grad) {
+            torch::autograd::variable_list out = TokenLogprobs::apply(logits, *tokens, *scale, entropy, *top);
+            logprobs = out[0];
+            if (entropy) h = out[1];
+            if (*top > 0) {
+                top_logprobs = out[out.size() - 2];
+                top_tokens = out.back();
+            }
+        } else {
+            std::tie(logprobs, std::ignore, h, top_logprobs, top_tokens) = logprobs_of(
+                logits, tokens->dim() == 1 ? tokens->unsqueeze(1) : *tokens, tokens->sizes(), *scale, entropy, *top);
+        }
     }
-    const auto& [logprobs, stats, h, top_logprobs, top_tokens] = out;
     return py::make_tuple(wrap(logprobs), entropy ? wrap(h) : py::none(), *top > 0 ? wrap(top_logprobs) : py::none(),
                           *top > 0 ? wrap(top_tokens) : py::none());
 }

@@ -228,3 +228,59 @@ def test_empty():
     got = cf.token_logprobs(torch.empty(0, 9, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda"),
                             entropy=True, top=3)
     assert got.logprobs.shape == (0,) and got.top_tokens.shape == (0, 3)
+
+
+@pytest.mark.parametrize("shape", [(6,), (6, 3)], ids=["one", "several"])
+@pytest.mark.parametrize("entropy, top", [(False, 0), (True, 0), (False, 4), (True, 4)])
+def test_gradients_of_the_native_node_equal_the_general_ones(shape, entropy, top):
+    # Three dimensions take the general way, two the native node: the same kernels.
+    logits = torch.randn(6, 700, device="cuda", dtype=torch.bfloat16)
+    tokens = torch.randint(-1, 700, shape, device="cuda")
+    two, three = logits.clone().requires_grad_(), logits.clone().view(1, 6, 700).requires_grad_()
+    a = cf.token_logprobs(two, tokens, 0.7, entropy, top)
+    b = cf.token_logprobs(three, tokens.view(1, *shape), 0.7, entropy, top)
+    assert a.logprobs.requires_grad and a.logprobs.shape == shape and torch.equal(a.logprobs, b.logprobs[0])
+    weights = torch.randn(shape, device="cuda")
+    losses = [(r.logprobs.view(shape) * weights).sum() for r in (a, b)]
+    if entropy:
+        losses = [l + r.entropy.square().sum() for l, r in zip(losses, (a, b))]
+    if top:
+        assert not a.top_logprobs.requires_grad and not a.top_tokens.requires_grad
+        assert torch.equal(a.top_tokens, b.top_tokens[0])
+    for loss in losses:
+        loss.backward()
+    assert torch.equal(two.grad, three.grad[0])
+
+
+def test_gradient_of_the_entropy_alone():
+    logits = torch.randn(5, 333, device="cuda", requires_grad=True)
+    got = cf.token_logprobs(logits, torch.zeros(5, dtype=torch.int64, device="cuda"), 1.0, True)
+    got.entropy.sum().backward()
+    x = logits.detach().cpu().double().requires_grad_()
+    p = x.log_softmax(-1)
+    (-(p.exp() * p).sum()).backward()
+    # p (ln p + H) in fp32: a few roundings of values below 8, times p.
+    assert (logits.grad.cpu().double() - x.grad).abs().max() <= 64 * 2.0 ** -24
+
+
+def test_saved_tensors_are_guarded_and_may_be_packed():
+    logits = torch.randn(4, 256, device="cuda", requires_grad=True)
+    tokens = torch.tensor([1, 2, 3, 4], device="cuda")
+    plain = cf.token_logprobs(logits, tokens).logprobs
+    want, = torch.autograd.grad(plain.sum(), logits)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        packed = cf.token_logprobs(logits, tokens).logprobs
+    got, = torch.autograd.grad(packed.sum(), logits)
+    assert torch.equal(got, want)
+    changed = cf.token_logprobs(logits, tokens).logprobs
+    tokens.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        changed.sum().backward()
+
+
+@pytest.mark.parametrize("scale, top, count", [(float("nan"), 0, 1), (float("inf"), 0, 1), (1e29, 0, 1), (1.0, 65, 1),
+                                               (1.0, 0, 1025)])
+def test_limits_are_refused_alike_on_the_gpu(scale, top, count):
+    with pytest.raises(ValueError):
+        cf.token_logprobs(torch.zeros(2, 100, device="cuda"), torch.zeros(2, count, dtype=torch.int64, device="cuda"),
+                          scale, top=top)
