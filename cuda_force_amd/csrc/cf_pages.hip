@@ -11,12 +11,18 @@
 // data. Results depend on the inputs alone: of two entries that claim the same
 // row or page the earlier one wins (an integer minimum), reference counts are
 // integer sums, and free pages come out of an ordered scan.
-//   * The plan of a list runs in one workgroup of 1024 threads (phases divided
-//     by barriers instead of launches). The search for free pages reads 16384
-//     counts a step and ends when it has enough: 4096 pages 5 us with everything
-//     else of a fork's plan.
+//   * The plan of a list runs in one workgroup of 1024 threads: phases divided
+//     by barriers instead of launches, and nothing but the order of the phases
+//     to keep between them. The search for free pages reads 16384 counts a step
+//     and ends when it has enough. Bound by the chain of loads and atomics:
+//     32 forks of 8 sequences 8 us, their extension 8 us, 1500 pairs of a copy 11 us.
 //   * Copies are bound by HBM: 16 KiB per workgroup and step, four 16-byte loads
-//     in flight per lane, streamed past the caches.
+//     in flight per lane, streamed past the caches. 1500 pages of 32 KiB in four
+//     tensors (393 MB read and written) 78 us, 5.0 TB/s; 32 KiB per workgroup
+//     took 80 us, and a grid that loops over the chunks 80 us.
+//   * Compaction: 48 sequences' 195 MB read and written 37 us, after 11 us that
+//     list the moves. Counting and listing in one launch where the pool is small
+//     took 9 us of those 11 but left the whole as it was, so there is one way.
 #include "cf_common.hpp"
 
 namespace cf {
@@ -46,9 +52,12 @@ __device__ __forceinline__ int peek(const int* p) {
 __device__ __forceinline__ void poke(int* p, int v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-/// Barrier between two phases of a plan: what they wrote to memory is visible.
+/// Barrier between two phases of a plan. One workgroup runs it, and all that
+/// its threads exchange through memory goes by peek, poke and atomics, past the
+/// CU's cache: it is enough that these have arrived. A fence at device scope
+/// writes L2 back as well, microseconds each time.
 __device__ __forceinline__ void phase() {
-    __threadfence();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 }
 
