@@ -1,0 +1,43 @@
+"""Continuations of shared prompts on the GPU, sampled together."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.continuations_util import run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_continuations_are_sampled_forked_and_compacted(dtype):
+    run("cuda", dtype)
+
+
+def test_a_captured_step_between_forks_and_a_compaction():
+    """The step is captured once and replayed; between its replays rows are
+    released, forked and moved eagerly on the same tensors."""
+
+    def captured(r):
+        kept = [t.clone() for t in (*r.caches, r.counts, r.tables, r.context)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            r.step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = r.step()
+        for t, was in zip((*r.caches, r.counts, r.tables, r.context), kept):
+            t.copy_(was)
+
+        def replay():
+            graph.replay()
+            torch.cuda.synchronize()
+            return results
+
+        return replay
+
+    run("cuda", torch.bfloat16, captured)
