@@ -15,9 +15,10 @@
 // group (sequences x heads of a KV head) against the prefix, on the matrix
 // cores. The rests stay bound by HBM.
 //   * A work item is (row tile, KV head, token range) of a prefix or (sequence,
-//     KV head, token range) of a rest, one workgroup of four waves each, both
-//     kinds in one launch. Long ranges are split over workgroups from the
-//     lengths found on the device; a second kernel joins the pieces.
+//     KV head, token range) of a rest, a workgroup of four waves each (a wave,
+//     where there are many rests), both kinds in one launch, the items of all
+//     groups laid end to end. Long ranges are split from the lengths found on
+//     the device; a second kernel joins the pieces.
 //   * Scores are formed transposed, S^T = K Q^T: a lane then holds one query
 //     row and several tokens, so a row's maximum and sum are lane-local but for
 //     one exchange, and the probabilities are in place as the B operand of
@@ -31,6 +32,12 @@
 //     caches 16 x 16 x 4 fp32 MFMA over 16 rows and 16 tokens (fp32 products).
 //     Probabilities are rounded to the cache's type for the second product
 //     (relative error half an ulp each, of either sign); sums stay in fp32.
+//   * Measured, 32 query and 8 KV heads of 128 in bf16, with the join: 128
+//     sequences behind 32768 tokens 98 + 9.5 us, 704 TFLOP/s: neither the matrix
+//     cores (31% busy) nor the vector units (34%), but the chain from one product
+//     through the probabilities to the next at two waves per SIMD. 64 sequences
+//     behind 4099 tokens 26 + 6.5 us, 3.2 TB/s: one round of work, a third of it
+//     filling and draining. 8 behind 1000 tokens 9 + 4 us: the launches' chains.
 // Tokens behind a range's end, and tokens whose page is not in the cache, get
 // no weight: their scores are replaced and their V rows are cleared in LDS, so
 // that whatever lies there (NaN, infinities) stays out.
@@ -1142,7 +1149,7 @@ void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
             run_matrix<T, 256>(a, p, grid, stream);
         }
     }
-    // A wave per row from a round of the GPU's waves on (2048 rows: 5.9 -> 4.6 us).
+    // A wave per row from a round of the GPU's waves on (2048 rows: 9.4 -> 6.5 us).
     const bool one_wave = rows >= 1024 && a.head_dim <= 256;
     auto* join = one_wave ? (a.head_dim <= 64    ? shared_attention_join_kernel<T, 64, 1>
                              : a.head_dim <= 128 ? shared_attention_join_kernel<T, 128, 1>
