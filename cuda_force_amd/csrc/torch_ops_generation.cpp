@@ -95,8 +95,12 @@ torch::Tensor token_logprobs_backward_hip(const torch::Tensor& logits, const tor
         TORCH_CHECK(entropy.scalar_type() == torch::kFloat32 && entropy.numel() == rows, "entropy must be float32 [",
                     rows, "]");
     }
-    // Laid out as the logits: rows padded to an aligned pitch stay aligned.
-    torch::Tensor grad = torch::empty_strided(logits.sizes(), {row_stride(logits), 1}, logits.options());
+    // Laid out as the logits where their rows are padded to an aligned pitch, so
+    // that the gradient's are aligned too; not where they are a small part of a
+    // larger tensor's rows (the last position of each sequence), which it would
+    // take the memory of.
+    const int64_t pitch = row_stride(logits) - vocab <= 128 ? row_stride(logits) : vocab;
+    torch::Tensor grad = torch::empty_strided(logits.sizes(), {pitch, 1}, logits.options());
     check_status(cf_token_logprobs_backward(logits.data_ptr(), to_cf(logits, "logits"), rows, vocab,
                                             row_stride(logits), tokens.data_ptr<int64_t>(), tokens.size(1),
                                             static_cast<float>(scale), stats.data_ptr<float>(),

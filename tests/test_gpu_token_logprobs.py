@@ -284,3 +284,51 @@ def test_limits_are_refused_alike_on_the_gpu(scale, top, count):
     with pytest.raises(ValueError):
         cf.token_logprobs(torch.zeros(2, 100, device="cuda"), torch.zeros(2, count, dtype=torch.int64, device="cuda"),
                           scale, top=top)
+
+
+@pytest.mark.parametrize("padding, pitch", [(0, 500), (12, 512), (4500, 500)])
+def test_the_gradient_takes_no_more_memory_than_the_logits(padding, pitch):
+    # Rows behind a little padding keep their pitch; rows far apart (the last
+    # position of every sequence) do not.
+    whole = torch.randn(4, 500 + padding, device="cuda")
+    logits = whole[:, :500].requires_grad_()
+    tokens = torch.tensor([0, 1, 498, 499], device="cuda")
+    got = cf.token_logprobs(logits, tokens).logprobs
+    grad, = torch.autograd.grad(got.sum(), logits)
+    ref, size = gradient(logits, tokens[:, None], 1.0, torch.ones(4, 1), None)
+    close(grad, ref, 2.0**-24 * ref.abs() + (2.0**-18 + 8 * 2.0**-24 * 500 / 256) * size)
+    direct = torch.ops.cudaforge.token_logprobs_backward(
+        logits.detach(), tokens[:, None].contiguous(), 1.0,
+        torch.ops.cudaforge.token_logprobs(logits.detach(), tokens[:, None].contiguous(), 1.0, False, 0)[1],
+        torch.empty(0, device="cuda"), torch.ones(4, 1, device="cuda"), None)
+    assert direct.stride() == (pitch, 1) and torch.equal(direct, grad)
+
+
+def test_forward_and_backward_captured_and_replayed():
+    """No eager graph of the same leaf lives while the capture runs."""
+    logits = torch.randn(33, 1000, device="cuda", dtype=torch.bfloat16)
+    tokens = torch.randint(-1, 1000, (33,), device="cuda")
+    weights = torch.randn(33, device="cuda")
+
+    def step(leaf):
+        got = cf.token_logprobs(leaf, tokens, 0.9, True)
+        grad, = torch.autograd.grad([got.logprobs, got.entropy], [leaf], [weights, weights])
+        return got.logprobs.detach(), got.entropy.detach(), grad
+
+    static = logits.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(static.detach().requires_grad_())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        results = step(static.detach().requires_grad_())
+    for i in range(4):
+        logits = torch.randn_like(logits)
+        static.copy_(logits)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(results, step(logits.clone().requires_grad_())):
+            assert torch.equal(got, want)
