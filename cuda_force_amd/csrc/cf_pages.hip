@@ -15,7 +15,8 @@
 //     by barriers instead of launches, and nothing but the order of the phases
 //     to keep between them. The search for free pages reads 16384 counts a step
 //     and ends when it has enough. Bound by the chain of loads and atomics:
-//     32 forks of 8 sequences 8 us, their extension 8 us, 1500 pairs of a copy 11 us.
+//     32 forks of 8 sequences 5.6 us, their extension 5.5 us, 1500 pairs of a copy
+//     4.9 us; claims and short lists of pages are exchanged in LDS for that.
 //   * Copies are bound by HBM: 16 KiB per workgroup and step, four 16-byte loads
 //     in flight per lane, streamed past the caches. 1500 pages of 32 KiB in four
 //     tensors (393 MB read and written) 78 us, 5.0 TB/s; 32 KiB per workgroup
@@ -23,6 +24,8 @@
 //   * Compaction: 48 sequences' 195 MB read and written 37 us, after 11 us that
 //     list the moves. Counting and listing in one launch where the pool is small
 //     took 9 us of those 11 but left the whole as it was, so there is one way.
+#include <type_traits>
+
 #include "cf_common.hpp"
 
 namespace cf {
@@ -36,6 +39,11 @@ constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;
 constexpr int64_t kChunkBytes = int64_t{kCopyThreads} * kCopyUnroll * 16;
 constexpr int kTilePages = kCopyThreads * kCountsPerThread;  // counts per workgroup of the compaction's scan
+/// Plans over at most so many rows (a copy: pages) exchange their claims in LDS,
+/// those of forks and extensions if they want at most kPlanThreads pages: atomics
+/// and loads past the CU's cache cost most of a plan's time otherwise (32 forks
+/// 8.1 -> 5.6 us, 32 rows extended 8.0 -> 5.5, 1500 pairs copied 10.6 -> 4.9).
+constexpr int kSmallRows = 8192;
 constexpr int kUnclaimed = 0x7FFFFFFF;
 
 struct Tensors {
@@ -61,21 +69,38 @@ __device__ __forceinline__ void phase() {
     __syncthreads();
 }
 
-/// Sum of v over lower threads; `total` over all. Every thread calls it.
+/// Numbers that a plan's threads exchange: in the workspace, or in LDS.
+struct InMemory {
+    int* p;
+    __device__ __forceinline__ int get(int64_t i) const { return peek(p + i); }
+    __device__ __forceinline__ void put(int64_t i, int v) const { poke(p + i, v); }
+    __device__ __forceinline__ void lower(int64_t i, int v) const { atomicMin(p + i, v); }
+    __device__ __forceinline__ static void phase() { cf::phase(); }
+};
+struct InLds {
+    int* p;
+    __device__ __forceinline__ int get(int64_t i) const { return p[i]; }
+    __device__ __forceinline__ void put(int64_t i, int v) const { p[i] = v; }
+    __device__ __forceinline__ void lower(int64_t i, int v) const { atomicMin(p + i, v); }
+    __device__ __forceinline__ static void phase() { __syncthreads(); }
+};
+
+/// Sum of v over lower threads; `total` over all. Every thread calls it. Sums
+/// of pages, entries or tokens wanted: at most kMostInts.
 template <int kWaves>
-__device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* slots, int64_t& total) {
+__device__ __forceinline__ int scan_before(int v, int* slots, int& total) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
     const int wave = static_cast<int>(threadIdx.x) / kWaveSize;
-    int64_t sum = v;
+    int sum = v;
 #pragma unroll
     for (int d = 1; d < kWaveSize; d <<= 1) {
-        const int64_t o = __shfl_up(sum, d);
+        const int o = __shfl_up(sum, d);
         if (lane >= d) sum += o;
     }
     __syncthreads();  // the last call's slots have been read
     if (lane == kWaveSize - 1) slots[wave] = sum;
     __syncthreads();
-    int64_t before = 0;
+    int before = 0;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
@@ -105,7 +130,8 @@ __device__ __forceinline__ void load_counts(const int* counts, int64_t pages, in
 
 /// The lowest `wanted` free pages into `list`, ascending; returns how many
 /// there are (at most `wanted`). The whole planning workgroup calls it.
-__device__ int64_t find_free(const int* counts, int64_t pages, int64_t wanted, int* list, int64_t* slots) {
+template <typename Ints>
+__device__ int64_t find_free(const int* counts, int64_t pages, int64_t wanted, const Ints& list, int* slots) {
     int64_t found = 0;
     const bool aligned = aligned16(counts);
     for (int64_t base = 0; base < pages && found < wanted; base += int64_t{kPlanThreads} * kCountsPerThread) {
@@ -115,12 +141,12 @@ __device__ int64_t find_free(const int* counts, int64_t pages, int64_t wanted, i
         int mine = 0;
 #pragma unroll
         for (int i = 0; i < kCountsPerThread; ++i) mine += c[i] <= 0 ? 1 : 0;
-        int64_t total;
+        int total;
         int64_t at = found + scan_before<kPlanWaves>(mine, slots, total);
 #pragma unroll
         for (int i = 0; i < kCountsPerThread; ++i) {
             if (c[i] > 0) continue;
-            if (at < wanted) poke(list + at, static_cast<int>(first + i));
+            if (at < wanted) list.put(at, static_cast<int>(first + i));
             ++at;
         }
         found += total;
@@ -163,20 +189,25 @@ __device__ __forceinline__ void copy_bytes(const uint8_t* from, uint8_t* to, int
 
 /// Which pairs of a copy take part: status 0, or 1 for a pair out of range,
 /// whose dst an earlier pair names, or whose src any pair names as its dst.
+/// kSmall: claims in LDS.
+template <bool kSmall>
 __global__ __launch_bounds__(kPlanThreads) void copy_plan_kernel(const int* src, const int* dst, int64_t count,
-                                                                 int64_t pages, int* claims, int* status) {
+                                                                 int64_t pages, int* claims_, int* status) {
+    using Ints = typename std::conditional<kSmall, InLds, InMemory>::type;
+    __shared__ int lds[kSmall ? kSmallRows : 1];
+    const Ints claims{kSmall ? lds : claims_};
     for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (within(src[i], pages)) poke(claims + src[i], kUnclaimed);
-        if (within(dst[i], pages)) poke(claims + dst[i], kUnclaimed);
+        if (within(src[i], pages)) claims.put(src[i], kUnclaimed);
+        if (within(dst[i], pages)) claims.put(dst[i], kUnclaimed);
     }
-    phase();
+    Ints::phase();
     for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (within(dst[i], pages)) atomicMin(claims + dst[i], static_cast<int>(i));
+        if (within(dst[i], pages)) claims.lower(dst[i], static_cast<int>(i));
     }
-    phase();
+    Ints::phase();
     for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        const bool good = within(src[i], pages) && within(dst[i], pages) && peek(claims + dst[i]) == i &&
-                          peek(claims + src[i]) == kUnclaimed;
+        const bool good = within(src[i], pages) && within(dst[i], pages) && claims.get(dst[i]) == i &&
+                          claims.get(src[i]) == kUnclaimed;
         status[i] = good ? 0 : 1;
     }
 }
@@ -210,55 +241,74 @@ struct TableArgs {
 };
 
 /// Fork's plan. `fresh[i]`: the page that pair i's child gets in the place of
-/// its parent's partial last page, -1 for none.
+/// its parent's partial last page, -1 for none. kSmall: a pair a thread at most,
+/// and claims and free pages in LDS.
+template <bool kSmall>
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(TableArgs a, const int* parents, const int* children,
-                                                                 int64_t count, int* claims, int* fresh, int* free_list,
-                                                                 int* status) {
-    __shared__ int64_t slots[kPlanWaves];
-    const int64_t rounds = (count + kPlanThreads - 1) / kPlanThreads;
+                                                                 int64_t count, int* claims_, int* fresh,
+                                                                 int* free_list, int* status) {
+    using Ints = typename std::conditional<kSmall, InLds, InMemory>::type;
+    __shared__ int slots[kPlanWaves];
+    __shared__ int lds[kSmall ? kSmallRows + kPlanThreads : 1];
+    const Ints claims{kSmall ? lds : claims_};
+    const Ints list{kSmall ? lds + kSmallRows : free_list};
+    const int64_t rounds = kSmall ? 1 : (count + kPlanThreads - 1) / kPlanThreads;
+    // A pair's parent's length where it may be forked, else 0.
     auto eligible = [&](int64_t i) {
-        if (i >= count || !within(parents[i], a.sequences) || !within(children[i], a.sequences)) return false;
+        if (i >= count || !within(parents[i], a.sequences) || !within(children[i], a.sequences)) return 0;
         const int length = a.context[parents[i]];
-        return length > 0 && length <= a.capacity && a.context[children[i]] <= 0;
+        return length > 0 && length <= a.capacity && a.context[children[i]] <= 0 ? length : 0;
     };
-    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (within(children[i], a.sequences)) poke(claims + children[i], kUnclaimed);
-    }
-    phase();
-    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (eligible(i)) atomicMin(claims + children[i], static_cast<int>(i));
-    }
-    phase();
-    // Which pairs need a page, and how many before each do.
-    int64_t wanted = 0;
+    int mine = 0;  // kSmall: the thread's pair's
     for (int64_t r = 0; r < rounds; ++r) {
         const int64_t i = r * kPlanThreads + threadIdx.x;
-        const bool wins = eligible(i) && peek(claims + children[i]) == i;
-        const bool needs = wins && a.context[parents[i]] % a.block != 0;
-        int64_t total;
+        if (i < count && within(children[i], a.sequences)) claims.put(children[i], kUnclaimed);
+    }
+    if (kSmall) mine = eligible(threadIdx.x);
+    Ints::phase();
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t i = r * kPlanThreads + threadIdx.x;
+        if (kSmall ? mine > 0 : eligible(i) > 0) claims.lower(children[i], static_cast<int>(i));
+    }
+    Ints::phase();
+    // Which pairs need a page, and how many before each do.
+    int64_t wanted = 0;
+    int rank = -1;
+    bool wins = false;
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t i = r * kPlanThreads + threadIdx.x;
+        const int length = kSmall ? mine : eligible(i);
+        wins = length > 0 && claims.get(children[i]) == i;
+        const bool needs = wins && static_cast<uint32_t>(length) % static_cast<uint32_t>(a.block) != 0;
+        int total;
         const int64_t before = wanted + scan_before<kPlanWaves>(needs ? 1 : 0, slots, total);
-        if (i < count) {
-            poke(fresh + i, needs ? static_cast<int>(before) : -1);
+        rank = needs ? static_cast<int>(before) : -1;
+        if (!kSmall && i < count) {
+            poke(fresh + i, rank);
             poke(status + i, wins ? 0 : 1);
         }
         wanted += total;
     }
-    const int64_t found = find_free(a.counts, a.pages, wanted < a.pages ? wanted : a.pages, free_list, slots);
-    phase();
-    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (peek(status + i) != 0) continue;
-        const int rank = peek(fresh + i);
-        if (rank >= found) {
-            poke(status + i, 2);
-            poke(fresh + i, -1);
-            continue;
+    const int64_t found = find_free(a.counts, a.pages, wanted < a.pages ? wanted : a.pages, list, slots);
+    Ints::phase();
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t i = r * kPlanThreads + threadIdx.x;
+        if (i >= count) break;
+        if (!kSmall) {
+            wins = peek(status + i) == 0;
+            rank = peek(fresh + i);
         }
-        if (rank >= 0) {
-            const int page = peek(free_list + rank);
-            poke(fresh + i, page);
-            a.counts[page] = 1;
+        const bool enough = rank < found;
+        int page = -1;
+        if (wins && enough) {
+            if (rank >= 0) {
+                page = list.get(rank);
+                a.counts[page] = 1;
+            }
+            a.context[children[i]] = a.context[parents[i]];
         }
-        a.context[children[i]] = a.context[parents[i]];
+        fresh[i] = page;
+        status[i] = !wins ? 1 : enough ? 0 : 2;
     }
 }
 
@@ -298,62 +348,82 @@ __global__ __launch_bounds__(kCopyThreads) void fork_move_kernel(TableArgs a, Te
 
 /// The flat slot of token `at` of a table row; -1 where the row names no page.
 __device__ __forceinline__ int64_t slot_of(const TableArgs& a, int64_t sequence, int64_t at) {
-    const uint32_t page = a.tables[sequence * a.width + at / a.block];
-    return page < a.pages ? page * a.block + at % a.block : -1;
+    const uint32_t block = static_cast<uint32_t>(a.block);
+    const uint32_t token = static_cast<uint32_t>(at);  // below the capacity
+    const uint32_t page = a.tables[sequence * a.width + token / block];
+    return page < a.pages ? page * a.block + token % block : -1;
 }
 
 /// Extend, whole for one token a sequence (slots then holds count entries);
-/// else slots are left to extend_slots_kernel.
+/// else slots are left to extend_slots_kernel. kSmall: an entry a thread at
+/// most, and claims and free pages in LDS.
+template <bool kSmall>
 __global__ __launch_bounds__(kPlanThreads) void extend_kernel(TableArgs a, const int* sequences, int64_t count,
-                                                              int64_t tokens, int* claims, int64_t* ranks,
+                                                              int64_t tokens, int* claims_, int64_t* ranks,
                                                               int* free_list, int* status, int64_t* slots_out) {
-    __shared__ int64_t slots[kPlanWaves];
-    const int64_t rounds = (count + kPlanThreads - 1) / kPlanThreads;
-    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (within(sequences[i], a.sequences)) poke(claims + sequences[i], kUnclaimed);
-    }
-    phase();
-    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (within(sequences[i], a.sequences)) atomicMin(claims + sequences[i], static_cast<int>(i));
-    }
-    phase();
-    auto length_of = [&](int64_t i) { return static_cast<int64_t>(a.context[sequences[i]] > 0 ? a.context[sequences[i]] : 0); };
-    auto pages_of = [&](int64_t n) { return (n + a.block - 1) / a.block; };
-    int64_t wanted = 0;
+    using Ints = typename std::conditional<kSmall, InLds, InMemory>::type;
+    __shared__ int slots[kPlanWaves];
+    __shared__ int lds[kSmall ? kSmallRows + kPlanThreads : 1];
+    const Ints claims{kSmall ? lds : claims_};
+    const Ints list{kSmall ? lds + kSmallRows : free_list};
+    const int64_t rounds = kSmall ? 1 : (count + kPlanThreads - 1) / kPlanThreads;
     for (int64_t r = 0; r < rounds; ++r) {
         const int64_t i = r * kPlanThreads + threadIdx.x;
-        const bool wins = i < count && within(sequences[i], a.sequences) && peek(claims + sequences[i]) == i &&
-                          length_of(i) + tokens <= a.capacity;
-        const int64_t need = wins ? pages_of(length_of(i) + tokens) - pages_of(length_of(i)) : 0;
-        int64_t total;
-        const int64_t before = wanted + scan_before<kPlanWaves>(need, slots, total);
-        if (i < count) {
-            ranks[i] = before;  // read by this thread alone
+        if (i < count && within(sequences[i], a.sequences)) claims.put(sequences[i], kUnclaimed);
+    }
+    Ints::phase();
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t i = r * kPlanThreads + threadIdx.x;
+        if (i < count && within(sequences[i], a.sequences)) claims.lower(sequences[i], static_cast<int>(i));
+    }
+    Ints::phase();
+    auto length_of = [&](int64_t i) { return static_cast<int64_t>(a.context[sequences[i]] > 0 ? a.context[sequences[i]] : 0); };
+    // Lengths up to the capacity fit 31 bits, and the block 30.
+    const uint32_t block = static_cast<uint32_t>(a.block);
+    auto pages_of = [&](int64_t n) { return static_cast<int>((static_cast<uint32_t>(n) + block - 1) / block); };
+    int64_t wanted = 0;
+    int64_t rank = 0;
+    bool wins = false;
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t i = r * kPlanThreads + threadIdx.x;
+        wins = i < count && within(sequences[i], a.sequences) && claims.get(sequences[i]) == i &&
+               length_of(i) + tokens <= a.capacity;
+        const int need = wins ? pages_of(length_of(i) + tokens) - pages_of(length_of(i)) : 0;
+        int total;
+        rank = wanted + scan_before<kPlanWaves>(need, slots, total);
+        if (!kSmall && i < count) {
+            ranks[i] = rank;  // read by this thread alone
             poke(status + i, wins ? 0 : 1);
         }
         wanted += total;
     }
-    const int64_t found = find_free(a.counts, a.pages, wanted < a.pages ? wanted : a.pages, free_list, slots);
-    phase();
-    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        bool good = peek(status + i) == 0;
+    const int64_t found = find_free(a.counts, a.pages, wanted < a.pages ? wanted : a.pages, list, slots);
+    Ints::phase();
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t i = r * kPlanThreads + threadIdx.x;
+        if (i >= count) break;
+        if (!kSmall) {
+            wins = peek(status + i) == 0;
+            rank = ranks[i];
+        }
+        bool good = wins;
         int64_t length = 0;
         if (good) {
             length = length_of(i);
             const int64_t first = pages_of(length);
-            const int64_t need = pages_of(length + tokens) - first;
-            if (need > 0 && ranks[i] + need > found) {
+            const int need = pages_of(length + tokens) - static_cast<int>(first);
+            if (need > 0 && rank + need > found) {
                 good = false;
-                poke(status + i, 2);
             } else {
-                for (int64_t k = 0; k < need; ++k) {
-                    const int page = peek(free_list + ranks[i] + k);
+                for (int k = 0; k < need; ++k) {
+                    const int page = list.get(rank + k);
                     a.tables[sequences[i] * a.width + first + k] = static_cast<uint32_t>(page);
                     a.counts[page] = 1;
                 }
                 a.context[sequences[i]] = static_cast<int>(length + tokens);
             }
         }
+        status[i] = good ? 0 : wins ? 2 : 1;
         if (tokens == 1) slots_out[i] = good ? slot_of(a, sequences[i], length) : -1;
     }
 }
@@ -410,14 +480,14 @@ struct CompactArgs {
 };
 
 __global__ __launch_bounds__(kCopyThreads) void compact_count_kernel(CompactArgs a) {
-    __shared__ int64_t slots[kCopyThreads / kWaveSize];
+    __shared__ int slots[kCopyThreads / kWaveSize];
     const int64_t first = int64_t{blockIdx.x} * kTilePages + int64_t{threadIdx.x} * kCountsPerThread;
     int c[kCountsPerThread];
     load_counts(a.counts, a.pages, first, aligned16(a.counts), c);
     int live = 0;
 #pragma unroll
     for (int i = 0; i < kCountsPerThread; ++i) live += c[i] > 0 && first + i < a.pages ? 1 : 0;
-    int64_t total;
+    int total;
     scan_before<kCopyThreads / kWaveSize>(live, slots, total);
     if (threadIdx.x == 0) a.tile_live[blockIdx.x] = static_cast<int>(total);
 }
@@ -425,23 +495,23 @@ __global__ __launch_bounds__(kCopyThreads) void compact_count_kernel(CompactArgs
 /// Every workgroup: the lists' entries of one tile of pages.
 __global__ __launch_bounds__(kCopyThreads) void compact_list_kernel(CompactArgs a) {
     constexpr int kWaves = kCopyThreads / kWaveSize;
-    __shared__ int64_t slots[kWaves];
+    __shared__ int slots[kWaves];
     const int64_t tile = blockIdx.x;
     // Live pages in all, before this tile, and before the tile that the live
     // count falls into.
-    int64_t all = 0, before = 0;
+    int all = 0, before = 0;
     for (int64_t i = threadIdx.x; i < a.tiles; i += kCopyThreads) {
         all += a.tile_live[i];
         if (i < tile) before += a.tile_live[i];
     }
-    int64_t live, base, unused;
+    int live, base, unused;
     scan_before<kWaves>(all, slots, live);
     scan_before<kWaves>(before, slots, base);
     const bool aligned = aligned16(a.counts);
     int c[kCountsPerThread];
     // Live pages below the live count: what is not moved.
     const int64_t edge = live / kTilePages;
-    int64_t low = 0;
+    int low = 0;
     for (int64_t i = threadIdx.x; i < edge && i < a.tiles; i += kCopyThreads) low += a.tile_live[i];
     if (edge < a.tiles) {
         const int64_t first = edge * kTilePages + int64_t{threadIdx.x} * kCountsPerThread;
@@ -449,7 +519,7 @@ __global__ __launch_bounds__(kCopyThreads) void compact_list_kernel(CompactArgs 
 #pragma unroll
         for (int i = 0; i < kCountsPerThread; ++i) low += c[i] > 0 && first + i < live ? 1 : 0;
     }
-    int64_t kept;
+    int kept;
     scan_before<kWaves>(low, slots, kept);
     const int64_t first = tile * kTilePages + int64_t{threadIdx.x} * kCountsPerThread;
     load_counts(a.counts, a.pages, first, aligned, c);
@@ -607,7 +677,8 @@ cf_status cf_cache_copy(void* const* caches, int64_t num_caches, int64_t page_by
     CF_REQUIRE(most == 0 || count <= ((int64_t{1} << 31) - 1) / most / chunks, "%s: %lld pairs exceed the grid", who,
                static_cast<long long>(count));
     auto s = static_cast<hipStream_t>(stream);
-    cf::launch(cf::copy_plan_kernel, dim3(1), dim3(cf::kPlanThreads), 0, s, src, dst, count, num_pages,
+    const bool small = num_pages <= cf::kSmallRows;
+    cf::launch(small ? cf::copy_plan_kernel<true> : cf::copy_plan_kernel<false>, dim3(1), dim3(cf::kPlanThreads), 0, s, src, dst, count, num_pages,
                static_cast<int*>(workspace), status);
     if (num_caches > 0) {
         const int unit = cf::unit_of(caches, num_caches, page_bytes, page_bytes);
@@ -651,7 +722,8 @@ cf_status cf_cache_fork(void* const* caches, int64_t num_caches, int64_t page_by
     auto* fresh = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + cf::align_up(static_cast<size_t>(rows) * 4));
     auto* free_list = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(fresh) + cf::align_up(static_cast<size_t>(count) * 8));
     auto s = static_cast<hipStream_t>(stream);
-    cf::launch(cf::fork_plan_kernel, dim3(1), dim3(cf::kPlanThreads), 0, s, a, parents, children, count, claims, fresh,
+    const bool small = count <= cf::kPlanThreads && num_sequences <= cf::kSmallRows;
+    cf::launch(small ? cf::fork_plan_kernel<true> : cf::fork_plan_kernel<false>, dim3(1), dim3(cf::kPlanThreads), 0, s, a, parents, children, count, claims, fresh,
                free_list, status);
     const int unit = num_caches > 0 ? cf::unit_of(caches, num_caches, page_bytes, page_bytes / block_size) : 16;
     cf::by_tensors(caches, num_caches, [&](const cf::Tensors& t, int n, bool first) {
@@ -690,7 +762,9 @@ cf_status cf_cache_extend(int32_t* ref_counts, uint32_t* block_tables, int32_t* 
     at += cf::align_up(static_cast<size_t>(count) * 8);
     auto* free_list = reinterpret_cast<int*>(at);
     auto s = static_cast<hipStream_t>(stream);
-    cf::launch(cf::extend_kernel, dim3(1), dim3(cf::kPlanThreads), 0, s, a, sequences, count, tokens, claims, ranks,
+    const bool small = num_sequences <= cf::kSmallRows &&
+                       count * cf::ceil_div<int64_t>(tokens, block_size) <= cf::kPlanThreads;  // pages wanted
+    cf::launch(small ? cf::extend_kernel<true> : cf::extend_kernel<false>, dim3(1), dim3(cf::kPlanThreads), 0, s, a, sequences, count, tokens, claims, ranks,
                free_list, status, slots);
     if (tokens > 1) {
         cf::launch(cf::extend_slots_kernel,

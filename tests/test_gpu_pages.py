@@ -203,3 +203,24 @@ def test_another_stream_and_a_replayed_graph():
         torch.cuda.synchronize()
         same(out, eager)
         same(state_, after)
+
+
+@pytest.mark.parametrize("count", [1023, 1024, 1025, 4000])
+@pytest.mark.parametrize("rows", [8192, 8193])
+def test_lists_and_tables_on_both_sides_of_what_a_plan_keeps_to_itself(count, rows):
+    """Plans of up to 1024 pages over up to 8192 rows (or a copy's pages) work
+    in LDS, longer ones in memory."""
+    gen = torch.Generator().manual_seed(count)
+    lengths = [int(n) for n in random_rows(gen, 300, 1, 12)] + [0] * (rows - 300)
+    caches, counts, tables, context = state(lengths, 4, 3, rows, shape=(1, 2))
+    parents = random_rows(gen, count, 0, 301)
+    children = random_rows(gen, count, 299, rows + 1)
+    children[:20] = rows - 1  # the same row again and again, the last one
+    both(cf.cache_fork, plain._fork_reference, [caches, counts, tables, context, parents, children])
+    sequences = random_rows(gen, count, -1, rows + 1)
+    sequences[5:9] = rows - 1
+    for tokens in (1, 4, 5):
+        both(cf.cache_extend, plain._extend_reference, [counts, tables, context, sequences], (4, tokens))
+    src, dst = random_rows(gen, count, 0, rows), random_rows(gen, count, 0, rows)
+    dst[3] = src[7] = rows - 1
+    both(cf.cache_copy, plain._copy_reference, [caches, src, dst])
