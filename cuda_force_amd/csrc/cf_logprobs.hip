@@ -28,12 +28,12 @@
 //     teams' (otherwise k larger ones exist), so only those k teams' vectors
 //     (k / 64 of the chunk) are read again, from L2, and filtered by the k-th
 //     best team's logit. Teams of four against single threads: 64 keys to rank
-//     and not 256 (5 of 131072, 600 rows in fp16: 41 -> 39 us, with the batches below);
+//     and not 256 (5 of 131072, 600 rows in fp16: 41 -> 38 us, with the batches below);
 //     a row of equal logits leaves more keys, which are sieved twice.
 //   * Measured: 4096 rows of 32000 bf16 logits (262 MB) with entropy 47 us, 5.6
 //     TB/s, from memory that nothing has written to before; 79 us straight after a
 //     kernel that wrote as much, whose lines are then written back meanwhile.
-//     1001 rows of 32000 floats (128 MB) 24 us, 5.3 TB/s. A batch of four vectors with one
+//     1001 rows of 32000 floats (128 MB) 23.4 us, 5.5 TB/s. A batch of four vectors with one
 //     maximum and the next on its way, against a vector at a time: 27 -> 24 us.
 //     Few rows are bound by the chain of steps behind the loads: 8 rows of
 //     50257 with 20 tokens 7.3 us, and 5.8 us to join them.
@@ -785,11 +785,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(GradArgs a) {
     }
 }
 
-/// Chunks per row: about four workgroups a CU where there are few rows, but no
-/// chunk under a vector a thread, and none above 128 vectors a thread.
+/// Chunks per row: about eight workgroups a CU where there are few rows, but no
+/// chunk under a vector a thread, and none above 128 vectors a thread. (Four a
+/// CU: 600 rows of 131072 in fp16 39.4 -> 38.2 us, 1001 of 32000 floats 24.4 -> 23.4;
+/// sixteen 44.4 and 24.4 us.)
 int chunks_of(int64_t rows, int64_t vocab, size_t size) {
     const int64_t vectors = ceil_div<int64_t>(vocab * static_cast<int64_t>(size), 16);
-    const int64_t wanted = ceil_div<int64_t>(1024, rows);
+    const int64_t many = ceil_div<int64_t>(2048, rows);
+    const int64_t wanted = many < kCandidates ? many : kCandidates;  // the joining kernel holds a key of each
     const int64_t most = ceil_div<int64_t>(vectors, kThreads);
     const int64_t least = ceil_div<int64_t>(vectors, 128 * kThreads);
     int64_t chunks = wanted < most ? wanted : most;

@@ -332,3 +332,10 @@ def test_forward_and_backward_captured_and_replayed():
         torch.cuda.synchronize()
         for got, want in zip(results, step(logits.clone().requires_grad_())):
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3])
+def test_as_many_chunks_as_a_row_can_have(rows):
+    vocab = (1 << 22) + 3
+    logits = torch.randn(rows, vocab, device="cuda", dtype=torch.bfloat16)
+    check(logits, torch.full((rows,), vocab - 1, device="cuda"), 1.0, 64)
