@@ -31,7 +31,8 @@
 //   * 16-bit caches run 32 x 32 x 16 MFMA over 32 rows and 32 tokens, fp32
 //     caches 16 x 16 x 4 fp32 MFMA over 16 rows and 16 tokens (fp32 products).
 //     Probabilities are rounded to the cache's type for the second product
-//     (relative error half an ulp each, of either sign); sums stay in fp32.
+//     (relative error half an ulp each, of either sign; for fp16's smallest
+//     numbers see kLift); sums stay in fp32.
 //   * Measured, 32 query and 8 KV heads of 128 in bf16, with the join: 128
 //     sequences behind 32768 tokens 98 + 9.5 us, 704 TFLOP/s: neither the matrix
 //     cores (31% busy) nor the vector units (34%), but the chain from one product
@@ -279,6 +280,16 @@ struct Tile {
     static constexpr int kScores = kRows * kTokens / kWaveSize;   // scores per lane
     static constexpr int kAcc = kRows * kD / kWaveSize;           // output values per lane
     static constexpr int kOutPitch = kD + 4;                      // floats per row of the output area
+    /// A row's maximum may lag the true one by up to kLag (base 2): sums and
+    /// outputs are rescaled only when it would lag more. Probabilities, and with
+    /// them weighted values and sums, are kept 2^kLift times as large: fp16
+    /// holds them up to 2^15, so one is a full number down to 2^-27 of the row's
+    /// largest, and off by at most 2^-38 of that below (kept at most 1, one
+    /// below 2^-25 was 0: 32767 tokens 17.5 nats behind a leading one without
+    /// a value gave 0 for 8.2e-4). A lag of 2 against 8 costs nothing, none at
+    /// all 5% (128 sequences behind 32768 tokens in fp16: 125, 125 and 131 us).
+    static constexpr float kLag = std::is_same<T, f16_t>::value ? 2.0f : 8.0f;
+    static constexpr float kLift = std::is_same<T, f16_t>::value ? 13.0f : 0.0f;
 
     /// Order of the 16-byte pieces of a K row: a fragment read takes the same
     /// piece of 16 rows.
@@ -574,17 +585,14 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             }
         }
     };
-    // Scores to probabilities, and the running values. m may lag the true
-    // maximum by up to kLag (base 2): sums and outputs are rescaled only when it
-    // would lag more (fp32 holds the factor, and so does fp16: 2^8 at most).
-    constexpr float kLag = 8.0f;
+    // Scores to probabilities, and the running values.
     auto soften = [&](typename L::Score& s) {
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < L::kScores; ++i) top = fmaxf(top, s[i]);
         top = groups_max<L::kRows>(top);
         const float m_new = fmaxf(m, top * a.c);
-        if (__builtin_amdgcn_ballot_w64(m_new > m + kLag) != 0) {
+        if (__builtin_amdgcn_ballot_w64(m_new > m + L::kLag) != 0) {
             const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
             l *= f;
 #pragma unroll
@@ -594,7 +602,7 @@ __device__ void attend(const SharedArgs& a, const Item& w, uint8_t* lds, float (
             }
             m = m_new;
         }
-        const float shift = m == -INFINITY ? 0.0f : m;
+        const float shift = (m == -INFINITY ? 0.0f : m) - L::kLift;
 #pragma unroll
         for (int i = 0; i < L::kScores; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -shift));

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import cuda_force_amd as cf
-from tests.shared_util import build, check
+from tests.shared_util import build, check, reference
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -188,3 +188,31 @@ def test_another_stream_and_a_replayed_graph():
         torch.cuda.synchronize()
         check(out, c)
         assert torch.equal(out, cf.paged_attention_shared(*args)), step
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [8.0, 12.0, 14.0, 16.0, 17.5, 18.0, 25.0])
+@pytest.mark.parametrize("prefix", [0, 5000])
+def test_a_leading_key_without_a_value(dtype, nats, prefix):
+    """One key leads all others by so much that these hold little weight, and
+    the result is theirs alone."""
+    c = build([(prefix, [5000, 4000 + prefix, 5001 + prefix])], 4, 2, 64, 16, dtype, fill=0.0)
+    c.query[:] = 0
+    c.query[..., :2] = 1.0
+    c.k[..., 0] = 0
+    c.v[:] = (c.v.float().abs() / 4 + 0.5).to(dtype)  # nothing cancels
+    for s in range(3):
+        page = int(c.tables[s, 0])
+        c.k[page, 0, :, 0], c.k[page, 0, :, 1], c.v[page, 0] = 8 * nats, 0.0, 0.0
+    got = cf.paged_attention_shared(*c.args()).cpu().double()
+    ref, size = reference(c)
+    # As shared_util.check; and fp16 probabilities below 2^-14 of the 2^13 that
+    # stand for the largest are off by half of 2^-24, whatever their size.
+    half = torch.finfo(dtype).eps / 2
+    f32 = 2.0**-16 + 2.0**-24 * float(c.context.max()) / 32
+    tolerance = (f32 + (half if dtype != torch.float32 else 0.0)) * size + half * ref.abs()
+    if dtype == torch.float16:
+        tolerance += 2.0**-25  # the result's own smallest step, halved
+        tolerance += 2.0**-38 * c.context.double()[:, None, None] * c.v.double().abs().max()
+    worst = ((got - ref).abs() - tolerance).max().item()
+    assert worst <= 0, worst
