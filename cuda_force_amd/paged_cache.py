@@ -412,8 +412,11 @@ def cache_extend(
     ``cache.view(-1, kv_heads, head_dim)``. They are -1 for an entry left out: a
     row out of range or named before, one whose table would overflow, or one for
     which not all pages were free (nor then for a later entry that needs one).
-    The last page of a row must be its own (``cache_fork`` sees to that): the new
-    tokens go there. Not in the reference's API.
+    An index of -1 is the last token of the cache, in whosever page that lies:
+    send such tokens elsewhere before storing through the slots, for instance
+    ``slots.clamp(min=0)`` to a page 0 whose count the program set to 1 before
+    it stored anything. The last page of a row must be its own (``cache_fork``
+    sees to that): the new tokens go there. Not in the reference's API.
 
     Raises:
         ValueError: for shapes, devices or layouts that do not match, or sizes

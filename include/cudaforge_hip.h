@@ -580,7 +580,8 @@ cf_status cf_cache_fork(void* const* caches, int64_t num_caches, int64_t page_by
  * tokens go, page * block_size + offset; all -1 for an entry left out: a row out
  * of range, named by an earlier entry, or whose table would overflow, or for
  * which not all pages were free (nor then for any later entry that needs one).
- * Slots in a last page that the table names wrongly are -1 alone. Needs
+ * Slots in a last page that the table names wrongly are -1 alone. Nothing may be
+ * stored through a slot of -1. Needs
  * cf_cache_workspace_bytes(num_pages, num_sequences, count). It has no
  * counterpart in the reference. */
 cf_status cf_cache_extend(int32_t* ref_counts, uint32_t* block_tables, int32_t* context_lens,

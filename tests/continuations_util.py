@@ -133,3 +133,37 @@ def run(device, dtype, step=None):
         r.check(*make())
     r.release(1, *CHILDREN)
     assert (r.counts == 0).all() and (r.context == 0).all()
+
+
+def step_without_pages(device, make=None):
+    """Three sequences take a step of which one finds no free page: its token
+    goes to page 0, which no sequence has, and nothing else is touched. `make`:
+    how the step is called."""
+    pages, block, kv_heads, dim = 6, 4, 2, 8
+    gen = torch.Generator().manual_seed(5)
+    caches = [torch.randn(pages, block, kv_heads, dim, generator=gen).to(device) for _ in range(2)]
+    counts, context = (torch.zeros(n, dtype=torch.int32, device=device) for n in (pages, 3))
+    tables = torch.zeros(3, 3, dtype=torch.int32, device=device)
+    rows = torch.arange(3, dtype=torch.int32, device=device)
+    counts[0] = 1
+    for row, length in enumerate((7, 4, 8)):
+        assert (cf.cache_extend(counts, tables, context, rows[row : row + 1], block, length) > 0).all()
+    assert (counts == 1).all()
+    new = torch.randn(3, kv_heads, dim, generator=gen).to(device)
+
+    def step():
+        slots = cf.cache_extend(counts, tables, context, rows, block)[:, 0]
+        for cache in caches:
+            cache.view(-1, kv_heads, dim)[slots.clamp(min=0)] = new
+        return slots
+
+    before = [[t.clone() for t in (counts, tables, context)], [c.clone() for c in caches]]
+    slots = (step if make is None else make(step, [counts, tables, context, *caches]))()
+    own = int(tables[0, 1]) * block + 3
+    assert slots.tolist() == [own, -1, -1] and context.tolist() == [8, 4, 8]
+    assert torch.equal(counts, before[0][0]) and torch.equal(tables, before[0][1])
+    for cache, was in zip(caches, before[1]):
+        now, was = cache.view(-1, kv_heads, dim), was.view(-1, kv_heads, dim)
+        assert torch.equal(now[own], new[0])
+        rest = [i for i in range(block, pages * block) if i != own]
+        assert torch.equal(now[rest], was[rest])

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.continuations_util import run
+from tests.continuations_util import run, step_without_pages
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,30 @@ def test_a_captured_step_between_forks_and_a_compaction():
         return replay
 
     run("cuda", torch.bfloat16, captured)
+
+
+def test_a_step_that_finds_no_page_leaves_the_others_alone():
+    step_without_pages("cuda")
+
+    def captured(step, state):
+        kept = [t.clone() for t in state]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            slots = step()
+
+        def replay():
+            for _ in range(3):
+                for t, was in zip(state, kept):
+                    t.copy_(was)
+                graph.replay()
+                torch.cuda.synchronize()
+            return slots
+
+        return replay
+
+    step_without_pages("cuda", captured)
