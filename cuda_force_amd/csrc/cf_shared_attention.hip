@@ -46,6 +46,7 @@
 
 #include "cf_common.hpp"
 #include "cf_lds_dma.hpp"
+#include "cf_ranges.hpp"
 
 namespace cf {
 namespace {
@@ -133,15 +134,6 @@ __device__ Group group_of(const SharedArgs& a, int s) {
 
 __device__ __forceinline__ int context_of(const SharedArgs& a, int s) { return clamp_to(a.context[s], a.capacity); }
 
-/// Tokens of each of at most `splits` ranges of `length` tokens: whole steps,
-/// and about `least` or more (a range has fixed costs, its piece of the result
-/// among them).
-__device__ __forceinline__ int split_length(int length, int splits, int step, int least) {
-    const int wanted = min(splits, max(1, (length + least - 1) / least));
-    const int each = (length + wanted - 1) / wanted;
-    return (each + step - 1) / step * step;
-}
-
 /// One XCD's share of the prefixes' work: a group, its row tile, and the place
 /// of a (range, KV head) pair in the XCD's run of them.
 struct PrefixItem {
@@ -176,7 +168,7 @@ __device__ PrefixItem prefix_item(const SharedArgs& a, int rows, int step, int l
         end = there ? max(start, end) : start;
         const int tiles = prefix > 0 ? ((end - start) * a.per + rows - 1) / rows : 0;
         const int each = split_length(max(prefix, 1), a.prefix_splits, step, least);
-        const int run = ((prefix + each - 1) / each * a.kv_heads + 7) / 8;
+        const int run = (range_count(prefix, each) * a.kv_heads + 7) / 8;
         const int items = tiles * run;
         int total = items;
         if (a.groups > 1) {
@@ -820,8 +812,9 @@ __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void shared_attention_
         const int pair = id % 8 * p.run + p.place;
         const int split = pair / a.kv_heads;
         w.kv_head = pair % a.kv_heads;
-        w.lo = split * p.each;
-        w.hi = min(g.prefix, w.lo + p.each);
+        const Range range = range_of(0, g.prefix, p.each, split);
+        w.lo = range.lo;
+        w.hi = range.hi;
         if (w.lo >= w.hi) return;
         // The pages of the first sequence that holds the whole prefix.
         int holder = -1;
@@ -860,8 +853,9 @@ __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void shared_attention_
         const Group g = a.groups > 0 ? group_of(a, s) : Group{0, 0, 0};
         const int first = g.end > 0 && g.prefix <= context ? g.prefix : 0;
         const int each = split_length(context - first, a.rest_splits, a.rest_step, a.rest_least);
-        w.lo = first + split * each;
-        w.hi = min(context, w.lo + each);
+        const Range range = range_of(first, context - first, each, split);
+        w.lo = range.lo;
+        w.hi = range.hi;
         if (w.lo >= w.hi) return;
         w.table = a.tables + static_cast<int64_t>(s) * a.max_blocks;
         w.last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
@@ -891,8 +885,9 @@ __global__ __launch_bounds__(kThreads) void shared_attention_any_kernel(SharedAr
     const int s = static_cast<int>(out_row / a.heads);
     const int context = context_of(a, s);
     const int each = split_length(context, a.rest_splits, a.rest_step, a.rest_least);
-    const int lo = split * each;
-    const int hi = min(context, lo + each);
+    const Range range = range_of(0, context, each, split);
+    const int lo = range.lo;
+    const int hi = range.hi;
     if (lo >= hi) return;
     const T* q = static_cast<const T*>(a.query) + out_row * a.head_dim;
     float qv[kPer];
@@ -961,13 +956,13 @@ __global__ __launch_bounds__(kThreads) void shared_attention_join_kernel(SharedA
         if (g.end > 0 && g.prefix <= context && g.prefix > 0) {
             first = g.prefix;
             const int each = split_length(first, a.prefix_splits, a.prefix_step, a.prefix_least);
-            prefix_pieces = (first + each - 1) / each;
+            prefix_pieces = range_count(first, each);
         }
     }
     int rest_pieces = 0;
     if (context > first) {
         const int each = split_length(context - first, a.rest_splits, a.rest_step, a.rest_least);
-        rest_pieces = (context - first + each - 1) / each;
+        rest_pieces = range_count(context - first, each);
     }
     const int pieces = prefix_pieces + rest_pieces;
     auto slot_of = [&](int i) { return i < prefix_pieces ? i : a.prefix_splits + i - prefix_pieces; };
@@ -1109,8 +1104,7 @@ Plan plan_of(cf_dtype dtype, int64_t sequences, int64_t groups, int64_t heads, i
 }
 
 int64_t capacity_of(int64_t max_blocks, int64_t block_size) {
-    const int64_t most = (int64_t{1} << 31) - 4096;  // token positions and the steps behind them stay in 32 bits
-    return max_blocks > most / block_size ? most : max_blocks * block_size;
+    return max_blocks > kMostTokens / block_size ? kMostTokens : max_blocks * block_size;
 }
 
 size_t workspace_of(const Plan& p, int64_t sequences, int64_t heads, int64_t head_dim) {
@@ -1215,7 +1209,7 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
                    cf::host_aligned(out, size),
                "%s: misaligned pointer", who);
     // Cache rows, token positions and work items are counted in 32 bits.
-    constexpr int64_t kMost = (int64_t{1} << 31) - 4096;
+    constexpr int64_t kMost = cf::kMostTokens;
     CF_REQUIRE(num_pages <= kMost / block_size && max_blocks_per_sequence <= kMost && num_kv_heads <= (1 << 14) && num_groups <= (1 << 20) &&
                    num_sequences <= kMost / num_heads,
                "%s: %lld pages of %lld tokens, %lld sequences of %lld heads, %lld KV heads or %lld groups exceed 32-bit counts", who,

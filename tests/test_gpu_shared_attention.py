@@ -216,3 +216,28 @@ def test_a_leading_key_without_a_value(dtype, nats, prefix):
         tolerance += 2.0**-38 * c.context.double()[:, None, None] * c.v.double().abs().max()
     worst = ((got - ref).abs() - tolerance).max().item()
     assert worst <= 0, worst
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+def test_lengths_at_the_end_of_32_bits(grouped):
+    """Contexts of 2^31 - 4096 tokens, the most there are, of which the table
+    names the first and the last block alone."""
+    most, block, dim = 2**31 - 4096, 1 << 16, 64
+    gen = torch.Generator().manual_seed(0)
+    query = torch.randn(3, 2, dim, generator=gen).bfloat16()
+    k, v = (torch.randn(2, block, 1, dim, generator=gen).bfloat16() for _ in range(2))
+    tables = torch.full((3, 1 << 15), -1, dtype=torch.int32)
+    tables[:, 0], tables[:, -1] = 1, 0
+    lengths = [most, 2**31 - 1, 70000]
+    starts, prefix = ([0, 3], [most - 1]) if grouped else ([0], [])
+    args = [t.cuda() for t in (query, k, v, torch.tensor(starts, dtype=torch.int32),
+                               torch.tensor(prefix, dtype=torch.int32), tables, torch.tensor(lengths, dtype=torch.int32))]
+    got = cf.paged_attention_shared(*args).cpu().double()
+    half = torch.finfo(torch.bfloat16).eps / 2
+    for s, last in enumerate((block - 4096, block - 4096, 0)):
+        keys, values = (torch.cat([x[1, :, 0], x[0, :last, 0]]).double() for x in (k, v))
+        p = torch.softmax(query[s].double() @ keys.T * dim**-0.5, -1)
+        ref, size = p @ values, p @ values.abs()
+        # As shared_util.check, with the tokens that the table names.
+        tolerance = (2.0**-16 + 2.0**-24 * len(keys) / 32 + half) * size + half * ref.abs()
+        assert ((got[s] - ref).abs() <= tolerance).all()
