@@ -42,6 +42,10 @@ inline constexpr int kQuantBlockSize = 64;
 /// of a CU.
 inline constexpr int kDefaultBlockSize = 256;
 
+/// Most workgroups of kDefaultBlockSize threads in one launch: its threads are
+/// counted in 32 bits.
+inline constexpr int64_t kMaxWorkgroups = (int64_t{1} << 24) - 1;
+
 /// Largest workgroup HIP permits on gfx950.
 inline constexpr int kMaxBlockSize = 1024;
 

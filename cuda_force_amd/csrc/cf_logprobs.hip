@@ -818,31 +818,65 @@ cf_status validate(const char* who, const void* logits, cf_dtype dtype, int64_t 
                static_cast<long long>(token_count), kTokensMax);
     CF_REQUIRE(scale > 0.0f && scale * kLog2e < 1.0e30f, "%s: scale must be positive and finite", who);
     CF_REQUIRE(host_aligned(logits, dtype_size(dtype)) && host_aligned(tokens, 8), "%s: misaligned pointer", who);
-    CF_REQUIRE(rows * chunks_of(rows, vocab, dtype_size(dtype)) < (1LL << 31), "%s: %lld rows exceed the grid", who,
+    CF_REQUIRE(rows * chunks_of(rows, vocab, dtype_size(dtype)) < (1LL << 31), "%s: %lld rows are too many", who,
                static_cast<long long>(rows));
     return CF_OK;
 }
 
+/// p + n, or null.
+template <typename P>
+P* at(P* p, int64_t n) {
+    return p == nullptr ? nullptr : p + n;
+}
+
+/// As many rows a launch as it takes workgroups.
 template <typename T>
-void run_forward(const RowArgs& a, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(a.rows * a.chunks));
-    const dim3 block(kThreads);
-    const bool entropy = a.entropy != nullptr;
-    if (a.top > 0) {
-        launch(entropy ? logprobs_kernel<T, true, true> : logprobs_kernel<T, false, true>, grid, block, 0, stream, a);
-    } else {
-        launch(entropy ? logprobs_kernel<T, true, false> : logprobs_kernel<T, false, false>, grid, block, 0, stream, a);
-    }
-    if (a.chunks > 1) {
-        launch(logprobs_join_kernel<T>, dim3(static_cast<unsigned>(a.rows)), block, 0, stream, a);
+void run_forward(const RowArgs& all, hipStream_t stream) {
+    const int64_t most = kMaxWorkgroups / all.chunks;
+    for (int64_t row = 0; row < all.rows; row += most) {
+        RowArgs a = all;
+        a.rows = all.rows - row < most ? all.rows - row : most;
+        a.logits = static_cast<const T*>(all.logits) + row * all.stride;
+        a.tokens = all.tokens + row * all.count;
+        a.logprobs = all.logprobs + row * all.count;
+        a.stats = at(all.stats, 2 * row);
+        a.entropy = at(all.entropy, row);
+        a.top_logprobs = at(all.top_logprobs, row * all.top);
+        a.top_tokens = at(all.top_tokens, row * all.top);
+        a.partial = at(all.partial, 4 * row * all.chunks);
+        a.keys = at(all.keys, row * all.chunks * all.top);
+        const dim3 grid(static_cast<unsigned>(a.rows * a.chunks));
+        const dim3 block(kThreads);
+        const bool entropy = a.entropy != nullptr;
+        if (a.top > 0) {
+            launch(entropy ? logprobs_kernel<T, true, true> : logprobs_kernel<T, false, true>, grid, block, 0, stream,
+                   a);
+        } else {
+            launch(entropy ? logprobs_kernel<T, true, false> : logprobs_kernel<T, false, false>, grid, block, 0,
+                   stream, a);
+        }
+        if (a.chunks > 1) {
+            launch(logprobs_join_kernel<T>, dim3(static_cast<unsigned>(a.rows)), block, 0, stream, a);
+        }
     }
 }
 
 template <typename T>
-void run_backward(const GradArgs& a, int64_t rows, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(rows * a.chunks));
-    launch(a.grad_entropy != nullptr ? logprobs_grad_kernel<T, true> : logprobs_grad_kernel<T, false>, grid,
-           dim3(kThreads), 0, stream, a);
+void run_backward(const GradArgs& all, int64_t rows, hipStream_t stream) {
+    const int64_t most = kMaxWorkgroups / all.chunks;
+    for (int64_t row = 0; row < rows; row += most) {
+        GradArgs a = all;
+        a.logits = static_cast<const T*>(all.logits) + row * all.stride;
+        a.tokens = all.tokens + row * all.count;
+        a.stats = all.stats + 2 * row;
+        a.entropy = at(all.entropy, row);
+        a.grad_logprobs = at(all.grad_logprobs, row * all.count);
+        a.grad_entropy = at(all.grad_entropy, row);
+        a.grad = static_cast<T*>(all.grad) + row * all.grad_stride;
+        const dim3 grid(static_cast<unsigned>((rows - row < most ? rows - row : most) * a.chunks));
+        launch(a.grad_entropy != nullptr ? logprobs_grad_kernel<T, true> : logprobs_grad_kernel<T, false>, grid,
+               dim3(kThreads), 0, stream, a);
+    }
 }
 
 }  // namespace

@@ -639,6 +639,21 @@ void by_tensors(void* const* caches, int64_t tensors, Body body) {
     }
 }
 
+/// Runs `body` with entries [first, first + n) of a list of `count`, each of
+/// which takes `each` workgroups, in launches of no more than there may be; a
+/// single entry's have to fit.
+bool one_entry_fits(int64_t tensors, int64_t chunks) {
+    return (tensors < kTensors ? tensors : kTensors) * chunks + 1 <= kMaxWorkgroups;
+}
+
+template <typename Body>
+void by_entries(int64_t count, int64_t each, Body body) {
+    const int64_t most = kMaxWorkgroups / each;
+    for (int64_t first = 0; first < count; first += most) {
+        body(first, count - first < most ? count - first : most);
+    }
+}
+
 }  // namespace
 }  // namespace cf
 
@@ -673,9 +688,8 @@ cf_status cf_cache_copy(void* const* caches, int64_t num_caches, int64_t page_by
     CF_REQUIRE(workspace != nullptr && workspace_bytes >= needed && cf::host_aligned(workspace, 16),
                "%s: needs %zu bytes of 16-byte aligned workspace", who, needed);
     const int64_t chunks = cf::ceil_div<int64_t>(page_bytes, cf::kChunkBytes);
-    const int64_t most = num_caches < cf::kTensors ? num_caches : cf::kTensors;
-    CF_REQUIRE(most == 0 || count <= ((int64_t{1} << 31) - 1) / most / chunks, "%s: %lld pairs exceed the grid", who,
-               static_cast<long long>(count));
+    CF_REQUIRE(cf::one_entry_fits(num_caches, chunks), "%s: pages of %lld bytes", who,
+               static_cast<long long>(page_bytes));
     auto s = static_cast<hipStream_t>(stream);
     const bool small = num_pages <= cf::kSmallRows;
     cf::launch(small ? cf::copy_plan_kernel<true> : cf::copy_plan_kernel<false>, dim3(1), dim3(cf::kPlanThreads), 0, s, src, dst, count, num_pages,
@@ -685,8 +699,10 @@ cf_status cf_cache_copy(void* const* caches, int64_t num_caches, int64_t page_by
         cf::by_tensors(caches, num_caches, [&](const cf::Tensors& t, int n, bool) {
             auto* kernel = unit == 16 ? cf::copy_pages_kernel<16>
                            : unit == 4 ? cf::copy_pages_kernel<4> : cf::copy_pages_kernel<1>;
-            cf::launch(kernel, dim3(static_cast<unsigned>(count * n * chunks)), dim3(cf::kCopyThreads), 0, s, t, n,
-                       page_bytes, chunks, src, dst, static_cast<const int*>(status));
+            cf::by_entries(count, n * chunks, [&](int64_t at, int64_t pairs) {
+                cf::launch(kernel, dim3(static_cast<unsigned>(pairs * n * chunks)), dim3(cf::kCopyThreads), 0, s, t, n,
+                           page_bytes, chunks, src + at, dst + at, static_cast<const int*>(status + at));
+            });
         });
     }
     return cf::check_launch("launching the page copies", s);
@@ -714,9 +730,8 @@ cf_status cf_cache_fork(void* const* caches, int64_t num_caches, int64_t page_by
     CF_REQUIRE(workspace != nullptr && workspace_bytes >= needed && cf::host_aligned(workspace, 16),
                "%s: needs %zu bytes of 16-byte aligned workspace", who, needed);
     const int64_t chunks = num_caches > 0 ? cf::ceil_div<int64_t>(page_bytes, cf::kChunkBytes) : 1;
-    const int64_t most = num_caches < cf::kTensors ? num_caches : cf::kTensors;
-    CF_REQUIRE(count <= ((int64_t{1} << 31) - 1) / (most * chunks + 1), "%s: %lld pairs exceed the grid", who,
-               static_cast<long long>(count));
+    CF_REQUIRE(cf::one_entry_fits(num_caches, chunks), "%s: pages of %lld bytes", who,
+               static_cast<long long>(page_bytes));
     auto* claims = static_cast<int*>(workspace);
     const int64_t rows = num_pages > num_sequences ? num_pages : num_sequences;
     auto* fresh = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + cf::align_up(static_cast<size_t>(rows) * 4));
@@ -729,9 +744,12 @@ cf_status cf_cache_fork(void* const* caches, int64_t num_caches, int64_t page_by
     cf::by_tensors(caches, num_caches, [&](const cf::Tensors& t, int n, bool first) {
         auto* kernel = unit == 16 ? cf::fork_move_kernel<16>
                        : unit == 4 ? cf::fork_move_kernel<4> : cf::fork_move_kernel<1>;
-        cf::launch(kernel, dim3(static_cast<unsigned>(count * (n * chunks + (first ? 1 : 0)))), dim3(cf::kCopyThreads),
-                   0, s, a, t, n, page_bytes, chunks, first, parents, children, static_cast<const int*>(fresh),
-                   static_cast<const int*>(status));
+        const int64_t pieces = n * chunks + (first ? 1 : 0);
+        cf::by_entries(count, pieces, [&](int64_t at, int64_t pairs) {
+            cf::launch(kernel, dim3(static_cast<unsigned>(pairs * pieces)), dim3(cf::kCopyThreads), 0, s, a, t, n,
+                       page_bytes, chunks, first, parents + at, children + at, static_cast<const int*>(fresh + at),
+                       static_cast<const int*>(status + at));
+        });
     });
     return cf::check_launch("launching the fork", s);
 }
@@ -787,7 +805,10 @@ cf_status cf_cache_release(int32_t* ref_counts, uint32_t* block_tables, int32_t*
     CF_REQUIRE(sequences != nullptr, "%s: null pointer", who);
     CF_REQUIRE(count <= cf::kMostInts, "%s: %lld sequences", who, static_cast<long long>(count));
     auto s = static_cast<hipStream_t>(stream);
-    cf::launch(cf::release_kernel, dim3(static_cast<unsigned>(count)), dim3(cf::kCopyThreads), 0, s, a, sequences);
+    cf::by_entries(count, 1, [&](int64_t at, int64_t rows) {
+        cf::launch(cf::release_kernel, dim3(static_cast<unsigned>(rows)), dim3(cf::kCopyThreads), 0, s, a,
+                   sequences + at);
+    });
     return cf::check_launch("launching the release", s);
 }
 

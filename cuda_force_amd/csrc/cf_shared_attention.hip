@@ -1119,6 +1119,9 @@ bool sizes_ok(int64_t sequences, int64_t groups, int64_t heads, int64_t kv_heads
            block_size > 0 && max_blocks > 0 && heads % kv_heads == 0;
 }
 
+/// A wave per row from a round of the GPU's waves on (2048 rows: 9.4 -> 6.5 us).
+bool join_by_wave(int64_t rows, int64_t head_dim) { return rows >= 1024 && head_dim <= 256; }
+
 template <typename T, int kD>
 void run_matrix(const SharedArgs& a, const Plan& p, dim3 grid, hipStream_t stream) {
     if (p.row_waves == 4) {
@@ -1151,8 +1154,7 @@ void run(const SharedArgs& a, const Plan& p, hipStream_t stream) {
             run_matrix<T, 256>(a, p, grid, stream);
         }
     }
-    // A wave per row from a round of the GPU's waves on (2048 rows: 9.4 -> 6.5 us).
-    const bool one_wave = rows >= 1024 && a.head_dim <= 256;
+    const bool one_wave = join_by_wave(rows, a.head_dim);
     auto* join = one_wave ? (a.head_dim <= 64    ? shared_attention_join_kernel<T, 64, 1>
                              : a.head_dim <= 128 ? shared_attention_join_kernel<T, 128, 1>
                                                  : shared_attention_join_kernel<T, 256, 1>)
@@ -1263,6 +1265,17 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
     const int64_t rest_items = num_sequences * num_kv_heads * (p.rest_tiles > 0 ? p.rest_tiles : 1) * p.rest_splits;
     CF_REQUIRE(prefix_items + rest_items < kMost && num_sequences * num_heads * p.rest_splits < kMost,
                "%s: too many work items", who);
+    const int64_t rows_in_all = num_sequences * num_heads;
+    const int64_t workgroups =
+        p.dim == 0 ? cf::ceil_div<int64_t>(rows_in_all * p.rest_splits, cf::kWaves)
+                   : prefix_items + (p.rest_solo ? cf::ceil_div<int64_t>(rest_items / p.rest_splits, cf::kWaves) *
+                                                       p.rest_splits
+                                                 : rest_items);
+    const int64_t joins =
+        cf::join_by_wave(rows_in_all, head_dim) ? cf::ceil_div<int64_t>(rows_in_all, cf::kWaves) : rows_in_all;
+    CF_REQUIRE(workgroups <= cf::kMaxWorkgroups && joins <= cf::kMaxWorkgroups,
+               "%s: %lld sequences of %lld heads are too many for a launch", who,
+               static_cast<long long>(num_sequences), static_cast<long long>(num_heads));
     a.prefix_items = static_cast<int>(prefix_items);
     // The kernels take maxima of unscaled scores, so the factor must not be
     // negative, nor 0 (which times a masked score is NaN).

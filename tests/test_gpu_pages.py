@@ -224,3 +224,33 @@ def test_lists_and_tables_on_both_sides_of_what_a_plan_keeps_to_itself(count, ro
     src, dst = random_rows(gen, count, 0, rows), random_rows(gen, count, 0, rows)
     dst[3] = src[7] = rows - 1
     both(cf.cache_copy, plain._copy_reference, [caches, src, dst])
+
+
+def test_lists_that_take_more_than_one_launch():
+    """More workgroups (an entry takes one for each of 64 tensors) than a launch
+    may have: 2^24 of 256 threads."""
+    n = 2**18 + 5
+    caches = [torch.zeros(2 * n, 2, 1, 1, device="cuda") for _ in range(64)]
+    for i, cache in enumerate(caches):
+        cache.copy_(torch.arange(2 * n, device="cuda").view(-1, 1, 1, 1) + i)
+    src = torch.arange(n, dtype=torch.int32, device="cuda")
+    assert (cf.cache_copy(caches, src, src + n) == 0).all()
+    for i, cache in enumerate(caches):
+        assert torch.equal(cache[n:], cache[:n]) and cache[n - 1, 0, 0, 0] == n - 1 + i
+    # One token in a page of two: every child gets a page of its own.
+    counts = torch.zeros(2 * n, dtype=torch.int32, device="cuda")
+    counts[0] = 1
+    tables = torch.zeros(n + 1, 1, dtype=torch.int32, device="cuda")
+    context = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    context[0] = 1
+    for i, cache in enumerate(caches):
+        cache[0] = -1.0 - i
+    assert (cf.cache_fork(caches, counts, tables, context, torch.zeros_like(src), src + 1) == 0).all()
+    assert torch.equal(tables[1:, 0], src + 1) and (context == 1).all()
+    for i, cache in enumerate(caches):
+        assert (cache[: n + 1, 0] == -1.0 - i).all() and (cache[n + 1 :, 0] >= 0).all()
+    sequences = torch.full((2**24 + 10,), -1, dtype=torch.int32, device="cuda")
+    sequences[3], sequences[-1] = 7, n
+    cf.cache_release(counts, tables, context, sequences, 2)
+    assert context.sum() == n - 1 and context[7] == 0 and context[n] == 0
+    assert counts.sum() == n - 1 and counts[7] == 0 and counts[n] == 0

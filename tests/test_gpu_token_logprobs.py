@@ -339,3 +339,21 @@ def test_as_many_chunks_as_a_row_can_have(rows):
     vocab = (1 << 22) + 3
     logits = torch.randn(rows, vocab, device="cuda", dtype=torch.bfloat16)
     check(logits, torch.full((rows,), vocab - 1, device="cuda"), 1.0, 64)
+
+
+def test_rows_that_take_more_than_one_launch():
+    """More rows than a launch has workgroups (2^24 of 256 threads)."""
+    rows, vocab = 2**24 + 100, 8
+    logits = torch.randn(rows, vocab, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    tokens = torch.randint(0, vocab, (rows,), device="cuda")
+    got = cf.token_logprobs(logits, tokens, 0.7, True, 2)
+    g, h = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    grad, = torch.autograd.grad([got.logprobs, got.entropy], [logits], [g, h])
+    for at in (slice(0, 50), slice(2**24 - 50, rows)):
+        ref = reference(logits[at], tokens[at, None], 0.7, 2)
+        close(got.logprobs[at, None], ref[0], logprob_tolerance(ref[0], vocab))
+        close(got.entropy[at], ref[1], entropy_tolerance(ref[1], vocab))
+        close(got.top_logprobs[at], ref[2], logprob_tolerance(ref[2], vocab))
+        assert torch.equal(got.top_tokens[at].cpu(), ref[3])
+        want, size = gradient(logits[at], tokens[at, None], 0.7, g[at, None], h[at])
+        close(grad[at], want, 2.0**-8 * want.abs() + 2.0**-18 * size + 2.0**-130)

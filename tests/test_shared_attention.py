@@ -87,3 +87,18 @@ def test_c_abi_refusals_before_any_launch():
     assert size(_lib.CF_BF16, 4, 1, 8, 3, 64, 16, 10) == 0
     # 128 sequences of 32 heads over 32768 shared tokens: tens of MB, not GB.
     assert size(_lib.CF_BF16, 128, 1, 32, 8, 128, 32, 1040) < 64e6
+
+
+def test_more_rows_than_a_launch_takes_are_refused_before_any():
+    lib = _lib.load()
+    fake, null = ctypes.c_void_p(0x1000), ctypes.c_void_p(0)
+
+    def call(sequences, heads, kv_heads, dim):
+        return lib.cf_paged_attention_shared(fake, fake, fake, null, null, fake, fake, fake, _lib.CF_BF16, 100,
+                                             sequences, 0, heads, kv_heads, dim, 16, 1, 1.0, fake, 2**62, null)
+
+    bad = _lib.CF_ERR_INVALID_ARGUMENT
+    assert call(2**23, 32, 32, 64) == bad     # a wave a rest: 2^26 workgroups
+    assert call(2**22, 32, 2, 64) == bad      # rows to join, a wave each: 2^25
+    assert call(2**20, 17, 1, 300) == bad     # rows to join, a workgroup each
+    assert b"too many" in lib.cf_last_error()
