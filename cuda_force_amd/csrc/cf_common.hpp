@@ -552,11 +552,17 @@ void note_launch_error(hipError_t error);
 /// entry point's first kernel its start, each kernel its completion, so their
 /// elapsed time is the entry point's GPU time from its first kernel's start to
 /// its last kernel's end, without the queue packets an event pair around the
-/// call adds.
+/// call adds. A grid of 2^32 threads or more in a dimension is an error here: the
+/// runtime starts a remainder of it and reports nothing.
 template <typename... KArgs, typename... Args>
 inline void launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, uint32_t lds_bytes,
                    hipStream_t stream, Args&&... args) {
     static_assert(sizeof...(KArgs) == sizeof...(Args), "argument count of the kernel");
+    if (uint64_t{grid.x} * block.x > UINT32_MAX || uint64_t{grid.y} * block.y > UINT32_MAX ||
+        uint64_t{grid.z} * block.z > UINT32_MAX) {
+        note_launch_error(hipErrorInvalidConfiguration);
+        return;
+    }
     const LaunchEvents events = next_launch_events();
     if (events.start == nullptr && events.stop == nullptr) {
         kernel<<<grid, block, lds_bytes, stream>>>(std::forward<Args>(args)...);

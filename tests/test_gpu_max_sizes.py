@@ -104,3 +104,26 @@ def test_sum_past_2_31_elements():
     # fp32 partial sums of ones are exact below 2^24 per partial; the final
     # fixed-order tree over <= 4096 partials rounds at most ~12 times.
     assert abs(out.item() - n) <= n * 2.0**-20
+
+
+def test_a_grid_of_2_32_threads_is_refused():
+    """A launch counts its threads in 32 bits; here a wave per (sequence, head)
+    asks for a few more."""
+    sequences, heads, dim, block = (1 << 21) + 1, 32, 5, 4
+    g.announce(f"paged attention fp32, {sequences} sequences of {heads} heads of {dim}")
+    q = torch.ones(sequences, heads, dim, device="cuda")
+    k, v = torch.ones(1, block, 1, dim, device="cuda"), torch.full((1, block, 1, dim), 3.0, device="cuda")
+    tables, context = (torch.full((sequences,), n, dtype=torch.int32, device="cuda") for n in (0, 1))
+    out = g.poison_like(q)
+
+    def run(n):
+        g.call("cf_paged_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), tables.data_ptr(), context.data_ptr(),
+               out.data_ptr(), g.cf("f32"), n, heads, 1, dim, block, 1, 1.0, None, 0, g.stream())
+
+    with pytest.raises(RuntimeError, match="invalid configuration"):
+        run(sequences)
+    torch.cuda.synchronize()
+    assert bool(out.isnan().all())
+    run(sequences - 2)  # the most that a launch counts, nearly
+    torch.cuda.synchronize()
+    assert bool((out[: sequences - 2] == 3.0).all()) and bool(out[sequences - 2 :].isnan().all())
