@@ -711,13 +711,17 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(GradArgs a) {
     const int64_t* tokens = a.tokens + row * a.count;
     const float* given = a.grad_logprobs == nullptr ? nullptr : a.grad_logprobs + row * a.count;
 
+    // Given token i's part of G: none where no log probability is differentiated.
+    auto weight = [&](int64_t i, int64_t token) {
+        return given == nullptr ? 0.0f : token >= a.vocab ? __uint_as_float(0x7FC00000u) : given[i];
+    };
     float total = 0.0f;
     bool any = false;
     for (int64_t i = tid; i < a.count; i += kThreads) {
         const int64_t token = tokens[i];
         if (token < 0) continue;
         any = true;
-        total += token >= a.vocab ? __uint_as_float(0x7FC00000u) : (given != nullptr ? given[i] : 0.0f);
+        total += weight(i, token);
     }
     if (a.count > 1) {
         total = block_reduce_f32<kWaves, AddF32>(total, slots);
@@ -725,7 +729,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(GradArgs a) {
     } else {
         const int64_t token = tokens[0];
         any = token >= 0;
-        total = !any ? 0.0f : token >= a.vocab ? __uint_as_float(0x7FC00000u) : (given != nullptr ? given[0] : 0.0f);
+        total = any ? weight(0, token) : 0.0f;
     }
     const float h = kEntropy ? a.grad_entropy[row] : 0.0f;
     const float big_h = kEntropy ? a.entropy[row] : 0.0f;

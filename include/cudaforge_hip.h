@@ -226,7 +226,8 @@ cf_status cf_token_logprobs(const void* logits, cf_dtype dtype, int64_t rows, in
 
 /* The gradient of cf_token_logprobs's logprobs and entropy: with g =
  * grad_logprobs [rows, token_count] and h = grad_entropy [rows] (NULL: zeros),
- * G = sum of g over the row's tokens that are not padding, H = entropy,
+ * G = sum of g over the row's tokens that are not padding (NaN with one >= vocab,
+ * unless grad_logprobs is NULL), H = entropy,
  *   grad_logits_j = scale * (sum_{i: tokens_i = j} g_i - p_j (G + h (ln p_j + H)))
  * in the logits' dtype, rounded once; grad_row_stride elements between rows
  * (what lies between them is left alone). A row whose tokens are all padding

@@ -357,3 +357,19 @@ def test_rows_that_take_more_than_one_launch():
         assert torch.equal(got.top_tokens[at].cpu(), ref[3])
         want, size = gradient(logits[at], tokens[at, None], 0.7, g[at, None], h[at])
         close(grad[at], want, 2.0**-8 * want.abs() + 2.0**-18 * size + 2.0**-130)
+
+
+def test_the_entropys_gradient_does_not_ask_for_the_tokens():
+    """A token past the vocabulary gives a log probability of NaN, and its
+    gradient too, but where only the entropy is differentiated no token counts."""
+    for dtype in DTYPES:
+        for count in (1, 3):
+            logits = torch.randn(3, 300, device="cuda").to(dtype).requires_grad_()
+            tokens = torch.tensor([[5], [300], [-1]], device="cuda").repeat(1, count)
+            got = cf.token_logprobs(logits, tokens, 0.8, True)
+            h = torch.randn(3, device="cuda")
+            grad, = torch.autograd.grad(got.entropy, logits, h, retain_graph=True)
+            ref, size = gradient(logits, tokens.clamp(max=0), 0.8, None, h)
+            close(grad, ref, torch.finfo(dtype).eps / 2 * ref.abs() + 2.0**-18 * size + torch.finfo(dtype).tiny)
+            both, = torch.autograd.grad([got.entropy, got.logprobs], logits, [h, torch.ones_like(got.logprobs)])
+            assert both[1].isnan().all() and not both[0].isnan().any() and not both[2].isnan().any()

@@ -138,3 +138,13 @@ def test_c_abi_refusals_before_any_launch():
     for case in ({"stats": null}, {"grad": null}, {"entropy": null, "h": fake}, {"stride": 99},
                  {"grad": ctypes.c_void_p(0x1001)}):
         assert backward(**case) == bad, case
+
+
+def test_the_entropys_gradient_does_not_ask_for_the_tokens():
+    logits = torch.randn(3, 30)
+    tokens = torch.tensor([[5], [30], [-1]])
+    h = torch.randn(3)
+    _, stats, entropy, _, _ = torch.ops.cudaforge.token_logprobs(logits, tokens, 0.8, True, 0)
+    got = torch.ops.cudaforge.token_logprobs_backward(logits, tokens, 0.8, stats, entropy, None, h)
+    ref, size = gradient(logits, tokens.clamp(max=0), 0.8, None, h)
+    close(got, ref, 2.0**-20 * (size + 1e-6))
