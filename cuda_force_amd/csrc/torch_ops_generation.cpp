@@ -143,19 +143,19 @@ torch::Tensor token_logprobs_backward_cpu(const torch::Tensor& logits, const tor
     const torch::Tensor p = logp.exp();
     torch::Tensor held;
     torch::Tensor grad = torch::zeros_like(p);
-    const bool has_h = gradient(grad_entropy, logits, {rows}, "grad_entropy", held) != nullptr;
-    if (has_h) {
+    torch::Tensor padding = (tokens < 0).all(1, true);  // of rows that have no gradient, whatever they hold
+    if (gradient(grad_entropy, logits, {rows}, "grad_entropy", held) != nullptr) {
         const torch::Tensor kept = torch::where(p == 0, torch::zeros_like(p), logp);
         grad -= held.unsqueeze(1) * p * (kept + entropy.unsqueeze(1));
+        padding = padding & (held == 0).unsqueeze(1);
     }
     if (gradient(grad_logprobs, logits, tokens.sizes(), "grad_logprobs", held) != nullptr) {
         torch::Tensor g = held.masked_fill(tokens < 0, 0.0);
         g = g.masked_fill(tokens >= vocab, std::numeric_limits<float>::quiet_NaN());
         grad -= g.sum(1, true) * p;
         grad.scatter_add_(1, tokens.clamp(0, vocab - 1), g);
-        if (!has_h) grad.masked_fill_((tokens < 0).all(1, true), 0.0);
     }
-    return (scale * grad).to(logits.scalar_type());
+    return (scale * grad.masked_fill_(padding, 0.0)).to(logits.scalar_type());
 }
 
 // ---- pages of a paged cache ------------------------------------------------

@@ -148,3 +148,25 @@ def test_the_entropys_gradient_does_not_ask_for_the_tokens():
     got = torch.ops.cudaforge.token_logprobs_backward(logits, tokens, 0.8, stats, entropy, None, h)
     ref, size = gradient(logits, tokens.clamp(max=0), 0.8, None, h)
     close(got, ref, 2.0**-20 * (size + 1e-6))
+
+
+@pytest.mark.parametrize("through", ["ops", "kernels"])
+def test_a_row_of_padding_alone_has_no_gradient_whatever_it_holds(through):
+    logits = torch.randn(4, 6)
+    logits[1] = float("-inf")
+    logits[2, 3] = float("nan")
+    tokens = torch.tensor([[1, 2], [-1, -100], [-1, -1], [-1, 5]])
+    g, h = torch.ones(4, 2), torch.tensor([0.5, 0.0, 0.0, 0.0])
+    for with_h in (False, True):
+        if through == "ops":
+            leaf = logits.clone().requires_grad_()
+            got = cf.token_logprobs(leaf, tokens, 0.9, entropy=True)
+            grad, = torch.autograd.grad(got.logprobs, leaf, g)
+        else:
+            _, stats, entropy, _, _ = torch.ops.cudaforge.token_logprobs(logits, tokens, 0.9, True, 0)
+            grad = torch.ops.cudaforge.token_logprobs_backward(logits, tokens, 0.9, stats, entropy, g,
+                                                               h if with_h else None)
+        assert (grad[1:3] == 0).all() and torch.isfinite(grad).all() and (grad[[0, 3]] != 0).all()
+    if through == "kernels":
+        alone = torch.ops.cudaforge.token_logprobs_backward(logits, tokens, 0.9, stats, entropy, None, h)
+        assert (alone[1:] == 0).all() and (alone[0] != 0).all()
