@@ -348,13 +348,18 @@ def _token_logprobs_reference(
     where the logits are."""
     vocab = logits.shape[1]
     wide = logits if logits.dtype == torch.float64 else logits.float()
+
+    def log_softmax(x: torch.Tensor) -> torch.Tensor:
+        # Differences first: a scaled logit may leave its type's range.
+        return torch.log_softmax((x - x.detach().amax(-1, keepdim=True)) * scale, dim=-1)
+
     # A row of padding alone has no gradient, whatever it holds.
     given = wide.masked_fill((tokens < 0).all(-1, keepdim=True), 0.0)
-    picked = torch.log_softmax(given * scale, dim=-1).gather(1, tokens.clamp(0, vocab - 1))
+    picked = log_softmax(given).gather(1, tokens.clamp(0, vocab - 1))
     picked = picked.masked_fill(tokens < 0, 0.0).masked_fill(tokens >= vocab, float("nan"))
     if not entropy and top == 0:
         return picked, None, None, None
-    logp = torch.log_softmax(wide * scale, dim=-1)
+    logp = log_softmax(wide)
     h = None
     if entropy:
         p = logp.exp()

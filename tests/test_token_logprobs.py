@@ -170,3 +170,21 @@ def test_a_row_of_padding_alone_has_no_gradient_whatever_it_holds(through):
     if through == "kernels":
         alone = torch.ops.cudaforge.token_logprobs_backward(logits, tokens, 0.9, stats, entropy, None, h)
         assert (alone[1:] == 0).all() and (alone[0] != 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_logits_at_the_ends_of_their_type_keep_their_differences_when_scaled(dtype):
+    low = torch.finfo(dtype).min
+    logits = torch.full((2, 8), low, dtype=dtype)
+    logits[1, 3] = 1.0
+    tokens = torch.tensor([2, 3])
+    leaf = logits.clone().requires_grad_()
+    for got in (cf.token_logprobs(logits, tokens, 2.0, entropy=True, top=2),
+                cf.token_logprobs(leaf, tokens, 2.0, entropy=True, top=2)):
+        assert abs(got.logprobs[0] + torch.tensor(8.0).log()) < 1e-6 and got.logprobs[1] == 0
+        assert abs(got.entropy[0] - torch.tensor(8.0).log()) < 1e-6 and got.entropy[1] == 0
+        assert got.top_tokens.tolist() == [[0, 1], [3, 0]]
+    got.logprobs.sum().backward()
+    want = torch.full((8,), -0.25)
+    want[2] += 2.0
+    assert (leaf.grad[0].float() - want).abs().max() < 1e-6 and (leaf.grad[1] == 0).all()
