@@ -313,12 +313,12 @@ __device__ void chunk_top(const Span<T>& s, u64 best, int top, Shared& sh, u64* 
     }
     // More logits than fit (they would have to be dealt so that the same few
     // threads hold them): one search over the chunk for each place.
-    u64 previous = ~0ull;
+    u64 previous = 0;  // of the place before; the first has none (a NaN as token 0 has the largest key there is)
     for (int place = 0; place < top; ++place) {
         u64 mine = 0;
         auto look = [&](float v, uint32_t index) {
             const u64 key = key_of(v, index);
-            if (key < previous && key > mine) mine = key;
+            if ((place == 0 || key < previous) && key > mine) mine = key;
         };
         const uint32_t h = s.head_element(tid);
         const uint32_t e = s.tail_element(tid);

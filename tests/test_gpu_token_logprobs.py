@@ -373,3 +373,27 @@ def test_the_entropys_gradient_does_not_ask_for_the_tokens():
             close(grad, ref, torch.finfo(dtype).eps / 2 * ref.abs() + 2.0**-18 * size + torch.finfo(dtype).tiny)
             both, = torch.autograd.grad([got.entropy, got.logprobs], logits, [h, torch.ones_like(got.logprobs)])
             assert both[1].isnan().all() and not both[0].isnan().any() and not both[2].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,vocab", [(2, 9000), (1100, 4096), (1100, 4103)])
+@pytest.mark.parametrize("top", [32, 33, 64])
+def test_rows_of_one_value_with_many_alternatives(dtype, rows, vocab, top):
+    """All of a row equal, masked or NaN: as many equal logits as the search for
+    the likeliest may meet, the first token among them."""
+    logits = torch.randn(rows, vocab, device="cuda").to(dtype)
+    logits[0] = float("nan")
+    logits[1] = 0.0
+    if rows > 2:
+        logits[2, 1:] = -1.0
+        logits[2, 0] = float("nan")
+        logits[3] = float("-inf")
+        logits[4, 40:] = float("-inf")
+        logits[5] = torch.finfo(dtype).min
+        logits[6, ::2] = float("nan")
+        logits[7, :] = float("inf")
+    tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    got = cf.token_logprobs(logits, tokens, 1.5, True, top)
+    ref = reference(logits[:8], tokens[:8, None], 1.5, top)
+    assert torch.equal(got.top_tokens[:8].cpu(), ref[3])
+    close(got.top_logprobs[:8], ref[2], logprob_tolerance(ref[2], vocab))
