@@ -51,7 +51,15 @@ constexpr int kTopMax = 64;
 /// likeliest: as many teams as tokens may be asked for.
 constexpr int kTeam = kThreads / kTopMax;
 constexpr int kTokensMax = 1024;
-constexpr int kCandidates = 1024;  // keys that the filter may keep before the slow search takes over
+/// Keys that the filter may keep before the slow search takes over. Logits that
+/// are all equal (a masked row) leave the first vector of each thread of as many
+/// teams as tokens are asked for, and up to seven logits before the first vector:
+/// 2031 in 16 bits. (With room for 1024, 600 rows of 131072 in fp16, all but 100
+/// logits masked, took 1904 us for 64 tokens and take 99 now, like any others.)
+constexpr int kCandidates = 2048;
+static_assert(kTopMax * kTeam * 8 <= kCandidates, "equal 16-bit logits");
+constexpr int kChunksMax = 1024;  // of a row
+static_assert(kChunksMax + kTopMax <= kCandidates, "the joining kernel holds the first keys of every chunk");
 constexpr int kUnroll = 4;  // vectors of a batch; two batches are in flight
 constexpr int kHeld = 8;           // keys that a thread of the joining kernel keeps in registers
 constexpr float kLog2e = 1.4426950408889634f;
@@ -61,9 +69,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNothing = -256.0f;
 constexpr float kLowest = -3.0e38f;
 /// Most logits per row: a row's chunks (at most 128 vectors a thread) then
-/// stay within kCandidates, which the joining kernel relies on.
+/// stay within kChunksMax.
 constexpr int64_t kVocabMax = int64_t{1} << 27;
-static_assert(kVocabMax * 4 / 16 / (128 * kThreads) <= kCandidates, "chunks of the longest row");
+static_assert(kVocabMax * 4 / 16 / (128 * kThreads) <= kChunksMax, "chunks of the longest row");
 
 typedef unsigned long long u64;
 
@@ -286,12 +294,19 @@ __device__ void chunk_top(const Span<T>& s, u64 best, int top, Shared& sh, u64* 
     if (kept <= kCandidates) {
         if (kept > 2 * kThreads / kTeam) {
             // Many equal logits (a masked row): the same sieve once more, over
-            // the keys, since ranking them costs their number squared.
-            u64 held[kCandidates / kThreads];
+            // the keys, since ranking them costs their number squared. They
+            // lie as the waves brought them, neighbours beside each other; a
+            // team takes every kSpread-th (the golden section of them all), so
+            // that each has some of the best.
+            constexpr int kEach = kCandidates / kThreads;
+            constexpr int kSpread = 1265;
+            static_assert(kCandidates == 2048, "kSpread");
+            u64 held[kEach];
             best = 0;
 #pragma unroll
-            for (int i = 0; i < kCandidates / kThreads; ++i) {
-                held[i] = i * kThreads + tid < kept ? sh.candidates[i * kThreads + tid] : 0;
+            for (int i = 0; i < kEach; ++i) {
+                const int from = (tid * kEach + i) * kSpread % kCandidates;
+                held[i] = from < kept ? sh.candidates[from] : 0;
                 best = held[i] > best ? held[i] : best;
             }
             if (tid == 0) sh.threshold = 0;
@@ -301,7 +316,7 @@ __device__ void chunk_top(const Span<T>& s, u64 best, int top, Shared& sh, u64* 
             if (best != 0 && rank == top - 1 && tid % kTeam == 0) sh.threshold = best;
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kCandidates / kThreads; ++i) {
+            for (int i = 0; i < kEach; ++i) {
                 if (held[i] != 0 && held[i] >= sh.threshold) sh.candidates[atomicAdd(&sh.kept, 1)] = held[i];
             }
             __syncthreads();
@@ -312,7 +327,7 @@ __device__ void chunk_top(const Span<T>& s, u64 best, int top, Shared& sh, u64* 
         return;
     }
     // More logits than fit (they would have to be dealt so that the same few
-    // threads hold them): one search over the chunk for each place.
+    // teams hold them): one search over the chunk for each place.
     u64 previous = 0;  // of the place before; the first has none (a NaN as token 0 has the largest key there is)
     for (int place = 0; place < top; ++place) {
         u64 mine = 0;
@@ -796,7 +811,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(GradArgs a) {
 int chunks_of(int64_t rows, int64_t vocab, size_t size) {
     const int64_t vectors = ceil_div<int64_t>(vocab * static_cast<int64_t>(size), 16);
     const int64_t many = ceil_div<int64_t>(2048, rows);
-    const int64_t wanted = many < kCandidates ? many : kCandidates;  // the joining kernel holds a key of each
+    const int64_t wanted = many < kChunksMax ? many : kChunksMax;
     const int64_t most = ceil_div<int64_t>(vectors, kThreads);
     const int64_t least = ceil_div<int64_t>(vectors, 128 * kThreads);
     int64_t chunks = wanted < most ? wanted : most;
