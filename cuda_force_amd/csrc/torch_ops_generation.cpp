@@ -480,8 +480,8 @@ py::object try_token_logprobs(py::handle logits_, py::handle tokens_, py::handle
     const bool entropy = entropy_.ptr() == Py_True;
     if (!kernel_dtype(logits.scalar_type()) || tokens->scalar_type() != torch::kInt64 ||
         tokens->device() != logits.device() || logits.dim() != 2 || logits.numel() == 0 || logits.stride(1) != 1 ||
-        (logits.size(0) > 1 && logits.stride(0) < logits.size(1)) || tokens->size(0) != logits.size(0) ||
-        tokens->dim() > 2 || (tokens->dim() == 2 && tokens->size(1) > kLogprobsTokens) ||
+        (logits.size(0) > 1 && logits.stride(0) < logits.size(1)) || tokens->dim() < 1 || tokens->dim() > 2 ||
+        tokens->size(0) != logits.size(0) || (tokens->dim() == 2 && tokens->size(1) > kLogprobsTokens) ||
         !(*scale > 0 && *scale < 1e29) || *top < 0 || *top > std::min(kLogprobsTop, logits.size(1))) {
         return py::none();
     }

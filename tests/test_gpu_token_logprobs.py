@@ -397,3 +397,11 @@ def test_rows_of_one_value_with_many_alternatives(dtype, rows, vocab, top):
     ref = reference(logits[:8], tokens[:8, None], 1.5, top)
     assert torch.equal(got.top_tokens[:8].cpu(), ref[3])
     close(got.top_logprobs[:8], ref[2], logprob_tolerance(ref[2], vocab))
+
+
+@pytest.mark.parametrize("shape", [(), (3,), (1, 2), (2, 1, 1), (2, 0)])
+def test_tokens_that_do_not_fit_are_refused_alike_on_the_gpu(shape):
+    tokens = torch.zeros(shape, dtype=torch.int64, device="cuda")
+    for logits in (torch.zeros(2, 100, device="cuda"), torch.zeros(2, 100, device="cuda", requires_grad=True)):
+        with pytest.raises(ValueError):
+            cf.token_logprobs(logits, tokens)
