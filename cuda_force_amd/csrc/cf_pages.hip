@@ -45,6 +45,7 @@ constexpr int kTilePages = kCopyThreads * kCountsPerThread;  // counts per workg
 /// 8.1 -> 5.6 us, 32 rows extended 8.0 -> 5.5, 1500 pairs copied 10.6 -> 4.9).
 constexpr int kSmallRows = 8192;
 constexpr int kUnclaimed = 0x7FFFFFFF;
+constexpr int kNamed = kUnclaimed - 1;
 
 struct Tensors {
     uint8_t* p[kTensors];
@@ -188,7 +189,8 @@ __device__ __forceinline__ void copy_bytes(const uint8_t* from, uint8_t* to, int
 // ---- copy -------------------------------------------------------------------
 
 /// Which pairs of a copy take part: status 0, or 1 for a pair out of range,
-/// whose dst an earlier pair names, or whose src any pair names as its dst.
+/// whose dst an earlier pair in range names, or whose src any pair names as its
+/// dst (one out of range by its src too: such a dst is kNamed, claimed by none).
 /// kSmall: claims in LDS.
 template <bool kSmall>
 __global__ __launch_bounds__(kPlanThreads) void copy_plan_kernel(const int* src, const int* dst, int64_t count,
@@ -202,7 +204,7 @@ __global__ __launch_bounds__(kPlanThreads) void copy_plan_kernel(const int* src,
     }
     Ints::phase();
     for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
-        if (within(dst[i], pages)) claims.lower(dst[i], static_cast<int>(i));
+        if (within(dst[i], pages)) claims.lower(dst[i], within(src[i], pages) ? static_cast<int>(i) : kNamed);
     }
     Ints::phase();
     for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {

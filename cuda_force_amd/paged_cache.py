@@ -150,10 +150,11 @@ def _copy_reference(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torc
     pages = caches[0].shape[0]
     pairs = list(zip(src.tolist(), dst.tolist()))
     owner: dict[int, int] = {}
-    for i, (_, d) in enumerate(pairs):
-        if 0 <= d < pages:
+    named = {d for _, d in pairs}
+    for i, (s, d) in enumerate(pairs):
+        if 0 <= s < pages and 0 <= d < pages:
             owner.setdefault(d, i)
-    status = [0 if 0 <= s < pages and owner.get(d) == i and s not in owner else 1 for i, (s, d) in enumerate(pairs)]
+    status = [0 if owner.get(d) == i and s not in named else 1 for i, (s, d) in enumerate(pairs)]
     good = [i for i, bad in enumerate(status) if not bad]
     if good:
         for cache in caches:
@@ -339,8 +340,8 @@ def cache_copy(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
     ``caches`` are tensors ``[pages, ...]`` of one shape and any dtype, ``src``
     and ``dst`` int32 ``[n]`` on their device. Returns int32 ``[n]``: 0 for a
     copied page, 1 for an entry left out (a page out of range, a ``dst`` that an
-    earlier entry names, or a ``src`` that some entry names as its ``dst``). Not
-    in the reference's API.
+    earlier entry whose pages are in range names, or a ``src`` that some entry
+    names as its ``dst``). Not in the reference's API.
 
     Raises:
         ValueError: for caches that differ, are not contiguous or require

@@ -254,3 +254,10 @@ def test_lists_that_take_more_than_one_launch():
     cf.cache_release(counts, tables, context, sequences, 2)
     assert context.sum() == n - 1 and context[7] == 0 and context[n] == 0
     assert counts.sum() == n - 1 and counts[7] == 0 and counts[n] == 0
+
+
+@pytest.mark.parametrize("pages", [10, 9000])
+def test_a_copy_out_of_range_blocks_no_other(pages):
+    caches, *_ = state([], 4, 1, pages, shape=(1, 2))
+    arguments = [caches, ints(-1, 2, 3, 6, pages, 4), ints(5, 5, 5, 7, 6, 8)]
+    assert both(cf.cache_copy, plain._copy_reference, arguments).tolist() == [1, 0, 1, 1, 1, 0]

@@ -185,3 +185,15 @@ def test_c_abi_refusals_before_any_launch():
 
     for case in ({"counts": null}, {"new": null}, {"live": null}, {"pages": 0}, {"tables": null}, {"size": 0}):
         assert compact(**case) == bad, case
+
+
+def test_a_copy_out_of_range_blocks_no_other():
+    caches, *_ = state([], 4, 1, 10)
+    before = [c.clone() for c in caches]
+    #      out of range, good all the same, taken, from a page that one names as its dst, out of range
+    src, dst = ints(-1, 2, 3, 6, 10, 4), ints(5, 5, 5, 7, 6, 8)
+    assert cf.cache_copy(caches, src, dst).tolist() == [1, 0, 1, 1, 1, 0]
+    for cache, old in zip(caches, before):
+        expect = old.clone()
+        expect[5], expect[8] = old[2], old[4]
+        assert torch.equal(cache, expect)
