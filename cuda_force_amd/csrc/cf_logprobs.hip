@@ -804,13 +804,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(GradArgs a) {
     }
 }
 
-/// Chunks per row: about eight workgroups a CU where there are few rows, but no
-/// chunk under a vector a thread, and none above 128 vectors a thread. (Four a
-/// CU: 600 rows of 131072 in fp16 39.4 -> 38.2 us, 1001 of 32000 floats 24.4 -> 23.4;
-/// sixteen 44.4 and 24.4 us.)
-int chunks_of(int64_t rows, int64_t vocab, size_t size) {
+/// Chunks per row: the given number of workgroups in all where there are few
+/// rows, but no chunk under a vector a thread, and none above 128 vectors a thread.
+int chunks_of(int64_t rows, int64_t vocab, size_t size, int64_t workgroups) {
     const int64_t vectors = ceil_div<int64_t>(vocab * static_cast<int64_t>(size), 16);
-    const int64_t many = ceil_div<int64_t>(2048, rows);
+    const int64_t many = ceil_div<int64_t>(workgroups, rows);
     const int64_t wanted = many < kChunksMax ? many : kChunksMax;
     const int64_t most = ceil_div<int64_t>(vectors, kThreads);
     const int64_t least = ceil_div<int64_t>(vectors, 128 * kThreads);
@@ -818,6 +816,26 @@ int chunks_of(int64_t rows, int64_t vocab, size_t size) {
     if (chunks < least) chunks = least;
     return static_cast<int>(chunks < 1 ? 1 : chunks);
 }
+
+/// The forward: 512 workgroups, since a row that is not cut needs no join. Many
+/// of the likeliest tokens of long rows: 2048, since a chunk's sieve reads its
+/// teams' vectors again, and takes the longer the more there are. Whole calls in
+/// us at 512 | 1024 | 2048 workgroups, rows of bf16 out of memory:
+///   600 x 32000, none of the likeliest  12.1 | 15.5 | 15.1;   5: 16.6 | 22.5 | 22.7
+///   1001 x 32000                        16.9 | 20.7 | 22.6;      21.9 | 28.1 | 32.2
+///   600 x 131072                        32.9 | 36.3 | 35.3;      43.0 | 47.0 | 44.5
+///   600 x 131072, 20 of the likeliest   57.9 | 58.3 | 54.2;  48: 89.5 | 78.7 | 74.6
+/// Against 2048 throughout, over 1 to 3000 rows of 4099 to 131072 in bf16 and
+/// fp32 with 0 to 64 of the likeliest, calls take 14% less on average, 9% more at
+/// most (200 rows of 131072 floats) and a third at least (1001 rows of 4099).
+int64_t forward_groups(int64_t vocab, size_t size, int64_t top) {
+    return top > 8 && vocab * static_cast<int64_t>(size) / 16 > 32 * kThreads ? 2048 : 512;
+}
+
+/// The backward joins nothing, and is bound by its stores: 1024 workgroups (300
+/// rows of 131072 in bf16 39.2 us at 512, 28.9 at 1024, 32.2 at 2048; 600 rows 77.3,
+/// 56.7 and 60.0; 1700 rows of 32000 39.4, 39.3 and 37.4).
+constexpr int64_t kBackwardGroups = 1024;
 
 int64_t vectors_per_chunk(int64_t vocab, size_t size, int chunks) {
     return ceil_div<int64_t>(ceil_div<int64_t>(vocab * static_cast<int64_t>(size), 16), chunks);
@@ -837,7 +855,7 @@ cf_status validate(const char* who, const void* logits, cf_dtype dtype, int64_t 
                static_cast<long long>(token_count), kTokensMax);
     CF_REQUIRE(scale > 0.0f && scale * kLog2e < 1.0e30f, "%s: scale must be positive and finite", who);
     CF_REQUIRE(host_aligned(logits, dtype_size(dtype)) && host_aligned(tokens, 8), "%s: misaligned pointer", who);
-    CF_REQUIRE(rows * chunks_of(rows, vocab, dtype_size(dtype)) < (1LL << 31), "%s: %lld rows are too many", who,
+    CF_REQUIRE(rows * chunks_of(rows, vocab, dtype_size(dtype), 1) < (1LL << 31), "%s: %lld rows are too many", who,
                static_cast<long long>(rows));
     return CF_OK;
 }
@@ -905,7 +923,8 @@ extern "C" {
 
 size_t cf_token_logprobs_workspace_bytes(cf_dtype dtype, int64_t rows, int64_t vocab, int64_t top) {
     if (!cf::valid_dtype(dtype) || rows <= 0 || vocab <= 0 || top < 0) return 0;
-    const int chunks = cf::chunks_of(rows, vocab, cf::dtype_size(dtype));
+    const size_t size = cf::dtype_size(dtype);
+    const int chunks = cf::chunks_of(rows, vocab, size, cf::forward_groups(vocab, size, top));
     if (chunks == 1) return 0;
     return cf::round_up(static_cast<size_t>(rows) * chunks * 16) + static_cast<size_t>(rows) * chunks * top * 8;
 }
@@ -938,7 +957,8 @@ cf_status cf_token_logprobs(const void* logits, cf_dtype dtype, int64_t rows, in
     a.vocab = vocab;
     a.stride = row_stride;
     a.count = token_count;
-    a.chunks = cf::chunks_of(rows, vocab, cf::dtype_size(dtype));
+    const size_t size = cf::dtype_size(dtype);
+    a.chunks = cf::chunks_of(rows, vocab, size, cf::forward_groups(vocab, size, top));
     a.vectors_per_chunk = cf::vectors_per_chunk(vocab, cf::dtype_size(dtype), a.chunks);
     a.top = static_cast<int>(top);
     a.scale = scale;
@@ -984,7 +1004,7 @@ cf_status cf_token_logprobs_backward(const void* logits, cf_dtype dtype, int64_t
     a.stride = row_stride;
     a.grad_stride = grad_row_stride;
     a.count = token_count;
-    a.chunks = cf::chunks_of(rows, vocab, cf::dtype_size(dtype));
+    a.chunks = cf::chunks_of(rows, vocab, cf::dtype_size(dtype), cf::kBackwardGroups);
     a.vectors_per_chunk = cf::vectors_per_chunk(vocab, cf::dtype_size(dtype), a.chunks);
     a.scale = scale;
     a.c = scale * cf::kLog2e;

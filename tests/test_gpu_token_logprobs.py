@@ -405,3 +405,38 @@ def test_tokens_that_do_not_fit_are_refused_alike_on_the_gpu(shape):
     for logits in (torch.zeros(2, 100, device="cuda"), torch.zeros(2, 100, device="cuda", requires_grad=True)):
         with pytest.raises(ValueError):
             cf.token_logprobs(logits, tokens)
+
+
+@pytest.mark.parametrize("top", [0, 64])
+def test_the_longest_row_there_is(top):
+    """2^27 floats: as many chunks as the join takes."""
+    vocab = 2**27
+    logits = torch.randn(1, vocab, device="cuda")
+    peaks = torch.randperm(vocab, device="cuda")[:64]
+    logits[0, peaks] = 40.0 - 0.25 * torch.arange(64, device="cuda")
+    got = cf.token_logprobs(logits, peaks[None, :3].contiguous(), 1.0, True, top)
+    if top:
+        assert torch.equal(got.top_tokens[0], peaks)
+    x = logits[0].double()
+    logp = x - x.logsumexp(0)
+    ref = logp[peaks[:3]][None].cpu()
+    close(got.logprobs, ref, logprob_tolerance(ref, vocab // 1024))
+    entropy = -(logp.exp() * logp).sum()[None].cpu()
+    close(got.entropy, entropy, entropy_tolerance(entropy, vocab // 1024))
+
+
+@pytest.mark.parametrize("rows", [255, 256, 257, 511, 512, 513, 1023, 1025])
+@pytest.mark.parametrize("vocab,top", [(4103, 3), (66000, 9), (66000, 8)])
+def test_rows_on_both_sides_of_where_they_are_cut(rows, vocab, top):
+    logits = torch.randn(rows, vocab, device="cuda").bfloat16().requires_grad_()
+    tokens = torch.randint(0, vocab, (rows,), device="cuda")
+    got = cf.token_logprobs(logits, tokens, 0.9, True, top)
+    g, h = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    grad, = torch.autograd.grad([got.logprobs, got.entropy], [logits], [g, h])
+    at = torch.tensor([0, 1, rows // 2, rows - 1])
+    ref = reference(logits[at], tokens[at, None], 0.9, top)
+    close(got.logprobs[at, None], ref[0], logprob_tolerance(ref[0], vocab))
+    close(got.entropy[at], ref[1], entropy_tolerance(ref[1], vocab))
+    assert torch.equal(got.top_tokens[at].cpu(), ref[3])
+    want, size = gradient(logits[at], tokens[at, None], 0.9, g[at, None], h[at])
+    close(grad[at], want, 2.0**-8 * want.abs() + (2.0**-18 + 8 * 2.0**-24 * vocab / 256) * size + 2.0**-130)
