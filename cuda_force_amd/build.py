@@ -65,7 +65,7 @@ HIP_LIBRARY = PACKAGE_DIR / "libcudaforge_hip.so"
 OFFLOAD_ARCH = "gfx950"
 
 # -packed-fp32-ops keeps the compiler from emitting packed fp32 VALU ops
-# (v_pk_add/mul/fma_f32), which this hardware pool has miscomputed
+# (v_pk_add/mul/fma_f32), which this hardware has miscomputed
 # intermittently. No -ffast-math: the quantiser relies on IEEE division and
 # the default correctly-rounded sqrt. -fvisibility=hidden: only the C ABI
 # (declared default-visible in include/cudaforge_hip.h) is exported.

@@ -28,15 +28,16 @@
 //     teams' (otherwise k larger ones exist), so only those k teams' vectors
 //     (k / 64 of the chunk) are read again, from L2, and filtered by the k-th
 //     best team's logit. Teams of four against single threads: 64 keys to rank
-//     and not 256 (5 of 131072, 600 rows in fp16: 41 -> 38 us, with the batches below);
-//     a row of equal logits leaves more keys, which are sieved twice.
-//   * Measured: 4096 rows of 32000 bf16 logits (262 MB) with entropy 47 us, 5.6
-//     TB/s, from memory that nothing has written to before; 79 us straight after a
+//     and not 256 (5 of 131072, 600 rows in fp16 cut in four: 41 -> 38 us, with the
+//     batches below); a row of equal logits leaves more keys, which are sieved twice.
+//   * Measured: 4096 rows of 32000 bf16 logits (262 MB) with entropy 52 us, 5.0
+//     TB/s, from memory that nothing has written to before; 78 us straight after a
 //     kernel that wrote as much, whose lines are then written back meanwhile.
-//     1001 rows of 32000 floats (128 MB) 23.4 us, 5.5 TB/s. A batch of four vectors with one
-//     maximum and the next on its way, against a vector at a time: 27 -> 24 us.
-//     Few rows are bound by the chain of steps behind the loads: 8 rows of
-//     50257 with 20 tokens 7.3 us, and 5.8 us to join them.
+//     1001 rows of 32000 floats (128 MB) 24.7 us a call, 5.2 TB/s. A batch of four
+//     vectors with one maximum and the next on its way, against a vector at a
+//     time: 27 -> 24 us (two workgroups a row). Few rows are bound by the chain of
+//     steps behind the loads: 8 rows of 50257 with 20 tokens 7 to 9 us, and 5.1 us
+//     to join them.
 #include <type_traits>
 
 #include "cf_common.hpp"

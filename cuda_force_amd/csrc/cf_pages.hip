@@ -15,7 +15,7 @@
 //     by barriers instead of launches, and nothing but the order of the phases
 //     to keep between them. The search for free pages reads 16384 counts a step
 //     and ends when it has enough. Bound by the chain of loads and atomics:
-//     32 forks of 8 sequences 5.6 us, their extension 5.5 us, 1500 pairs of a copy
+//     32 forks of 8 sequences 5.1 us, their extension 5.4 us, 1500 pairs of a copy
 //     4.9 us; claims and short lists of pages are exchanged in LDS for that.
 //   * Copies are bound by HBM: 16 KiB per workgroup and step, four 16-byte loads
 //     in flight per lane, streamed past the caches. 1500 pages of 32 KiB in four
@@ -42,7 +42,8 @@ constexpr int kTilePages = kCopyThreads * kCountsPerThread;  // counts per workg
 /// Plans over at most so many rows (a copy: pages) exchange their claims in LDS,
 /// those of forks and extensions if they want at most kPlanThreads pages: atomics
 /// and loads past the CU's cache cost most of a plan's time otherwise (32 forks
-/// 8.1 -> 5.6 us, 32 rows extended 8.0 -> 5.5, 1500 pairs copied 10.6 -> 4.9).
+/// 8.1 -> 5.6 us, 32 rows extended 8.0 -> 5.5, 1500 pairs copied 10.6 -> 4.9; these
+/// take 14 us in a pool of 100000 pages).
 constexpr int kSmallRows = 8192;
 constexpr int kUnclaimed = 0x7FFFFFFF;
 constexpr int kNamed = kUnclaimed - 1;

@@ -34,11 +34,13 @@
 //     (relative error half an ulp each, of either sign; for fp16's smallest
 //     numbers see kLift); sums stay in fp32.
 //   * Measured, 32 query and 8 KV heads of 128 in bf16, with the join: 128
-//     sequences behind 32768 tokens 98 + 9.5 us, 704 TFLOP/s: neither the matrix
+//     sequences behind 32768 tokens 100 + 9.9 us, 690 TFLOP/s: neither the matrix
 //     cores (31% busy) nor the vector units (34%), but the chain from one product
 //     through the probabilities to the next at two waves per SIMD. 64 sequences
-//     behind 4099 tokens 26 + 6.5 us, 3.2 TB/s: one round of work, a third of it
-//     filling and draining. 8 behind 1000 tokens 9 + 4 us: the launches' chains.
+//     behind 4099 tokens 26 + 6.7 us, 3.2 TB/s: one round of work, the CUs busy
+//     for 57% of it. 8 behind 1000 tokens 9 + 3.5 us: the launches' chains. 16 in
+//     two groups behind 2048 tokens in fp32 27 + 4.7 us: 680 workgroups on 512
+//     places, matrix cores 12% busy.
 // Tokens behind a range's end, and tokens whose page is not in the cache, get
 // no weight: their scores are replaced and their V rows are cleared in LDS, so
 // that whatever lies there (NaN, infinities) stays out.
