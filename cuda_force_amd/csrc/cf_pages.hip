@@ -642,13 +642,14 @@ void by_tensors(void* const* caches, int64_t tensors, Body body) {
     }
 }
 
-/// Runs `body` with entries [first, first + n) of a list of `count`, each of
-/// which takes `each` workgroups, in launches of no more than there may be; a
-/// single entry's have to fit.
+/// Whether a launch takes the workgroups of one entry: every chunk of its page in
+/// every tensor, and one for its tables.
 bool one_entry_fits(int64_t tensors, int64_t chunks) {
     return (tensors < kTensors ? tensors : kTensors) * chunks + 1 <= kMaxWorkgroups;
 }
 
+/// Runs `body` with entries [first, first + n) of a list of `count`, each of
+/// which takes `each` workgroups, in launches of no more than there may be.
 template <typename Body>
 void by_entries(int64_t count, int64_t each, Body body) {
     const int64_t most = kMaxWorkgroups / each;

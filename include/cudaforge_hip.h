@@ -639,7 +639,8 @@ size_t cf_paged_attention_shared_workspace_bytes(cf_dtype dtype, int64_t num_seq
  * tables' reach. num_groups 0: nothing is shared, both may be NULL.
  * k_cache and v_cache hold num_pages blocks: a token whose table entry is not
  * below num_pages is left out, as are contexts' tokens past the table, and past
- * 2^31 - 4096. Sequences without tokens get zeros, and so does a row all of whose scores are -inf.
+ * 2^31 - 4096. Sequences without tokens get zeros, and so does a row all of
+ * whose scores are -inf.
  * Cache rows behind a context's end are never used, whatever they hold.
  * Matrix-core kernels take head sizes that are multiples of 8 up to 256 (fp32:
  * multiples of 4 up to 128) with 16-byte aligned query and caches; every other
