@@ -21,8 +21,10 @@ from cuda_force_amd.ops import (
     gelu,
     kernel_supports,
     lora_linear,
+    matmul_int8,
     quantization_error,
     quantize_int8,
+    quantize_int8_rows,
     rmsnorm,
     row_sum,
     silu,
@@ -38,7 +40,10 @@ from cuda_force_amd.paged_cache import (
     cache_copy,
     cache_extend,
     cache_fork,
+    cache_read,
     cache_release,
+    cache_write,
+    paged_attention_chunk,
     paged_attention_shared,
 )
 
@@ -56,16 +61,21 @@ __all__ = [
     "cache_copy",
     "cache_extend",
     "cache_fork",
+    "cache_read",
     "cache_release",
+    "cache_write",
     "dequantize_int8",
     "fake_quantize_int8",
     "fused_residual_rmsnorm",
     "gelu",
     "kernel_supports",
     "lora_linear",
+    "matmul_int8",
+    "paged_attention_chunk",
     "paged_attention_shared",
     "quantization_error",
     "quantize_int8",
+    "quantize_int8_rows",
     "rmsnorm",
     "row_sum",
     "silu",

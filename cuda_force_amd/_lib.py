@@ -30,6 +30,10 @@ CF_F32 = 0
 CF_F16 = 1
 CF_BF16 = 2
 
+CF_CACHE_PLAIN = 0
+CF_CACHE_INT8 = 1
+CF_CACHE_E4M3 = 2
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int
@@ -106,6 +110,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I32,
         [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P, _SZ, _P],
     ),
+    "cf_cache_write": (
+        _I32,
+        [_P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _P, _I64, _P],
+    ),
+    "cf_cache_read": (_I32, [_P, _P, _I32, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _I32, _P]),
+    "cf_paged_attention_chunk_workspace_bytes": (
+        _SZ,
+        [_I32, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    ),
+    "cf_paged_attention_chunk": (
+        _I32,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P,
+         _SZ, _P],
+    ),
+    "cf_quantize_int8_rows": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "cf_matmul_int8": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _P]),
     "cf_reduce_sum_workspace_bytes": (_SZ, [_I64]),
     "cf_reduce_sum": (_I32, [_P, _I32, _P, _I64, _P, _SZ, _I32, _P]),
     "cf_reduce_sum_noalloc": (_I32, [_P, _I32, _P, _I64, _I32, _P]),

@@ -49,9 +49,12 @@ HIP_SOURCES = (
     "cf_logprobs.hip",
     "cf_pages.hip",
     "cf_shared_attention.hip",
+    "cf_cache_store.hip",
+    "cf_chunk_attention.hip",
+    "cf_matmul_int8.hip",
 )
 
-TORCH_SOURCES = ("torch_ops.cpp", "torch_ops_generation.cpp")
+TORCH_SOURCES = ("torch_ops.cpp", "torch_ops_generation.cpp", "torch_ops_serving.cpp")
 
 # Per-source additions. The fused LoRA kernel accumulates in VGPRs: the
 # compiler's AGPR accumulator allocation rotates registers every K-step.

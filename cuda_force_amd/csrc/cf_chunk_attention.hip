@@ -1,0 +1,1195 @@
+// Causal attention of the newest tokens of every sequence over a paged cache,
+// in the query's type or in 8-bit codes with a scale per row.
+//
+// Row i of sequence s, of n_s new tokens in a context of c_s, is at position
+// p = c_s - n_s + i; for head h and KV head h / (H / KVH):
+//   out = sum_{t <= p} softmax_t(scale q . k[t]) v[t].
+//
+// The rows of a sequence and KV head (tokens x heads of the KV head) against its
+// keys are a matrix product; a row tile of a long chunk is bound by the matrix
+// and vector units, a single token's few rows by HBM.
+//   * A work item is (row tile, KV head, range of the context), a workgroup of
+//     four waves. Tiles with more rows than a wave takes are shared by the
+//     waves, a quarter of the rows each; with fewer, the waves take different
+//     tokens of the same rows. Ranges are cut only where there are few items;
+//     a second kernel joins their pieces.
+//   * 8-bit codes are exact in fp16, so they are widened to it on their way to
+//     LDS and the products run on fp16 tiles whatever the query's type: a bf16
+//     query is scaled by a power of two per row (it has fewer bits than fp16
+//     holds, and what falls below fp16's smallest number is 2^-39 of the row's
+//     largest), an fp32 query is taken as the sum of two fp16 numbers. Keys'
+//     scales multiply the scores, values' scales the probabilities, relative to
+//     a power of two above all scales met so far, all in fp32.
+//   * Tokens that are not there (behind the range, in no page) get no weight and
+//     their values are cleared in LDS.
+#include "cf_attention_tile.hpp"
+#include "cf_codes.hpp"
+#include "cf_common.hpp"
+#include "cf_lds_dma.hpp"
+#include "cf_ranges.hpp"
+
+namespace cf {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWaveSize;
+constexpr int kMaxSplits = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct ChunkArgs {
+    const void* query;
+    const uint8_t* k_cache;
+    const uint8_t* v_cache;
+    const float* k_scales;
+    const float* v_scales;
+    const int32_t* starts;  // [sequences + 1]
+    const uint32_t* tables;
+    const int32_t* context;
+    void* out;
+    float* ml;   // [splits][tokens * heads][2]: maximum (base 2), sum
+    float* acc;  // [splits][tokens * heads][pitch]
+    uint32_t pages;
+    uint32_t block_size;
+    int block_shift;  // log2(block_size), or -1
+    int tokens;
+    int sequences;
+    int heads;
+    int kv_heads;
+    int per;  // query heads per KV head
+    int head_dim;
+    int pitch;  // head_dim rounded up to 4
+    int max_blocks;
+    int capacity;  // tokens a table row reaches
+    int splits;
+    int step;  // tokens of a range are a multiple of this
+    int least;  // and at least about this
+    bool query_bf16;  // of 8-bit caches: the query's and the result's 16-bit type
+    float c;              // |scale| log2(e), above 0
+    uint32_t query_sign;  // flips the query's signs for a negative scale
+};
+
+__device__ __forceinline__ int clamp_to(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
+
+// ---- items ----------------------------------------------------------------------
+
+/// Neighbouring rows (tokens) of one sequence, or of none.
+struct Segment {
+    int sequence;  // -1: rows that no sequence holds
+    int first;     // token
+    int count;
+    int tile;  // of the segment
+};
+
+/// Tile `index` (uniform) of all segments' tiles laid end to end: the rows before
+/// the first start, the sequences', the rows behind the last one. Starts are
+/// taken as the largest so far, so that segments never overlap whatever is
+/// stored. count = 0: no such tile.
+__device__ Segment segment_of(const ChunkArgs& a, int rows, int index) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    int before = 0;  // largest start so far
+    const int segments = a.sequences + 2;
+    for (int base = 0; base < segments; base += kWaveSize) {
+        const int i = base + lane;  // from starts[i - 1] to starts[i]
+        int end = i <= a.sequences ? clamp_to(a.starts[min(i, a.sequences)], a.tokens) : a.tokens;
+        end = max(end, before);
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) {
+            const int o = __shfl_up(end, d);
+            if (lane >= d) end = max(end, o);
+        }
+        int start = __shfl_up(end, 1);
+        if (lane == 0) start = before;
+        const int tiles = i < segments ? static_cast<int>((static_cast<int64_t>(end - start) * a.per + rows - 1) / rows) : 0;
+        int total = tiles;
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) {
+            const int o = __shfl_up(total, d);
+            if (lane >= d) total += o;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(total > index);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            const int n = __builtin_amdgcn_readlane(tiles, at);
+            const int first = __builtin_amdgcn_readlane(start, at);
+            const int sequence = base + at - 1;
+            index -= __builtin_amdgcn_readlane(total, at) - n;
+            // The last tiles of a chunk see most tokens: they come first.
+            return Segment{sequence < a.sequences ? sequence : -1, first, __builtin_amdgcn_readlane(end, at) - first,
+                           n - 1 - index};
+        }
+        index -= __builtin_amdgcn_readlane(total, kWaveSize - 1);
+        before = __builtin_amdgcn_readlane(end, kWaveSize - 1);
+    }
+    return Segment{-1, 0, 0, 0};
+}
+
+/// The segment of one token (uniform).
+__device__ Segment segment_of_token(const ChunkArgs& a, int token) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    int before = 0;
+    const int segments = a.sequences + 2;
+    for (int base = 0; base < segments; base += kWaveSize) {
+        const int i = base + lane;
+        int end = i <= a.sequences ? clamp_to(a.starts[min(i, a.sequences)], a.tokens) : a.tokens;
+        end = max(end, before);
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) {
+            const int o = __shfl_up(end, d);
+            if (lane >= d) end = max(end, o);
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(end > token);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            const int first = at > 0 ? __builtin_amdgcn_readlane(end, at - 1) : before;
+            const int sequence = base + at - 1;
+            return Segment{sequence < a.sequences ? sequence : -1, first, __builtin_amdgcn_readlane(end, at) - first, 0};
+        }
+        before = __builtin_amdgcn_readlane(end, kWaveSize - 1);
+    }
+    return Segment{-1, 0, 0, 0};
+}
+
+/// What a tile of a segment's rows sees.
+struct Reach {
+    int offset;  // position of the segment's first token
+    int hi;      // tokens that the tile's last row sees, at least 0
+    int each;    // tokens per range
+};
+
+__device__ __forceinline__ Reach reach_of(const ChunkArgs& a, const Segment& s, int rows) {
+    Reach r{};
+    const int context = clamp_to(a.context[s.sequence], a.capacity);
+    r.offset = context - s.count;
+    const int64_t last_row = static_cast<int64_t>(s.tile + 1) * rows - 1;
+    const int64_t last_token = last_row / a.per;
+    r.hi = r.offset + (last_token < s.count ? static_cast<int>(last_token) + 1 : s.count);
+    r.hi = r.hi < 0 ? 0 : r.hi;
+    r.each = split_length(r.hi, a.splits, a.step, a.least);
+    return r;
+}
+
+// ---- one work item ----------------------------------------------------------------
+
+struct Item {
+    const uint32_t* table;
+    int lo, hi;
+    int offset;     // position of the segment's first token
+    int first;      // the segment's first token
+    int rows;       // of the segment: tokens x heads of the KV head
+    int first_row;  // of the tile
+    int kv_head;
+    int split;
+    bool direct;    // the only piece: straight to the result
+};
+
+/// kHeld: how the cache holds its rows. T: the type of the tiles. kSplit: an
+/// fp32 query of an 8-bit cache.
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
+struct Kind {
+    using L = Tile<T, kD>;
+    static constexpr bool kCodes = kHeld != CF_CACHE_PLAIN;
+    static constexpr int kStages = kCodes ? 2 : 4;  // of a ring that the waves share
+    static constexpr int kScales = kCodes ? 2 * L::kTokens : 0;  // floats per tile
+    static constexpr int kTileBytes = 2 * L::kBytes + 4 * kScales;
+    static constexpr int lds_bytes() {
+        constexpr int ring = kStages * kTileBytes;
+        constexpr int own = kWaves * kTileBytes;
+        constexpr int outputs = kWaves * L::kRows * L::kOutPitch * 4;
+        constexpr int tiles = ring > own ? ring : own;
+        return tiles > outputs ? tiles : outputs;
+    }
+};
+
+/// 16 codes as fp16, 8 to a vector.
+template <cf_cache_format kHeld>
+__device__ __forceinline__ void widen16(const u32x4_t& codes, u32x4_t& lo, u32x4_t& hi) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t a, b;
+        if constexpr (kHeld == CF_CACHE_INT8) {
+            // 0x64uu is 1024 + u in fp16: u = code + 128 below it, 1152 taken off.
+            typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+            const uint32_t u = codes[i] ^ 0x80808080u;
+            const f16x2_v less = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+            a = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - less);
+            b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - less);
+        } else {
+            typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+            float f[4];
+            unpack4_codes<CF_CACHE_E4M3>(codes[i], f);
+            a = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(f[0]), static_cast<_Float16>(f[1])});
+            b = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(f[2]), static_cast<_Float16>(f[3])});
+        }
+        if (i < 2) {
+            lo[2 * i] = a;
+            lo[2 * i + 1] = b;
+        } else {
+            hi[2 * i - 4] = a;
+            hi[2 * i - 3] = b;
+        }
+    }
+}
+
+/// kShared: the waves take different rows of the tile, else different tokens of
+/// the same rows.
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit, bool kShared>
+__device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
+                       uint32_t* lds_bad) {
+    using K = Kind<T, kD, kHeld, kSplit>;
+    using L = typename K::L;
+    constexpr bool kCodes = K::kCodes;
+    constexpr int kRowWaves = kShared ? kWaves : 1;
+    constexpr int kTokenWaves = kShared ? 1 : kWaves;
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & (kWaveSize - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
+    const int row_wave = kShared ? wave : 0;
+    const int token_wave = kShared ? 0 : wave;
+
+    // This lane's query row; rows past the end are zeros.
+    const int row = w.first_row + row_wave * L::kRows + L::row_of(lane);
+    const bool inside = row < w.rows;
+    const int token = inside ? row / a.per : 0;
+    const int limit = inside ? w.offset + token : -1;  // the last token it sees
+    typename L::Query q[L::kQueries];
+    [[maybe_unused]] typename L::Query q_low[kSplit ? L::kQueries : 1];
+    float c = a.c;
+    {
+        const int64_t out_row = static_cast<int64_t>(w.first + token) * a.heads + w.kv_head * a.per + (inside ? row % a.per : 0);
+        if constexpr (!kCodes) {
+            const T* from = static_cast<const T*>(a.query) + out_row * a.head_dim;
+#pragma unroll
+            for (int u = 0; u < L::kQueries; ++u) {
+                const int dim = L::query_dim(u, lane);
+                u32x4_t raw = {0u, 0u, 0u, 0u};
+                if (inside && dim < a.head_dim) raw = *reinterpret_cast<const u32x4_t*>(from + dim) ^ a.query_sign;
+                q[u] = __builtin_bit_cast(typename L::Query, raw);
+            }
+        } else {
+            // Scaled by a power of two to magnitudes of up to 2^15; the inverse goes to
+            // the scores' factor.
+            float f[L::kQueries][8];
+            float top = 0.0f;
+#pragma unroll
+            for (int u = 0; u < L::kQueries; ++u) {
+                const int dim = L::query_dim(u, lane);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[u][e] = 0.0f;
+                if (inside && dim < a.head_dim) {
+                    if constexpr (kSplit) {
+                        const float* from = static_cast<const float*>(a.query) + out_row * a.head_dim + dim;
+                        unpack16<float>(*reinterpret_cast<const uint4*>(from), f[u]);
+                        unpack16<float>(*reinterpret_cast<const uint4*>(from + 4), f[u] + 4);
+                    } else {
+                        const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) +
+                                                                         out_row * a.head_dim + dim);
+                        if (a.query_bf16) unpack16<bf16_t>(raw, f[u]); else unpack16<f16_t>(raw, f[u]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[u][e]));
+            }
+            top = groups_max<L::kRows>(top);
+            const int lift = 15 - __builtin_amdgcn_frexp_expf(top);
+            // Not 0, which times a masked score is NaN.
+            c = fmaxf(__builtin_amdgcn_ldexpf(c, -lift), 0x1p-126f);
+            const float sign = a.query_sign != 0 ? -1.0f : 1.0f;
+            typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int u = 0; u < L::kQueries; ++u) {
+                u32x4_t high, low;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x0 = __builtin_amdgcn_ldexpf(f[u][2 * e] * sign, lift);
+                    const float x1 = __builtin_amdgcn_ldexpf(f[u][2 * e + 1] * sign, lift);
+                    const f16x2_v h = {static_cast<_Float16>(x0), static_cast<_Float16>(x1)};
+                    high[e] = __builtin_bit_cast(uint32_t, h);
+                    if constexpr (kSplit) {
+                        low[e] = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(x0 - static_cast<float>(h[0])),
+                                                                      static_cast<_Float16>(x1 - static_cast<float>(h[1]))});
+                    }
+                }
+                q[u] = __builtin_bit_cast(typename L::Query, high);
+                if constexpr (kSplit) q_low[u] = __builtin_bit_cast(typename L::Query, low);
+            }
+        }
+    }
+    // The smallest of the wave's limits: tiles up to it need no mask.
+    int least = inside ? limit : 0x7FFFFFFF;
+#pragma unroll
+    for (int d = 1; d < L::kRows; d <<= 1) least = min(least, __shfl_xor(least, d));
+    const int wave_least = __builtin_amdgcn_readfirstlane(least);
+
+    uint8_t* const own = lds + (kShared ? 0 : wave * K::kTileBytes);
+    if (a.head_dim < kD) {  // the copies leave the end of every row as it is
+        constexpr int kPieces = (kShared ? K::kStages : 1) * K::kTileBytes / 16;
+        for (int i = kShared ? tid : lane; i < kPieces; i += kShared ? kThreads : kWaveSize) {
+            reinterpret_cast<u32x4_t*>(own)[i] = u32x4_t{0u, 0u, 0u, 0u};
+        }
+        if constexpr (kShared) __syncthreads(); else wait_lds();
+    }
+
+    // Tiles begin at multiples of kTokens (ranges do).
+    const int begin = w.lo + token_wave * L::kTokens;
+    constexpr int kStride = kTokenWaves * L::kTokens;
+    const int tiles = begin < w.hi ? (w.hi - begin + kStride - 1) / kStride : 0;
+    const int last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
+
+    // 64 entries of the block table in lane registers: looking a page up is then
+    // no load that would have to wait behind the copies.
+    auto block_of = [&](int t) {
+        return static_cast<int>(a.block_shift >= 0 ? static_cast<uint32_t>(t) >> a.block_shift
+                                                   : static_cast<uint32_t>(t) / a.block_size);
+    };
+    int window_base = block_of(begin < w.hi ? begin : w.lo);
+    uint32_t window = w.table[min(window_base + lane, last_block)];
+    uint32_t valid = 0;  // tokens of the tile looked up last, a bit each
+    uint32_t place = 0;  // of token lane % kTokens: row of the cache, 0 where it is not there
+    constexpr uint32_t kAll = 0xFFFFFFFFu >> (32 - L::kTokens);
+    auto look_up = [&](int first) {
+        const int last = min(first + L::kTokens, w.hi) - 1;
+        if (block_of(last) >= window_base + kWaveSize) {
+            window_base = block_of(first);
+            window = w.table[min(window_base + lane, last_block)];
+            // Waited for here, not behind the branch, whether or not this ran.
+            asm volatile("" : "+v"(window));
+        }
+        const int t = min(first + (lane & (L::kTokens - 1)), last);
+        const int block = block_of(t);
+        const uint32_t page = static_cast<uint32_t>(__shfl(static_cast<int>(window), block - window_base));
+        const bool there = page < a.pages && first + (lane & (L::kTokens - 1)) < w.hi;
+        place = there ? page * a.block_size + (static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size) : 0u;
+        valid = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(there)) & kAll;
+    };
+
+    const uint32_t lds_own = __builtin_amdgcn_readfirstlane(lds_address(own));
+    const int held_size = kCodes ? 1 : static_cast<int>(sizeof(T));
+    const uint64_t token_bytes = static_cast<uint64_t>(a.kv_heads) * a.head_dim * held_size;
+    const uint64_t head_bytes = static_cast<uint64_t>(w.kv_head) * a.head_dim * held_size;
+    const uint8_t* k_head = a.k_cache + head_bytes;
+    const uint8_t* v_head = a.v_cache + head_bytes;
+
+    // Plain caches: this wave's copies of a tile to LDS; of a shared one half of the
+    // waves copy K, the others V.
+    constexpr int kPerCopy = kWaveSize / L::kChunks;
+    constexpr int kCopies = kShared ? 2 * L::kCopies / kWaves : L::kCopies;
+    const bool shared_v = kShared && wave >= kWaves / 2;
+    const int first_copy = kShared ? wave % (kWaves / 2) * kCopies : 0;
+    const int row_pieces = a.head_dim * held_size / 16;
+    [[maybe_unused]] auto copy = [&](uint32_t dst, bool is_v) {
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) {
+            const int r = (first_copy + n) * kPerCopy + lane / L::kChunks;
+            const uint64_t from = static_cast<uint32_t>(__shfl(static_cast<int>(place), r)) * token_bytes;
+            const int piece = (lane % L::kChunks) ^ (is_v ? L::v_swizzle(r) : L::k_swizzle(r));
+            if (piece < row_pieces) {
+                copy16_to_lds((is_v ? v_head : k_head) + from + piece * 16,
+                              dst + static_cast<uint32_t>(first_copy + n) * 16 * kWaveSize);
+            }
+        }
+    };
+    // 8-bit caches: 16 codes a lane and load, this wave's share of a tile, and one
+    // scale (lanes 0 .. kTokens - 1 of K, the others of V).
+    constexpr int kCodeLanes = kD / 16;                  // per token
+    constexpr int kCodeTokens = kWaveSize / kCodeLanes;  // per load
+    constexpr int kLoads = L::kTokens / kCodeTokens;     // of K or V of a tile
+    constexpr int kShare = kShared ? 2 * kLoads / kWaves : 2 * kLoads;
+    static_assert(!kCodes || kShare * (kShared ? kWaves : 1) == 2 * kLoads, "loads per wave");
+    [[maybe_unused]] u32x4_t raw[kCodes ? kShare : 1];
+    [[maybe_unused]] float raw_scale = 0.0f;
+    [[maybe_unused]] uint32_t raw_valid = 0;
+    [[maybe_unused]] auto load_codes = [&]() {
+#pragma unroll
+        for (int n = 0; n < kShare; ++n) {
+            const int at = (kShared ? wave * kShare : 0) + n;  // K's loads, then V's
+            const int r = at % kLoads * kCodeTokens + lane / kCodeLanes;
+            const uint64_t from = static_cast<uint32_t>(__shfl(static_cast<int>(place), r)) * token_bytes;
+            const int piece = lane % kCodeLanes;
+            raw[n] = u32x4_t{0u, 0u, 0u, 0u};
+            if (piece < row_pieces && ((valid >> r) & 1) != 0) {
+                raw[n] = *reinterpret_cast<const u32x4_t*>((at < kLoads ? k_head : v_head) + from + piece * 16);
+            }
+        }
+        const int t = lane & (L::kTokens - 1);
+        const int64_t scale_at = static_cast<int64_t>(static_cast<uint32_t>(place)) * a.kv_heads + w.kv_head;
+        raw_scale = ((valid >> t) & 1) != 0 ? (lane < L::kTokens ? a.k_scales : a.v_scales)[scale_at] : 0.0f;
+        raw_valid = valid;
+    };
+    [[maybe_unused]] auto store_codes = [&](uint8_t* tile) {
+#pragma unroll
+        for (int n = 0; n < kShare; ++n) {
+            const int at = (kShared ? wave * kShare : 0) + n;
+            const int r = at % kLoads * kCodeTokens + lane / kCodeLanes;
+            const bool is_v = at >= kLoads;
+            const int sw = is_v ? L::v_swizzle(r) : L::k_swizzle(r);
+            const int piece = lane % kCodeLanes;
+            u32x4_t lo, hi;
+            widen16<kCodes ? kHeld : CF_CACHE_INT8>(raw[n], lo, hi);
+            uint8_t* to = tile + (is_v ? L::kBytes : 0) + r * L::kRowBytes;
+            if (piece < row_pieces) {
+                *reinterpret_cast<u32x4_t*>(to + (((2 * piece) ^ sw) << 4)) = lo;
+                *reinterpret_cast<u32x4_t*>(to + (((2 * piece + 1) ^ sw) << 4)) = hi;
+            }
+        }
+        // Of a shared tile every wave has all scales.
+        if (!kShared || wave == 0) reinterpret_cast<float*>(tile + 2 * L::kBytes)[lane] = raw_scale;
+    };
+
+    float m = -INFINITY;  // the row's running maximum
+    float l = 0.0f;       // this lane's share of the running sum
+    [[maybe_unused]] float unit = 0.0f;     // above all values' scales the row met, a power of two
+    [[maybe_unused]] float inverse = 0.0f;  // of it
+    typename L::Score acc[L::kAcc / L::kScores];
+#pragma unroll
+    for (int b = 0; b < L::kAcc / L::kScores; ++b) {
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) acc[b][i] = 0.0f;
+    }
+    auto rescale = [&](float f) {
+#pragma unroll
+        for (int b = 0; b < L::kAcc / L::kScores; ++b) {
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) acc[b][i] *= f;
+        }
+    };
+    // The tokens of the tile at `first` that this lane's row sees, of the valid ones.
+    auto seen = [&](int first, uint32_t there) {
+        const int count = limit - first + 1;
+        return there & (count >= L::kTokens ? kAll : count <= 0 ? 0u : (1u << count) - 1u);
+    };
+    auto clear = [&](uint8_t* v, uint32_t there, int start, int step) {
+        for (int i = start; i < L::kTokens * L::kChunks; i += step) {
+            if (((there >> (i / L::kChunks)) & 1) == 0) reinterpret_cast<u32x4_t*>(v)[i] = u32x4_t{0u, 0u, 0u, 0u};
+        }
+    };
+    // Scores of a tile to weights, and the running values.
+    auto soften = [&](typename L::Score& s, const uint8_t* tile, int first, uint32_t there) {
+        const bool masked = there != kAll || first + L::kTokens - 1 > wave_least;
+        const uint32_t mine = masked ? seen(first, there) >> (4 * L::part_of(lane)) : 0u;
+        [[maybe_unused]] const float* scales = reinterpret_cast<const float*>(tile + 2 * L::kBytes) + 4 * L::part_of(lane);
+        if constexpr (kCodes) {
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) s[i] *= scales[L::token_of(i)];
+        }
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) s[i] = (mine & (1u << L::token_of(i))) != 0 ? s[i] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < L::kScores; ++i) top = fmaxf(top, s[i]);
+        top = groups_max<L::kRows>(top);
+        const float m_new = fmaxf(m, top * c);
+        if (__builtin_amdgcn_ballot_w64(m_new > m + L::kLag) != 0) {
+            const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+            l *= f;
+            rescale(f);
+            m = m_new;
+        }
+        const float shift = (m == -INFINITY ? 0.0f : m) - L::kLift;
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -shift));
+            l += s[i];
+        }
+        if constexpr (kCodes) {
+            float by[L::kScores];
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) {
+                by[i] = scales[L::kTokens + L::token_of(i)];
+                // What a row does not see may be NaN, or far above its own scales.
+                if (masked) by[i] = (mine & (1u << L::token_of(i))) != 0 ? by[i] : 0.0f;
+                most = fmaxf(most, fabsf(by[i]));
+            }
+            most = groups_max<L::kRows>(most);
+            if (__builtin_amdgcn_ballot_w64(most >= unit) != 0) {
+                uint32_t exponent = __float_as_uint(most) >> 23;
+                exponent = exponent < 1 ? 1 : exponent > 252 ? 252 : exponent;
+                const float above = __uint_as_float((exponent + 1) << 23);
+                const float old = unit;
+                if (above > unit) {
+                    unit = above;
+                    inverse = __uint_as_float((253 - exponent) << 23);
+                }
+                rescale(old * inverse);
+            }
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) s[i] *= by[i] * inverse;
+        }
+    };
+    auto scores = [&](const uint8_t* k) {
+        typename L::Score s = L::scores(k, q, lane);
+        if constexpr (kSplit) {
+            const typename L::Score low = L::scores(k, q_low, lane);
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) s[i] += low[i];
+        }
+        return s;
+    };
+    // A token that a row of the tile does not see may hold NaN or infinities, which
+    // times a weight of 0 would reach that row. In such tiles they are replaced by 0,
+    // and a row that sees one gets a sum of NaN.
+    auto guard = [&](uint8_t* v, int first, uint32_t there) {
+        if (min(first + L::kTokens, w.hi) - 1 <= w.offset + w.first_row / a.per) return;
+        constexpr uint32_t kExponent = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, f16_t>::value ? 0x7C00u : 0x7F80u;
+        uint32_t bad = 0;  // tokens
+#pragma unroll 1
+        for (int i = kShared ? tid : lane; i < L::kTokens * L::kChunks; i += kShared ? kThreads : kWaveSize) {
+            u32x4_t four = reinterpret_cast<const u32x4_t*>(v)[i];
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool low = (four[e] & kExponent) == kExponent;
+                const bool high = sizeof(T) == 2 && (four[e] >> 16 & kExponent) == kExponent;
+                any = any || low || high;
+                four[e] &= (low ? (sizeof(T) == 2 ? 0xFFFF0000u : 0u) : 0xFFFFFFFFu) & (high ? 0xFFFFu : 0xFFFFFFFFu);
+            }
+            if (any) {
+                reinterpret_cast<u32x4_t*>(v)[i] = four;
+                bad |= 1u << (i / L::kChunks);
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) bad |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(bad), d));
+        if constexpr (kShared) {
+            if (lane == 0) lds_bad[wave] = bad;
+            __syncthreads();
+            bad = lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3];
+        } else {
+            wait_lds();
+        }
+        if ((bad & seen(first, there)) != 0) l = __uint_as_float(0x7FC00000u);
+    };
+    auto add_values = [&](uint8_t* v, typename L::Score& s, int first, uint32_t there) {
+        guard(v, first, there);
+        L::values(v, s, acc, lane);
+        if constexpr (kSplit) {
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) s[i] -= static_cast<float>(static_cast<_Float16>(s[i]));
+            L::values(v, s, acc, lane);
+        }
+    };
+
+    if constexpr (kCodes) {
+        if (tiles > 0) {
+            look_up(begin);
+            load_codes();
+        }
+        // A tile is widened into LDS while the next one's codes are on their way; of a
+        // shared ring each barrier ends the reading of one stage and the writing of
+        // the other.
+        if constexpr (kShared) {
+            store_codes(own);
+            uint32_t there = raw_valid;
+            if (tiles > 1) {
+                look_up(begin + kStride);
+                load_codes();
+            }
+            __syncthreads();
+            for (int i = 0; i < tiles; ++i) {
+                uint8_t* tile = lds + (i & 1) * K::kTileBytes;
+                const int first = begin + i * kStride;
+                const uint32_t now = there;
+                if (i + 1 < tiles) {
+                    store_codes(lds + ((i + 1) & 1) * K::kTileBytes);
+                    there = raw_valid;
+                    if (i + 2 < tiles) {
+                        look_up(first + 2 * kStride);
+                        load_codes();
+                    }
+                }
+                typename L::Score s = scores(tile);
+                soften(s, tile, first, now);
+                add_values(tile + L::kBytes, s, first, now);
+                __syncthreads();
+            }
+        } else {
+            for (int i = 0; i < tiles; ++i) {
+                const int first = begin + i * kStride;
+                store_codes(own);
+                const uint32_t there = raw_valid;
+                if (i + 1 < tiles) {
+                    look_up(first + kStride);
+                    load_codes();
+                }
+                wait_lds();
+                typename L::Score s = scores(own);
+                soften(s, own, first, there);
+                add_values(own + L::kBytes, s, first, there);
+                wait_lds();
+            }
+        }
+    } else if constexpr (!kShared) {
+        // The wave's own K and V tile, one copied while the other is used.
+        const uint32_t v_dst = lds_own + L::kBytes;
+        uint8_t* v = own + L::kBytes;
+        if (tiles > 0) {
+            look_up(begin);
+            copy(lds_own, false);
+            copy(v_dst, true);
+        }
+        for (int i = 0; i < tiles; ++i) {
+            const int first = begin + i * kStride;
+            const bool more = i + 1 < tiles;
+            // K has landed: only V's copies may be in flight. (Copies that no lane takes
+            // part in are not issued, so a head narrower than kD waits for all.)
+            if (a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
+            const uint32_t there = valid;
+            typename L::Score s = scores(own);
+            wait_lds();
+            if (more) {
+                look_up(first + kStride);
+                copy(lds_own, false);
+            }
+            soften(s, own, first, there);
+            if (more && a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
+            if (there != kAll) {
+                clear(v, there, lane, kWaveSize);
+                wait_lds();
+            }
+            add_values(v, s, first, there);
+            wait_lds();
+            if (more) copy(v_dst, true);
+        }
+    } else {
+        // A ring of tiles, all but one of them in flight.
+        constexpr int kStages = K::kStages;
+        uint32_t there[kStages];
+        auto issue = [&](int i, int at) {
+            look_up(begin + i * kStride);
+            there[at] = valid;
+            const uint32_t dst = lds_own + static_cast<uint32_t>(at) * K::kTileBytes;
+            copy(shared_v ? dst + L::kBytes : dst, shared_v);
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) {
+            there[i] = 0;
+            if (i < tiles) issue(i, i);
+        }
+        there[kStages - 1] = 0;
+        // The ring's steps written out, so that LDS addresses are constants.
+        auto step = [&](auto at, int i) {
+            constexpr int kAt = decltype(at)::value;
+            // This wave's copies of tile i have landed; those of the tiles behind it
+            // (fewer at the end) are in flight.
+            if (i + kStages - 2 < tiles && a.head_dim == kD) wait_vm<(kStages - 2) * kCopies>(); else wait_vm<0>();
+            bare_barrier();  // and every wave is past tile i - 1, whose place is filled next
+            const uint32_t now = there[kAt];
+            if (i + kStages - 1 < tiles) issue(i + kStages - 1, (kAt + kStages - 1) % kStages);
+            uint8_t* k = lds + kAt * K::kTileBytes;
+            uint8_t* v = k + L::kBytes;
+            typename L::Score s = scores(k);
+            soften(s, k, begin + i * kStride, now);
+            if (now != kAll) {
+                clear(v, now, tid, kThreads);
+                __syncthreads();
+            }
+            add_values(v, s, begin + i * kStride, now);
+            wait_lds();  // before the barrier that lets the tile be overwritten
+        };
+        static_assert(kStages == 4, "four steps");
+        for (int i = 0; i < tiles; i += kStages) {
+            step(std::integral_constant<int, 0>{}, i);
+            if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
+            if (i + 2 < tiles) step(std::integral_constant<int, 2>{}, i + 2);
+            if (i + 3 < tiles) step(std::integral_constant<int, 3>{}, i + 3);
+        }
+    }
+
+#pragma unroll
+    for (int d = L::kRows; d < kWaveSize; d <<= 1) l += __shfl_xor(l, d);
+    if constexpr (kCodes) rescale(unit);  // units may differ between waves
+    wait_vm<0>();
+    __syncthreads();  // all tiles are done with: their space takes the outputs
+    float* mine = reinterpret_cast<float*>(lds) + wave * L::kRows * L::kOutPitch;
+#pragma unroll
+    for (int i = 0; i < L::kAcc; i += 4) {
+        f32x4_t four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = acc[(i + e) / L::kScores][(i + e) % L::kScores];
+        *reinterpret_cast<f32x4_t*>(mine + L::row_of(lane) * L::kOutPitch + L::dim_of(i, lane)) = four;
+    }
+    if (L::part_of(lane) == 0) {
+        lds_m[wave][L::row_of(lane)] = m;
+        lds_l[wave][L::row_of(lane)] = l;
+    }
+    __syncthreads();
+    // Rows x groups of four dims, over the workgroup; token waves are joined.
+    constexpr int kOutRows = kRowWaves * L::kRows;
+    constexpr int kFours = kD / 4;
+    constexpr int kRounds = (kOutRows * kFours + kThreads - 1) / kThreads;
+#pragma unroll 2
+    for (int n = 0; n < kRounds; ++n) {
+        const int i = n * kThreads + tid;
+        const int r = i / kFours;
+        const int dim = (i % kFours) * 4;
+        if (r >= kOutRows) break;
+        const int out = w.first_row + r;
+        if (out >= w.rows || dim >= a.head_dim) continue;
+        const int owner = kShared ? r / L::kRows : 0;
+        const int lr = r % L::kRows;
+        const int64_t out_row = static_cast<int64_t>(w.first + out / a.per) * a.heads + w.kv_head * a.per + out % a.per;
+        float mm = lds_m[owner][lr];
+#pragma unroll
+        for (int t = 1; t < kTokenWaves; ++t) mm = fmaxf(mm, lds_m[t][lr]);
+        float ll = 0.0f;
+        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < kTokenWaves; ++t) {
+            const int src = owner + t;
+            const float f = kTokenWaves == 1 ? 1.0f : lds_m[src][lr] == -INFINITY ? 0.0f : exp2f(lds_m[src][lr] - mm);
+            // A wave without a finite score still passes its NaN on.
+            ll += kTokenWaves > 1 && lds_m[src][lr] == -INFINITY ? lds_l[src][lr] : lds_l[src][lr] * f;
+            const f32x4_t four = *reinterpret_cast<const f32x4_t*>(
+                reinterpret_cast<const float*>(lds) + (src * L::kRows + lr) * L::kOutPitch + dim);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(four[e], f, sum[e]);
+        }
+        if (w.direct) {
+            const float by = ll == 0.0f ? 0.0f : 1.0f / ll;
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = ll == 0.0f ? 0.0f : sum[e] * by;
+            const int64_t at = out_row * a.head_dim + dim;
+            if constexpr (kSplit || (!kCodes && sizeof(T) == 4)) {
+                *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at) = f32x4_t{o[0], o[1], o[2], o[3]};
+            } else {
+                const bool bf16 = kCodes ? a.query_bf16 : std::is_same<T, bf16_t>::value;
+                uint2 two;
+                if (bf16) {
+                    two = make_uint2(Storage<bf16_t>::to_bits2(o[0], o[1]), Storage<bf16_t>::to_bits2(o[2], o[3]));
+                } else {
+                    two = make_uint2(Storage<f16_t>::to_bits2(o[0], o[1]), Storage<f16_t>::to_bits2(o[2], o[3]));
+                }
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = two;
+            }
+            continue;
+        }
+        const int64_t at = static_cast<int64_t>(w.split) * a.tokens * a.heads + out_row;
+        if (dim == 0) {
+            a.ml[2 * at] = mm;
+            a.ml[2 * at + 1] = ll;
+        }
+        *reinterpret_cast<f32x4_t*>(a.acc + at * a.pitch + dim) = sum;
+    }
+}
+
+/// Zeros for the rows first_row .. first_row + count - 1 of a KV head's heads,
+/// counted from token `first`.
+template <typename O>
+__device__ void zero_rows(const ChunkArgs& a, int first, int kv_head, int first_row, int end_row) {
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(end_row - first_row) * a.head_dim; i += kThreads) {
+        const int r = first_row + static_cast<int>(i / a.head_dim);
+        const int64_t out_row = static_cast<int64_t>(first + r / a.per) * a.heads + kv_head * a.per + r % a.per;
+        static_cast<O*>(a.out)[out_row * a.head_dim + i % a.head_dim] = O{};
+    }
+}
+
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_kernel(ChunkArgs a) {
+    using K = Kind<T, kD, kHeld, kSplit>;
+    using L = typename K::L;
+    using O = std::conditional_t<kSplit, float, T>;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[K::lds_bytes()];
+    __shared__ float lds_m[kWaves][32];
+    __shared__ float lds_l[kWaves][32];
+    __shared__ uint32_t lds_bad[kWaves];
+    constexpr int kRows = kWaves * L::kRows;
+    // KV heads vary fastest: workgroup i runs on XCD i % 8, so with 8 of them an
+    // XCD reads one head's keys and values.
+    int id = static_cast<int>(blockIdx.x);
+    Item w{};
+    w.kv_head = id % a.kv_heads;
+    id /= a.kv_heads;
+    w.split = id % a.splits;
+    const Segment s = segment_of(a, kRows, id / a.splits);
+    if (s.count == 0) return;
+    w.first = s.first;
+    w.rows = s.count * a.per;
+    w.first_row = s.tile * kRows;
+    const int end_row = min(w.rows, w.first_row + kRows);
+    Reach reach{};
+    if (s.sequence >= 0) reach = reach_of(a, s, kRows);
+    const Range range = range_of(0, reach.hi, reach.each, w.split);
+    if (range.lo >= range.hi) {
+        if (reach.hi == 0 && w.split == 0) zero_rows<O>(a, s.first, w.kv_head, w.first_row, end_row);
+        return;
+    }
+    w.lo = range.lo;
+    w.hi = range.hi;
+    w.offset = reach.offset;
+    w.table = a.tables + static_cast<int64_t>(s.sequence) * a.max_blocks;
+    w.direct = reach.each >= reach.hi;
+    if (end_row - w.first_row > L::kRows) {
+        attend<T, kD, kHeld, kSplit, true>(a, w, lds, lds_m, lds_l, lds_bad);
+    } else {
+        attend<T, kD, kHeld, kSplit, false>(a, w, lds, lds_m, lds_l, lds_bad);
+    }
+}
+
+/// The general kernel: any head size and alignment, a wave per (token, head,
+/// range), a token of the context at a time, dims over the lanes.
+template <typename T, cf_cache_format kHeld, int kPer>
+__global__ __launch_bounds__(kThreads) void chunk_attention_any_kernel(ChunkArgs a) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * kWaves +
+                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWaveSize);
+    if (id >= static_cast<int64_t>(a.tokens) * a.heads * a.splits) return;
+    const int split = static_cast<int>(id % a.splits);
+    const int64_t out_row = id / a.splits;
+    const int head = static_cast<int>(out_row % a.heads);
+    const int token = static_cast<int>(out_row / a.heads);
+    Segment s = segment_of_token(a, token);
+    T* out = static_cast<T*>(a.out) + out_row * a.head_dim;
+    Reach reach{};
+    if (s.sequence >= 0) {
+        s.tile = token - s.first;
+        reach = reach_of(a, s, a.per);
+    }
+    const Range range = range_of(0, reach.hi, reach.each, split);
+    if (range.lo >= range.hi) {
+        if (reach.hi == 0 && split == 0) {
+            for (int d = lane; d < a.head_dim; d += kWaveSize) Storage<T>::store(out + d, 0.0f);
+        }
+        return;
+    }
+    const T* q = static_cast<const T*>(a.query) + out_row * a.head_dim;
+    float qv[kPer];
+    float acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int d = lane + i * kWaveSize;
+        qv[i] = d < a.head_dim ? Storage<T>::load(q + d) : 0.0f;
+        acc[i] = 0.0f;
+    }
+    auto value = [&](const uint8_t* cache, int64_t at) {
+        if constexpr (kHeld == CF_CACHE_PLAIN) {
+            return Storage<T>::load(reinterpret_cast<const T*>(cache) + at);
+        } else {
+            float f[4];
+            unpack4_codes<kHeld>(cache[at], f);
+            return f[0];
+        }
+    };
+    float m = -INFINITY;
+    float l = 0.0f;
+    for (int t = range.lo; t < range.hi; ++t) {
+        const uint32_t block = static_cast<uint32_t>(t) / a.block_size;
+        const uint32_t page = a.tables[static_cast<int64_t>(s.sequence) * a.max_blocks + block];
+        if (page >= a.pages) continue;
+        const int64_t row = static_cast<int64_t>(page) * a.block_size + (static_cast<uint32_t>(t) - block * a.block_size);
+        const int64_t held = row * a.kv_heads + head / a.per;
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int d = lane + i * kWaveSize;
+            if (d < a.head_dim) dot = fmaf(qv[i], value(a.k_cache, held * a.head_dim + d), dot);
+        }
+        float y = wave_reduce_f32<AddF32>(dot) * (a.query_sign != 0 ? -a.c : a.c);
+        float by = 1.0f;
+        if constexpr (kHeld != CF_CACHE_PLAIN) {
+            y *= a.k_scales[held];
+            by = a.v_scales[held];
+        }
+        const float m_new = fmaxf(m, y);
+        const float shift = m_new == -INFINITY ? 0.0f : m_new;
+        const float f = exp2f(m - shift);
+        const float p = exp2f(y - shift);
+        m = m_new;
+        l = fmaf(l, f, p);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int d = lane + i * kWaveSize;
+            if (d < a.head_dim) acc[i] = fmaf(acc[i], f, p * by * value(a.v_cache, held * a.head_dim + d));
+        }
+    }
+    if (reach.each >= reach.hi) {
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int d = lane + i * kWaveSize;
+            if (d < a.head_dim) Storage<T>::store(out + d, l == 0.0f ? 0.0f : acc[i] * by);
+        }
+        return;
+    }
+    const int64_t at = static_cast<int64_t>(split) * a.tokens * a.heads + out_row;
+    if (lane == 0) {
+        a.ml[2 * at] = m;
+        a.ml[2 * at + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int d = lane + i * kWaveSize;
+        if (d < a.head_dim) a.acc[at * a.pitch + d] = acc[i];
+    }
+}
+
+/// Joins the pieces of one (token, head), a wave each. Rows of one piece are there
+/// already. `rows`: of the first kernel's tiles.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void chunk_attention_join_kernel(ChunkArgs a, int rows) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
+    const int64_t all = static_cast<int64_t>(a.tokens) * a.heads;
+    const int64_t out_row = static_cast<int64_t>(blockIdx.x) * kWaves +
+                            __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWaveSize);
+    if (out_row >= all) return;
+    const int token = static_cast<int>(out_row / a.heads);
+    Segment s = segment_of_token(a, token);
+    if (s.sequence < 0) return;
+    const int64_t row = static_cast<int64_t>(token - s.first) * a.per + out_row % a.heads % a.per;
+    s.tile = static_cast<int>(row / rows);
+    const Reach reach = reach_of(a, s, rows);
+    const int pieces = range_count(reach.hi, reach.each);
+    if (pieces <= 1) return;
+    static_assert(kMaxSplits <= kWaveSize, "a piece per lane");
+    float pm = -INFINITY;
+    float pl = 0.0f;
+    if (lane < pieces) {
+        pm = a.ml[2 * (lane * all + out_row)];
+        pl = a.ml[2 * (lane * all + out_row) + 1];
+    }
+    const float m = wave_reduce_f32<MaxF32>(pm);
+    const float weight = pm == -INFINITY ? 0.0f : exp2f(pm - m);
+    const float l = wave_reduce_f32<AddF32>(pm == -INFINITY ? pl : pl * weight);
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + out_row * a.head_dim;
+    for (int d = lane; d < (a.head_dim + kWaveSize - 1) / kWaveSize * kWaveSize; d += kWaveSize) {
+        float o = 0.0f;
+        for (int i = 0; i < pieces; ++i) {
+            const float f = readlane_f32(weight, i);
+            if (d < a.head_dim) o = fmaf(a.acc[(i * all + out_row) * a.pitch + d], f, o);
+        }
+        if (d < a.head_dim) Storage<T>::store(out + d, l == 0.0f ? 0.0f : o * inverse);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------
+
+struct Plan {
+    int dim;   // head size of the matrix kernel, or 0: the general kernel
+    int rows;  // of a tile
+    int splits;
+    int step;
+    int least;
+};
+
+Plan plan_of(cf_dtype dtype, cf_cache_format format, int64_t tokens, int64_t sequences, int64_t heads,
+             int64_t kv_heads, int64_t head_dim, int64_t capacity) {
+    Plan p{};
+    const int64_t per = heads / kv_heads;
+    const bool wide = dtype == CF_F32 && format == CF_CACHE_PLAIN;
+    const int64_t vec = format != CF_CACHE_PLAIN ? 16 : wide ? 4 : 8;
+    if (head_dim % vec == 0 && head_dim <= (wide ? 128 : 256)) p.dim = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    const int64_t wave_rows = wide ? 16 : 32;
+    p.rows = static_cast<int>(p.dim == 0 ? per : kWaves * wave_rows);
+    auto splits = [&](int64_t items, int64_t target, int64_t least) {
+        int64_t n = items > 0 ? target / items : 1;
+        const int64_t most = ceil_div<int64_t>(capacity, least);
+        if (n > most) n = most;
+        if (n > kMaxSplits) n = kMaxSplits;
+        return static_cast<int>(n < 1 ? 1 : n);
+    };
+    if (p.dim == 0) {
+        p.step = 32;
+        p.least = 64;
+        p.splits = splits(tokens * heads, 4096, p.least);
+        return p;
+    }
+    p.step = static_cast<int>(kWaves * wave_rows);
+    p.least = 256;
+    const int64_t tiles = tokens * per / p.rows + (sequences < tokens ? sequences : tokens);
+    p.splits = splits(tiles * kv_heads, 512, p.least);
+    return p;
+}
+
+int64_t capacity_of(int64_t max_blocks, int64_t block_size) {
+    return max_blocks > kMostTokens / block_size ? kMostTokens : max_blocks * block_size;
+}
+
+size_t workspace_of(const Plan& p, int64_t tokens, int64_t heads, int64_t head_dim) {
+    if (p.splits == 1) return 0;
+    const size_t rows = static_cast<size_t>(p.splits) * tokens * heads;
+    return (rows * 8 + 15) / 16 * 16 + rows * ((head_dim + 3) / 4 * 4) * 4;
+}
+
+bool sizes_ok(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
+              int64_t block_size, int64_t max_blocks) {
+    return tokens > 0 && sequences >= 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && head_dim <= 1024 &&
+           block_size > 0 && max_blocks > 0 && heads % kv_heads == 0;
+}
+
+/// Row tiles of all segments, at most: one more than the rows fill for each.
+int64_t tiles_of(const Plan& p, int64_t tokens, int64_t sequences, int64_t per) {
+    return tokens * per / p.rows + sequences + 2;
+}
+
+template <typename T, cf_cache_format kHeld, bool kSplit>
+void run_matrix(const ChunkArgs& a, const Plan& p, dim3 grid, hipStream_t stream) {
+    if (p.dim == 64) {
+        launch(chunk_attention_kernel<T, 64, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
+    } else if (p.dim == 128) {
+        launch(chunk_attention_kernel<T, 128, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
+    } else if constexpr (kHeld != CF_CACHE_PLAIN || sizeof(T) == 2) {
+        launch(chunk_attention_kernel<T, 256, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
+    }
+}
+
+template <typename T, cf_cache_format kHeld>
+void run(const ChunkArgs& a, const Plan& p, int64_t tiles, hipStream_t stream) {
+    const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+    if (p.dim == 0) {
+        const dim3 grid(static_cast<unsigned>(ceil_div<int64_t>(rows * a.splits, kWaves)));
+        if (a.head_dim <= 128) {
+            launch(chunk_attention_any_kernel<T, kHeld, 2>, grid, dim3(kThreads), 0, stream, a);
+        } else {
+            launch(chunk_attention_any_kernel<T, kHeld, 16>, grid, dim3(kThreads), 0, stream, a);
+        }
+    } else {
+        const dim3 grid(static_cast<unsigned>(tiles * a.splits * a.kv_heads));
+        if constexpr (kHeld == CF_CACHE_PLAIN) {
+            run_matrix<T, kHeld, false>(a, p, grid, stream);
+        } else if constexpr (sizeof(T) == 4) {
+            run_matrix<f16_t, kHeld, true>(a, p, grid, stream);
+        } else {
+            run_matrix<f16_t, kHeld, false>(a, p, grid, stream);
+        }
+    }
+    if (a.splits > 1) {
+        launch(chunk_attention_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div<int64_t>(rows, kWaves))),
+               dim3(kThreads), 0, stream, a, p.rows);
+    }
+}
+
+template <typename T>
+void run_format(cf_cache_format format, const ChunkArgs& a, const Plan& p, int64_t tiles, hipStream_t stream) {
+    switch (format) {
+        case CF_CACHE_PLAIN: run<T, CF_CACHE_PLAIN>(a, p, tiles, stream); break;
+        case CF_CACHE_INT8: run<T, CF_CACHE_INT8>(a, p, tiles, stream); break;
+        case CF_CACHE_E4M3: run<T, CF_CACHE_E4M3>(a, p, tiles, stream); break;
+    }
+}
+
+}  // namespace
+}  // namespace cf
+
+extern "C" {
+
+size_t cf_paged_attention_chunk_workspace_bytes(cf_dtype dtype, cf_cache_format format, int64_t num_tokens,
+                                                int64_t num_sequences, int64_t num_heads, int64_t num_kv_heads,
+                                                int64_t head_dim, int64_t block_size,
+                                                int64_t max_blocks_per_sequence) {
+    if (!cf::valid_dtype(dtype) || !cf::valid_format(format) ||
+        !cf::sizes_ok(num_tokens, num_sequences, num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_sequence)) {
+        return 0;
+    }
+    const cf::Plan p = cf::plan_of(dtype, format, num_tokens, num_sequences, num_heads, num_kv_heads, head_dim,
+                                   cf::capacity_of(max_blocks_per_sequence, block_size));
+    return cf::workspace_of(p, num_tokens, num_heads, head_dim);
+}
+
+cf_status cf_paged_attention_chunk(const void* query, const void* k_cache, const void* v_cache, const float* k_scales,
+                                   const float* v_scales, const int32_t* query_starts, const uint32_t* block_tables,
+                                   const int32_t* context_lens, void* out, cf_dtype dtype, cf_cache_format format,
+                                   int64_t num_pages, int64_t num_tokens, int64_t num_sequences, int64_t num_heads,
+                                   int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                   int64_t max_blocks_per_sequence, float scale, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+    CF_ENTRY();
+    const char* who = "cf_paged_attention_chunk";
+    if (num_tokens <= 0 || num_heads <= 0 || head_dim <= 0) return CF_OK;
+    CF_REQUIRE(cf::valid_dtype(dtype), "%s: unknown dtype %d", who, static_cast<int>(dtype));
+    CF_REQUIRE(cf::valid_format(format), "%s: unknown cache format %d", who, static_cast<int>(format));
+    CF_REQUIRE(cf::sizes_ok(num_tokens, num_sequences, num_heads, num_kv_heads, head_dim, block_size,
+                            max_blocks_per_sequence) && num_pages > 0,
+               "%s: %lld heads over %lld KV heads of %lld (at most 1024), blocks of %lld, %lld per sequence, %lld "
+               "pages, %lld sequences",
+               who, static_cast<long long>(num_heads), static_cast<long long>(num_kv_heads),
+               static_cast<long long>(head_dim), static_cast<long long>(block_size),
+               static_cast<long long>(max_blocks_per_sequence), static_cast<long long>(num_pages),
+               static_cast<long long>(num_sequences));
+    CF_REQUIRE(query != nullptr && k_cache != nullptr && v_cache != nullptr && query_starts != nullptr &&
+                   block_tables != nullptr && context_lens != nullptr && out != nullptr,
+               "%s: null pointer", who);
+    CF_REQUIRE(format == CF_CACHE_PLAIN || (k_scales != nullptr && v_scales != nullptr),
+               "%s: an 8-bit cache needs scales", who);
+    const size_t size = cf::dtype_size(dtype);
+    const size_t held = format == CF_CACHE_PLAIN ? size : 1;
+    CF_REQUIRE(cf::host_aligned(query, size) && cf::host_aligned(out, size) && cf::host_aligned(k_cache, held) &&
+                   cf::host_aligned(v_cache, held) && cf::host_aligned(k_scales, 4) && cf::host_aligned(v_scales, 4),
+               "%s: misaligned pointer", who);
+    // Cache rows, token positions, query rows and work items are counted in 32 bits.
+    constexpr int64_t kMost = cf::kMostTokens;
+    CF_REQUIRE(num_pages <= kMost / block_size && max_blocks_per_sequence <= kMost && num_kv_heads <= (1 << 14) &&
+                   num_sequences <= kMost - 2 && num_tokens <= kMost / num_heads,
+               "%s: %lld pages of %lld tokens, %lld sequences, %lld tokens of %lld heads or %lld KV heads exceed "
+               "32-bit counts",
+               who, static_cast<long long>(num_pages), static_cast<long long>(block_size),
+               static_cast<long long>(num_sequences), static_cast<long long>(num_tokens),
+               static_cast<long long>(num_heads), static_cast<long long>(num_kv_heads));
+    cf::Plan p = cf::plan_of(dtype, format, num_tokens, num_sequences, num_heads, num_kv_heads, head_dim,
+                             cf::capacity_of(max_blocks_per_sequence, block_size));
+    const size_t needed = cf::workspace_of(p, num_tokens, num_heads, head_dim);
+    CF_REQUIRE(needed == 0 || (workspace != nullptr && workspace_bytes >= needed && cf::host_aligned(workspace, 16)),
+               "%s: needs %zu bytes of 16-byte aligned workspace", who, needed);
+    if (p.dim != 0 && !(cf::host_aligned(query, 16) && cf::host_aligned(k_cache, 16) &&
+                        cf::host_aligned(v_cache, 16) && cf::host_aligned(out, 16))) {
+        p.dim = 0;  // within the same workspace: as many ranges at most
+        p.rows = static_cast<int>(num_heads / num_kv_heads);
+        p.step = 32;
+        p.least = 64;
+    }
+    cf::ChunkArgs a{};
+    a.query = query;
+    a.k_cache = static_cast<const uint8_t*>(k_cache);
+    a.v_cache = static_cast<const uint8_t*>(v_cache);
+    a.k_scales = k_scales;
+    a.v_scales = v_scales;
+    a.starts = query_starts;
+    a.tables = block_tables;
+    a.context = context_lens;
+    a.out = out;
+    a.pages = static_cast<uint32_t>(num_pages);
+    a.block_size = static_cast<uint32_t>(block_size);
+    a.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll(static_cast<uint64_t>(block_size)) : -1;
+    a.tokens = static_cast<int>(num_tokens);
+    a.sequences = static_cast<int>(num_sequences);
+    a.heads = static_cast<int>(num_heads);
+    a.kv_heads = static_cast<int>(num_kv_heads);
+    a.per = static_cast<int>(num_heads / num_kv_heads);
+    a.head_dim = static_cast<int>(head_dim);
+    a.pitch = (a.head_dim + 3) / 4 * 4;
+    a.max_blocks = static_cast<int>(max_blocks_per_sequence);
+    a.capacity = static_cast<int>(cf::capacity_of(max_blocks_per_sequence, block_size));
+    a.splits = p.splits;
+    a.step = p.step;
+    a.least = p.least;
+    a.query_bf16 = dtype == CF_BF16;
+    const int64_t tiles = cf::tiles_of(p, num_tokens, num_sequences, a.per);
+    const int64_t rows = num_tokens * num_heads;
+    const int64_t workgroups = p.dim == 0 ? cf::ceil_div<int64_t>(rows * p.splits, cf::kWaves)
+                                          : tiles * p.splits * num_kv_heads;
+    CF_REQUIRE(workgroups <= cf::kMaxWorkgroups && cf::ceil_div<int64_t>(rows, cf::kWaves) <= cf::kMaxWorkgroups,
+               "%s: %lld tokens of %lld heads are too many for a launch", who, static_cast<long long>(num_tokens),
+               static_cast<long long>(num_heads));
+    // The kernels take maxima of unscaled scores, so the factor must not be
+    // negative, nor 0 (which times a masked score is NaN).
+    const float c = scale * cf::kLog2e;
+    a.c = c == 0.0f ? 1.0e-37f : c < 0.0f ? -c : c;
+    const bool flip = c < 0.0f;
+    a.query_sign = flip ? (dtype == CF_F32 ? 0x80000000u : 0x80008000u) : 0u;
+    const size_t pieces = static_cast<size_t>(p.splits) * rows;
+    a.ml = static_cast<float*>(workspace);
+    a.acc = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (pieces * 8 + 15) / 16 * 16);
+    auto s = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case CF_F32: cf::run_format<float>(format, a, p, tiles, s); break;
+        case CF_F16: cf::run_format<cf::f16_t>(format, a, p, tiles, s); break;
+        case CF_BF16: cf::run_format<cf::bf16_t>(format, a, p, tiles, s); break;
+    }
+    return cf::check_launch("launching paged attention of chunks", s);
+}
+
+}  // extern "C"

@@ -1,0 +1,534 @@
+// Products of 8-bit integers, with a scale for each row of the one and each row
+// of the other operand, and the row-wise quantisation that makes the operand of
+// activations:
+//
+//   y[i, j] = T(x_scales[i] w_scales[j] sum_k x[i, k] w[j, k] + bias[j])
+//
+// x [m, k] and w [n, k] are int8, both dense along k (w is a torch Linear's
+// weight), sums exact in int32.
+#include "cf_codes.hpp"
+#include "cf_common.hpp"
+#include "cf_lds_dma.hpp"
+
+#include <type_traits>
+
+namespace cf {
+namespace {
+
+typedef int i32x4v_t __attribute__((ext_vector_type(4)));
+typedef int i32x16v_t __attribute__((ext_vector_type(16)));
+typedef float f32x4v_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
+
+// ---- quantisation of rows ------------------------------------------------------
+
+struct RowsArgs {
+    const void* x;
+    int8_t* codes;
+    float* scales;
+    int64_t rows;
+    int64_t cols;
+    int64_t stride;
+};
+
+constexpr int kRowThreads = 256;
+
+/// kVecs 16-byte vectors per thread of kPerRow; the row stays in registers.
+template <typename T, int kPerRow, int kVecs>
+__global__ __launch_bounds__(kPerRow < kRowThreads ? kRowThreads : kPerRow) void quantize_rows_kernel(RowsArgs a) {
+    constexpr int kThreads = kPerRow < kRowThreads ? kRowThreads : kPerRow;
+    constexpr int kRows = kThreads / kPerRow;
+    constexpr int kWaves = kPerRow / kWaveSize;
+    constexpr int kPer = Storage<T>::kPerVec;
+    __shared__ uint32_t tops[kWaves];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int part = tid % kPerRow;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + tid / kPerRow; row < a.rows;
+         row += static_cast<int64_t>(gridDim.x) * kRows) {
+        const T* x = static_cast<const T*>(a.x) + row * a.stride;
+        float f[kVecs][kPer];
+        uint4 raw[kVecs];
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int d = (v * kPerRow + part) * kPer;
+            raw[v] = d < a.cols ? *reinterpret_cast<const uint4*>(x + d) : make_uint4(0, 0, 0, 0);
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            unpack16<T>(raw[v], f[v]);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) top = MaxU32::apply(top, __float_as_uint(f[v][e]) & 0x7FFFFFFFu);
+        }
+        top = group_reduce_u32<16, MaxU32>(top);
+        // Bits of finite magnitudes, infinities and NaN: never negative as integers.
+        int wave_top = __builtin_amdgcn_readlane(static_cast<int>(top), 0);
+#pragma unroll
+        for (int l = 16; l < kWaveSize; l += 16) {
+            const int o = __builtin_amdgcn_readlane(static_cast<int>(top), l);
+            wave_top = o > wave_top ? o : wave_top;
+        }
+        top = static_cast<uint32_t>(wave_top);
+        if constexpr (kWaves > 1) {  // a row per workgroup: all its threads are here
+            if ((tid & (kWaveSize - 1)) == 0) tops[tid / kWaveSize] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) top = MaxU32::apply(top, tops[w]);
+            __syncthreads();
+        }
+        const RowScale s = row_scale<CF_CACHE_INT8>(top);
+        int8_t* to = a.codes + row * a.cols;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int d = (v * kPerRow + part) * kPer;
+            uint32_t w[kPer / 4];
+#pragma unroll
+            for (int e = 0; e < kPer / 4; ++e) w[e] = pack4_codes<CF_CACHE_INT8>(f[v] + 4 * e, s);
+            if (d < a.cols) {
+                if constexpr (kPer == 8) {
+                    *reinterpret_cast<uint2*>(to + d) = make_uint2(w[0], w[1]);
+                } else {
+                    *reinterpret_cast<uint32_t*>(to + d) = w[0];
+                }
+            }
+        }
+        if (part == 0) a.scales[row] = s.s;
+    }
+}
+
+/// Rows of any length and alignment, read twice.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void quantize_rows_any_kernel(RowsArgs a) {
+    constexpr int kWaves = kRowThreads / kWaveSize;
+    __shared__ uint32_t tops[kWaves];
+    const int tid = static_cast<int>(threadIdx.x);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.stride;
+        uint32_t top = 0;
+        for (int64_t d = tid; d < a.cols; d += kRowThreads) {
+            top = MaxU32::apply(top, __float_as_uint(Storage<T>::load(x + d)) & 0x7FFFFFFFu);
+        }
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) {
+            top = MaxU32::apply(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+        }
+        if ((tid & (kWaveSize - 1)) == 0) tops[tid / kWaveSize] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = MaxU32::apply(top, tops[w]);
+        __syncthreads();
+        const RowScale s = row_scale<CF_CACHE_INT8>(top);
+        for (int64_t d = tid; d < a.cols; d += kRowThreads) {
+            const float f[4] = {Storage<T>::load(x + d), 0.0f, 0.0f, 0.0f};
+            a.codes[row * a.cols + d] = static_cast<int8_t>(pack4_codes<CF_CACHE_INT8>(f, s));
+        }
+        if (tid == 0) a.scales[row] = s.s;
+    }
+}
+
+template <typename T>
+void launch_rows(const RowsArgs& a, hipStream_t stream) {
+    constexpr int kPer = Storage<T>::kPerVec;
+    const int64_t vecs = a.cols / kPer;
+    auto capped = [](int64_t n) { return dim3(static_cast<unsigned>(n < kMaxWorkgroups ? n : kMaxWorkgroups)); };
+    const bool vectors = a.cols % kPer == 0 && host_aligned(a.x, 16) && a.stride % kPer == 0 &&
+                         host_aligned(a.codes, kPer) && vecs <= 1024 * 8;
+    if (!vectors) {
+        launch(quantize_rows_any_kernel<T>, capped(a.rows), dim3(kRowThreads), 0, stream, a);
+        return;
+    }
+    // A wave per row where there are rows enough to fill the GPU with that.
+    if (vecs <= 64 * 8 && a.rows >= 2048) {
+        const dim3 grid = capped(ceil_div<int64_t>(a.rows, 4));
+        auto* kernel = vecs <= 64    ? quantize_rows_kernel<T, 64, 1>
+                       : vecs <= 128 ? quantize_rows_kernel<T, 64, 2>
+                       : vecs <= 256 ? quantize_rows_kernel<T, 64, 4>
+                                     : quantize_rows_kernel<T, 64, 8>;
+        launch(kernel, grid, dim3(kRowThreads), 0, stream, a);
+    } else if (vecs <= 256 * 8) {
+        auto* kernel = vecs <= 256    ? quantize_rows_kernel<T, 256, 1>
+                       : vecs <= 512  ? quantize_rows_kernel<T, 256, 2>
+                       : vecs <= 1024 ? quantize_rows_kernel<T, 256, 4>
+                                      : quantize_rows_kernel<T, 256, 8>;
+        launch(kernel, capped(a.rows), dim3(256), 0, stream, a);
+    } else {
+        launch(quantize_rows_kernel<T, 1024, 8>, capped(a.rows), dim3(1024), 0, stream, a);
+    }
+}
+
+// ---- products -------------------------------------------------------------------
+
+struct Int8Args {
+    const int8_t* x;
+    const int8_t* w;
+    const float* x_scales;
+    const float* w_scales;
+    const void* bias;
+    void* y;
+    int m;
+    int n;
+    int k;
+    int tiles_m;
+    int tiles_n;
+};
+
+constexpr int kStep = 128;  // bytes of k per stage: a line of every row
+
+/// Order of the 16-byte pieces of a row of 128: a fragment read takes the same
+/// piece of 32 rows, eight rows and those 24 further on (or eight apart) at a
+/// time, which bit 3 of the row sends to different halves.
+__device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+/// One result: as the header has it.
+template <typename T>
+__device__ __forceinline__ float result(int sum, float xs, float ws, float bias) {
+    return static_cast<float>(sum) * xs * ws + bias;
+}
+
+template <typename T>
+__device__ __forceinline__ float bias_at(const Int8Args& a, int j) {
+    return a.bias != nullptr ? Storage<T>::load(static_cast<const T*>(a.bias) + j) : 0.0f;
+}
+
+/// Four neighbouring columns j .. j + 3 of row i.
+template <typename T>
+__device__ __forceinline__ void store4(const Int8Args& a, int i, int j, const int (&sum)[4], float xs, bool vectors) {
+    T* y = static_cast<T*>(a.y) + static_cast<int64_t>(i) * a.n + j;
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int col = j + e < a.n ? j + e : a.n - 1;
+        v[e] = result<T>(sum[e], xs, a.w_scales[col], bias_at<T>(a, col));
+    }
+    if (vectors && j + 3 < a.n) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            *reinterpret_cast<uint2*>(y) = make_uint2(Storage<T>::to_bits2(v[0], v[1]), Storage<T>::to_bits2(v[2], v[3]));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (j + e < a.n) Storage<T>::store(y + e, v[e]);
+        }
+    }
+}
+
+/// kBM x kBN results per workgroup, kWM x kWN per wave, kStages stages of 128
+/// bytes of k in LDS. The product is formed transposed (w the first operand), so
+/// a lane holds runs of four columns of one row.
+template <typename T, int kBM, int kBN, int kWM, int kWN, int kStages>
+__global__ __launch_bounds__(kBM / kWM * (kBN / kWN) * kWaveSize) void matmul_int8_kernel(Int8Args a) {
+    constexpr int kWavesM = kBM / kWM;
+    constexpr int kWavesN = kBN / kWN;
+    constexpr int kWaves = kWavesM * kWavesN;
+    constexpr int kCopies = (kBM + kBN) / 8 / kWaves;  // of 1 KiB, per wave and stage
+    constexpr int kStageBytes = (kBM + kBN) * kStep;
+    static_assert((kBM + kBN) / 8 % kWaves == 0 && kBM / 8 % kCopies == 0, "a wave copies rows of one operand");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kStages * kStageBytes];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm;
+    int tn;
+    tile_of(static_cast<int>(blockIdx.x), a.tiles_m, a.tiles_n, tm, tn);
+    const int m0 = tm * kBM;
+    const int n0 = tn * kBN;
+
+    // This wave's copies: rows 8 c .. + 7 of one operand, lane l row l / 8 and
+    // piece l % 8 as it lies in LDS.
+    const bool of_x = wave * kCopies < kBM / 8;
+    const int first_copy = of_x ? wave * kCopies : wave * kCopies - kBM / 8;
+    const int rows_here = of_x ? (a.m - m0 < kBM ? a.m - m0 : kBM) : (a.n - n0 < kBN ? a.n - n0 : kBN);
+    const int8_t* base = of_x ? a.x + static_cast<int64_t>(m0) * a.k : a.w + static_cast<int64_t>(n0) * a.k;
+    const i32x4_t buffer = uniform(raw_buffer_words(base, static_cast<uint32_t>(rows_here) * static_cast<uint32_t>(a.k)));
+    uint32_t offset[2];  // of even and odd copies
+    uint32_t tail[2];    // in the last stage: zeros behind the end of x's rows
+    const int steps = (a.k + kStep - 1) / kStep;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int piece = (lane & 7) ^ (lane >> 3) ^ b;
+        offset[b] = static_cast<uint32_t>((lane >> 3) * a.k + piece * 16);
+        tail[b] = of_x && (steps - 1) * kStep + piece * 16 >= a.k ? kOutOfRange : offset[b];
+    }
+    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8_t*)lds)) +
+                              static_cast<uint32_t>(wave * kCopies) * 1024;
+    auto issue = [&](int step) {
+        const uint32_t dst = lds_base + static_cast<uint32_t>(step % kStages) * kStageBytes;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+            const uint32_t at = static_cast<uint32_t>((first_copy + c) * 8) * static_cast<uint32_t>(a.k) +
+                                static_cast<uint32_t>(step) * kStep;
+            const int odd = (first_copy + c) & 1;
+            const uint32_t lane_at = step == steps - 1 ? (odd ? tail[1] : tail[0]) : (odd ? offset[1] : offset[0]);
+            dma16_m0(buffer, dst + static_cast<uint32_t>(c) * 1024, lane_at, at);
+        }
+    };
+
+    constexpr int kM = kWM / 32;
+    constexpr int kN = kWN / 32;
+    const int wm = wave / kWavesN;
+    const int wn = wave % kWavesN;
+    i32x16v_t acc[kN][kM];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+#pragma unroll
+        for (int i = 0; i < kM; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][i][e] = 0;
+        }
+    }
+    const int row = lane & 31;
+    const int sw = swizzle(row);
+    const int h = lane >> 5;
+
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+        if (s < steps) issue(s);
+    }
+    for (int step = 0; step < steps; ++step) {
+        // This wave's copies of the step have landed, then everyone's.
+        if (step + kStages - 2 < steps) {
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm((kStages - 2) * kCopies));
+        } else {
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        }
+        bare_barrier();
+        if (step + kStages - 1 < steps) issue(step + kStages - 1);
+        const uint8_t* xs = lds + step % kStages * kStageBytes + wm * kWM * kStep;
+        const uint8_t* ws = lds + step % kStages * kStageBytes + (kBM + wn * kWN) * kStep;
+#pragma unroll
+        for (int u = 0; u < kStep / 32; ++u) {
+            const int at = row * kStep + (((2 * u + h) ^ sw) << 4);
+            i32x4v_t xf[kM];
+            i32x4v_t wf[kN];
+#pragma unroll
+            for (int i = 0; i < kM; ++i) xf[i] = *reinterpret_cast<const i32x4v_t*>(xs + i * 32 * kStep + at);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) wf[j] = *reinterpret_cast<const i32x4v_t*>(ws + j * 32 * kStep + at);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+#pragma unroll
+                for (int i = 0; i < kM; ++i) {
+                    acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+                }
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0xF | (3 << 14) | (7 << 4));  // LDS reads are done before the next barrier
+    }
+
+    const bool vectors = a.n % 4 == 0;
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+        const int gi = m0 + wm * kWM + 32 * i + (lane & 31);
+        if (gi >= a.m) continue;
+        const float xs = a.x_scales[gi];
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int gj = n0 + wn * kWN + 32 * j + 8 * q + 4 * h;
+                if (gj >= a.n) continue;
+                const int sum[4] = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+                store4<T>(a, gi, gj, sum, xs, vectors);
+            }
+        }
+    }
+}
+
+/// Few rows: 16 columns per workgroup, whose waves split k; w goes from memory
+/// to the matrix cores without LDS.
+template <typename T, int kM>
+__global__ __launch_bounds__(512) void matmul_int8_rows_kernel(Int8Args a) {
+    constexpr int kWaves = 8;
+    constexpr int kAhead = 4;
+    __shared__ i32x4v_t sums[kWaves][kM][kWaveSize];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = static_cast<int>(blockIdx.x) * 16;
+    const int g = lane >> 4;
+    const int col = n0 + (lane & 15) < a.n ? n0 + (lane & 15) : a.n - 1;
+    const int8_t* w = a.w + static_cast<int64_t>(col) * a.k;
+    const int8_t* x[kM];
+    i32x4v_t acc[kM];
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+        const int r = 16 * i + (lane & 15) < a.m ? 16 * i + (lane & 15) : a.m - 1;
+        x[i] = a.x + static_cast<int64_t>(r) * a.k;
+        acc[i] = i32x4v_t{0, 0, 0, 0};
+    }
+    const i32x4v_t none = {0, 0, 0, 0};
+    // Steps of 64 bytes, a quarter for each 16 lanes; waves take runs of kAhead.
+    for (int k0 = wave * kAhead * 64; k0 < a.k; k0 += kWaves * kAhead * 64) {
+        i32x4v_t wf[kAhead];
+        i32x4v_t xf[kAhead][kM];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int at = k0 + u * 64 + g * 16;
+            const bool in = at < a.k;
+            wf[u] = in ? *reinterpret_cast<const i32x4v_t*>(w + at) : none;
+#pragma unroll
+            for (int i = 0; i < kM; ++i) xf[u][i] = in ? *reinterpret_cast<const i32x4v_t*>(x[i] + at) : none;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+            for (int i = 0; i < kM; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[u][i], acc[i], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kM; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    // Row tile i of the results: wave i adds the waves' parts.
+    for (int i = wave; i < kM; i += kWaves) {
+        int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+            const i32x4v_t part = sums[v][i][lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += part[e];
+        }
+        const int gi = 16 * i + (lane & 15);
+        const int gj = n0 + 4 * g;
+        if (gi < a.m && gj < a.n) store4<T>(a, gi, gj, sum, a.x_scales[gi], a.n % 4 == 0);
+    }
+}
+
+/// Any k and alignment.
+template <typename T>
+__global__ __launch_bounds__(256) void matmul_int8_any_kernel(Int8Args a) {
+    constexpr int kTile = 16;
+    constexpr int kDeep = 64;
+    __shared__ int8_t xs[kTile][kDeep + 4];
+    __shared__ int8_t ws[kTile][kDeep + 4];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int tm = static_cast<int>(blockIdx.x) / a.tiles_n;
+    const int tn = static_cast<int>(blockIdx.x) % a.tiles_n;
+    const int i = tm * kTile + tid / kTile;
+    const int j = tn * kTile + tid % kTile;
+    int sum = 0;
+    for (int k0 = 0; k0 < a.k; k0 += kDeep) {
+        for (int c = tid; c < kTile * kDeep; c += 256) {
+            const int r = c / kDeep;
+            const int k = k0 + c % kDeep;
+            const int xr = tm * kTile + r;
+            const int wr = tn * kTile + r;
+            xs[r][c % kDeep] = xr < a.m && k < a.k ? a.x[static_cast<int64_t>(xr) * a.k + k] : static_cast<int8_t>(0);
+            ws[r][c % kDeep] = wr < a.n && k < a.k ? a.w[static_cast<int64_t>(wr) * a.k + k] : static_cast<int8_t>(0);
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int k = 0; k < kDeep; k += 4) {
+            sum = __builtin_amdgcn_sdot4(*reinterpret_cast<const int*>(&xs[tid / kTile][k]),
+                                         *reinterpret_cast<const int*>(&ws[tid % kTile][k]), sum, false);
+        }
+        __syncthreads();
+    }
+    if (i < a.m && j < a.n) {
+        Storage<T>::store(static_cast<T*>(a.y) + static_cast<int64_t>(i) * a.n + j,
+                          result<T>(sum, a.x_scales[i], a.w_scales[j], bias_at<T>(a, j)));
+    }
+}
+
+// ---- host -----------------------------------------------------------------------
+
+enum class Way { kAny, kRows, kTile64, kTile128, kTile256 };
+
+Way way_of(const Int8Args& a) {
+    if (a.k % 16 != 0 || !host_aligned(a.x, 16) || !host_aligned(a.w, 16) || !host_aligned(a.y, 16)) return Way::kAny;
+    if (a.m <= 64) return Way::kRows;
+    const int64_t big = ceil_div<int64_t>(a.m, 256) * ceil_div<int64_t>(a.n, 256);
+    const int64_t mid = ceil_div<int64_t>(a.m, 128) * ceil_div<int64_t>(a.n, 128);
+    return big >= 192 ? Way::kTile256 : mid >= 192 ? Way::kTile128 : Way::kTile64;
+}
+
+void tiles(Int8Args& a, int bm, int bn) {
+    a.tiles_m = (a.m + bm - 1) / bm;
+    a.tiles_n = (a.n + bn - 1) / bn;
+}
+
+template <typename T>
+cf_status run(Int8Args a, hipStream_t stream) {
+    const Way way = way_of(a);
+    int threads = 256;
+    void (*kernel)(Int8Args) = nullptr;
+    switch (way) {
+        case Way::kAny: tiles(a, 16, 16); kernel = matmul_int8_any_kernel<T>; break;
+        case Way::kRows:
+            tiles(a, a.m, 16);
+            threads = 512;
+            kernel = a.m <= 16   ? matmul_int8_rows_kernel<T, 1>
+                     : a.m <= 32 ? matmul_int8_rows_kernel<T, 2>
+                                 : matmul_int8_rows_kernel<T, 4>;
+            break;
+        case Way::kTile64: tiles(a, 64, 64); kernel = matmul_int8_kernel<T, 64, 64, 32, 32, 4>; break;
+        case Way::kTile128: tiles(a, 128, 128); kernel = matmul_int8_kernel<T, 128, 128, 64, 64, 2>; break;
+        case Way::kTile256: tiles(a, 256, 256); threads = 512; kernel = matmul_int8_kernel<T, 256, 256, 64, 128, 2>; break;
+    }
+    const int64_t grid = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+    CF_REQUIRE(grid <= kMaxWorkgroups / 2, "cf_matmul_int8: %d x %d results are too many for a launch", a.m, a.n);
+    launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, a);
+    return check_launch("launching the int8 product", stream);
+}
+
+}  // namespace
+}  // namespace cf
+
+extern "C" {
+
+cf_status cf_quantize_int8_rows(const void* x, cf_dtype dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                                int8_t* codes, float* scales, void* stream) {
+    CF_ENTRY();
+    const char* who = "cf_quantize_int8_rows";
+    if (rows <= 0 || cols <= 0) return CF_OK;
+    CF_REQUIRE(cf::valid_dtype(dtype), "%s: unknown dtype %d", who, static_cast<int>(dtype));
+    CF_REQUIRE(x != nullptr && codes != nullptr && scales != nullptr, "%s: null pointer", who);
+    CF_REQUIRE(row_stride >= cols || rows == 1, "%s: rows of %lld are %lld apart", who, static_cast<long long>(cols),
+               static_cast<long long>(row_stride));
+    CF_REQUIRE(cf::host_aligned(x, cf::dtype_size(dtype)) && cf::host_aligned(scales, 4), "%s: misaligned pointer", who);
+    const cf::RowsArgs a{x, codes, scales, rows, cols, row_stride};
+    auto s = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case CF_F32: cf::launch_rows<float>(a, s); break;
+        case CF_F16: cf::launch_rows<cf::f16_t>(a, s); break;
+        case CF_BF16: cf::launch_rows<cf::bf16_t>(a, s); break;
+    }
+    return cf::check_launch("launching the row quantiser", s);
+}
+
+cf_status cf_matmul_int8(const int8_t* x, const int8_t* w, const float* x_scales, const float* w_scales,
+                         const void* bias, void* y, cf_dtype dtype, int64_t m, int64_t n, int64_t k, void* stream) {
+    CF_ENTRY();
+    const char* who = "cf_matmul_int8";
+    if (m <= 0 || n <= 0) return CF_OK;
+    CF_REQUIRE(cf::valid_dtype(dtype), "%s: unknown dtype %d", who, static_cast<int>(dtype));
+    CF_REQUIRE(k >= 0 && k <= 131071 && m <= INT32_MAX - 256 && n <= INT32_MAX - 256,
+               "%s: %lld x %lld results of %lld products (at most 131071)", who, static_cast<long long>(m),
+               static_cast<long long>(n), static_cast<long long>(k));
+    CF_REQUIRE((x != nullptr && w != nullptr) || k == 0, "%s: null pointer", who);
+    CF_REQUIRE(x_scales != nullptr && w_scales != nullptr && y != nullptr, "%s: null pointer", who);
+    const size_t size = cf::dtype_size(dtype);
+    CF_REQUIRE(cf::host_aligned(y, size) && cf::host_aligned(bias, size) && cf::host_aligned(x_scales, 4) &&
+                   cf::host_aligned(w_scales, 4),
+               "%s: misaligned pointer", who);
+    cf::Int8Args a{};
+    a.x = x;
+    a.w = w;
+    a.x_scales = x_scales;
+    a.w_scales = w_scales;
+    a.bias = bias;
+    a.y = y;
+    a.m = static_cast<int>(m);
+    a.n = static_cast<int>(n);
+    a.k = static_cast<int>(k);
+    auto s = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case CF_F32: return cf::run<float>(a, s);
+        case CF_F16: return cf::run<cf::f16_t>(a, s);
+        case CF_BF16: return cf::run<cf::bf16_t>(a, s);
+    }
+    return CF_OK;
+}
+
+}  // extern "C"

@@ -916,4 +916,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("try_attention_pv", torch::wrap_pybind_function(&cudaforge_amd::try_attention_pv));
     m.def("try_lora_linear", torch::wrap_pybind_function(&cudaforge_amd::try_lora_linear));
     cudaforge_amd::bind_generation(m);
+    cudaforge_amd::bind_serving(m);
 }

@@ -69,6 +69,19 @@ inline void check_same_device(const torch::Tensor& a, const torch::Tensor& b, co
                 a.device());
 }
 
+inline void check_ints(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, const char* name) {
+    TORCH_CHECK(t.dim() == dim, name, " must have ", dim, " dimensions, got ", t.dim());
+    TORCH_CHECK(t.scalar_type() == torch::kInt32, name, " must be int32, got ", t.scalar_type());
+    check_contiguous(t, name);
+    check_same_device(like, t, name);
+}
+
+/// Counts a write for autograd's saved-tensor checks, as the mutating
+/// operators of torch do.
+inline void mark_written(const torch::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 /// PyTorch's current stream on the tensor's device, as the C ABI's void*.
 inline void* stream_for(const torch::Tensor& t) {
     return static_cast<void*>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
@@ -174,9 +187,23 @@ inline bool ordinary_set(std::initializer_list<const at::Tensor*> tensors) {
     return kernel_dtype(first->scalar_type()) && !grad_needed(tensors);
 }
 
+/// Ordinary int32 tensors of the given dimensions, all on one device.
+inline bool ordinary_ints(std::initializer_list<std::pair<const at::Tensor*, int64_t>> tensors) {
+    const at::Tensor* first = tensors.begin()->first;
+    for (const auto& [t, dim] : tensors) {
+        if (t == nullptr || t->scalar_type() != torch::kInt32 || t->dim() != dim || t->device() != first->device()) {
+            return false;
+        }
+    }
+    return true;
+}
+
 inline py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
 
 /// Adds the entries of torch_ops_generation.cpp to the extension module.
 void bind_generation(py::module_& m);
+
+/// And those of torch_ops_serving.cpp.
+void bind_serving(py::module_& m);
 
 }  // namespace cudaforge_amd

@@ -160,13 +160,6 @@ torch::Tensor token_logprobs_backward_cpu(const torch::Tensor& logits, const tor
 
 // ---- pages of a paged cache ------------------------------------------------
 
-void check_ints(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, const char* name) {
-    TORCH_CHECK(t.dim() == dim, name, " must have ", dim, " dimensions, got ", t.dim());
-    TORCH_CHECK(t.scalar_type() == torch::kInt32, name, " must be int32, got ", t.scalar_type());
-    check_contiguous(t, name);
-    check_same_device(like, t, name);
-}
-
 /// Caches as the C ABI takes them: pointers, and the bytes of a page.
 struct CacheList {
     std::vector<void*> pointers;
@@ -191,12 +184,6 @@ CacheList cache_list(at::TensorList caches, bool by_token) {
     }
     list.page_bytes = list.pages > 0 ? first.numel() / list.pages * first.element_size() : 0;
     return list;
-}
-
-/// Counts a write for autograd's saved-tensor checks, as the mutating
-/// operators of torch do.
-void mark_written(const torch::Tensor& t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 torch::Tensor page_workspace(const torch::Tensor& like, int64_t pages, int64_t sequences, int64_t count) {
@@ -520,17 +507,6 @@ std::optional<std::vector<at::Tensor>> ordinary_list(py::handle object) {
         list.push_back(*t);
     }
     return list.empty() ? std::nullopt : std::make_optional(std::move(list));
-}
-
-/// Ordinary int32 tensors of the given dimensions, all on one device.
-bool ordinary_ints(std::initializer_list<std::pair<const at::Tensor*, int64_t>> tensors) {
-    const at::Tensor* first = tensors.begin()->first;
-    for (const auto& [t, dim] : tensors) {
-        if (t == nullptr || t->scalar_type() != torch::kInt32 || t->dim() != dim || t->device() != first->device()) {
-            return false;
-        }
-    }
-    return true;
 }
 
 py::object try_cache_copy(py::handle caches_, py::handle src_, py::handle dst_) {

@@ -753,6 +753,128 @@ def dequantize_int8(
     return _dequantize_int8_reference(quantised, scales).to(target)
 
 
+def _nearest_codes(x: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes (of ``dtype``: int8 or float8_e4m3fn) and fp32 scales of the rows
+    along the last dimension. A code is the one nearest to x / scale, ties to
+    even; the quotient is taken in fp64, which rounds none of fp32 numbers onto
+    the middle of two codes."""
+    top = 127.0 if dtype == torch.int8 else 448.0
+    wide = x.double()
+    largest = wide.abs().amax(-1).float() if x.shape[-1] else wide.new_zeros(x.shape[:-1], dtype=torch.float32)
+    scales = largest / top
+    scales = torch.where(scales == 0, torch.ones_like(scales), scales)
+    scales = torch.where(torch.isfinite(largest), scales, torch.full_like(scales, float("nan")))
+    q = (wide / scales.double().unsqueeze(-1)).clamp(-top, top)
+    q = torch.where(torch.isnan(scales).unsqueeze(-1), torch.zeros_like(q), q)
+    if dtype != torch.int8:
+        # Three bits behind the leading one, steps of 2^-9 at least.
+        steps = 4 - torch.frexp(q)[1].clamp(min=-5)
+        return torch.ldexp(torch.ldexp(q, steps).round(), -steps).float().to(dtype), scales
+    return q.round().to(dtype), scales
+
+
+def _matmul_int8_reference(
+    x: torch.Tensor, weight: torch.Tensor, x_scales: torch.Tensor, w_scales: torch.Tensor,
+    bias: torch.Tensor | None, dtype: torch.dtype,
+) -> torch.Tensor:
+    """2-D; the sums are exact in fp64."""
+    y = (x.double() @ weight.double().t()).float() * x_scales.unsqueeze(1) * w_scales
+    return (y if bias is None else y + bias.float()).to(dtype)
+
+
+if _EXTENSION_LOADED:
+    _CPU = torch.library.Library("cudaforge", "IMPL")
+    _CPU.impl("quantize_int8_rows", lambda x: _nearest_codes(x, torch.int8), "CPU")
+    _CPU.impl("matmul_int8", _matmul_int8_reference, "CPU")
+
+
+def quantize_int8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Symmetric int8 quantisation with one scale per row of the last dimension
+    (per token, of activations; per output channel, of a Linear's weight).
+
+    ``scale = absmax / 127`` in fp32 (1 for a row of zeros), and each code is the
+    integer nearest to ``x / scale``, ties to even: of the exact quotient, where
+    :func:`quantize_int8` rounds the fp32 quotient. A row that holds NaN or an
+    infinity gets codes of 0 and the scale NaN, so what is made of it is NaN.
+    ``x`` is ``[..., cols]`` of fp32, fp16 or bf16 (rows may be padded). Not in
+    the reference's API.
+
+    Returns:
+        ``(codes, scales)``: int8 shaped like ``x`` and fp32 ``[...]``.
+    """
+    if _DIRECT is not None and not _compiling():
+        direct = _DIRECT.try_quantize_int8_rows(x)
+        if direct is not None:
+            return direct
+    if x.ndim < 1:
+        raise ValueError("x must have at least one dimension")
+    rows = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.new_empty(x.shape[:-1].numel(), 0)
+    if (rows.shape[1] > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
+        rows = rows.contiguous()
+    if _dispatch_available("quantize_int8_rows", x) and x.dtype in KERNEL_DTYPES:
+        codes, scales = torch.ops.cudaforge.quantize_int8_rows(rows)
+    else:
+        _refuse_gpu_fallback("quantize_int8_rows", x)
+        codes, scales = _nearest_codes(rows, torch.int8)
+    return codes.view(x.shape), scales.view(x.shape[:-1])
+
+
+#: Most products that matmul_int8 adds up: 2^14 times as many stay in 32 bits.
+MATMUL_INT8_MAX_K = 131071
+
+
+def matmul_int8(
+    x: torch.Tensor, weight: torch.Tensor, x_scales: torch.Tensor, w_scales: torch.Tensor,
+    bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """Product of 8-bit integers with a scale for each row of either operand:
+    ``y[..., j] = x_scales[...] * w_scales[j] * sum_k x[..., k] * weight[j, k] +
+    bias[j]``.
+
+    ``x`` is int8 ``[..., k]`` with fp32 ``x_scales`` ``[...]`` (a scale per
+    token), ``weight`` int8 ``[n, k]`` with fp32 ``w_scales`` ``[n]`` (per output
+    channel): both as :func:`quantize_int8_rows` gives them, the weight from a
+    torch Linear's. Sums are exact in int32 (k <= 131071), scaled in fp32 and
+    rounded once to ``dtype`` (fp32, fp16 or bf16; also the bias's). Not
+    differentiable on the kernels. Not in the reference's API.
+
+    Raises:
+        ValueError: for shapes, devices or layouts that do not match.
+        TypeError: for operands that are not int8, scales that are not fp32 or a
+            bias that is not of ``dtype``.
+    """
+    if _DIRECT is not None and not _compiling():
+        direct = _DIRECT.try_matmul_int8(x, weight, x_scales, w_scales, bias, dtype)
+        if direct is not None:
+            return direct
+    for t, name, kind in ((x, "x", torch.int8), (weight, "weight", torch.int8), (x_scales, "x_scales", torch.float32),
+                          (w_scales, "w_scales", torch.float32), (bias, "bias", dtype)):
+        if t is not None and t.dtype != kind:
+            raise TypeError(f"{name} must be {kind}, got {t.dtype}")
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, expected {x.device}")
+    if x.ndim < 1 or weight.ndim != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x of {tuple(x.shape)} and weight of {tuple(weight.shape)} do not match")
+    n, k = weight.shape
+    if k > MATMUL_INT8_MAX_K:
+        raise ValueError(f"k must be at most {MATMUL_INT8_MAX_K}, got {k}")
+    if x_scales.shape != x.shape[:-1] or w_scales.shape != (n,):
+        raise ValueError(
+            f"scales must be {tuple(x.shape[:-1])} and {(n,)}, got {tuple(x_scales.shape)} and {tuple(w_scales.shape)}")
+    if bias is not None and bias.shape != (n,):
+        raise ValueError(f"bias must be {(n,)}, got {tuple(bias.shape)}")
+    rows = x.reshape(-1, k).contiguous() if k else x.new_empty(x.shape[:-1].numel(), 0)
+    operands = (rows, weight.contiguous(), x_scales.reshape(-1).contiguous(), w_scales.contiguous(),
+                None if bias is None else bias.contiguous())
+    floats = [t for t in operands[2:] if t is not None]
+    if _dispatch_available("matmul_int8", rows, *floats) and dtype in KERNEL_DTYPES:
+        y = torch.ops.cudaforge.matmul_int8(*operands, dtype)
+    else:
+        _refuse_gpu_fallback("matmul_int8", rows, *floats)
+        y = _matmul_int8_reference(*operands, dtype)
+    return y.view(*x.shape[:-1], n)
+
+
 def fake_quantize_int8(x: torch.Tensor) -> torch.Tensor:
     """Quantise and dequantise in one pass, in x's dtype (the reference's
     launch_quantize_dequantize, which it never exposed as an operator)."""

@@ -142,6 +142,293 @@ def paged_attention_shared(
 
 
 # ---------------------------------------------------------------------------
+# Storing, reading back, and attention of chunks. A cache holds its rows in a
+# float type, or as 8-bit codes with an fp32 scale per token and KV head.
+# ---------------------------------------------------------------------------
+
+#: Types of codes that a cache may hold.
+CODE_DTYPES: frozenset[torch.dtype] = frozenset({torch.int8, torch.float8_e4m3fn})
+
+
+def _check_held(
+    k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor | None, v_scales: torch.Tensor | None,
+    like: torch.Tensor,
+) -> bool:
+    """Whether the caches hold codes."""
+    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError(
+            f"caches must be [pages, block, kv_heads, head_dim] and alike, got {tuple(k_cache.shape)} {k_cache.dtype} "
+            f"and {tuple(v_cache.shape)} {v_cache.dtype}"
+        )
+    codes = k_cache.dtype in CODE_DTYPES
+    if not codes and not k_cache.dtype.is_floating_point:
+        raise TypeError(f"no cache holds {k_cache.dtype}")
+    if (k_scales is not None) != codes or (v_scales is not None) != codes:
+        raise ValueError("k_scales and v_scales are given for 8-bit caches, and for those alone")
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache"), (k_scales, "k_scales"), (v_scales, "v_scales")):
+        if t is None:
+            continue
+        if t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32, got {t.dtype}")
+        if t is not None and t.shape != k_cache.shape[:3]:
+            raise ValueError(f"{name} must be {tuple(k_cache.shape[:3])}, got {tuple(t.shape)}")
+    return codes
+
+
+def _check_slots(slots: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    if slots.dtype != torch.int64:
+        raise TypeError(f"slots must be int64, got {slots.dtype}")
+    if slots.ndim != 1:
+        raise ValueError(f"slots must be [tokens], got shape {tuple(slots.shape)}")
+    if slots.device != like.device:
+        raise ValueError(f"slots are on {slots.device}, expected {like.device}")
+    return slots.contiguous()
+
+
+def _rows_of(cache: torch.Tensor) -> torch.Tensor:
+    """[slots, kv_heads, head_dim], float8 as the bytes that indexing takes."""
+    flat = cache.view(cache.shape[0] * cache.shape[1], *cache.shape[2:])
+    return flat.view(torch.int8) if cache.dtype == torch.float8_e4m3fn else flat
+
+
+def _values_at(cache: torch.Tensor, scales: torch.Tensor | None, at: torch.Tensor) -> torch.Tensor:
+    """What the cache holds at slots, in fp32 (fp64 where the cache is)."""
+    rows = _rows_of(cache)[at].view(cache.dtype)
+    wide = rows if rows.dtype == torch.float64 else rows.float()
+    return wide if scales is None else wide * scales.view(-1, scales.shape[2])[at].unsqueeze(-1)
+
+
+def _write_reference(
+    keys: torch.Tensor, values: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+    k_scales: torch.Tensor | None, v_scales: torch.Tensor | None,
+) -> None:
+    last = {s: i for i, s in enumerate(slots.tolist()) if 0 <= s < k_cache.shape[0] * k_cache.shape[1]}
+    at = torch.tensor(list(last), dtype=torch.int64, device=slots.device)
+    rows = torch.tensor(list(last.values()), dtype=torch.int64, device=slots.device)
+    for x, cache, scales in ((keys, k_cache, k_scales), (values, v_cache, v_scales)):
+        given = x.detach()[rows]
+        if scales is not None:
+            given, scale = ops._nearest_codes(given, cache.dtype)
+            scales.view(-1, scales.shape[2])[at] = scale
+        flat = _rows_of(cache)
+        flat[at] = given.view(flat.dtype)
+
+
+def _read_reference(
+    k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, k_scales: torch.Tensor | None,
+    v_scales: torch.Tensor | None, dtype: torch.dtype,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    there = (slots >= 0) & (slots < k_cache.shape[0] * k_cache.shape[1])
+    out = []
+    for cache, scales in ((k_cache, k_scales), (v_cache, v_scales)):
+        rows = torch.zeros(slots.shape[0], *cache.shape[2:], dtype=dtype, device=cache.device)
+        rows[there] = _values_at(cache, scales, slots[there]).to(dtype)
+        out.append(rows)
+    return out[0], out[1]
+
+
+def _chunk_reference(
+    query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_starts: torch.Tensor,
+    block_tables: torch.Tensor, context_lens: torch.Tensor, k_scales: torch.Tensor | None,
+    v_scales: torch.Tensor | None, scale: float,
+) -> torch.Tensor:
+    """Sequence by sequence in plain PyTorch (fp32, or fp64 where the query is)."""
+    pages, block, kv_heads, dim = k_cache.shape
+    tokens, heads = query.shape[:2]
+    wide = torch.float64 if query.dtype == torch.float64 else torch.float32
+    parts, done = [], 0
+    ends = [min(max(n, 0), tokens) for n in query_starts.tolist()]
+    for s, length in enumerate(context_lens.tolist()):
+        first = max(done, ends[s])
+        end = max(first, ends[s + 1])
+        parts.append(query.new_zeros(first - done, heads, dim, dtype=wide))
+        done = end
+        if end == first:
+            continue
+        length = min(max(length, 0), block_tables.shape[1] * block)
+        t = torch.arange(length, device=query.device)
+        page = block_tables[s].long()[t // max(block, 1)]
+        there = (page >= 0) & (page < pages)
+        at = (page * block + t % max(block, 1))[there]
+        if at.numel() == 0:
+            parts.append(query.new_zeros(end - first, heads, dim, dtype=wide))
+            continue
+        k = _values_at(k_cache, k_scales, at).to(wide).permute(1, 2, 0).contiguous()  # [KVH, D, L]
+        v = _values_at(v_cache, v_scales, at).to(wide).permute(1, 0, 2).contiguous()
+        q = query[first:end].to(wide).view(end - first, kv_heads, -1, dim).permute(1, 2, 0, 3)  # [KVH, per, n, D]
+        position = length - (end - first) + torch.arange(end - first, device=query.device)
+        hidden = t[there] > position[:, None]
+        scores = (q @ k.unsqueeze(1)).mul(scale).masked_fill(hidden, float("-inf"))
+        none = (scores == float("-inf")).all(-1, keepdim=True)
+        p = torch.softmax(scores.masked_fill(none, 0.0), -1).masked_fill(none | hidden, 0.0)
+        # What a row does not see stays out, whatever it holds.
+        bad = ~torch.isfinite(v).all(0).all(-1)
+        o = p @ v.masked_fill(bad[:, None], 0.0).unsqueeze(1)
+        for j in bad.nonzero().view(-1).tolist():
+            o = o + torch.where(hidden[:, j, None], torch.zeros_like(o), p[..., j, None] * v[:, None, None, j])
+        parts.append(o.permute(2, 0, 1, 3).reshape(end - first, heads, dim))
+    parts.append(query.new_zeros(tokens - done, heads, dim, dtype=wide))
+    return torch.cat(parts).to(query.dtype)
+
+
+def cache_write(
+    keys: torch.Tensor, values: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+    k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
+) -> None:
+    """Store the keys and values of new tokens into a paged cache, quantised on
+    the way where the cache holds 8 bits.
+
+    ``keys`` and ``values`` are ``[tokens, kv_heads, head_dim]`` of fp32, fp16 or
+    bf16 (views of a fused projection are read as they lie: only head_dim has to
+    be dense), ``slots`` int64 ``[tokens]`` as :func:`cache_extend` gives them
+    (``page * block + offset``, flattened): token i goes to slot ``slots[i]``, and
+    one whose slot is negative or past the cache is left out. Of several tokens
+    with one slot the last one stays.
+
+    Caches ``[pages, block, kv_heads, head_dim]`` are of the tokens' type, or int8
+    or float8_e4m3fn with fp32 ``k_scales`` and ``v_scales`` ``[pages, block,
+    kv_heads]``. A row's scale is its largest magnitude over 127 (448), 1 for a
+    row of zeros, and a code the one nearest to ``x / scale``, ties to even; a row
+    that holds NaN or an infinity gets codes of 0 and the scale NaN. Caches and
+    scales are written in place. Not differentiable. Not in the reference's API.
+
+    Raises:
+        ValueError: for shapes, devices or layouts that do not match, or tensors
+            that require gradients.
+        TypeError: for slots that are not int64, scales that are not fp32 or a
+            cache of another type.
+    """
+    if ops._DIRECT is not None and not ops._compiling():
+        if ops._DIRECT.try_cache_write(keys, values, k_cache, v_cache, slots, k_scales, v_scales):
+            return
+    codes = _check_held(k_cache, v_cache, k_scales, v_scales, keys)
+    slots = _check_slots(slots, keys)
+    shape = (slots.shape[0], *k_cache.shape[2:])
+    for x, name in ((keys, "keys"), (values, "values")):
+        if tuple(x.shape) != shape:
+            raise ValueError(f"{name} must be {shape}, got {tuple(x.shape)}")
+        if x.device != keys.device:
+            raise ValueError(f"{name} are on {x.device}, expected {keys.device}")
+        if not x.is_floating_point() or x.dtype in CODE_DTYPES or x.dtype != (keys.dtype if codes else k_cache.dtype):
+            raise TypeError(f"{name} are {x.dtype}, the caches {k_cache.dtype} and keys {keys.dtype}")
+    tensors = [t for t in (k_cache, v_cache, k_scales, v_scales) if t is not None]
+    if any(t.requires_grad for t in tensors) or ops._needs_autograd(keys, values):
+        raise ValueError("cache_write is not differentiable: detach its arguments")
+    dense = [x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous() for x in (keys, values)]
+    if _dispatch_available("cache_write", keys, values) and keys.dtype in KERNEL_DTYPES:
+        torch.ops.cudaforge.cache_write(*dense, k_cache, v_cache, slots, k_scales, v_scales)
+        return
+    _refuse_gpu_fallback("cache_write", keys, values, k_cache)
+    _write_reference(*dense, k_cache, v_cache, slots, k_scales, v_scales)
+
+
+def cache_read(
+    k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """What a paged cache holds at ``slots`` (int64 ``[tokens]``): ``(keys,
+    values)``, each ``[tokens, kv_heads, head_dim]``, zeros for a slot out of range.
+
+    Caches and scales are as in :func:`cache_write`. 8-bit caches give ``code *
+    scale`` in ``dtype`` (fp32, fp16 or bf16; default fp32), rounded once; others
+    their own type. Token t of sequence s lies at slot ``block_tables[s, t //
+    block] * block + t % block``. Not differentiable on the kernels. Not in the
+    reference's API.
+
+    Raises:
+        ValueError: for shapes, devices or layouts that do not match, or another
+            ``dtype`` than a plain cache's.
+        TypeError: for slots that are not int64, or scales that are not fp32.
+    """
+    if ops._DIRECT is not None and not ops._compiling():
+        direct = ops._DIRECT.try_cache_read(k_cache, v_cache, slots, k_scales, v_scales, dtype)
+        if direct is not None:
+            return direct
+    codes = _check_held(k_cache, v_cache, k_scales, v_scales, k_cache)
+    slots = _check_slots(slots, k_cache)
+    if dtype is None:
+        dtype = torch.float32 if codes else k_cache.dtype
+    if not codes and dtype != k_cache.dtype:
+        raise ValueError(f"a cache of {k_cache.dtype} is read back as that, not as {dtype}")
+    tensors = [t for t in (k_cache, v_cache, k_scales, v_scales) if t is not None]
+    if _dispatch_available("cache_read", *tensors) and dtype in KERNEL_DTYPES:
+        return torch.ops.cudaforge.cache_read(k_cache, v_cache, slots, k_scales, v_scales, dtype)
+    _refuse_gpu_fallback("cache_read", *tensors)
+    return _read_reference(k_cache, v_cache, slots, k_scales, v_scales, dtype)
+
+
+def paged_attention_chunk(
+    query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_starts: torch.Tensor,
+    block_tables: torch.Tensor, context_lens: torch.Tensor, k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None, scale: float | None = None,
+) -> torch.Tensor:
+    """Causal attention of the newest tokens of every sequence over a paged cache
+    that holds them already: chunks of prompts, single tokens, or both in one
+    batch.
+
+    ``query`` is ``[tokens, heads, head_dim]``: rows ``query_starts[s] ..
+    query_starts[s + 1] - 1`` (int32 ``[sequences + 1]``, ascending) are the last
+    tokens of sequence s, in order; a sequence may have none. The row at position
+    p attends to tokens 0 .. p of its sequence, so its last row to all
+    ``context_lens[s]`` of them. Caches and scales are as in :func:`cache_write`
+    (caches of the query's type, or 8-bit codes for any query), heads a multiple
+    of kv_heads, ``block_tables`` ``[sequences, width]``. ``scale`` defaults to
+    ``1 / sqrt(head_dim)``.
+
+    Returns ``[tokens, heads, head_dim]``; zeros for a row that no sequence holds
+    (padding behind the last one), or whose position is below 0. A table entry
+    that names no page leaves its tokens out. fp32, fp16 and bf16; not
+    differentiable on the kernels (a call that needs a gradient runs the PyTorch
+    composition). Not in the reference's API.
+
+    Raises:
+        ValueError: for shapes or devices that do not match, or caches that are
+            not contiguous (a copy of a cache is never made).
+        TypeError: for integer arguments that are not int32, or scales that are
+            not fp32.
+    """
+    if scale is None:
+        scale = 1.0 / math.sqrt(query.shape[-1]) if query.ndim and query.shape[-1] else 1.0
+    if ops._DIRECT is not None and not ops._compiling():
+        direct = ops._DIRECT.try_paged_attention_chunk(
+            query, k_cache, v_cache, query_starts, block_tables, context_lens, k_scales, v_scales, scale)
+        if direct is not None:
+            return direct
+    if query.ndim != 3:
+        raise ValueError(f"query must be [tokens, heads, head_dim], got shape {tuple(query.shape)}")
+    codes = _check_held(k_cache, v_cache, k_scales, v_scales, query)
+    heads, dim = query.shape[1:]
+    if k_cache.shape[3] != dim or k_cache.shape[2] == 0 or heads % k_cache.shape[2]:
+        raise ValueError(
+            f"query of {heads} heads of {dim} does not fit a cache of {k_cache.shape[2]} heads of {k_cache.shape[3]}"
+        )
+    if dim > 1024:
+        raise ValueError(f"head_dim {dim} is above 1024")
+    if not codes and k_cache.dtype != query.dtype:
+        raise ValueError(f"query and caches differ in dtype: {query.dtype} and {k_cache.dtype}")
+    starts = _check_int32(query_starts, 1, query, "query_starts").contiguous()
+    tables = _check_int32(block_tables, 2, query, "block_tables").contiguous()
+    context = _check_int32(context_lens, 1, query, "context_lens").contiguous()
+    if tables.shape[0] != context.shape[0] or starts.shape[0] != context.shape[0] + 1:
+        raise ValueError(
+            f"block_tables, context_lens and query_starts have {tables.shape[0]}, {context.shape[0]} and "
+            f"{starts.shape[0]} rows: for n sequences n, n and n + 1"
+        )
+    query = query.contiguous()
+    arguments = (query, k_cache, v_cache, starts, tables, context, k_scales, v_scales, float(scale))
+    tensors = [t for t in (query, k_cache, v_cache, k_scales, v_scales) if t is not None]
+    if _dispatch_available("paged_attention_chunk", *tensors) and query.dtype in KERNEL_DTYPES:
+        return torch.ops.cudaforge.paged_attention_chunk(*arguments)
+    _refuse_gpu_fallback("paged_attention_chunk", *tensors)
+    return _chunk_reference(*arguments)
+
+
+# ---------------------------------------------------------------------------
 # Pages. Plain forms first: one entry of a list after the other, in place.
 # ---------------------------------------------------------------------------
 
@@ -285,7 +572,8 @@ if ops._EXTENSION_LOADED:
     _CPU = torch.library.Library("cudaforge", "IMPL")
     for _name, _form in (("cache_copy", _copy_reference), ("cache_fork", _fork_reference),
                          ("cache_extend", _extend_reference), ("cache_release", _release_reference),
-                         ("cache_compact", _compact_reference)):
+                         ("cache_compact", _compact_reference), ("cache_write", _write_reference),
+                         ("cache_read", _read_reference), ("paged_attention_chunk", _chunk_reference)):
         _CPU.impl(_name, _form, "CPU")
 
 

@@ -61,6 +61,14 @@ typedef enum cf_dtype {
     CF_BF16 = 2,
 } cf_dtype;
 
+/* How a paged cache holds its rows (one token's head_dim values of one KV head):
+ * in a cf_dtype, or in 8 bits with an fp32 scale per row. */
+typedef enum cf_cache_format {
+    CF_CACHE_PLAIN = 0,
+    CF_CACHE_INT8 = 1, /* int8 codes in -127 .. 127  */
+    CF_CACHE_E4M3 = 2, /* OCP e4m3fn codes           */
+} cf_cache_format;
+
 /* Elements per quantisation block. Same value as kQuantBlockSize
  * (cuda/include/cudaforge/quantization.cuh:18) and QUANT_BLOCK_SIZE
  * (python/cudaforge/ops.py:41). */
@@ -656,6 +664,101 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
                                     int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
                                     int64_t max_blocks_per_sequence, float scale, void* workspace,
                                     size_t workspace_bytes, void* stream);
+
+/* ---- storing into a paged cache ------------------------------------------ */
+
+/* Writes the keys and values of `tokens` tokens into a paged cache: token i goes
+ * to place slots[i] = page * block_size + offset of k_cache and v_cache
+ * [num_slots, num_kv_heads, head_dim] (num_slots = pages * block_size); a token
+ * whose slot is below 0 or not below num_slots is left out. Of several tokens
+ * with one slot the last one stays.
+ * keys and values are [tokens, num_kv_heads, head_dim] of `dtype`, dense along
+ * head_dim, tokens and heads a stride of elements apart (columns of a fused
+ * projection, say). CF_CACHE_PLAIN: the caches are of `dtype` too, and the scales
+ * NULL. CF_CACHE_INT8 and CF_CACHE_E4M3: a row's scale s, fp32 in k_scales and
+ * v_scales [num_slots, num_kv_heads], is absmax / 127 or absmax / 448 (1 where
+ * that is 0; NaN, with codes of 0, for a row that is not finite), and each code
+ * the one nearest to x / s: exactly, ties to even.
+ * Rows of up to 1024 bytes of whole 16-byte vectors, aligned, move fastest.
+ * num_slots is at most 2^31 - 4096. It has no counterpart in the reference. */
+cf_status cf_cache_write(const void* keys, const void* values, cf_dtype dtype, int64_t tokens,
+                         int64_t num_kv_heads, int64_t head_dim, int64_t key_token_stride,
+                         int64_t key_head_stride, int64_t value_token_stride,
+                         int64_t value_head_stride, const int64_t* slots, void* k_cache,
+                         void* v_cache, cf_cache_format format, float* k_scales, float* v_scales,
+                         int64_t num_slots, void* stream);
+
+/* Reads places back: row i of keys and values [tokens, num_kv_heads, head_dim]
+ * (dense, of `dtype`) is what slot slots[i] holds, code * scale rounded once for
+ * 8-bit caches, and zeros for a slot out of range. CF_CACHE_PLAIN caches are of
+ * `dtype`. It has no counterpart in the reference. */
+cf_status cf_cache_read(const void* k_cache, const void* v_cache, cf_cache_format format,
+                        const float* k_scales, const float* v_scales, int64_t num_slots,
+                        const int64_t* slots, int64_t tokens, int64_t num_kv_heads,
+                        int64_t head_dim, void* keys, void* values, cf_dtype dtype, void* stream);
+
+/* ---- paged attention of chunks of new tokens ------------------------------ */
+
+/* Workspace bytes cf_paged_attention_chunk needs: the pieces of split contexts
+ * (0 where it splits none). It has no counterpart in the reference. */
+size_t cf_paged_attention_chunk_workspace_bytes(cf_dtype dtype, cf_cache_format format,
+                                                int64_t num_tokens, int64_t num_sequences,
+                                                int64_t num_heads, int64_t num_kv_heads,
+                                                int64_t head_dim, int64_t block_size,
+                                                int64_t max_blocks_per_sequence);
+
+/* Causal attention of the newest tokens of every sequence over a paged cache
+ * that holds them already: query / out [num_tokens, num_heads, head_dim], rows
+ * query_starts[s] .. query_starts[s + 1] - 1 the last n_s tokens of sequence s, in
+ * order (n_s may be 0, 1 or more; query_starts [num_sequences + 1] is int32 on the
+ * device). The row at position p of its sequence attends to tokens 0 .. p of it:
+ * the last one to all context_lens[s] of them. Caches, tables and context lengths
+ * are as in cf_paged_attention_shared, or the caches hold 8-bit codes (`format`)
+ * with k_scales and v_scales [num_pages, block_size, num_kv_heads]. Keys and
+ * values are used as code * scale.
+ * Rows whose position is below 0 (more rows than context), rows that no sequence
+ * holds, rows all of whose tokens are left out or whose scores are all -inf get
+ * zeros. Starts are taken in ascending order (one below an earlier one counts as
+ * that one) and within 0 .. num_tokens; a token whose table entry is not below
+ * num_pages is left out, as are contexts past the table and past 2^31 - 4096.
+ * Cache rows and scales behind a row's position are never used, whatever they
+ * hold.
+ * Matrix-core kernels take head sizes that are multiples of 8 (8-bit caches:
+ * 16) up to 256 (plain fp32 caches: multiples of 4 up to 128) with 16-byte
+ * aligned query and caches; every other head size up to 1024 runs a general
+ * kernel. Deterministic. The workspace is 16-byte aligned, in any state;
+ * overlapping calls need their own. It has no counterpart in the reference. */
+cf_status cf_paged_attention_chunk(const void* query, const void* k_cache, const void* v_cache,
+                                   const float* k_scales, const float* v_scales,
+                                   const int32_t* query_starts, const uint32_t* block_tables,
+                                   const int32_t* context_lens, void* out, cf_dtype dtype,
+                                   cf_cache_format format, int64_t num_pages, int64_t num_tokens,
+                                   int64_t num_sequences, int64_t num_heads, int64_t num_kv_heads,
+                                   int64_t head_dim, int64_t block_size,
+                                   int64_t max_blocks_per_sequence, float scale, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* ---- products of 8-bit integers ------------------------------------------ */
+
+/* Quantises rows to int8 with one scale each: scales[r] and codes[r, :] of row r
+ * of x by the rule of cf_cache_write's CF_CACHE_INT8 rows. x is [rows, cols] of
+ * `dtype`, dense along cols, rows row_stride (>= cols) elements apart; codes
+ * [rows, cols] and scales [rows] are dense. It has no counterpart in the
+ * reference, whose scales go by blocks of 64 (python/cudaforge/ops.py:215-229). */
+cf_status cf_quantize_int8_rows(const void* x, cf_dtype dtype, int64_t rows, int64_t cols,
+                                int64_t row_stride, int8_t* codes, float* scales, void* stream);
+
+/* y[i, j] = x_scales[i] * w_scales[j] * sum_k x[i, k] * w[j, k] (+ bias[j]): x
+ * [m, k] and w [n, k] dense int8, scales fp32, bias (may be NULL) and y [m, n] of
+ * `dtype`. The sum is exact in 32 bits; it is converted to fp32, multiplied by
+ * x's scale and then by w's, the bias is added, and the result rounded to `dtype`.
+ * k at most 131071 (a sum of k products of -128 stays in 32 bits). k a multiple
+ * of 16 and 16-byte aligned operands run on the matrix cores, others a general
+ * kernel. It has no counterpart in the reference, whose 8-bit codes are
+ * dequantised before use. */
+cf_status cf_matmul_int8(const int8_t* x, const int8_t* w, const float* x_scales,
+                         const float* w_scales, const void* bias, void* y, cf_dtype dtype,
+                         int64_t m, int64_t n, int64_t k, void* stream);
 
 /* ---- causal attention products ------------------------------------------ */
 
