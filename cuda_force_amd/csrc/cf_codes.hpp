@@ -1,8 +1,8 @@
 // Rows held in 8 bits: a scale per row and a code per value, int8 or OCP
 // e4m3fn, for caches and for the int8 product's activations.
 //
-//   s = absmax / M in fp32 (M = 127 or 448, the largest code); 1 where that is
-//       0; NaN where the row holds a NaN or an infinity
+//   s = absmax (1 / M), both in fp32 (M = 127 or 448, the largest code); 1 where
+//       that is 0; NaN where the row holds a NaN or an infinity
 //   code = the code nearest to x / s, ties to the even code, at most M either
 //       way; 0 where s is NaN
 //
@@ -37,7 +37,7 @@ struct RowScale {
 template <cf_cache_format kFormat>
 __device__ __forceinline__ RowScale row_scale(uint32_t absmax_bits) {
     RowScale r;
-    const float s = __uint_as_float(absmax_bits) / kLargestCode<kFormat>;
+    const float s = __uint_as_float(absmax_bits) * (1.0f / kLargestCode<kFormat>);
     r.s = s > 0.0f ? s : 1.0f;
     r.lift = r.s < 0x1p-80f ? 0x1p100f : 1.0f;
     r.lifted = r.s * r.lift;

@@ -761,7 +761,7 @@ def _nearest_codes(x: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, t
     top = 127.0 if dtype == torch.int8 else 448.0
     wide = x.double()
     largest = wide.abs().amax(-1).float() if x.shape[-1] else wide.new_zeros(x.shape[:-1], dtype=torch.float32)
-    scales = largest / top
+    scales = largest * (1.0 / top)  # the factor rounded to fp32, too
     scales = torch.where(scales == 0, torch.ones_like(scales), scales)
     scales = torch.where(torch.isfinite(largest), scales, torch.full_like(scales, float("nan")))
     q = (wide / scales.double().unsqueeze(-1)).clamp(-top, top)
@@ -792,7 +792,7 @@ def quantize_int8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Symmetric int8 quantisation with one scale per row of the last dimension
     (per token, of activations; per output channel, of a Linear's weight).
 
-    ``scale = absmax / 127`` in fp32 (1 for a row of zeros), and each code is the
+    ``scale = absmax * (1 / 127)`` in fp32 (1 for a row of zeros), and each code is the
     integer nearest to ``x / scale``, ties to even: of the exact quotient, where
     :func:`quantize_int8` rounds the fp32 quotient. A row that holds NaN or an
     infinity gets codes of 0 and the scale NaN, so what is made of it is NaN.

@@ -292,8 +292,8 @@ def cache_write(
 
     Caches ``[pages, block, kv_heads, head_dim]`` are of the tokens' type, or int8
     or float8_e4m3fn with fp32 ``k_scales`` and ``v_scales`` ``[pages, block,
-    kv_heads]``. A row's scale is its largest magnitude over 127 (448), 1 for a
-    row of zeros, and a code the one nearest to ``x / scale``, ties to even; a row
+    kv_heads]``. A row's scale is its largest magnitude times fp32's 1 / 127 (1 /
+    448), 1 for a row of zeros, and a code the one nearest to ``x / scale``, ties to even; a row
     that holds NaN or an infinity gets codes of 0 and the scale NaN. Caches and
     scales are written in place. Not differentiable. Not in the reference's API.
 

@@ -28,7 +28,7 @@ def rows(x: torch.Tensor, codes: torch.dtype) -> tuple[torch.Tensor, torch.Tenso
         if not np.isfinite(row).all():
             scales[i] = np.nan
             continue
-        s = np.float32(np.abs(row).max() / top) if len(row) else np.float32(0)
+        s = np.abs(row).max() * (np.float32(1) / top) if len(row) else np.float32(0)
         scales[i] = s if s > 0 else 1.0
         out[i] = [float(nearest(Fraction(float(v)) / Fraction(float(scales[i])), codes)) for v in row]
     return torch.from_numpy(out).view(x.shape), torch.from_numpy(scales).view(x.shape[:-1])
