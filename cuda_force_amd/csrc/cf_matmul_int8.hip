@@ -180,7 +180,6 @@ constexpr int kStep = 128;  // bytes of k per stage: a line of every row
 __device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 /// One result: as the header has it.
-template <typename T>
 __device__ __forceinline__ float result(int sum, float xs, float ws, float bias) {
     return static_cast<float>(sum) * xs * ws + bias;
 }
@@ -198,7 +197,7 @@ __device__ __forceinline__ void store4(const Int8Args& a, int i, int j, const in
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int col = j + e < a.n ? j + e : a.n - 1;
-        v[e] = result<T>(sum[e], xs, a.w_scales[col], bias_at<T>(a, col));
+        v[e] = result(sum[e], xs, a.w_scales[col], bias_at<T>(a, col));
     }
     if (vectors && j + 3 < a.n) {
         if constexpr (sizeof(T) == 4) {
@@ -336,6 +335,251 @@ __global__ __launch_bounds__(kBM / kWM * (kBN / kWN) * kWaveSize) void matmul_in
     }
 }
 
+// ---- products with one wave per SIMD ----------------------------------------------
+// 256 x 256 results per workgroup of four waves, 128 x 128 each as 4 x 4 blocks in
+// the accumulation registers (a wave has 512 registers when it is alone on its
+// SIMD): per MFMA half of the LDS reads that a 64 x 128 wave tile needs.
+//   * Stages of 128 bytes of k, two in LDS, of 32 KiB for either operand. Every
+//     wave copies a quarter of each: 16 copies.
+//   * Fragments are double-buffered in registers by halves of 64 bytes: the 32
+//     MFMAs of one half issue while the next half's fragments are read.
+//   * One barrier per stage, between its halves: by then every wave has read all
+//     of it, so the stage after next takes its place, a copy behind every second
+//     MFMA of the second half; and the next stage, sent one stage ago, has landed.
+//     (Waiting for it twelve MFMAs later, at a second barrier, was 7% slower.)
+constexpr int kBigTile = 256;
+constexpr int kBigOperand = kBigTile * kStep;  // 32 KiB
+constexpr int kBigLds = 4 * kBigOperand;       // x of both stages, then w
+
+template <typename T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void matmul_int8_big_kernel(Int8Args a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBigLds];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1;
+    const int wn = wave & 1;
+    int tm;
+    int tn;
+    tile_of(static_cast<int>(blockIdx.x), a.tiles_m, a.tiles_n, tm, tn);
+    const int m0 = tm * kBigTile;
+    const int n0 = tn * kBigTile;
+    const uint32_t k = static_cast<uint32_t>(a.k);
+    const int rows_here = a.m - m0 < kBigTile ? a.m - m0 : kBigTile;
+    const int cols_here = a.n - n0 < kBigTile ? a.n - n0 : kBigTile;
+    const i32x4_t xbuf = uniform(raw_buffer_words(a.x + static_cast<int64_t>(m0) * a.k, static_cast<uint32_t>(rows_here) * k));
+    const i32x4_t wbuf = uniform(raw_buffer_words(a.w + static_cast<int64_t>(n0) * a.k, static_cast<uint32_t>(cols_here) * k));
+    // Copy i (0 .. 7) of an operand: rows 64 wave + 8 i + l / 8, piece l % 8 as it
+    // lies in LDS. The row's swizzle takes l / 8 and bit 0 of i, so two lane offsets
+    // serve all eight; 16 (i / 2) rows go into the scalar offset.
+    const int steps = (a.k + kStep - 1) / kStep;
+    uint32_t offset[2];
+    uint32_t tail[2];  // of x in the last stage: zeros behind the rows' end
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int row = 64 * wave + 8 * b + (lane >> 3);
+        const int piece = (lane & 7) ^ swizzle(row);
+        offset[b] = static_cast<uint32_t>(row) * k + static_cast<uint32_t>(piece) * 16;
+        tail[b] = (steps - 1) * kStep + piece * 16 >= a.k ? kOutOfRange : offset[b];
+    }
+    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8_t*)lds)) +
+                              static_cast<uint32_t>(wave) * 8192;
+    // Copy s (0 .. 15) of a stage: x's for even s, w's for odd ones.
+    auto issue = [&](int step, int s, bool last) {
+        const int i = s >> 1;
+        const uint32_t dst = lds_base + static_cast<uint32_t>((step & 1) * kBigOperand + i * 1024) + ((s & 1) ? 2 * kBigOperand : 0);
+        const uint32_t at = static_cast<uint32_t>(step) * kStep + static_cast<uint32_t>(i >> 1) * 16 * k;
+        const uint32_t lane_at = (s & 1) == 0 && last ? tail[i & 1] : offset[i & 1];
+        dma16_m0((s & 1) ? wbuf : xbuf, dst, lane_at, at);
+    };
+
+    // Block i of x (second operand): rows wm 128 + 32 i + l % 32; of w (first): wn
+    // 128 + 32 j + l % 32. A lane takes bytes 32 (l / 32) .. + 31 of a half, 16 to
+    // an MFMA: whatever the order along k, it is the same for both.
+    const int h = lane >> 5;
+    const int sw = swizzle(lane & 31);
+    const int rd0 = (lane & 31) * kStep + (((2 * h) ^ sw) << 4);
+    const int rd1 = (lane & 31) * kStep + (((2 * h + 1) ^ sw) << 4);
+    struct Pair {
+        i32x4v_t lo, hi;
+    };
+    struct Frags {
+        Pair w[4];
+        Pair x[4];
+    };
+    auto read_pair = [&](int base, int half) {
+        return Pair{*reinterpret_cast<const i32x4v_t*>(lds + base + (rd0 ^ (half << 6))),
+                    *reinterpret_cast<const i32x4v_t*>(lds + base + (rd1 ^ (half << 6)))};
+    };
+    // Fragment r (0 .. 7) of a half in the order in which the MFMAs use them: w0, x0
+    // .. x3, w1 .. w3.
+    auto read_frag = [&](Frags& f, int stage, int half, int r) {
+        if (r >= 1 && r <= 4) {
+            f.x[r - 1] = read_pair(stage * kBigOperand + (wm * 128 + (r - 1) * 32) * kStep, half);
+        } else {
+            const int j = r == 0 ? 0 : r - 4;
+            f.w[j] = read_pair((2 + stage) * kBigOperand + (wn * 128 + j * 32) * kStep, half);
+        }
+    };
+    i32x16v_t acc[4][4];  // [w block][x block]
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][i][e] = 0;
+        }
+    }
+    // The 32 MFMAs of a half, `between(s)` behind MFMA s; the scheduling barriers
+    // keep the order. The two MFMAs of a block lie four apart: the second needs the
+    // first's sums.
+    auto multiply = [&](const Frags& f, auto between) {
+#pragma unroll
+        for (int s = 0; s < 32; ++s) {
+            const int j = s >> 3;
+            const int i = s & 3;
+            if ((s & 4) == 0) {
+                acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[j].lo, f.x[i].lo, acc[j][i], 0, 0, 0);
+            } else {
+                acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[j].hi, f.x[i].hi, acc[j][i], 0, 0, 0);
+            }
+            between(s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+#pragma unroll
+    for (int s = 0; s < 16; ++s) issue(0, s, steps == 1);
+    if (steps > 1) {
+#pragma unroll
+        for (int s = 0; s < 16; ++s) issue(1, s, steps == 2);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(16));
+    } else {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    }
+    bare_barrier();
+    Frags f0;
+    Frags f1;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) read_frag(f0, 0, 0, r);
+    using yes = std::true_type;
+    using no = std::false_type;
+    auto stage = [&](int step, auto send, auto more) {
+        multiply(f0, [&](int s) {
+            if (s % 4 == 0) read_frag(f1, step & 1, 1, s >> 2);
+        });
+        // Every wave has read all of the stage; the next one has landed.
+        __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));
+        if constexpr (decltype(more)::value) {
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            bare_barrier();
+        }
+        multiply(f1, [&](int s) {
+            if constexpr (decltype(more)::value) {
+                if (s % 4 == 0) read_frag(f0, (step & 1) ^ 1, 0, s >> 2);
+            }
+            if constexpr (decltype(send)::value) {
+                if (s & 1) issue(step + 2, s >> 1, step + 3 == steps);
+            }
+        });
+    };
+    // The last two stages apart, so that the loop has no branch to move MFMAs across.
+    int step = 0;
+    for (; step + 2 < steps; ++step) stage(step, yes{}, yes{});
+    if (steps >= 2) stage(step++, no{}, yes{});
+    stage(step, no{}, no{});
+
+    // acc[j][i] element 4 q + e of lane l: row wm 128 + 32 i + l % 32, column wn 128 +
+    // 32 j + 8 q + 4 (l / 32) + e. 32 rows at a time go through the wave's part of LDS
+    // to be stored as whole pieces of rows.
+    __syncthreads();
+    constexpr int kPer = Storage<T>::kPerVec;
+    const int col0 = n0 + wn * 128;
+    float4 ws[4][4];
+    float4 bias[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int col = col0 + 32 * j + 8 * q + 4 * h;
+            float w4[4];
+            float b4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = col + e < a.n ? col + e : a.n - 1;
+                w4[e] = a.w_scales[at];
+                b4[e] = bias_at<T>(a, at);
+            }
+            ws[j][q] = make_float4(w4[0], w4[1], w4[2], w4[3]);
+            bias[j][q] = make_float4(b4[0], b4[1], b4[2], b4[3]);
+        }
+    }
+    uint8_t* stage_out = lds + wave * (32 * 128 * 4);
+    const bool whole = a.n % kPer == 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = lane & 31;
+        const int row0 = m0 + wm * 128 + 32 * i;
+        const float xs = a.x_scales[row0 + r < a.m ? row0 + r : a.m - 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const i32x16v_t& c = acc[j][i];
+                const float v[4] = {result(c[4 * q], xs, ws[j][q].x, bias[j][q].x),
+                                    result(c[4 * q + 1], xs, ws[j][q].y, bias[j][q].y),
+                                    result(c[4 * q + 2], xs, ws[j][q].z, bias[j][q].z),
+                                    result(c[4 * q + 3], xs, ws[j][q].w, bias[j][q].w)};
+                if constexpr (sizeof(T) == 4) {
+                    const int piece = 8 * j + 2 * q + h;
+                    *reinterpret_cast<float4*>(stage_out + r * 512 + ((piece ^ r) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    const int piece = 4 * j + q;
+                    *reinterpret_cast<uint2*>(stage_out + r * 256 + ((piece ^ (r & 15)) << 4) + ((h ^ (r >> 4)) << 3)) =
+                        make_uint2(Storage<T>::to_bits2(v[0], v[1]), Storage<T>::to_bits2(v[2], v[3]));
+                }
+            }
+        }
+        // Only this wave reads what it wrote.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        constexpr int kPieces = 128 / kPer;          // of 16 bytes per row
+        constexpr int kRowsAt = kWaveSize / kPieces;  // per store
+        const int piece = lane % kPieces;
+        const int col = col0 + piece * kPer;
+#pragma unroll
+        for (int s = 0; s < 32 / kRowsAt; ++s) {
+            const int out = s * kRowsAt + lane / kPieces;
+            uint4 v;
+            if constexpr (sizeof(T) == 4) {
+                v = *reinterpret_cast<const uint4*>(stage_out + out * 512 + ((piece ^ out) << 4));
+            } else {
+                v = *reinterpret_cast<const uint4*>(stage_out + out * 256 + ((piece ^ (out & 15)) << 4));
+                if (out >> 4) v = make_uint4(v.z, v.w, v.x, v.y);
+            }
+            if (row0 + out >= a.m || col >= a.n) continue;
+            T* y = static_cast<T*>(a.y) + static_cast<int64_t>(row0 + out) * a.n + col;
+            if (whole) {
+                store_stream16(y, v);
+            } else {
+                const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    if (col + e >= a.n) continue;
+                    if constexpr (sizeof(T) == 4) {
+                        reinterpret_cast<uint32_t*>(y)[e] = words[e];
+                    } else {
+                        reinterpret_cast<uint16_t*>(y)[e] = static_cast<uint16_t>(words[e / 2] >> (16 * (e & 1)));
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 /// Few rows: 16 columns per workgroup, whose waves split k; w goes from memory
 /// to the matrix cores without LDS.
 template <typename T, int kM>
@@ -427,7 +671,7 @@ __global__ __launch_bounds__(256) void matmul_int8_any_kernel(Int8Args a) {
     }
     if (i < a.m && j < a.n) {
         Storage<T>::store(static_cast<T*>(a.y) + static_cast<int64_t>(i) * a.n + j,
-                          result<T>(sum, a.x_scales[i], a.w_scales[j], bias_at<T>(a, j)));
+                          result(sum, a.x_scales[i], a.w_scales[j], bias_at<T>(a, j)));
     }
 }
 
@@ -464,7 +708,7 @@ cf_status run(Int8Args a, hipStream_t stream) {
             break;
         case Way::kTile64: tiles(a, 64, 64); kernel = matmul_int8_kernel<T, 64, 64, 32, 32, 4>; break;
         case Way::kTile128: tiles(a, 128, 128); kernel = matmul_int8_kernel<T, 128, 128, 64, 64, 2>; break;
-        case Way::kTile256: tiles(a, 256, 256); threads = 512; kernel = matmul_int8_kernel<T, 256, 256, 64, 128, 2>; break;
+        case Way::kTile256: tiles(a, 256, 256); kernel = matmul_int8_big_kernel<T>; break;
     }
     const int64_t grid = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
     CF_REQUIRE(grid <= kMaxWorkgroups / 2, "cf_matmul_int8: %d x %d results are too many for a launch", a.m, a.n);
