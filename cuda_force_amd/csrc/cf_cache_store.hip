@@ -19,7 +19,8 @@ namespace cf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxOwn = 2048;  // tokens per workgroup at most
+constexpr int kManyThreads = 1024;
+constexpr int kMaxOwn = 1024;  // tokens per workgroup at most: 52 KiB of LDS
 
 struct StoreArgs {
     const void* x[2];  // keys, values (read: the results)
@@ -34,6 +35,7 @@ struct StoreArgs {
     int dim;
     int own;    // tokens per workgroup
     int table;  // entries of the hash table, a power of two, 2 own at least
+    int bits;   // of the filter before it, a power of two
 };
 
 /// The largest over groups of kLanes lanes (8 to 64) of magnitudes' bits.
@@ -50,12 +52,15 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 
 __device__ __forceinline__ uint32_t abs_of(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-/// Which of the workgroup's tokens are written: keep[i] = 1 for those whose slot
-/// lies in the cache and is no later token's.
+/// Which of the workgroup's tokens are written: those whose slot lies in the
+/// cache and is no later token's. The own slots are set in a hash table, and in a
+/// filter of one bit per slot modulo its size, which nearly all slots of later
+/// tokens miss (8192 tokens: the search took 7 of 21 us with the table alone).
 struct Own {
-    int32_t* slot;   // [own] -1: left out
-    int32_t* key;    // [table] slot or -1
-    int32_t* last;   // [table] the last own token of that slot; own behind a later workgroup's
+    int32_t* slot;     // [own] -1: left out
+    int32_t* key;      // [table] slot or -1
+    int32_t* last;     // [table] the last own token of that slot; `own` behind a later workgroup's
+    uint32_t* filter;  // [bits / 32]
 };
 
 __device__ __forceinline__ uint32_t place_of(uint32_t slot, int table) {
@@ -64,12 +69,25 @@ __device__ __forceinline__ uint32_t place_of(uint32_t slot, int table) {
 
 __device__ void find_kept(const StoreArgs& a, const Own& own, int64_t first, int count) {
     const int tid = static_cast<int>(threadIdx.x);
-    for (int i = tid; i < a.table; i += kThreads) {
+    const int threads = static_cast<int>(blockDim.x);
+    if (a.own == 1) {  // one token: its slot against all later ones
+        const int64_t s = a.slots[first];
+        bool again = false;
+        for (int64_t j = first + 1 + tid; j < a.tokens; j += threads) again = again || a.slots[j] == s;
+        if (tid == 0) own.slot[0] = s >= 0 && s < a.num_slots ? static_cast<int>(s) : -1;
+        __syncthreads();
+        if (again) own.slot[0] = -1;
+        __syncthreads();
+        return;
+    }
+    for (int i = tid; i < a.table; i += threads) {
         own.key[i] = -1;
         own.last[i] = -1;
     }
+    for (int i = tid; i < a.bits / 32; i += threads) own.filter[i] = 0;
     __syncthreads();
-    for (int i = tid; i < count; i += kThreads) {
+    const uint32_t mask = static_cast<uint32_t>(a.bits - 1);
+    for (int i = tid; i < count; i += threads) {
         const int64_t s = a.slots[first + i];
         const int slot = s >= 0 && s < a.num_slots ? static_cast<int>(s) : -1;
         own.slot[i] = slot;
@@ -81,22 +99,39 @@ __device__ void find_kept(const StoreArgs& a, const Own& own, int64_t first, int
             at = (at + 1) & static_cast<uint32_t>(a.table - 1);
         }
         atomicMax(&own.last[at], i);
+        atomicOr(&own.filter[(static_cast<uint32_t>(slot) & mask) >> 5], 1u << (slot & 31));
     }
     __syncthreads();
-    for (int64_t j = first + count + tid; j < a.tokens; j += kThreads) {
-        const int64_t s = a.slots[j];
-        if (s < 0 || s >= a.num_slots) continue;
-        const int slot = static_cast<int>(s);
-        uint32_t at = place_of(static_cast<uint32_t>(slot), a.table);
-        for (;;) {
-            const int held = own.key[at];
-            if (held == slot) own.last[at] = a.own;
-            if (held == slot || held == -1) break;
-            at = (at + 1) & static_cast<uint32_t>(a.table - 1);
+    constexpr int kBatch = 8;  // loads of a thread in flight
+    for (int64_t j0 = first + count + tid; j0 < a.tokens; j0 += kBatch * threads) {
+        int64_t later[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const int64_t j = j0 + n * threads;
+            later[n] = j < a.tokens ? a.slots[j] : -1;
+        }
+        uint32_t hits = 0;
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const uint32_t low = static_cast<uint32_t>(later[n]);
+            hits |= ((own.filter[(low & mask) >> 5] >> (low & 31)) & 1u) << n;
+        }
+        if (hits == 0) continue;
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            if ((hits >> n & 1) == 0 || later[n] < 0 || later[n] >= a.num_slots) continue;
+            const int slot = static_cast<int>(later[n]);
+            uint32_t at = place_of(static_cast<uint32_t>(slot), a.table);
+            for (;;) {
+                const int held = own.key[at];
+                if (held == slot) own.last[at] = a.own;
+                if (held == slot || held == -1) break;
+                at = (at + 1) & static_cast<uint32_t>(a.table - 1);
+            }
         }
     }
     __syncthreads();
-    for (int i = tid; i < count; i += kThreads) {
+    for (int i = tid; i < count; i += threads) {
         const int slot = own.slot[i];
         if (slot < 0) continue;
         uint32_t at = place_of(static_cast<uint32_t>(slot), a.table);
@@ -106,86 +141,137 @@ __device__ void find_kept(const StoreArgs& a, const Own& own, int64_t first, int
     __syncthreads();
 }
 
+/// The rows of K or of V that a group of lanes takes in turn: (token, head) pairs
+/// of the workgroup, `step` apart, without a division or product per row.
+struct Rows {
+    int token;
+    int head;
+    int step_tokens, step_heads, heads;
+
+    __device__ __forceinline__ Rows(int first, int step, int kv_heads)
+        : token(first / kv_heads), head(first - token * kv_heads), step_tokens(step / kv_heads),
+          step_heads(step - step_tokens * kv_heads), heads(kv_heads) {}
+    __device__ __forceinline__ void next() {
+        token += step_tokens;
+        head += step_heads;
+        const bool wraps = head >= heads;
+        token += wraps ? 1 : 0;
+        head -= wraps ? heads : 0;
+    }
+};
+
 /// kVecs 16-byte vectors per lane of a group of kLanes; kVecs 0: rows of any
-/// length and alignment, a wave each, read twice.
+/// length and alignment, a wave each, read twice. The first half of a workgroup
+/// takes keys, the second values.
 template <typename T, cf_cache_format kFormat, int kLanes, int kVecs>
-__global__ __launch_bounds__(kThreads) void cache_write_kernel(StoreArgs a) {
+__global__ __launch_bounds__(kManyThreads) void cache_write_kernel(StoreArgs a) {
     extern __shared__ int32_t lds[];
-    const Own own{lds, lds + a.own, lds + a.own + a.table};
-    const int tid = static_cast<int>(threadIdx.x);
+    const Own own{lds, lds + a.own, lds + a.own + a.table, reinterpret_cast<uint32_t*>(lds) + a.own + 2 * a.table};
+    const int half = static_cast<int>(blockDim.x) / 2;
+    const int which = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >= half ? 1 : 0);
+    const int tid = static_cast<int>(threadIdx.x) - which * half;  // of the half
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.own;
     const int count = static_cast<int>(a.tokens - first < a.own ? a.tokens - first : a.own);
-    find_kept(a, own, first, count);
-    constexpr int kPer = Storage<T>::kPerVec;
-    constexpr int kGroups = kThreads / kLanes;
+    const int64_t token_stride = which ? a.token_stride[1] : a.token_stride[0];
+    const int64_t head_stride = which ? a.head_stride[1] : a.head_stride[0];
+    const T* given = static_cast<const T*>(which ? a.x[1] : a.x[0]) + first * token_stride;
+    void* const cache = which ? a.cache[1] : a.cache[0];
+    float* const scales = which ? a.scales[1] : a.scales[0];
+    const int groups = half / kLanes;
     const int part = tid % kLanes;
-    const int per_token = 2 * a.kv_heads;
-    // Rows of a workgroup are counted in 32 bits: 2048 tokens of 2^15 heads.
-    const int rows = count * per_token;
-    for (int r = tid / kLanes; r < rows; r += kGroups) {
-        const int token = r / per_token;
-        const int slot = own.slot[token];
-        if (slot < 0) continue;
-        const int which = r % per_token / a.kv_heads;
-        const int head = r % a.kv_heads;
-        const T* x = static_cast<const T*>(which ? a.x[1] : a.x[0]) +
-                     (first + token) * (which ? a.token_stride[1] : a.token_stride[0]) +
-                     head * (which ? a.head_stride[1] : a.head_stride[0]);
-        const int64_t row = static_cast<int64_t>(slot) * a.kv_heads + head;
-        void* cache = which ? a.cache[1] : a.cache[0];
-        float* scales = which ? a.scales[1] : a.scales[0];
-        if constexpr (kVecs > 0) {
+    Rows row(tid / kLanes, groups, a.kv_heads);
+    if constexpr (kVecs > 0) {
+        constexpr int kPer = Storage<T>::kPerVec;
+        constexpr int kAhead = kVecs == 1 ? 4 : 1;  // rows per group of lanes on their way
+        struct Given {
+            int token;
+            int head;
             uint4 raw[kVecs];
+        };
+        Given now[kAhead];
+        auto load = [&](Given& g) {
+            g.token = row.token;
+            g.head = row.head;
+            const T* x = given + row.token * token_stride + row.head * head_stride;
 #pragma unroll
             for (int v = 0; v < kVecs; ++v) {
                 const int d = (v * kLanes + part) * kPer;
-                raw[v] = d < a.dim ? load_stream16(x + d) : make_uint4(0, 0, 0, 0);
+                g.raw[v] = make_uint4(0, 0, 0, 0);
+                if (row.token < count && d < a.dim) g.raw[v] = load_stream16(x + d);
             }
-            if constexpr (kFormat == CF_CACHE_PLAIN) {
+            row.next();
+        };
 #pragma unroll
-                for (int v = 0; v < kVecs; ++v) {
-                    const int d = (v * kLanes + part) * kPer;
-                    if (d < a.dim) *reinterpret_cast<uint4*>(static_cast<T*>(cache) + row * a.dim + d) = raw[v];
-                }
-            } else {
-                float f[kVecs][kPer];
-                uint32_t top = 0;
+        for (int n = 0; n < kAhead; ++n) load(now[n]);
+        find_kept(a, own, first, count);
+        while (now[0].token < count) {
 #pragma unroll
-                for (int v = 0; v < kVecs; ++v) {
-                    unpack16<T>(raw[v], f[v]);
+            for (int n = 0; n < kAhead; ++n) {
+                // A row is stored while those behind it, the next round's among them, are
+                // on their way.
+                const Given g = now[n];
+                load(now[n]);
+                const int slot = g.token < count ? own.slot[g.token] : -1;
+                const int64_t at = static_cast<int64_t>(slot) * a.kv_heads + g.head;
+                if constexpr (kFormat == CF_CACHE_PLAIN) {
+                    T* to = static_cast<T*>(cache) + at * a.dim;
 #pragma unroll
-                    for (int e = 0; e < kPer; ++e) top = MaxU32::apply(top, abs_of(f[v][e]));
-                }
-                const RowScale s = row_scale<kFormat>(lanes_max<kLanes>(top));
+                    for (int v = 0; v < kVecs; ++v) {
+                        const int d = (v * kLanes + part) * kPer;
+                        if (slot >= 0 && d < a.dim) *reinterpret_cast<uint4*>(to + d) = g.raw[v];
+                    }
+                } else {
+                    float f[kVecs][kPer];
+                    uint32_t top = 0;
 #pragma unroll
-                for (int v = 0; v < kVecs; ++v) {
-                    const int d = (v * kLanes + part) * kPer;
-                    uint8_t* to = static_cast<uint8_t*>(cache) + row * a.dim + d;
-                    uint32_t w[kPer / 4];
+                    for (int v = 0; v < kVecs; ++v) {
+                        top = MaxU32::apply(top, largest16<T>(g.raw[v]));
+                        unpack16<T>(g.raw[v], f[v]);
+                    }
+                    const RowScale s = row_scale<kFormat>(lanes_max<kLanes>(top));
+                    const bool ordinary = ordinary_rows(s);
+                    uint8_t* to = static_cast<uint8_t*>(cache) + at * a.dim;
 #pragma unroll
-                    for (int e = 0; e < kPer / 4; ++e) w[e] = pack4_codes<kFormat>(f[v] + 4 * e, s);
-                    if (d < a.dim) {
-                        if constexpr (kPer == 8) {
-                            *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-                        } else {
-                            *reinterpret_cast<uint32_t*>(to) = w[0];
+                    for (int v = 0; v < kVecs; ++v) {
+                        const int d = (v * kLanes + part) * kPer;
+                        uint32_t w[kPer / 4];
+#pragma unroll
+                        for (int e = 0; e < kPer / 4; ++e) {
+                            w[e] = ordinary ? pack4_codes<kFormat, false>(f[v] + 4 * e, s)
+                                            : pack4_codes<kFormat, true>(f[v] + 4 * e, s);
+                        }
+                        if (slot >= 0 && d < a.dim) {
+                            if constexpr (kPer == 8) {
+                                *reinterpret_cast<uint2*>(to + d) = make_uint2(w[0], w[1]);
+                            } else {
+                                *reinterpret_cast<uint32_t*>(to + d) = w[0];
+                            }
                         }
                     }
+                    if (slot >= 0 && part == 0) scales[at] = s.s;
                 }
-                if (part == 0) scales[row] = s.s;
             }
-        } else if constexpr (kFormat == CF_CACHE_PLAIN) {
-            for (int d = part; d < a.dim; d += kLanes) static_cast<T*>(cache)[row * a.dim + d] = x[d];
-        } else {
-            uint32_t top = 0;
-            for (int d = part; d < a.dim; d += kLanes) top = MaxU32::apply(top, abs_of(Storage<T>::load(x + d)));
-            const RowScale s = row_scale<kFormat>(lanes_max<kLanes>(top));
-            uint8_t* to = static_cast<uint8_t*>(cache) + row * a.dim;
-            for (int d = part; d < a.dim; d += kLanes) {
-                const float f[4] = {Storage<T>::load(x + d), 0.0f, 0.0f, 0.0f};
-                to[d] = static_cast<uint8_t>(pack4_codes<kFormat>(f, s));
+        }
+    } else {
+        find_kept(a, own, first, count);
+        for (; row.token < count; row.next()) {
+            const int slot = own.slot[row.token];
+            if (slot < 0) continue;
+            const T* x = given + row.token * token_stride + row.head * head_stride;
+            const int64_t at = static_cast<int64_t>(slot) * a.kv_heads + row.head;
+            if constexpr (kFormat == CF_CACHE_PLAIN) {
+                for (int d = part; d < a.dim; d += kLanes) static_cast<T*>(cache)[at * a.dim + d] = x[d];
+            } else {
+                uint32_t top = 0;
+                for (int d = part; d < a.dim; d += kLanes) top = MaxU32::apply(top, abs_of(Storage<T>::load(x + d)));
+                const RowScale s = row_scale<kFormat>(lanes_max<kLanes>(top));
+                uint8_t* to = static_cast<uint8_t*>(cache) + at * a.dim;
+                for (int d = part; d < a.dim; d += kLanes) {
+                    const float f[4] = {Storage<T>::load(x + d), 0.0f, 0.0f, 0.0f};
+                    to[d] = static_cast<uint8_t>(pack4_codes<kFormat, true>(f, s));
+                }
+                if (part == 0) scales[at] = s.s;
             }
-            if (part == 0) scales[row] = s.s;
         }
     }
 }
@@ -255,9 +341,8 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(StoreArgs a) {
 /// Groups of lanes: vectors of 16 bytes of the given type a row holds, over at
 /// most 64 lanes and 4 steps (rows of 4 KiB); 0: the kernel for any row.
 template <template <typename, cf_cache_format, int, int> class Kernel, typename T, cf_cache_format kFormat>
-void launch_rows(const StoreArgs& a, bool vectors, dim3 grid, uint32_t lds_bytes, hipStream_t stream) {
+void launch_rows(const StoreArgs& a, bool vectors, dim3 grid, dim3 block, uint32_t lds_bytes, hipStream_t stream) {
     const int vecs = a.dim / Storage<T>::kPerVec;
-    const dim3 block(kThreads);
     if (!vectors || vecs > 256) {
         launch(Kernel<T, kFormat, 64, 0>::get(), grid, block, lds_bytes, stream, a);
     } else if (vecs <= 8) {
@@ -283,22 +368,22 @@ struct Read {
 };
 
 template <template <typename, cf_cache_format, int, int> class Kernel, typename T>
-void launch_format(cf_cache_format format, const StoreArgs& a, bool vectors, dim3 grid, uint32_t lds_bytes,
-                   hipStream_t stream) {
+void launch_format(cf_cache_format format, const StoreArgs& a, bool vectors, dim3 grid, dim3 block,
+                   uint32_t lds_bytes, hipStream_t stream) {
     switch (format) {
-        case CF_CACHE_PLAIN: launch_rows<Kernel, T, CF_CACHE_PLAIN>(a, vectors, grid, lds_bytes, stream); break;
-        case CF_CACHE_INT8: launch_rows<Kernel, T, CF_CACHE_INT8>(a, vectors, grid, lds_bytes, stream); break;
-        case CF_CACHE_E4M3: launch_rows<Kernel, T, CF_CACHE_E4M3>(a, vectors, grid, lds_bytes, stream); break;
+        case CF_CACHE_PLAIN: launch_rows<Kernel, T, CF_CACHE_PLAIN>(a, vectors, grid, block, lds_bytes, stream); break;
+        case CF_CACHE_INT8: launch_rows<Kernel, T, CF_CACHE_INT8>(a, vectors, grid, block, lds_bytes, stream); break;
+        case CF_CACHE_E4M3: launch_rows<Kernel, T, CF_CACHE_E4M3>(a, vectors, grid, block, lds_bytes, stream); break;
     }
 }
 
 template <template <typename, cf_cache_format, int, int> class Kernel>
-void launch_all(cf_dtype dtype, cf_cache_format format, const StoreArgs& a, bool vectors, dim3 grid,
+void launch_all(cf_dtype dtype, cf_cache_format format, const StoreArgs& a, bool vectors, dim3 grid, dim3 block,
                 uint32_t lds_bytes, hipStream_t stream) {
     switch (dtype) {
-        case CF_F32: launch_format<Kernel, float>(format, a, vectors, grid, lds_bytes, stream); break;
-        case CF_F16: launch_format<Kernel, f16_t>(format, a, vectors, grid, lds_bytes, stream); break;
-        case CF_BF16: launch_format<Kernel, bf16_t>(format, a, vectors, grid, lds_bytes, stream); break;
+        case CF_F32: launch_format<Kernel, float>(format, a, vectors, grid, block, lds_bytes, stream); break;
+        case CF_F16: launch_format<Kernel, f16_t>(format, a, vectors, grid, block, lds_bytes, stream); break;
+        case CF_BF16: launch_format<Kernel, bf16_t>(format, a, vectors, grid, block, lds_bytes, stream); break;
     }
 }
 
@@ -367,17 +452,21 @@ cf_status cf_cache_write(const void* keys, const void* values, cf_dtype dtype, i
     a.tokens = tokens;
     a.kv_heads = static_cast<int>(num_kv_heads);
     a.dim = static_cast<int>(head_dim);
-    // Two workgroups a CU, so that few read the list of later slots.
-    const int64_t own = cf::ceil_div<int64_t>(tokens, 512);
+    // A workgroup a CU, so that few read the list of later slots.
+    const int64_t own = cf::ceil_div<int64_t>(tokens, 256);
     a.own = static_cast<int>(own > cf::kMaxOwn ? cf::kMaxOwn : own);
     a.table = 64;
     while (a.table < 2 * a.own) a.table *= 2;
     const int64_t workgroups = cf::ceil_div<int64_t>(tokens, a.own);
     CF_REQUIRE(workgroups <= cf::kMaxWorkgroups, "%s: %lld tokens are too many", who, static_cast<long long>(tokens));
-    const uint32_t lds_bytes = static_cast<uint32_t>(a.own + 2 * a.table) * 4;
+    a.bits = 32768;
+    while (a.bits < 262144 && a.bits < 256 * a.own) a.bits *= 2;
+    const uint32_t lds_bytes = static_cast<uint32_t>(a.own + 2 * a.table) * 4 + static_cast<uint32_t>(a.bits) / 8;
+    // Large workgroups where each has values for them.
+    const int threads = int64_t{a.own} * num_kv_heads * head_dim >= 8 * cf::kManyThreads ? cf::kManyThreads : cf::kThreads;
     auto s = static_cast<hipStream_t>(stream);
     cf::launch_all<cf::Write>(dtype, format, a, cf::whole_vectors(a, dtype, format, true),
-                              dim3(static_cast<unsigned>(workgroups)), lds_bytes, s);
+                              dim3(static_cast<unsigned>(workgroups)), dim3(threads), lds_bytes, s);
     return cf::check_launch("launching the cache write", s);
 }
 
@@ -410,7 +499,7 @@ cf_status cf_cache_read(const void* k_cache, const void* v_cache, cf_cache_forma
     CF_REQUIRE(workgroups <= cf::kMaxWorkgroups, "%s: %lld tokens are too many", who, static_cast<long long>(tokens));
     auto s = static_cast<hipStream_t>(stream);
     cf::launch_all<cf::Read>(dtype, format, a, cf::whole_vectors(a, dtype, format, false),
-                             dim3(static_cast<unsigned>(workgroups)), 0, s);
+                             dim3(static_cast<unsigned>(workgroups)), dim3(cf::kThreads), 0, s);
     return cf::check_launch("launching the cache read", s);
 }
 

@@ -56,9 +56,8 @@ __global__ __launch_bounds__(kPerRow < kRowThreads ? kRowThreads : kPerRow) void
         uint32_t top = 0;
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) {
+            top = MaxU32::apply(top, largest16<T>(raw[v]));
             unpack16<T>(raw[v], f[v]);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) top = MaxU32::apply(top, __float_as_uint(f[v][e]) & 0x7FFFFFFFu);
         }
         top = group_reduce_u32<16, MaxU32>(top);
         // Bits of finite magnitudes, infinities and NaN: never negative as integers.
@@ -77,13 +76,17 @@ __global__ __launch_bounds__(kPerRow < kRowThreads ? kRowThreads : kPerRow) void
             __syncthreads();
         }
         const RowScale s = row_scale<CF_CACHE_INT8>(top);
+        const bool ordinary = ordinary_rows(s);
         int8_t* to = a.codes + row * a.cols;
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) {
             const int d = (v * kPerRow + part) * kPer;
             uint32_t w[kPer / 4];
 #pragma unroll
-            for (int e = 0; e < kPer / 4; ++e) w[e] = pack4_codes<CF_CACHE_INT8>(f[v] + 4 * e, s);
+            for (int e = 0; e < kPer / 4; ++e) {
+                w[e] = ordinary ? pack4_codes<CF_CACHE_INT8, false>(f[v] + 4 * e, s)
+                                : pack4_codes<CF_CACHE_INT8, true>(f[v] + 4 * e, s);
+            }
             if (d < a.cols) {
                 if constexpr (kPer == 8) {
                     *reinterpret_cast<uint2*>(to + d) = make_uint2(w[0], w[1]);
@@ -120,7 +123,7 @@ __global__ __launch_bounds__(kRowThreads) void quantize_rows_any_kernel(RowsArgs
         const RowScale s = row_scale<CF_CACHE_INT8>(top);
         for (int64_t d = tid; d < a.cols; d += kRowThreads) {
             const float f[4] = {Storage<T>::load(x + d), 0.0f, 0.0f, 0.0f};
-            a.codes[row * a.cols + d] = static_cast<int8_t>(pack4_codes<CF_CACHE_INT8>(f, s));
+            a.codes[row * a.cols + d] = static_cast<int8_t>(pack4_codes<CF_CACHE_INT8, true>(f, s));
         }
         if (tid == 0) a.scales[row] = s.s;
     }

@@ -69,6 +69,14 @@ def test_numbers_of_tokens_and_slots_named_again(held, tokens):
     run(x[:, 0], x[:, 2], torch.arange(tokens), (tokens + 31) // 16, 16, held)
 
 
+def test_more_tokens_than_a_round_of_workgroups_holds():
+    gen = torch.Generator().manual_seed(1)
+    tokens = 300_001
+    x = torch.randn(tokens, 2, 1, 16, generator=gen).to(torch.bfloat16)
+    slots = torch.randint(0, tokens, (tokens,), generator=gen)
+    run(x[:, 0], x[:, 1], slots, (tokens + 15) // 16, 16, torch.int8)
+
+
 @pytest.mark.parametrize("held", [torch.bfloat16, *CODES])
 def test_strides_and_alignment(held):
     fused = torch.randn(40, 6, 64).to(torch.bfloat16)
