@@ -35,6 +35,8 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWaveSize;
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f;
+/// Of 8-bit caches' values, scales below 2^-90 count as that (see soften).
+constexpr int kLeastUnit = -90;
 
 struct ChunkArgs {
     const void* query;
@@ -113,9 +115,12 @@ __device__ Segment segment_of(const ChunkArgs& a, int rows, int index) {
             const int first = __builtin_amdgcn_readlane(start, at);
             const int sequence = base + at - 1;
             index -= __builtin_amdgcn_readlane(total, at) - n;
-            // The last tiles of a chunk see most tokens: they come first.
+            // The last tiles of a chunk see most tokens: they come first, but those of
+            // the second half turned round, so that of a chunk that fills the GPU once
+            // (two workgroups a CU) a CU gets a long one and a short one.
+            const int half = (n + 1) / 2;
             return Segment{sequence < a.sequences ? sequence : -1, first, __builtin_amdgcn_readlane(end, at) - first,
-                           n - 1 - index};
+                           index < half ? n - 1 - index : index - half};
         }
         index -= __builtin_amdgcn_readlane(total, kWaveSize - 1);
         before = __builtin_amdgcn_readlane(end, kWaveSize - 1);
@@ -214,11 +219,8 @@ __device__ __forceinline__ void widen16(const u32x4_t& codes, u32x4_t& lo, u32x4
             a = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - less);
             b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - less);
         } else {
-            typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
-            float f[4];
-            unpack4_codes<CF_CACHE_E4M3>(codes[i], f);
-            a = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(f[0]), static_cast<_Float16>(f[1])});
-            b = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(f[2]), static_cast<_Float16>(f[3])});
+            a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], 1.0f, false));
+            b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], 1.0f, true));
         }
         if (i < 2) {
             lo[2 * i] = a;
@@ -230,15 +232,171 @@ __device__ __forceinline__ void widen16(const u32x4_t& codes, u32x4_t& lo, u32x4
     }
 }
 
+/// This lane's query row (token of the segment, head of the KV head): fragments
+/// q, and for kSplit what they leave; zeros outside. Returns the factor of its
+/// scores. 8-bit caches: scaled by a power of two to magnitudes of up to 2^15, the
+/// inverse in the factor.
+template <typename T, int kD, bool kCodes, bool kSplit>
+__device__ __forceinline__ float load_query(const ChunkArgs& a, const Item& w, bool inside, int token, int head, int lane,
+                                            typename Tile<T, kD>::Query (&q)[Tile<T, kD>::kQueries],
+                                            typename Tile<T, kD>::Query (&q_low)[kSplit ? Tile<T, kD>::kQueries : 1]) {
+    using L = Tile<T, kD>;
+    float c = a.c;
+    const int64_t out_row = static_cast<int64_t>(w.first + token) * a.heads + w.kv_head * a.per + head;
+    if constexpr (!kCodes) {
+        const T* from = static_cast<const T*>(a.query) + out_row * a.head_dim;
+#pragma unroll
+        for (int u = 0; u < L::kQueries; ++u) {
+            const int dim = L::query_dim(u, lane);
+            u32x4_t raw = {0u, 0u, 0u, 0u};
+            if (inside && dim < a.head_dim) raw = *reinterpret_cast<const u32x4_t*>(from + dim) ^ a.query_sign;
+            q[u] = __builtin_bit_cast(typename L::Query, raw);
+        }
+    } else {
+        float f[L::kQueries][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int u = 0; u < L::kQueries; ++u) {
+            const int dim = L::query_dim(u, lane);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[u][e] = 0.0f;
+            if (inside && dim < a.head_dim) {
+                if constexpr (kSplit) {
+                    const float* from = static_cast<const float*>(a.query) + out_row * a.head_dim + dim;
+                    unpack16<float>(*reinterpret_cast<const uint4*>(from), f[u]);
+                    unpack16<float>(*reinterpret_cast<const uint4*>(from + 4), f[u] + 4);
+                } else {
+                    const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) +
+                                                                     out_row * a.head_dim + dim);
+                    if (a.query_bf16) unpack16<bf16_t>(raw, f[u]); else unpack16<f16_t>(raw, f[u]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[u][e]));
+        }
+        top = groups_max<L::kRows>(top);
+        const int lift = 15 - __builtin_amdgcn_frexp_expf(top);
+        // Not 0, which times a masked score is NaN.
+        c = fmaxf(__builtin_amdgcn_ldexpf(c, -lift), 0x1p-126f);
+        const float sign = a.query_sign != 0 ? -1.0f : 1.0f;
+        typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int u = 0; u < L::kQueries; ++u) {
+            u32x4_t high, low;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x0 = __builtin_amdgcn_ldexpf(f[u][2 * e] * sign, lift);
+                const float x1 = __builtin_amdgcn_ldexpf(f[u][2 * e + 1] * sign, lift);
+                const f16x2_v h = {static_cast<_Float16>(x0), static_cast<_Float16>(x1)};
+                high[e] = __builtin_bit_cast(uint32_t, h);
+                if constexpr (kSplit) {
+                    low[e] = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(x0 - static_cast<float>(h[0])),
+                                                                  static_cast<_Float16>(x1 - static_cast<float>(h[1]))});
+                }
+            }
+            q[u] = __builtin_bit_cast(typename L::Query, high);
+            if constexpr (kSplit) q_low[u] = __builtin_bit_cast(typename L::Query, low);
+        }
+    }
+    return c;
+}
+
+/// The waves' outputs to the result, or to a piece of it. m in base 2.
+template <typename T, int kD, bool kCodes, bool kSplit, bool kShared>
+__device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32],
+                                       float (*lds_l)[32], float m, float l,
+                                       const typename Tile<T, kD>::Score (&acc)[Tile<T, kD>::kAcc / Tile<T, kD>::kScores]) {
+    using L = Tile<T, kD>;
+    constexpr int kRowWaves = kShared ? kWaves : 1;
+    constexpr int kTokenWaves = kShared ? 1 : kWaves;
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & (kWaveSize - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
+#pragma unroll
+    for (int d = L::kRows; d < kWaveSize; d <<= 1) l += __shfl_xor(l, d);
+    wait_vm<0>();
+    __syncthreads();  // all tiles are done with: their space takes the outputs
+    float* mine = reinterpret_cast<float*>(lds) + wave * L::kRows * L::kOutPitch;
+#pragma unroll
+    for (int i = 0; i < L::kAcc; i += 4) {
+        f32x4_t four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = acc[(i + e) / L::kScores][(i + e) % L::kScores];
+        *reinterpret_cast<f32x4_t*>(mine + L::row_of(lane) * L::kOutPitch + L::dim_of(i, lane)) = four;
+    }
+    if (L::part_of(lane) == 0) {
+        lds_m[wave][L::row_of(lane)] = m;
+        lds_l[wave][L::row_of(lane)] = l;
+    }
+    __syncthreads();
+    // Rows x groups of four dims, over the workgroup; token waves are joined.
+    constexpr int kOutRows = kRowWaves * L::kRows;
+    constexpr int kFours = kD / 4;
+    constexpr int kRounds = (kOutRows * kFours + kThreads - 1) / kThreads;
+#pragma unroll 2
+    for (int n = 0; n < kRounds; ++n) {
+        const int i = n * kThreads + tid;
+        const int r = i / kFours;
+        const int dim = (i % kFours) * 4;
+        if (r >= kOutRows) break;
+        const int out = w.first_row + r;
+        if (out >= w.rows || dim >= a.head_dim) continue;
+        const int owner = kShared ? r / L::kRows : 0;
+        const int lr = r % L::kRows;
+        const int64_t out_row = static_cast<int64_t>(w.first + out / a.per) * a.heads + w.kv_head * a.per + out % a.per;
+        float mm = lds_m[owner][lr];
+#pragma unroll
+        for (int t = 1; t < kTokenWaves; ++t) mm = fmaxf(mm, lds_m[t][lr]);
+        float ll = 0.0f;
+        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < kTokenWaves; ++t) {
+            const int src = owner + t;
+            const float f = kTokenWaves == 1 ? 1.0f : lds_m[src][lr] == -INFINITY ? 0.0f : exp2f(lds_m[src][lr] - mm);
+            // A wave without a finite score still passes its NaN on.
+            ll += kTokenWaves > 1 && lds_m[src][lr] == -INFINITY ? lds_l[src][lr] : lds_l[src][lr] * f;
+            const f32x4_t four = *reinterpret_cast<const f32x4_t*>(
+                reinterpret_cast<const float*>(lds) + (src * L::kRows + lr) * L::kOutPitch + dim);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(four[e], f, sum[e]);
+        }
+        if (w.direct) {
+            const float by = ll == 0.0f ? 0.0f : 1.0f / ll;
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = ll == 0.0f ? 0.0f : sum[e] * by;
+            const int64_t at = out_row * a.head_dim + dim;
+            if constexpr (kSplit || (!kCodes && sizeof(T) == 4)) {
+                *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at) = f32x4_t{o[0], o[1], o[2], o[3]};
+            } else {
+                const bool bf16 = kCodes ? a.query_bf16 : std::is_same<T, bf16_t>::value;
+                uint2 two;
+                if (bf16) {
+                    two = make_uint2(Storage<bf16_t>::to_bits2(o[0], o[1]), Storage<bf16_t>::to_bits2(o[2], o[3]));
+                } else {
+                    two = make_uint2(Storage<f16_t>::to_bits2(o[0], o[1]), Storage<f16_t>::to_bits2(o[2], o[3]));
+                }
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = two;
+            }
+            continue;
+        }
+        const int64_t at = static_cast<int64_t>(w.split) * a.tokens * a.heads + out_row;
+        if (dim == 0) {
+            a.ml[2 * at] = mm;
+            a.ml[2 * at + 1] = ll;
+        }
+        *reinterpret_cast<f32x4_t*>(a.acc + at * a.pitch + dim) = sum;
+    }
+}
+
 /// kShared: the waves take different rows of the tile, else different tokens of
 /// the same rows.
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit, bool kShared>
 __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
-                       uint32_t* lds_bad) {
+                       uint64_t* lds_bad) {
     using K = Kind<T, kD, kHeld, kSplit>;
     using L = typename K::L;
     constexpr bool kCodes = K::kCodes;
-    constexpr int kRowWaves = kShared ? kWaves : 1;
     constexpr int kTokenWaves = kShared ? 1 : kWaves;
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & (kWaveSize - 1);
@@ -253,67 +411,7 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
     const int limit = inside ? w.offset + token : -1;  // the last token it sees
     typename L::Query q[L::kQueries];
     [[maybe_unused]] typename L::Query q_low[kSplit ? L::kQueries : 1];
-    float c = a.c;
-    {
-        const int64_t out_row = static_cast<int64_t>(w.first + token) * a.heads + w.kv_head * a.per + (inside ? row % a.per : 0);
-        if constexpr (!kCodes) {
-            const T* from = static_cast<const T*>(a.query) + out_row * a.head_dim;
-#pragma unroll
-            for (int u = 0; u < L::kQueries; ++u) {
-                const int dim = L::query_dim(u, lane);
-                u32x4_t raw = {0u, 0u, 0u, 0u};
-                if (inside && dim < a.head_dim) raw = *reinterpret_cast<const u32x4_t*>(from + dim) ^ a.query_sign;
-                q[u] = __builtin_bit_cast(typename L::Query, raw);
-            }
-        } else {
-            // Scaled by a power of two to magnitudes of up to 2^15; the inverse goes to
-            // the scores' factor.
-            float f[L::kQueries][8];
-            float top = 0.0f;
-#pragma unroll
-            for (int u = 0; u < L::kQueries; ++u) {
-                const int dim = L::query_dim(u, lane);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[u][e] = 0.0f;
-                if (inside && dim < a.head_dim) {
-                    if constexpr (kSplit) {
-                        const float* from = static_cast<const float*>(a.query) + out_row * a.head_dim + dim;
-                        unpack16<float>(*reinterpret_cast<const uint4*>(from), f[u]);
-                        unpack16<float>(*reinterpret_cast<const uint4*>(from + 4), f[u] + 4);
-                    } else {
-                        const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) +
-                                                                         out_row * a.head_dim + dim);
-                        if (a.query_bf16) unpack16<bf16_t>(raw, f[u]); else unpack16<f16_t>(raw, f[u]);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[u][e]));
-            }
-            top = groups_max<L::kRows>(top);
-            const int lift = 15 - __builtin_amdgcn_frexp_expf(top);
-            // Not 0, which times a masked score is NaN.
-            c = fmaxf(__builtin_amdgcn_ldexpf(c, -lift), 0x1p-126f);
-            const float sign = a.query_sign != 0 ? -1.0f : 1.0f;
-            typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
-#pragma unroll
-            for (int u = 0; u < L::kQueries; ++u) {
-                u32x4_t high, low;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x0 = __builtin_amdgcn_ldexpf(f[u][2 * e] * sign, lift);
-                    const float x1 = __builtin_amdgcn_ldexpf(f[u][2 * e + 1] * sign, lift);
-                    const f16x2_v h = {static_cast<_Float16>(x0), static_cast<_Float16>(x1)};
-                    high[e] = __builtin_bit_cast(uint32_t, h);
-                    if constexpr (kSplit) {
-                        low[e] = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(x0 - static_cast<float>(h[0])),
-                                                                      static_cast<_Float16>(x1 - static_cast<float>(h[1]))});
-                    }
-                }
-                q[u] = __builtin_bit_cast(typename L::Query, high);
-                if constexpr (kSplit) q_low[u] = __builtin_bit_cast(typename L::Query, low);
-            }
-        }
-    }
+    const float c = load_query<T, kD, K::kCodes, kSplit>(a, w, inside, token, inside ? row % a.per : 0, lane, q, q_low);
     // The smallest of the wave's limits: tiles up to it need no mask.
     int least = inside ? limit : 0x7FFFFFFF;
 #pragma unroll
@@ -437,8 +535,8 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
 
     float m = -INFINITY;  // the row's running maximum
     float l = 0.0f;       // this lane's share of the running sum
-    [[maybe_unused]] float unit = 0.0f;     // above all values' scales the row met, a power of two
-    [[maybe_unused]] float inverse = 0.0f;  // of it
+    float shift = -L::kLift;  // of the exponents
+    [[maybe_unused]] int unit = kLeastUnit;  // 8-bit caches: see soften
     typename L::Score acc[L::kAcc / L::kScores];
 #pragma unroll
     for (int b = 0; b < L::kAcc / L::kScores; ++b) {
@@ -475,49 +573,53 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
 #pragma unroll
             for (int i = 0; i < L::kScores; ++i) s[i] = (mine & (1u << L::token_of(i))) != 0 ? s[i] : -INFINITY;
         }
-        float top = s[0];
-#pragma unroll
-        for (int i = 1; i < L::kScores; ++i) top = fmaxf(top, s[i]);
-        top = groups_max<L::kRows>(top);
-        const float m_new = fmaxf(m, top * c);
-        if (__builtin_amdgcn_ballot_w64(m_new > m + L::kLag) != 0) {
-            const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
-            l *= f;
-            rescale(f);
-            m = m_new;
-        }
-        const float shift = (m == -INFINITY ? 0.0f : m) - L::kLift;
-#pragma unroll
-        for (int i = 0; i < L::kScores; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -shift));
-            l += s[i];
-        }
+        // Probabilities are taken relative to a power of two 2^unit above all scales of
+        // values that the row met, sums too: times a scale they are at most 2^(kLift +
+        // kLag), as fp16 has to hold them.
+        [[maybe_unused]] float by[kCodes ? L::kScores : 1];
+        int most = kLeastUnit;
         if constexpr (kCodes) {
-            float by[L::kScores];
-            float most = 0.0f;
+            float largest = 0.0f;
 #pragma unroll
             for (int i = 0; i < L::kScores; ++i) {
                 by[i] = scales[L::kTokens + L::token_of(i)];
                 // What a row does not see may be NaN, or far above its own scales.
                 if (masked) by[i] = (mine & (1u << L::token_of(i))) != 0 ? by[i] : 0.0f;
-                most = fmaxf(most, fabsf(by[i]));
+                largest = fmaxf(largest, fabsf(by[i]));
             }
-            most = groups_max<L::kRows>(most);
-            if (__builtin_amdgcn_ballot_w64(most >= unit) != 0) {
-                uint32_t exponent = __float_as_uint(most) >> 23;
-                exponent = exponent < 1 ? 1 : exponent > 252 ? 252 : exponent;
-                const float above = __uint_as_float((exponent + 1) << 23);
-                const float old = unit;
-                if (above > unit) {
-                    unit = above;
-                    inverse = __uint_as_float((253 - exponent) << 23);
-                }
-                rescale(old * inverse);
-            }
+            most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(largest));
+        }
+        float top = s[0];
 #pragma unroll
-            for (int i = 0; i < L::kScores; ++i) s[i] *= by[i] * inverse;
+        for (int i = 1; i < L::kScores; ++i) top = fmaxf(top, s[i]);
+        top = groups_max<L::kRows>(top);
+        const float m_new = fmaxf(m, top * c);
+        if (__builtin_amdgcn_ballot_w64(m_new > m + L::kLag || (kCodes && most > unit)) != 0) {
+            float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+            m = m_new;
+            if constexpr (kCodes) {
+                const int old = unit;
+                unit = most > unit ? most : unit;
+                f = __builtin_amdgcn_ldexpf(f, old - unit);
+            }
+            l *= f;
+            rescale(f);
+            shift = (m == -INFINITY ? 0.0f : m) + (kCodes ? static_cast<float>(unit) : 0.0f) - L::kLift;
+        }
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -shift));
+            l += s[i];
+            if constexpr (kCodes) s[i] *= by[i];
+            // One value for both fp16 parts: the product could be rounded to fp16 at once.
+            if constexpr (kSplit) {
+                float x = s[i];
+                asm volatile("" : "+v"(x));
+                s[i] = x;
+            }
         }
     };
+    auto m_of = [&]() { return m + (kCodes ? static_cast<float>(unit) : 0.0f); };
     auto scores = [&](const uint8_t* k) {
         typename L::Score s = L::scores(k, q, lane);
         if constexpr (kSplit) {
@@ -555,7 +657,7 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
         if constexpr (kShared) {
             if (lane == 0) lds_bad[wave] = bad;
             __syncthreads();
-            bad = lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3];
+            bad = static_cast<uint32_t>(lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3]);
         } else {
             wait_lds();
         }
@@ -697,82 +799,466 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
         }
     }
 
-#pragma unroll
-    for (int d = L::kRows; d < kWaveSize; d <<= 1) l += __shfl_xor(l, d);
-    if constexpr (kCodes) rescale(unit);  // units may differ between waves
-    wait_vm<0>();
-    __syncthreads();  // all tiles are done with: their space takes the outputs
-    float* mine = reinterpret_cast<float*>(lds) + wave * L::kRows * L::kOutPitch;
-#pragma unroll
-    for (int i = 0; i < L::kAcc; i += 4) {
-        f32x4_t four;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) four[e] = acc[(i + e) / L::kScores][(i + e) % L::kScores];
-        *reinterpret_cast<f32x4_t*>(mine + L::row_of(lane) * L::kOutPitch + L::dim_of(i, lane)) = four;
+    finish<T, kD, kCodes, kSplit, kShared>(a, w, lds, lds_m, lds_l, m_of(), l, acc);
+}
+
+/// LDS of attend_rows: two tiles of 64 tokens of K and of V, and for codes their
+/// scales (K's, V's, and the exponent above V's).
+template <typename T, int kD, cf_cache_format kHeld>
+struct RowsKind {
+    using L = Tile<T, kD>;
+    static constexpr bool kCodes = kHeld != CF_CACHE_PLAIN;
+    static constexpr int kTokens = 64;
+    static constexpr int kOperand = kTokens * L::kRowBytes;
+    static constexpr int kScales = 2 * kTokens + 4;  // floats of a tile
+    static constexpr int kScalesAt = 4 * kOperand;
+    static constexpr int lds_bytes() {
+        constexpr int tiles = kScalesAt + (kCodes ? 2 * kScales * 4 : 0);
+        constexpr int outputs = kWaves * L::kRows * L::kOutPitch * 4;
+        return tiles > outputs ? tiles : outputs;
     }
-    if (L::part_of(lane) == 0) {
-        lds_m[wave][L::row_of(lane)] = m;
-        lds_l[wave][L::row_of(lane)] = l;
-    }
-    __syncthreads();
-    // Rows x groups of four dims, over the workgroup; token waves are joined.
-    constexpr int kOutRows = kRowWaves * L::kRows;
-    constexpr int kFours = kD / 4;
-    constexpr int kRounds = (kOutRows * kFours + kThreads - 1) / kThreads;
-#pragma unroll 2
-    for (int n = 0; n < kRounds; ++n) {
-        const int i = n * kThreads + tid;
-        const int r = i / kFours;
-        const int dim = (i % kFours) * 4;
-        if (r >= kOutRows) break;
-        const int out = w.first_row + r;
-        if (out >= w.rows || dim >= a.head_dim) continue;
-        const int owner = kShared ? r / L::kRows : 0;
-        const int lr = r % L::kRows;
-        const int64_t out_row = static_cast<int64_t>(w.first + out / a.per) * a.heads + w.kv_head * a.per + out % a.per;
-        float mm = lds_m[owner][lr];
-#pragma unroll
-        for (int t = 1; t < kTokenWaves; ++t) mm = fmaxf(mm, lds_m[t][lr]);
-        float ll = 0.0f;
-        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int t = 0; t < kTokenWaves; ++t) {
-            const int src = owner + t;
-            const float f = kTokenWaves == 1 ? 1.0f : lds_m[src][lr] == -INFINITY ? 0.0f : exp2f(lds_m[src][lr] - mm);
-            // A wave without a finite score still passes its NaN on.
-            ll += kTokenWaves > 1 && lds_m[src][lr] == -INFINITY ? lds_l[src][lr] : lds_l[src][lr] * f;
-            const f32x4_t four = *reinterpret_cast<const f32x4_t*>(
-                reinterpret_cast<const float*>(lds) + (src * L::kRows + lr) * L::kOutPitch + dim);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] = fmaf(four[e], f, sum[e]);
+};
+
+/// The waves take different rows, of 16-bit tiles: 64 tokens a step. In plain
+/// caches the next step's scores are formed while this one's are made
+/// probabilities, so that a wave has work for the matrix cores beside its vector
+/// instructions; codes, which need more of those, leave no registers for it.
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
+__device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
+                            uint64_t* lds_bad) {
+    using K = RowsKind<T, kD, kHeld>;
+    using L = typename K::L;
+    using Score = typename L::Score;
+    constexpr bool kCodes = K::kCodes;
+    constexpr int kTokens = K::kTokens;
+    static_assert(!L::kWide && L::kTokens == 32 && L::kRows == 32, "two halves of 32 tokens");
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & (kWaveSize - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
+    const int row = w.first_row + wave * L::kRows + L::row_of(lane);
+    const bool inside = row < w.rows;
+    const int token = inside ? row / a.per : 0;
+    const int limit = inside ? w.offset + token : -1;  // the last token the row sees
+    typename L::Query q[L::kQueries];
+    [[maybe_unused]] typename L::Query q_low[kSplit ? L::kQueries : 1];
+    const float c = load_query<T, kD, kCodes, kSplit>(a, w, inside, token, inside ? row % a.per : 0, lane, q, q_low);
+    // The smallest limit of the rows: tiles up to it need no mask.
+    const int tile_least = w.offset + w.first_row / a.per;
+    if (a.head_dim < kD) {  // the copies leave the end of every row as it is
+        for (int i = tid; i < 4 * K::kOperand / 16; i += kThreads) {
+            reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0u, 0u, 0u, 0u};
         }
-        if (w.direct) {
-            const float by = ll == 0.0f ? 0.0f : 1.0f / ll;
-            float o[4];
+        __syncthreads();
+    }
+
+    const int tiles = (w.hi - w.lo + kTokens - 1) / kTokens;
+    const int last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
+    auto block_of = [&](int t) {
+        return static_cast<int>(a.block_shift >= 0 ? static_cast<uint32_t>(t) >> a.block_shift
+                                                   : static_cast<uint32_t>(t) / a.block_size);
+    };
+    // 64 entries of the block table in lane registers (see attend).
+    int window_base = block_of(w.lo);
+    uint32_t window = w.table[min(window_base + lane, last_block)];
+    constexpr uint64_t kAll = ~uint64_t{0};
+    struct Place {
+        uint32_t row;    // of the cache: token `lane` of the tile; 0 where it is not there
+        uint64_t there;  // a bit per token
+    };
+    auto look_up = [&](int tile) {
+        const int first = w.lo + tile * kTokens;
+        const int last = min(first + kTokens, w.hi) - 1;
+        if (block_of(last) >= window_base + kWaveSize) {
+            window_base = block_of(first);
+            window = w.table[min(window_base + lane, last_block)];
+            asm volatile("" : "+v"(window));  // waited for here, not behind the branch
+        }
+        const int t = min(first + lane, last);
+        const int block = block_of(t);
+        const uint32_t page = static_cast<uint32_t>(__shfl(static_cast<int>(window), block - window_base));
+        const bool there = page < a.pages && first + lane < w.hi;
+        return Place{there ? page * a.block_size + (static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size) : 0u,
+                     __builtin_amdgcn_ballot_w64(there)};
+    };
+
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    const int held_size = kCodes ? 1 : static_cast<int>(sizeof(T));
+    const uint32_t token_bytes = static_cast<uint32_t>(a.kv_heads) * a.head_dim * held_size;
+    const uint64_t head_bytes = static_cast<uint64_t>(w.kv_head) * a.head_dim * held_size;
+    const int row_pieces = a.head_dim * held_size / 16;
+    // This wave's share of a tile: tokens 16 wave .. + 15 of K and of V.
+    constexpr int kMine = kTokens / kWaves;
+    constexpr int kPerCopy = kWaveSize / L::kChunks;  // plain: tokens a copy
+    constexpr int kCopies = kMine / kPerCopy;
+    constexpr int kBatch = kCopies < 4 ? kCopies : 4;
+    const bool whole = a.head_dim == kD;
+    // The lane's byte within a row of copy n (its order of pieces recurs after 16
+    // tokens).
+    [[maybe_unused]] auto piece_of = [&](int n, bool is_v) {
+        const int r = n * kPerCopy + lane / L::kChunks;
+        return (lane % L::kChunks) ^ (is_v ? L::v_swizzle(r) : L::k_swizzle(r));
+    };
+    [[maybe_unused]] auto send = [&](const Place& p, int slot, bool is_v) {
+        const uint8_t* base = (is_v ? a.v_cache : a.k_cache) + head_bytes;
+        const uint32_t dst = lds_base + static_cast<uint32_t>((is_v ? 2 + slot : slot) * K::kOperand + wave * kMine * L::kRowBytes);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = ll == 0.0f ? 0.0f : sum[e] * by;
-            const int64_t at = out_row * a.head_dim + dim;
-            if constexpr (kSplit || (!kCodes && sizeof(T) == 4)) {
-                *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at) = f32x4_t{o[0], o[1], o[2], o[3]};
-            } else {
-                const bool bf16 = kCodes ? a.query_bf16 : std::is_same<T, bf16_t>::value;
-                uint2 two;
-                if (bf16) {
-                    two = make_uint2(Storage<bf16_t>::to_bits2(o[0], o[1]), Storage<bf16_t>::to_bits2(o[2], o[3]));
-                } else {
-                    two = make_uint2(Storage<f16_t>::to_bits2(o[0], o[1]), Storage<f16_t>::to_bits2(o[2], o[3]));
-                }
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = two;
+        for (int n0 = 0; n0 < kCopies; n0 += kBatch) {
+            uint32_t at[kBatch];
+            const uint8_t* from[kBatch];
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                at[n] = static_cast<uint32_t>(
+                    __shfl(static_cast<int>(p.row), wave * kMine + (n0 + n) * kPerCopy + lane / L::kChunks));
             }
-            continue;
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                from[n] = base + piece_of(n0 + n, is_v) * 16 + static_cast<uint64_t>(at[n]) * token_bytes;
+            }
+            if constexpr (kBatch == 4) {
+                if (whole) {
+                    copy16x4_to_lds(from[0], from[1] - 1024, from[2] - 2048, from[3] - 3072,
+                                    dst + static_cast<uint32_t>(n0) * 16 * kWaveSize);
+                    continue;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                if (piece_of(n0 + n, is_v) < row_pieces) {
+                    copy16_to_lds(from[n], dst + static_cast<uint32_t>(n0 + n) * 16 * kWaveSize);
+                }
+            }
         }
-        const int64_t at = static_cast<int64_t>(w.split) * a.tokens * a.heads + out_row;
-        if (dim == 0) {
-            a.ml[2 * at] = mm;
-            a.ml[2 * at + 1] = ll;
+    };
+    // 8-bit caches: 16 codes a lane and load; wave 0 has K's scales, wave 1 V's.
+    constexpr int kCodeLanes = kD / 16;                  // per token
+    constexpr int kCodeTokens = kWaveSize / kCodeLanes;  // per load
+    constexpr int kLoads = kCodes ? kMine / kCodeTokens : 1;
+    static_assert(!kCodes || kMine % kCodeTokens == 0, "whole loads");
+    struct Codes {
+        u32x4_t raw[kLoads];
+    };
+    [[maybe_unused]] Codes k_codes, v_codes;
+    [[maybe_unused]] float raw_scale = 0.0f;
+    [[maybe_unused]] auto load_codes = [&](Codes& to, const Place& p, bool is_v) {
+        const uint8_t* base = (is_v ? a.v_cache : a.k_cache) + head_bytes;
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const int r = wave * kMine + n * kCodeTokens + lane / kCodeLanes;
+            const uint32_t at = static_cast<uint32_t>(__shfl(static_cast<int>(p.row), r));
+            const int piece = lane % kCodeLanes;
+            to.raw[n] = u32x4_t{0u, 0u, 0u, 0u};
+            if (piece < row_pieces && ((p.there >> r) & 1) != 0) {
+                to.raw[n] = *reinterpret_cast<const u32x4_t*>(base + static_cast<uint64_t>(at) * token_bytes + piece * 16);
+            }
         }
-        *reinterpret_cast<f32x4_t*>(a.acc + at * a.pitch + dim) = sum;
+        if (wave == (is_v ? 1 : 0)) {
+            // A value's scale that is not finite makes its key's one NaN and is 0 itself:
+            // rows that see the token are NaN, the others never meet it.
+            const int64_t at = static_cast<int64_t>(p.row) * a.kv_heads + w.kv_head;
+            const bool there = ((p.there >> lane) & 1) != 0;
+            const float of_v = there ? a.v_scales[at] : 0.0f;
+            const bool finite = __builtin_isfinite(of_v);
+            if (is_v) {
+                raw_scale = finite ? of_v : 0.0f;
+            } else {
+                raw_scale = there ? a.k_scales[at] : 0.0f;
+                raw_scale = finite ? raw_scale : __uint_as_float(0x7FC00000u);
+            }
+        }
+    };
+    [[maybe_unused]] auto scales_of = [&](int tile) {
+        return reinterpret_cast<float*>(lds + K::kScalesAt) + (tile & 1) * K::kScales;
+    };
+    [[maybe_unused]] auto store_codes = [&](const Codes& from, int tile, bool is_v) {
+        uint8_t* to = lds + ((is_v ? 2 : 0) + (tile & 1)) * K::kOperand;
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const int r = wave * kMine + n * kCodeTokens + lane / kCodeLanes;
+            const int sw = is_v ? L::v_swizzle(r) : L::k_swizzle(r);
+            const int piece = lane % kCodeLanes;
+            u32x4_t lo, hi;
+            widen16<kCodes ? kHeld : CF_CACHE_INT8>(from.raw[n], lo, hi);
+            if (piece < row_pieces) {
+                *reinterpret_cast<u32x4_t*>(to + r * L::kRowBytes + (((2 * piece) ^ sw) << 4)) = lo;
+                *reinterpret_cast<u32x4_t*>(to + r * L::kRowBytes + (((2 * piece + 1) ^ sw) << 4)) = hi;
+            }
+        }
+        if (wave == (is_v ? 1 : 0)) {
+            float* scales = scales_of(tile);
+            scales[(is_v ? kTokens : 0) + lane] = raw_scale;
+            if (is_v) {
+                const float top = wave_reduce_f32<MaxF32>(fabsf(raw_scale));
+                if (lane == 0) reinterpret_cast<int*>(scales)[2 * kTokens] = max(__builtin_amdgcn_frexp_expf(top), kLeastUnit);
+            }
+        }
+    };
+
+    float m = -INFINITY;  // the row's running maximum
+    float l = 0.0f;       // this lane's share of the running sum
+    float shift = -L::kLift;
+    [[maybe_unused]] int unit = kLeastUnit;  // see soften in attend
+    Score acc[L::kAcc / L::kScores];
+#pragma unroll
+    for (int b = 0; b < L::kAcc / L::kScores; ++b) {
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) acc[b][i] = 0.0f;
     }
+    auto scores = [&](int slot, int half) {
+        const uint8_t* k = lds + slot * K::kOperand + half * 32 * L::kRowBytes;
+        Score s = L::scores(k, q, lane);
+        if constexpr (kSplit) {
+            const Score low = L::scores(k, q_low, lane);
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) s[i] += low[i];
+        }
+        return s;
+    };
+    auto scale_scores = [&](Score& s, int tile, int half) {
+        if constexpr (kCodes) {
+            const float* scales = scales_of(tile) + 32 * half + 4 * L::part_of(lane);
+#pragma unroll
+            for (int i = 0; i < L::kScores; ++i) s[i] *= scales[L::token_of(i)];
+        }
+    };
+    auto rescale_to = [&](float top, int most) {
+        const float m_new = fmaxf(m, groups_max<L::kRows>(top) * c);
+        if (__builtin_amdgcn_ballot_w64(m_new > m + L::kLag || (kCodes && most > unit)) != 0) {
+            float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+            m = m_new;
+            if constexpr (kCodes) {
+                const int old = unit;
+                unit = most > unit ? most : unit;
+                f = __builtin_amdgcn_ldexpf(f, old - unit);
+            }
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < L::kAcc / L::kScores; ++b) {
+#pragma unroll
+                for (int i = 0; i < L::kScores; ++i) acc[b][i] *= f;
+            }
+            shift = (m == -INFINITY ? 0.0f : m) + (kCodes ? static_cast<float>(unit) : 0.0f) - L::kLift;
+        }
+    };
+    auto largest = [&](const Score& s0, const Score& s1) {
+        float top = fmaxf(s0[0], s1[0]);
+#pragma unroll
+        for (int i = 1; i < L::kScores; ++i) top = fmaxf(fmaxf(top, s0[i]), s1[i]);
+        return top;
+    };
+    // Scores to weights.
+    auto weigh = [&](Score& s, int tile, int half) {
+        [[maybe_unused]] const float* by = scales_of(tile) + kTokens + 32 * half + 4 * L::part_of(lane);
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -shift));
+            l += s[i];
+            if constexpr (kCodes) s[i] *= by[L::token_of(i)];
+            // One value for both fp16 parts: the product could be rounded to fp16 at once.
+            if constexpr (kSplit) {
+                float x = s[i];
+                asm volatile("" : "+v"(x));
+                s[i] = x;
+            }
+        }
+    };
+    // Values for the product of tokens 32 half + 16 u .. + 15 with dims 32 b .. + 31.
+    constexpr int kPieces = 2 * (kD / 32);  // of a half
+    auto read_values = [&](int slot, int half, int n) {
+        const int u = n & 1;
+        const int b = n >> 1;
+        const int j = lane & 15;
+        const int r = 16 * u + 4 * (lane >> 5) + (j >> 2);
+        const int piece = (4 * b + 2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ L::v_swizzle(r);
+        uint8_t* at = lds + (2 + slot) * K::kOperand + half * 32 * L::kRowBytes + r * L::kRowBytes + (piece << 4) + (j & 1) * 8;
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(lds_u8_t*)at);
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(lds_u8_t*)(at + 8 * L::kRowBytes));
+        return __builtin_bit_cast(u32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    struct Weights {
+        u32x4_t part[2];  // of 16 tokens each
+    };
+    auto pack = [&](const Score& s) {
+        Weights w2;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = s[8 * u + 2 * e];
+                const float p1 = s[8 * u + 2 * e + 1];
+                if constexpr (std::is_same<T, bf16_t>::value) {
+                    w2.part[u][e] = f32x2_to_bf16x2_bits(p0, p1);
+                } else {
+                    typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+                    w2.part[u][e] = __builtin_bit_cast(uint32_t, f16x2_v{static_cast<_Float16>(p0), static_cast<_Float16>(p1)});
+                }
+            }
+        }
+        return w2;
+    };
+    // What fp16 weights leave of s (kSplit).
+    auto rest_of = [&](const Score& s) {
+        Score r;
+#pragma unroll
+        for (int i = 0; i < L::kScores; ++i) r[i] = s[i] - static_cast<float>(static_cast<_Float16>(s[i]));
+        return r;
+    };
+    auto multiply = [&](const u32x4_t& v, const u32x4_t& p, Score& sum) {
+        if constexpr (std::is_same<T, bf16_t>::value) {
+            sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, p),
+                                                          sum, 0, 0, 0);
+        } else {
+            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, v), __builtin_bit_cast(f16x8_t, p),
+                                                         sum, 0, 0, 0);
+        }
+    };
+    // Values of tokens that are not there, and in tiles that some row does not see
+    // whole those that are not finite (see guard in attend), to 0. Returns the latter
+    // tokens, a bit each.
+    auto sanitise = [&](int slot, int first, uint64_t there) -> uint64_t {
+        const bool hidden = min(first + kTokens, w.hi) - 1 > tile_least;
+        if (there == kAll && !hidden) return 0;
+        constexpr uint32_t kExponent = std::is_same<T, f16_t>::value ? 0x7C00u : 0x7F80u;
+        u32x4_t* v = reinterpret_cast<u32x4_t*>(lds + (2 + slot) * K::kOperand);
+        uint64_t bad = 0;
+#pragma unroll 1
+        for (int i = tid; i < kTokens * L::kChunks; i += kThreads) {
+            u32x4_t four = v[i];
+            bool any = false;
+            const bool out = ((there >> (i / L::kChunks)) & 1) == 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool low = hidden && (four[e] & kExponent) == kExponent;
+                const bool high = hidden && (four[e] >> 16 & kExponent) == kExponent;
+                any = any || low || high;
+                four[e] = out ? 0u : four[e] & (low ? 0xFFFF0000u : 0xFFFFFFFFu) & (high ? 0xFFFFu : 0xFFFFFFFFu);
+            }
+            if (any || out) v[i] = four;
+            if (any && !out) bad |= uint64_t{1} << (i / L::kChunks);
+        }
+#pragma unroll
+        for (int d = 1; d < kWaveSize; d <<= 1) bad |= static_cast<uint64_t>(__shfl_xor(static_cast<long long>(bad), d));
+        if (lane == 0) lds_bad[wave] = bad;
+        __syncthreads();
+        return lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3];
+    };
+
+    Place here = look_up(0);  // of tile i
+    Place next{0u, 0u};       // of tile i + 1
+    if (tiles > 1) next = look_up(1);
+    Score s0, s1;
+    if constexpr (kCodes) {
+        load_codes(k_codes, here, false);
+        load_codes(v_codes, here, true);
+        store_codes(k_codes, 0, false);
+        store_codes(v_codes, 0, true);
+        if (tiles > 1) {
+            load_codes(k_codes, next, false);
+            load_codes(v_codes, next, true);
+        }
+    } else {
+        send(here, 0, false);
+        send(here, 0, true);
+        if (tiles > 1) send(next, 1, false);
+        wait_vm<0>();
+        bare_barrier();
+        s0 = scores(0, 0);
+        s1 = scores(0, 1);
+    }
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+        const int at = i & 1;
+        const int first = w.lo + i * kTokens;
+        Place far{0u, 0u};
+        [[maybe_unused]] Score n0, n1;
+        // Codes: tile i is in LDS, tile i + 1 in registers, loaded an iteration ago.
+        // Plain: K of tile i + 1 and V of tile i are in LDS. The places that the
+        // iteration before left are free.
+        if constexpr (!kCodes) wait_vm<0>();
+        wait_lds();
+        bare_barrier();
+        if constexpr (kCodes) {
+            if (i + 1 < tiles) {
+                store_codes(k_codes, i + 1, false);
+                store_codes(v_codes, i + 1, true);
+            }
+            if (i + 2 < tiles) {
+                far = look_up(i + 2);
+                load_codes(k_codes, far, false);
+                load_codes(v_codes, far, true);
+            }
+            s0 = scores(at, 0);
+            s1 = scores(at, 1);
+        } else {
+            if (i + 2 < tiles) {
+                far = look_up(i + 2);
+                send(far, at, false);
+            }
+            if (i + 1 < tiles) send(next, at ^ 1, true);
+        }
+        // (Behind the last tile these are scores of nothing, used by nobody.)
+        if constexpr (!kCodes) n0 = scores(at ^ 1, 0);
+        scale_scores(s0, i, 0);
+        scale_scores(s1, i, 1);
+        int most = 0;
+        if constexpr (kCodes) most = reinterpret_cast<const int*>(scales_of(i))[2 * kTokens];
+        const bool masked = here.there != kAll || first + kTokens - 1 > tile_least;
+        uint64_t sees = kAll;
+        if (masked) {
+            const int count = limit - first + 1;
+            sees = here.there & (count >= kTokens ? kAll : count <= 0 ? 0u : (uint64_t{1} << count) - 1u);
+            const uint32_t sees0 = static_cast<uint32_t>(sees) >> (4 * L::part_of(lane));
+            const uint32_t sees1 = static_cast<uint32_t>(sees >> 32) >> (4 * L::part_of(lane));
+            float above = 0.0f;
+#pragma unroll
+            for (int e = 0; e < L::kScores; ++e) {
+                const bool see0 = (sees0 & (1u << L::token_of(e))) != 0;
+                const bool see1 = (sees1 & (1u << L::token_of(e))) != 0;
+                s0[e] = see0 ? s0[e] : -INFINITY;
+                s1[e] = see1 ? s1[e] : -INFINITY;
+                if constexpr (kCodes) {
+                    const float* by = scales_of(i) + kTokens + 4 * L::part_of(lane) + L::token_of(e);
+                    above = fmaxf(above, see0 ? fabsf(by[0]) : 0.0f);
+                    above = fmaxf(above, see1 ? fabsf(by[32]) : 0.0f);
+                }
+            }
+            if constexpr (kCodes) most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(above));
+        }
+        rescale_to(largest(s0, s1), most);
+        if (masked) {
+            const uint64_t bad = sanitise(at, first, here.there);
+            if ((bad & sees) != 0) l = __uint_as_float(0x7FC00000u);
+        }
+        // Three stretches of products, each with the vector work of another part
+        // among them; values are read a stretch ahead of their product.
+        if constexpr (!kCodes) n1 = scores(at ^ 1, 1);
+        weigh(s0, i, 0);
+        const Weights p0 = pack(s0);
+        u32x4_t v[kPieces];
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n) v[n] = read_values(at, 0, n);
+        __builtin_amdgcn_sched_barrier(0);
+        weigh(s1, i, 1);
+        const Weights p1 = pack(s1);
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n) {
+            multiply(v[n], p0.part[n & 1], acc[n >> 1]);
+            if constexpr (kSplit) multiply(v[n], pack(rest_of(s0)).part[n & 1], acc[n >> 1]);
+            v[n] = read_values(at, 1, n);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n) {
+            multiply(v[n], p1.part[n & 1], acc[n >> 1]);
+            if constexpr (kSplit) multiply(v[n], pack(rest_of(s1)).part[n & 1], acc[n >> 1]);
+        }
+        if constexpr (!kCodes) {
+            s0 = n0;
+            s1 = n1;
+        }
+        here = next;
+        next = far;
+    }
+    finish<T, kD, kCodes, kSplit, true>(a, w, lds, lds_m, lds_l, m + (kCodes ? static_cast<float>(unit) : 0.0f), l, acc);
 }
 
 /// Zeros for the rows first_row .. first_row + count - 1 of a KV head's heads,
@@ -787,15 +1273,27 @@ __device__ void zero_rows(const ChunkArgs& a, int first, int kv_head, int first_
 }
 
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
+constexpr int lds_of() {
+    constexpr int own = Kind<T, kD, kHeld, kSplit>::lds_bytes();
+    if constexpr (Tile<T, kD>::kWide) {
+        return own;
+    } else {
+        constexpr int rows = RowsKind<T, kD, kHeld>::lds_bytes();
+        return own > rows ? own : rows;
+    }
+}
+
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_kernel(ChunkArgs a) {
     using K = Kind<T, kD, kHeld, kSplit>;
     using L = typename K::L;
     using O = std::conditional_t<kSplit, float, T>;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[K::lds_bytes()];
+    constexpr int kLds = lds_of<T, kD, kHeld, kSplit>();
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
     __shared__ float lds_m[kWaves][32];
     __shared__ float lds_l[kWaves][32];
-    __shared__ uint32_t lds_bad[kWaves];
+    __shared__ uint64_t lds_bad[kWaves];
     constexpr int kRows = kWaves * L::kRows;
     // KV heads vary fastest: workgroup i runs on XCD i % 8, so with 8 of them an
     // XCD reads one head's keys and values.
@@ -823,7 +1321,11 @@ __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_k
     w.table = a.tables + static_cast<int64_t>(s.sequence) * a.max_blocks;
     w.direct = reach.each >= reach.hi;
     if (end_row - w.first_row > L::kRows) {
-        attend<T, kD, kHeld, kSplit, true>(a, w, lds, lds_m, lds_l, lds_bad);
+        if constexpr (L::kWide) {
+            attend<T, kD, kHeld, kSplit, true>(a, w, lds, lds_m, lds_l, lds_bad);
+        } else {
+            attend_rows<T, kD, kHeld, kSplit>(a, w, lds, lds_m, lds_l, lds_bad);
+        }
     } else {
         attend<T, kD, kHeld, kSplit, false>(a, w, lds, lds_m, lds_l, lds_bad);
     }
