@@ -62,6 +62,7 @@ struct ChunkArgs {
     int pitch;  // head_dim rounded up to 4
     int max_blocks;
     int capacity;  // tokens a table row reaches
+    uint32_t token_pieces;  // 16 bytes of a token of the cache
     int splits;
     int step;  // tokens of a range are a multiple of this
     int least;  // and at least about this
@@ -862,7 +863,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     uint32_t window = w.table[min(window_base + lane, last_block)];
     constexpr uint64_t kAll = ~uint64_t{0};
     struct Place {
-        uint32_t row;    // of the cache: token `lane` of the tile; 0 where it is not there
+        uint32_t piece;  // of token `lane` of the tile: where its row begins in the cache, in 16 bytes;
+                         // 0 where it is not there
         uint64_t there;  // a bit per token
     };
     auto look_up = [&](int tile) {
@@ -877,13 +879,12 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         const int block = block_of(t);
         const uint32_t page = static_cast<uint32_t>(__shfl(static_cast<int>(window), block - window_base));
         const bool there = page < a.pages && first + lane < w.hi;
-        return Place{there ? page * a.block_size + (static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size) : 0u,
-                     __builtin_amdgcn_ballot_w64(there)};
+        const uint32_t row = page * a.block_size + (static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size);
+        return Place{there ? row * a.token_pieces : 0u, __builtin_amdgcn_ballot_w64(there)};
     };
 
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
     const int held_size = kCodes ? 1 : static_cast<int>(sizeof(T));
-    const uint32_t token_bytes = static_cast<uint32_t>(a.kv_heads) * a.head_dim * held_size;
     const uint64_t head_bytes = static_cast<uint64_t>(w.kv_head) * a.head_dim * held_size;
     const int row_pieces = a.head_dim * held_size / 16;
     // This wave's share of a tile: tokens 16 wave .. + 15 of K and of V.
@@ -908,11 +909,11 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
 #pragma unroll
             for (int n = 0; n < kBatch; ++n) {
                 at[n] = static_cast<uint32_t>(
-                    __shfl(static_cast<int>(p.row), wave * kMine + (n0 + n) * kPerCopy + lane / L::kChunks));
+                    __shfl(static_cast<int>(p.piece), wave * kMine + (n0 + n) * kPerCopy + lane / L::kChunks));
             }
 #pragma unroll
             for (int n = 0; n < kBatch; ++n) {
-                from[n] = base + piece_of(n0 + n, is_v) * 16 + static_cast<uint64_t>(at[n]) * token_bytes;
+                from[n] = base + (static_cast<uint64_t>(at[n] + static_cast<uint32_t>(piece_of(n0 + n, is_v))) << 4);
             }
             if constexpr (kBatch == 4) {
                 if (whole) {
@@ -944,17 +945,16 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
             const int r = wave * kMine + n * kCodeTokens + lane / kCodeLanes;
-            const uint32_t at = static_cast<uint32_t>(__shfl(static_cast<int>(p.row), r));
-            const int piece = lane % kCodeLanes;
-            to.raw[n] = u32x4_t{0u, 0u, 0u, 0u};
-            if (piece < row_pieces && ((p.there >> r) & 1) != 0) {
-                to.raw[n] = *reinterpret_cast<const u32x4_t*>(base + static_cast<uint64_t>(at) * token_bytes + piece * 16);
-            }
+            const uint32_t at = static_cast<uint32_t>(__shfl(static_cast<int>(p.piece), r));
+            // A row that is not there, or the end of a narrow one, is read from the cache's
+            // or row's beginning instead and not used.
+            const int piece = lane % kCodeLanes < row_pieces ? lane % kCodeLanes : 0;
+            to.raw[n] = *reinterpret_cast<const u32x4_t*>(base + (static_cast<uint64_t>(at + static_cast<uint32_t>(piece)) << 4));
         }
         if (wave == (is_v ? 1 : 0)) {
             // A value's scale that is not finite makes its key's one NaN and is 0 itself:
             // rows that see the token are NaN, the others never meet it.
-            const int64_t at = static_cast<int64_t>(p.row) * a.kv_heads + w.kv_head;
+            const int64_t at = static_cast<int64_t>(p.piece / a.token_pieces) * a.kv_heads + w.kv_head;
             const bool there = ((p.there >> lane) & 1) != 0;
             const float of_v = there ? a.v_scales[at] : 0.0f;
             const bool finite = __builtin_isfinite(of_v);
@@ -1063,6 +1063,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     };
     // Values for the product of tokens 32 half + 16 u .. + 15 with dims 32 b .. + 31.
     constexpr int kPieces = 2 * (kD / 32);  // of a half
+    static_assert(kPieces >= 4, "as many as are read ahead");
     auto read_values = [&](int slot, int half, int n) {
         const int u = n & 1;
         const int b = n >> 1;
@@ -1233,23 +1234,25 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         if constexpr (!kCodes) n1 = scores(at ^ 1, 1);
         weigh(s0, i, 0);
         const Weights p0 = pack(s0);
-        u32x4_t v[kPieces];
+        constexpr int kFar = 4;  // products that values are read ahead of theirs
+        u32x4_t v[kFar];
 #pragma unroll
-        for (int n = 0; n < kPieces; ++n) v[n] = read_values(at, 0, n);
+        for (int n = 0; n < kFar; ++n) v[n] = read_values(at, 0, n);
         __builtin_amdgcn_sched_barrier(0);
         weigh(s1, i, 1);
         const Weights p1 = pack(s1);
 #pragma unroll
         for (int n = 0; n < kPieces; ++n) {
-            multiply(v[n], p0.part[n & 1], acc[n >> 1]);
-            if constexpr (kSplit) multiply(v[n], pack(rest_of(s0)).part[n & 1], acc[n >> 1]);
-            v[n] = read_values(at, 1, n);
+            multiply(v[n % kFar], p0.part[n & 1], acc[n >> 1]);
+            if constexpr (kSplit) multiply(v[n % kFar], pack(rest_of(s0)).part[n & 1], acc[n >> 1]);
+            v[n % kFar] = n + kFar < kPieces ? read_values(at, 0, n + kFar) : read_values(at, 1, n + kFar - kPieces);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < kPieces; ++n) {
-            multiply(v[n], p1.part[n & 1], acc[n >> 1]);
-            if constexpr (kSplit) multiply(v[n], pack(rest_of(s1)).part[n & 1], acc[n >> 1]);
+            multiply(v[n % kFar], p1.part[n & 1], acc[n >> 1]);
+            if constexpr (kSplit) multiply(v[n % kFar], pack(rest_of(s1)).part[n & 1], acc[n >> 1]);
+            if (n + kFar < kPieces) v[n % kFar] = read_values(at, 1, n + kFar);
         }
         if constexpr (!kCodes) {
             s0 = n0;
@@ -1665,6 +1668,7 @@ cf_status cf_paged_attention_chunk(const void* query, const void* k_cache, const
     a.pitch = (a.head_dim + 3) / 4 * 4;
     a.max_blocks = static_cast<int>(max_blocks_per_sequence);
     a.capacity = static_cast<int>(cf::capacity_of(max_blocks_per_sequence, block_size));
+    a.token_pieces = static_cast<uint32_t>(num_kv_heads * head_dim * static_cast<int64_t>(held) / 16);
     a.splits = p.splits;
     a.step = p.step;
     a.least = p.least;
