@@ -35,7 +35,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWaveSize;
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f;
-/// Of 8-bit caches' values, scales below 2^-90 count as that (see soften).
+/// Of 8-bit caches' values, scales below 2^-90 count as that (see attend_few).
 constexpr int kLeastUnit = -90;
 
 struct ChunkArgs {
@@ -188,60 +188,56 @@ struct Item {
     bool direct;    // the only piece: straight to the result
 };
 
-/// kHeld: how the cache holds its rows. T: the type of the tiles. kSplit: an
-/// fp32 query of an 8-bit cache.
-template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
-struct Kind {
-    using L = Tile<T, kD>;
-    static constexpr bool kCodes = kHeld != CF_CACHE_PLAIN;
-    static constexpr int kStages = kCodes ? 2 : 4;  // of a ring that the waves share
-    static constexpr int kScales = kCodes ? 2 * L::kTokens : 0;  // floats per tile
-    static constexpr int kTileBytes = 2 * L::kBytes + 4 * kScales;
+/// LDS of attend: its tiles, a ring that the waves share or one for each of them.
+template <int kD>
+struct WideKind {
+    using L = Tile<float, kD>;
+    static constexpr int kStages = 4;
+    static constexpr int kTileBytes = 2 * L::kBytes;
     static constexpr int lds_bytes() {
+        static_assert(kStages >= kWaves, "a tile for each wave too");
         constexpr int ring = kStages * kTileBytes;
-        constexpr int own = kWaves * kTileBytes;
         constexpr int outputs = kWaves * L::kRows * L::kOutPitch * 4;
-        constexpr int tiles = ring > own ? ring : own;
-        return tiles > outputs ? tiles : outputs;
+        return ring > outputs ? ring : outputs;
     }
 };
+
+/// 4 codes as fp16, 2 to a word.
+template <cf_cache_format kHeld>
+__device__ __forceinline__ uint2 widen4(uint32_t codes) {
+    if constexpr (kHeld == CF_CACHE_INT8) {
+        // 0x64uu is 1024 + u in fp16: u = code + 128 below it, 1152 taken off.
+        typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+        const uint32_t u = codes ^ 0x80808080u;
+        const f16x2_v less = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+        const uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - less);
+        const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - less);
+        return make_uint2(lo, hi);
+    } else {
+        return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, false)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, true)));
+    }
+}
 
 /// 16 codes as fp16, 8 to a vector.
 template <cf_cache_format kHeld>
 __device__ __forceinline__ void widen16(const u32x4_t& codes, u32x4_t& lo, u32x4_t& hi) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t a, b;
-        if constexpr (kHeld == CF_CACHE_INT8) {
-            // 0x64uu is 1024 + u in fp16: u = code + 128 below it, 1152 taken off.
-            typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
-            const uint32_t u = codes[i] ^ 0x80808080u;
-            const f16x2_v less = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
-            a = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - less);
-            b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - less);
-        } else {
-            a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], 1.0f, false));
-            b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], 1.0f, true));
-        }
-        if (i < 2) {
-            lo[2 * i] = a;
-            lo[2 * i + 1] = b;
-        } else {
-            hi[2 * i - 4] = a;
-            hi[2 * i - 3] = b;
-        }
-    }
+    const uint2 w0 = widen4<kHeld>(codes[0]);
+    const uint2 w1 = widen4<kHeld>(codes[1]);
+    const uint2 w2 = widen4<kHeld>(codes[2]);
+    const uint2 w3 = widen4<kHeld>(codes[3]);
+    lo = u32x4_t{w0.x, w0.y, w1.x, w1.y};
+    hi = u32x4_t{w2.x, w2.y, w3.x, w3.y};
 }
 
-/// This lane's query row (token of the segment, head of the KV head): fragments
+/// This lane's query row in a tile of layout L (token of the segment, head of the KV head): fragments
 /// q, and for kSplit what they leave; zeros outside. Returns the factor of its
 /// scores. 8-bit caches: scaled by a power of two to magnitudes of up to 2^15, the
 /// inverse in the factor.
-template <typename T, int kD, bool kCodes, bool kSplit>
+template <typename L, typename T, bool kCodes, bool kSplit>
 __device__ __forceinline__ float load_query(const ChunkArgs& a, const Item& w, bool inside, int token, int head, int lane,
-                                            typename Tile<T, kD>::Query (&q)[Tile<T, kD>::kQueries],
-                                            typename Tile<T, kD>::Query (&q_low)[kSplit ? Tile<T, kD>::kQueries : 1]) {
-    using L = Tile<T, kD>;
+                                            typename L::Query (&q)[L::kQueries],
+                                            typename L::Query (&q_low)[kSplit ? L::kQueries : 1]) {
     float c = a.c;
     const int64_t out_row = static_cast<int64_t>(w.first + token) * a.heads + w.kv_head * a.per + head;
     if constexpr (!kCodes) {
@@ -302,14 +298,70 @@ __device__ __forceinline__ float load_query(const ChunkArgs& a, const Item& w, b
     return c;
 }
 
-/// The waves' outputs to the result, or to a piece of it. m in base 2.
+/// Four neighbouring dims of a row from all of the waves that have some of its
+/// tokens: `sums` of the first, the others `pitch` floats apart.
+struct Joined {
+    float m, l;
+    f32x4_t sum;
+};
+template <int kTeam>
+__device__ __forceinline__ Joined join_waves(const float* sums, int pitch, const float (*lds_m)[32],
+                                             const float (*lds_l)[32], int row) {
+    Joined j{lds_m[0][row], 0.0f, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int t = 1; t < kTeam; ++t) j.m = fmaxf(j.m, lds_m[t][row]);
+#pragma unroll
+    for (int t = 0; t < kTeam; ++t) {
+        const float mt = lds_m[t][row];
+        const float f = mt == -INFINITY ? 0.0f : exp2f(mt - j.m);
+        // A wave without a finite score still passes its NaN on.
+        j.l += mt == -INFINITY ? lds_l[t][row] : lds_l[t][row] * f;
+        const f32x4_t four = *reinterpret_cast<const f32x4_t*>(sums + t * pitch);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) j.sum[e] = fmaf(four[e], f, j.sum[e]);
+    }
+    return j;
+}
+
+/// Four dims of row `row` of the segment to the result, or to a piece of it. m in base 2.
+template <typename T, bool kCodes, bool kSplit>
+__device__ __forceinline__ void put(const ChunkArgs& a, const Item& w, int row, int dim, float m, float l,
+                                    const f32x4_t& sum) {
+    const int64_t out_row = static_cast<int64_t>(w.first + row / a.per) * a.heads + w.kv_head * a.per + row % a.per;
+    if (!w.direct) {
+        const int64_t at = static_cast<int64_t>(w.split) * a.tokens * a.heads + out_row;
+        if (dim == 0) {
+            a.ml[2 * at] = m;
+            a.ml[2 * at + 1] = l;
+        }
+        *reinterpret_cast<f32x4_t*>(a.acc + at * a.pitch + dim) = sum;
+        return;
+    }
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    float o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = l == 0.0f ? 0.0f : sum[e] * by;
+    const int64_t at = out_row * a.head_dim + dim;
+    if constexpr (kSplit || (!kCodes && sizeof(T) == 4)) {
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at) = f32x4_t{o[0], o[1], o[2], o[3]};
+    } else {
+        const bool bf16 = kCodes ? a.query_bf16 : std::is_same<T, bf16_t>::value;
+        uint2 two;
+        if (bf16) {
+            two = make_uint2(Storage<bf16_t>::to_bits2(o[0], o[1]), Storage<bf16_t>::to_bits2(o[2], o[3]));
+        } else {
+            two = make_uint2(Storage<f16_t>::to_bits2(o[0], o[1]), Storage<f16_t>::to_bits2(o[2], o[3]));
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = two;
+    }
+}
+
+/// The waves' outputs, of different rows (kShared) or of different tokens.
 template <typename T, int kD, bool kCodes, bool kSplit, bool kShared>
 __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32],
                                        float (*lds_l)[32], float m, float l,
                                        const typename Tile<T, kD>::Score (&acc)[Tile<T, kD>::kAcc / Tile<T, kD>::kScores]) {
     using L = Tile<T, kD>;
-    constexpr int kRowWaves = kShared ? kWaves : 1;
-    constexpr int kTokenWaves = kShared ? 1 : kWaves;
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & (kWaveSize - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
@@ -330,8 +382,8 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
         lds_l[wave][L::row_of(lane)] = l;
     }
     __syncthreads();
-    // Rows x groups of four dims, over the workgroup; token waves are joined.
-    constexpr int kOutRows = kRowWaves * L::kRows;
+    // Rows x groups of four dims, over the workgroup.
+    constexpr int kOutRows = (kShared ? kWaves : 1) * L::kRows;
     constexpr int kFours = kD / 4;
     constexpr int kRounds = (kOutRows * kFours + kThreads - 1) / kThreads;
 #pragma unroll 2
@@ -342,62 +394,24 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
         if (r >= kOutRows) break;
         const int out = w.first_row + r;
         if (out >= w.rows || dim >= a.head_dim) continue;
-        const int owner = kShared ? r / L::kRows : 0;
-        const int lr = r % L::kRows;
-        const int64_t out_row = static_cast<int64_t>(w.first + out / a.per) * a.heads + w.kv_head * a.per + out % a.per;
-        float mm = lds_m[owner][lr];
-#pragma unroll
-        for (int t = 1; t < kTokenWaves; ++t) mm = fmaxf(mm, lds_m[t][lr]);
-        float ll = 0.0f;
-        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int t = 0; t < kTokenWaves; ++t) {
-            const int src = owner + t;
-            const float f = kTokenWaves == 1 ? 1.0f : lds_m[src][lr] == -INFINITY ? 0.0f : exp2f(lds_m[src][lr] - mm);
-            // A wave without a finite score still passes its NaN on.
-            ll += kTokenWaves > 1 && lds_m[src][lr] == -INFINITY ? lds_l[src][lr] : lds_l[src][lr] * f;
-            const f32x4_t four = *reinterpret_cast<const f32x4_t*>(
-                reinterpret_cast<const float*>(lds) + (src * L::kRows + lr) * L::kOutPitch + dim);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] = fmaf(four[e], f, sum[e]);
+        const float* sums = reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim;
+        if constexpr (kShared) {
+            put<T, kCodes, kSplit>(a, w, out, dim, lds_m[r / L::kRows][r % L::kRows], lds_l[r / L::kRows][r % L::kRows],
+                                   *reinterpret_cast<const f32x4_t*>(sums));
+        } else {
+            const Joined j = join_waves<kWaves>(sums, L::kRows * L::kOutPitch, lds_m, lds_l, r);
+            put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
         }
-        if (w.direct) {
-            const float by = ll == 0.0f ? 0.0f : 1.0f / ll;
-            float o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = ll == 0.0f ? 0.0f : sum[e] * by;
-            const int64_t at = out_row * a.head_dim + dim;
-            if constexpr (kSplit || (!kCodes && sizeof(T) == 4)) {
-                *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at) = f32x4_t{o[0], o[1], o[2], o[3]};
-            } else {
-                const bool bf16 = kCodes ? a.query_bf16 : std::is_same<T, bf16_t>::value;
-                uint2 two;
-                if (bf16) {
-                    two = make_uint2(Storage<bf16_t>::to_bits2(o[0], o[1]), Storage<bf16_t>::to_bits2(o[2], o[3]));
-                } else {
-                    two = make_uint2(Storage<f16_t>::to_bits2(o[0], o[1]), Storage<f16_t>::to_bits2(o[2], o[3]));
-                }
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = two;
-            }
-            continue;
-        }
-        const int64_t at = static_cast<int64_t>(w.split) * a.tokens * a.heads + out_row;
-        if (dim == 0) {
-            a.ml[2 * at] = mm;
-            a.ml[2 * at + 1] = ll;
-        }
-        *reinterpret_cast<f32x4_t*>(a.acc + at * a.pitch + dim) = sum;
     }
 }
 
-/// kShared: the waves take different rows of the tile, else different tokens of
-/// the same rows.
-template <typename T, int kD, cf_cache_format kHeld, bool kSplit, bool kShared>
+/// fp32 caches. kShared: the waves take different rows of the tile, else different
+/// tokens of the same rows.
+template <int kD, bool kShared>
 __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
                        uint64_t* lds_bad) {
-    using K = Kind<T, kD, kHeld, kSplit>;
+    using K = WideKind<kD>;
     using L = typename K::L;
-    constexpr bool kCodes = K::kCodes;
     constexpr int kTokenWaves = kShared ? 1 : kWaves;
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & (kWaveSize - 1);
@@ -411,8 +425,8 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
     const int token = inside ? row / a.per : 0;
     const int limit = inside ? w.offset + token : -1;  // the last token it sees
     typename L::Query q[L::kQueries];
-    [[maybe_unused]] typename L::Query q_low[kSplit ? L::kQueries : 1];
-    const float c = load_query<T, kD, K::kCodes, kSplit>(a, w, inside, token, inside ? row % a.per : 0, lane, q, q_low);
+    typename L::Query unused[1];
+    const float c = load_query<L, float, false, false>(a, w, inside, token, inside ? row % a.per : 0, lane, q, unused);
     // The smallest of the wave's limits: tiles up to it need no mask.
     int least = inside ? limit : 0x7FFFFFFF;
 #pragma unroll
@@ -462,20 +476,19 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
     };
 
     const uint32_t lds_own = __builtin_amdgcn_readfirstlane(lds_address(own));
-    const int held_size = kCodes ? 1 : static_cast<int>(sizeof(T));
-    const uint64_t token_bytes = static_cast<uint64_t>(a.kv_heads) * a.head_dim * held_size;
-    const uint64_t head_bytes = static_cast<uint64_t>(w.kv_head) * a.head_dim * held_size;
+    const uint64_t token_bytes = static_cast<uint64_t>(a.kv_heads) * a.head_dim * 4;
+    const uint64_t head_bytes = static_cast<uint64_t>(w.kv_head) * a.head_dim * 4;
     const uint8_t* k_head = a.k_cache + head_bytes;
     const uint8_t* v_head = a.v_cache + head_bytes;
 
-    // Plain caches: this wave's copies of a tile to LDS; of a shared one half of the
-    // waves copy K, the others V.
+    // This wave's copies of a tile to LDS; of a shared one half of the waves copy K,
+    // the others V.
     constexpr int kPerCopy = kWaveSize / L::kChunks;
     constexpr int kCopies = kShared ? 2 * L::kCopies / kWaves : L::kCopies;
     const bool shared_v = kShared && wave >= kWaves / 2;
     const int first_copy = kShared ? wave % (kWaves / 2) * kCopies : 0;
-    const int row_pieces = a.head_dim * held_size / 16;
-    [[maybe_unused]] auto copy = [&](uint32_t dst, bool is_v) {
+    const int row_pieces = a.head_dim / 4;
+    auto copy = [&](uint32_t dst, bool is_v) {
 #pragma unroll
         for (int n = 0; n < kCopies; ++n) {
             const int r = (first_copy + n) * kPerCopy + lane / L::kChunks;
@@ -487,57 +500,9 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
             }
         }
     };
-    // 8-bit caches: 16 codes a lane and load, this wave's share of a tile, and one
-    // scale (lanes 0 .. kTokens - 1 of K, the others of V).
-    constexpr int kCodeLanes = kD / 16;                  // per token
-    constexpr int kCodeTokens = kWaveSize / kCodeLanes;  // per load
-    constexpr int kLoads = L::kTokens / kCodeTokens;     // of K or V of a tile
-    constexpr int kShare = kShared ? 2 * kLoads / kWaves : 2 * kLoads;
-    static_assert(!kCodes || kShare * (kShared ? kWaves : 1) == 2 * kLoads, "loads per wave");
-    [[maybe_unused]] u32x4_t raw[kCodes ? kShare : 1];
-    [[maybe_unused]] float raw_scale = 0.0f;
-    [[maybe_unused]] uint32_t raw_valid = 0;
-    [[maybe_unused]] auto load_codes = [&]() {
-#pragma unroll
-        for (int n = 0; n < kShare; ++n) {
-            const int at = (kShared ? wave * kShare : 0) + n;  // K's loads, then V's
-            const int r = at % kLoads * kCodeTokens + lane / kCodeLanes;
-            const uint64_t from = static_cast<uint32_t>(__shfl(static_cast<int>(place), r)) * token_bytes;
-            const int piece = lane % kCodeLanes;
-            raw[n] = u32x4_t{0u, 0u, 0u, 0u};
-            if (piece < row_pieces && ((valid >> r) & 1) != 0) {
-                raw[n] = *reinterpret_cast<const u32x4_t*>((at < kLoads ? k_head : v_head) + from + piece * 16);
-            }
-        }
-        const int t = lane & (L::kTokens - 1);
-        const int64_t scale_at = static_cast<int64_t>(static_cast<uint32_t>(place)) * a.kv_heads + w.kv_head;
-        raw_scale = ((valid >> t) & 1) != 0 ? (lane < L::kTokens ? a.k_scales : a.v_scales)[scale_at] : 0.0f;
-        raw_valid = valid;
-    };
-    [[maybe_unused]] auto store_codes = [&](uint8_t* tile) {
-#pragma unroll
-        for (int n = 0; n < kShare; ++n) {
-            const int at = (kShared ? wave * kShare : 0) + n;
-            const int r = at % kLoads * kCodeTokens + lane / kCodeLanes;
-            const bool is_v = at >= kLoads;
-            const int sw = is_v ? L::v_swizzle(r) : L::k_swizzle(r);
-            const int piece = lane % kCodeLanes;
-            u32x4_t lo, hi;
-            widen16<kCodes ? kHeld : CF_CACHE_INT8>(raw[n], lo, hi);
-            uint8_t* to = tile + (is_v ? L::kBytes : 0) + r * L::kRowBytes;
-            if (piece < row_pieces) {
-                *reinterpret_cast<u32x4_t*>(to + (((2 * piece) ^ sw) << 4)) = lo;
-                *reinterpret_cast<u32x4_t*>(to + (((2 * piece + 1) ^ sw) << 4)) = hi;
-            }
-        }
-        // Of a shared tile every wave has all scales.
-        if (!kShared || wave == 0) reinterpret_cast<float*>(tile + 2 * L::kBytes)[lane] = raw_scale;
-    };
-
     float m = -INFINITY;  // the row's running maximum
     float l = 0.0f;       // this lane's share of the running sum
     float shift = -L::kLift;  // of the exponents
-    [[maybe_unused]] int unit = kLeastUnit;  // 8-bit caches: see soften
     typename L::Score acc[L::kAcc / L::kScores];
 #pragma unroll
     for (int b = 0; b < L::kAcc / L::kScores; ++b) {
@@ -562,80 +527,36 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
         }
     };
     // Scores of a tile to weights, and the running values.
-    auto soften = [&](typename L::Score& s, const uint8_t* tile, int first, uint32_t there) {
+    auto soften = [&](typename L::Score& s, int first, uint32_t there) {
         const bool masked = there != kAll || first + L::kTokens - 1 > wave_least;
         const uint32_t mine = masked ? seen(first, there) >> (4 * L::part_of(lane)) : 0u;
-        [[maybe_unused]] const float* scales = reinterpret_cast<const float*>(tile + 2 * L::kBytes) + 4 * L::part_of(lane);
-        if constexpr (kCodes) {
-#pragma unroll
-            for (int i = 0; i < L::kScores; ++i) s[i] *= scales[L::token_of(i)];
-        }
         if (masked) {
 #pragma unroll
             for (int i = 0; i < L::kScores; ++i) s[i] = (mine & (1u << L::token_of(i))) != 0 ? s[i] : -INFINITY;
-        }
-        // Probabilities are taken relative to a power of two 2^unit above all scales of
-        // values that the row met, sums too: times a scale they are at most 2^(kLift +
-        // kLag), as fp16 has to hold them.
-        [[maybe_unused]] float by[kCodes ? L::kScores : 1];
-        int most = kLeastUnit;
-        if constexpr (kCodes) {
-            float largest = 0.0f;
-#pragma unroll
-            for (int i = 0; i < L::kScores; ++i) {
-                by[i] = scales[L::kTokens + L::token_of(i)];
-                // What a row does not see may be NaN, or far above its own scales.
-                if (masked) by[i] = (mine & (1u << L::token_of(i))) != 0 ? by[i] : 0.0f;
-                largest = fmaxf(largest, fabsf(by[i]));
-            }
-            most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(largest));
         }
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < L::kScores; ++i) top = fmaxf(top, s[i]);
         top = groups_max<L::kRows>(top);
         const float m_new = fmaxf(m, top * c);
-        if (__builtin_amdgcn_ballot_w64(m_new > m + L::kLag || (kCodes && most > unit)) != 0) {
-            float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+        if (__builtin_amdgcn_ballot_w64(m_new > m + L::kLag) != 0) {
+            const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
             m = m_new;
-            if constexpr (kCodes) {
-                const int old = unit;
-                unit = most > unit ? most : unit;
-                f = __builtin_amdgcn_ldexpf(f, old - unit);
-            }
             l *= f;
             rescale(f);
-            shift = (m == -INFINITY ? 0.0f : m) + (kCodes ? static_cast<float>(unit) : 0.0f) - L::kLift;
+            shift = (m == -INFINITY ? 0.0f : m) - L::kLift;
         }
 #pragma unroll
         for (int i = 0; i < L::kScores; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -shift));
             l += s[i];
-            if constexpr (kCodes) s[i] *= by[i];
-            // One value for both fp16 parts: the product could be rounded to fp16 at once.
-            if constexpr (kSplit) {
-                float x = s[i];
-                asm volatile("" : "+v"(x));
-                s[i] = x;
-            }
         }
-    };
-    auto m_of = [&]() { return m + (kCodes ? static_cast<float>(unit) : 0.0f); };
-    auto scores = [&](const uint8_t* k) {
-        typename L::Score s = L::scores(k, q, lane);
-        if constexpr (kSplit) {
-            const typename L::Score low = L::scores(k, q_low, lane);
-#pragma unroll
-            for (int i = 0; i < L::kScores; ++i) s[i] += low[i];
-        }
-        return s;
     };
     // A token that a row of the tile does not see may hold NaN or infinities, which
     // times a weight of 0 would reach that row. In such tiles they are replaced by 0,
     // and a row that sees one gets a sum of NaN.
     auto guard = [&](uint8_t* v, int first, uint32_t there) {
         if (min(first + L::kTokens, w.hi) - 1 <= w.offset + w.first_row / a.per) return;
-        constexpr uint32_t kExponent = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, f16_t>::value ? 0x7C00u : 0x7F80u;
         uint32_t bad = 0;  // tokens
 #pragma unroll 1
         for (int i = kShared ? tid : lane; i < L::kTokens * L::kChunks; i += kShared ? kThreads : kWaveSize) {
@@ -643,10 +564,9 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
             bool any = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const bool low = (four[e] & kExponent) == kExponent;
-                const bool high = sizeof(T) == 2 && (four[e] >> 16 & kExponent) == kExponent;
-                any = any || low || high;
-                four[e] &= (low ? (sizeof(T) == 2 ? 0xFFFF0000u : 0u) : 0xFFFFFFFFu) & (high ? 0xFFFFu : 0xFFFFFFFFu);
+                const bool out = (four[e] & 0x7F800000u) == 0x7F800000u;
+                any = any || out;
+                four[e] = out ? 0u : four[e];
             }
             if (any) {
                 reinterpret_cast<u32x4_t*>(v)[i] = four;
@@ -667,63 +587,9 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
     auto add_values = [&](uint8_t* v, typename L::Score& s, int first, uint32_t there) {
         guard(v, first, there);
         L::values(v, s, acc, lane);
-        if constexpr (kSplit) {
-#pragma unroll
-            for (int i = 0; i < L::kScores; ++i) s[i] -= static_cast<float>(static_cast<_Float16>(s[i]));
-            L::values(v, s, acc, lane);
-        }
     };
 
-    if constexpr (kCodes) {
-        if (tiles > 0) {
-            look_up(begin);
-            load_codes();
-        }
-        // A tile is widened into LDS while the next one's codes are on their way; of a
-        // shared ring each barrier ends the reading of one stage and the writing of
-        // the other.
-        if constexpr (kShared) {
-            store_codes(own);
-            uint32_t there = raw_valid;
-            if (tiles > 1) {
-                look_up(begin + kStride);
-                load_codes();
-            }
-            __syncthreads();
-            for (int i = 0; i < tiles; ++i) {
-                uint8_t* tile = lds + (i & 1) * K::kTileBytes;
-                const int first = begin + i * kStride;
-                const uint32_t now = there;
-                if (i + 1 < tiles) {
-                    store_codes(lds + ((i + 1) & 1) * K::kTileBytes);
-                    there = raw_valid;
-                    if (i + 2 < tiles) {
-                        look_up(first + 2 * kStride);
-                        load_codes();
-                    }
-                }
-                typename L::Score s = scores(tile);
-                soften(s, tile, first, now);
-                add_values(tile + L::kBytes, s, first, now);
-                __syncthreads();
-            }
-        } else {
-            for (int i = 0; i < tiles; ++i) {
-                const int first = begin + i * kStride;
-                store_codes(own);
-                const uint32_t there = raw_valid;
-                if (i + 1 < tiles) {
-                    look_up(first + kStride);
-                    load_codes();
-                }
-                wait_lds();
-                typename L::Score s = scores(own);
-                soften(s, own, first, there);
-                add_values(own + L::kBytes, s, first, there);
-                wait_lds();
-            }
-        }
-    } else if constexpr (!kShared) {
+    if constexpr (!kShared) {
         // The wave's own K and V tile, one copied while the other is used.
         const uint32_t v_dst = lds_own + L::kBytes;
         uint8_t* v = own + L::kBytes;
@@ -739,13 +605,13 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
             // part in are not issued, so a head narrower than kD waits for all.)
             if (a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
             const uint32_t there = valid;
-            typename L::Score s = scores(own);
+            typename L::Score s = L::scores(own, q, lane);
             wait_lds();
             if (more) {
                 look_up(first + kStride);
                 copy(lds_own, false);
             }
-            soften(s, own, first, there);
+            soften(s, first, there);
             if (more && a.head_dim == kD) wait_vm<kCopies>(); else wait_vm<0>();
             if (there != kAll) {
                 clear(v, there, lane, kWaveSize);
@@ -782,8 +648,8 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
             if (i + kStages - 1 < tiles) issue(i + kStages - 1, (kAt + kStages - 1) % kStages);
             uint8_t* k = lds + kAt * K::kTileBytes;
             uint8_t* v = k + L::kBytes;
-            typename L::Score s = scores(k);
-            soften(s, k, begin + i * kStride, now);
+            typename L::Score s = L::scores(k, q, lane);
+            soften(s, begin + i * kStride, now);
             if (now != kAll) {
                 clear(v, now, tid, kThreads);
                 __syncthreads();
@@ -800,7 +666,449 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
         }
     }
 
-    finish<T, kD, kCodes, kSplit, kShared>(a, w, lds, lds_m, lds_l, m_of(), l, acc);
+    finish<float, kD, false, false, kShared>(a, w, lds, lds_m, lds_l, m, l, acc);
+}
+
+/// Where a lane's values lie when 16 rows meet 32 tokens in 16 x 16 products.
+/// The four groups of 16 lanes hold different dims of the keys (any order that the
+/// query shares will do), and of tokens a group has 4 group .. + 3 and the four 16
+/// further on: of the scores as of the values, so that weights are in place.
+template <typename T, int kD, bool kCodes>
+struct FewTile {
+    static constexpr int kRows = 16;
+    static constexpr int kTokens = 32;
+    static constexpr int kSize = kCodes ? 1 : 2;  // bytes of a held value
+    using Query = u32x4_t;
+    static constexpr int kQueries = kD / 32;  // products of 16 tokens
+    __device__ __forceinline__ static int row_of(int lane) { return lane & 15; }
+    __device__ __forceinline__ static int part_of(int lane) { return lane >> 4; }
+    /// First of the 8 dims of a lane's query piece u. 16 codes are loaded at once.
+    __device__ __forceinline__ static int query_dim(int u, int lane) {
+        return kCodes ? 64 * (u / 2) + 16 * (lane >> 4) + 8 * (u & 1) : 32 * u + 8 * (lane >> 4);
+    }
+    static constexpr int kKeyLoads = kD * kSize / 64;  // of 16 tokens, 16 bytes a lane
+    /// Values: a lane has kBlocks dims of each of its tokens, in pieces of up to 16 bytes.
+    static constexpr int kBlocks = kD / 16;
+    static constexpr int kPiece = kBlocks * kSize < 16 ? kBlocks : 16 / kSize;  // dims
+    static constexpr int kPieces = kBlocks / kPiece;
+    static constexpr int kWords = kPiece * kSize / 4;  // 32-bit words of a piece
+    __device__ __forceinline__ static int value_dim(int of16, int block) {
+        return kPiece * of16 + block % kPiece + 16 * kPiece * (block / kPiece);
+    }
+    static constexpr int kOutPitch = kD + 4;
+    /// LDS of a wave: a tile's places and scales, then the query of 16 rows where it is
+    /// kept there, in two parts at most; the outputs at the end.
+    static constexpr int kQueryAt = kTokens * 16;
+    static constexpr int kQueryBytes = kQueries * kWaveSize * 16;
+    static constexpr int kOwnBytes = kQueryAt + 2 * kQueryBytes > kRows * kOutPitch * 4 ? kQueryAt + 2 * kQueryBytes
+                                                                                        : kRows * kOutPitch * 4;
+    static constexpr float kLag = Tile<T, kD>::kLag;
+    static constexpr float kLift = Tile<T, kD>::kLift;
+};
+
+/// Up to 16 kTiles rows, the team's waves on different tokens. Keys go from memory
+/// to the registers of the matrix products: a lane loads the dims that it
+/// multiplies. Values are transposed there, by byte permutations of the 8 tokens
+/// that a lane needs of each of its dims. So a wave keeps a tile of keys or values
+/// in flight while it works on the other, and LDS holds no more than the tile's
+/// places and scales.
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kTiles, int kTeam>
+__device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32]) {
+    constexpr bool kCodes = kHeld != CF_CACHE_PLAIN;
+    using L = FewTile<T, kD, kCodes>;
+    constexpr int kTokens = L::kTokens;
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & (kWaveSize - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
+    const int group = lane >> 4;
+    const int of16 = lane & 15;
+
+    // This lane's query rows; those past the end are zeros.
+    u32x4_t q[kTiles][L::kQueries];
+    [[maybe_unused]] u32x4_t q_low[kTiles][kSplit ? L::kQueries : 1];
+    float c[kTiles];
+    int limit[kTiles];  // the last token the row sees
+    int least = 0x7FFFFFFF;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+        const int row = w.first_row + n * L::kRows + of16;
+        const bool inside = row < w.rows;
+        const int token = inside ? row / a.per : 0;
+        limit[n] = inside ? w.offset + token : -1;
+        least = min(least, inside ? limit[n] : 0x7FFFFFFF);
+        c[n] = load_query<L, T, kCodes, kSplit>(a, w, inside, token, inside ? row % a.per : 0, lane, q[n], q_low[n]);
+    }
+    // The smallest of the limits: tiles up to it need no mask.
+#pragma unroll
+    for (int d = 1; d < L::kRows; d <<= 1) least = min(least, __shfl_xor(least, d));
+    const int wave_least = __builtin_amdgcn_readfirstlane(least);
+
+    uint8_t* const own = lds + wave * L::kOwnBytes;
+    // Teams of 8, four waves a SIMD, have registers for all but the query.
+    constexpr bool kParked = kTeam == 8;
+    static_assert(!kParked || kTiles == 1, "one tile's query");
+    u32x4_t* const parked = reinterpret_cast<u32x4_t*>(own + L::kQueryAt) + lane;
+    if constexpr (kParked) {
+#pragma unroll
+        for (int u = 0; u < L::kQueries; ++u) {
+            parked[u * kWaveSize] = q[0][u];
+            if constexpr (kSplit) parked[(L::kQueries + u) * kWaveSize] = q_low[0][u];
+        }
+    }
+
+    // Tiles begin at multiples of kTokens (ranges do).
+    const int begin = w.lo + wave * kTokens;
+    constexpr int kStride = kTeam * kTokens;
+    const int tiles = begin < w.hi ? (w.hi - begin + kStride - 1) / kStride : 0;
+    const int last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
+    auto block_of = [&](int t) {
+        return static_cast<int>(a.block_shift >= 0 ? static_cast<uint32_t>(t) >> a.block_shift
+                                                   : static_cast<uint32_t>(t) / a.block_size);
+    };
+    // 64 entries of the block table in lane registers: looking a page up is then
+    // no load that would have to wait behind the tiles'.
+    int window_base = block_of(begin < w.hi ? begin : w.lo);
+    uint32_t window = w.table[min(window_base + lane, last_block)];
+    uint64_t* const places = reinterpret_cast<uint64_t*>(own);  // of the tile looked up last, in bytes
+    float* const scales = reinterpret_cast<float*>(own + kTokens * 8);  // of the tile at hand: keys', values'
+    const uint64_t head_bytes = static_cast<uint64_t>(w.kv_head) * a.head_dim * L::kSize;
+    uint32_t row = 0;    // of the cache: token lane % kTokens of the tile looked up last, 0 where it is not there
+    uint32_t there = 0;  // its tokens that are, a bit each
+    auto look_up = [&](int first) {
+        const int last = min(first + kTokens, w.hi) - 1;
+        if (block_of(last) >= window_base + kWaveSize) {
+            window_base = block_of(first);
+            window = w.table[min(window_base + lane, last_block)];
+            asm volatile("" : "+v"(window));  // waited for here, not behind the branch
+        }
+        const int t = min(first + (lane & (kTokens - 1)), last);
+        const int block = block_of(t);
+        const uint32_t page = static_cast<uint32_t>(__shfl(static_cast<int>(window), block - window_base));
+        const bool is = page < a.pages && first + (lane & (kTokens - 1)) < w.hi;
+        row = is ? page * a.block_size + (static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size) : 0u;
+        there = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(is));
+        if (lane < kTokens) places[lane] = ((static_cast<uint64_t>(row) * a.token_pieces) << 4) + head_bytes;
+    };
+
+    // A row's end that a narrow head lacks is read from the row's beginning instead.
+    const int row_bytes = a.head_dim * L::kSize;
+    const bool whole = a.head_dim == kD;
+    u32x4_t keys[2][L::kKeyLoads];
+    auto load_keys = [&]() {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const uint8_t* from = a.k_cache + places[16 * s + of16];
+#pragma unroll
+            for (int n = 0; n < L::kKeyLoads; ++n) {
+                const int at = 64 * n + 16 * group;
+                keys[s][n] = *reinterpret_cast<const u32x4_t*>(from + (at < row_bytes ? at : 0));
+            }
+        }
+    };
+    typedef uint32_t piece_t __attribute__((ext_vector_type(L::kWords == 1 ? 2 : L::kWords)));  // (one word: see below)
+    uint32_t values[8][L::kPieces][L::kWords];
+    auto load_values = [&]() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint8_t* from = a.v_cache + places[16 * (j >> 2) + 4 * group + (j & 3)];
+#pragma unroll
+            for (int n = 0; n < L::kPieces; ++n) {
+                const int at = (of16 + 16 * n) * L::kPiece * L::kSize;
+                const uint8_t* piece = from + (at < row_bytes ? at : 0);
+                if constexpr (L::kWords == 1) {
+                    values[j][n][0] = *reinterpret_cast<const uint32_t*>(piece);
+                } else {
+                    const piece_t words = *reinterpret_cast<const piece_t*>(piece);
+#pragma unroll
+                    for (int e = 0; e < L::kWords; ++e) values[j][n][e] = words[e];
+                }
+            }
+        }
+    };
+    // Lanes below kTokens: a key's scale, the others a value's.
+    [[maybe_unused]] float scale = 0.0f;
+    // (A choice between the two pointers would be made in memory.)
+    [[maybe_unused]] const int64_t scale_from =
+        w.kv_head + (lane < kTokens ? 0 : (reinterpret_cast<int64_t>(a.v_scales) - reinterpret_cast<int64_t>(a.k_scales)) / 4);
+    [[maybe_unused]] auto load_scale = [&]() {
+        scale = a.k_scales[static_cast<int64_t>(static_cast<uint64_t>(row) * static_cast<uint32_t>(a.kv_heads)) + scale_from];
+    };
+
+    float m[kTiles];      // the row's running maximum
+    float l[kTiles];      // this lane's share of the running sum
+    float shift[kTiles];  // of the exponents
+    [[maybe_unused]] int unit[kTiles];
+    f32x4_t acc[kTiles][L::kBlocks];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+        shift[n] = -L::kLift;
+        unit[n] = kLeastUnit;
+#pragma unroll
+        for (int b = 0; b < L::kBlocks; ++b) acc[n][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    auto multiply = [](const u32x4_t& x, const u32x4_t& y, const f32x4_t& sum) {
+        if constexpr (std::is_same<T, bf16_t>::value) {
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y),
+                                                           sum, 0, 0, 0);
+        } else {
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, x), __builtin_bit_cast(f16x8_t, y),
+                                                          sum, 0, 0, 0);
+        }
+    };
+    constexpr int kScores = 8;  // a lane's, tokens 4 group + (i & 3) + 16 (i >> 2)
+    auto token_of = [](int i) { return (i & 3) + 16 * (i >> 2); };
+
+    if (tiles > 0) {
+        look_up(begin);
+        load_keys();
+        if constexpr (kCodes) load_scale();
+        __builtin_amdgcn_sched_barrier(0);  // in the loop's order
+        load_values();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+        const int first = begin + i * kStride;
+        const uint32_t now = there;
+        const bool masked = now != 0xFFFFFFFFu || first + kTokens - 1 > wave_least;
+        if constexpr (kCodes) scales[lane] = scale;
+        // The next tile; behind the last one its tokens are not there, and every lane reads
+        // row 0 of the cache, for nobody: loads behind a branch would be waited for
+        // wherever one of the others is.
+        look_up(first + kStride);
+
+        // Scores.
+        f32x4_t s[kTiles][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) s[n][h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < L::kKeyLoads; ++i) {
+                u32x4_t part[kCodes ? 2 : 1];
+                u32x4_t raw = keys[h][i];
+                if (!whole) raw = 64 * i + 16 * group < row_bytes ? raw : u32x4_t{0u, 0u, 0u, 0u};
+                if constexpr (kCodes) widen16<kHeld>(raw, part[0], part[1]); else part[0] = raw;
+#pragma unroll
+                for (int e = 0; e < (kCodes ? 2 : 1); ++e) {
+                    const int u = kCodes ? 2 * i + e : i;
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) {
+                        s[n][h] = multiply(part[e], kParked ? parked[u * kWaveSize] : q[n][u], s[n][h]);
+                        if constexpr (kSplit) {
+                            s[n][h] = multiply(part[e], kParked ? parked[(L::kQueries + u) * kWaveSize] : q_low[n][u], s[n][h]);
+                        }
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_keys();
+        if constexpr (kCodes) load_scale();
+        __builtin_amdgcn_sched_barrier(0);
+
+        // Weights.
+        u32x4_t weights[kTiles];
+        [[maybe_unused]] u32x4_t rest[kTiles];  // what fp16 weights leave (kSplit)
+        [[maybe_unused]] float of_key[kScores], of_value[kScores];
+        if constexpr (kCodes) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(scales + 16 * h + 4 * group);
+                const f32x4_t v4 = *reinterpret_cast<const f32x4_t*>(scales + kTokens + 16 * h + 4 * group);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    of_key[4 * h + e] = k4[e];
+                    of_value[4 * h + e] = v4[e];
+                }
+            }
+        }
+        uint32_t sees[kTiles];  // of the lane's tokens
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            float x[kScores];
+            [[maybe_unused]] float by[kScores];
+#pragma unroll
+            for (int i = 0; i < kScores; ++i) {
+                x[i] = s[n][i >> 2][i & 3];
+                if constexpr (kCodes) {
+                    x[i] *= of_key[i];
+                    by[i] = of_value[i];
+                }
+            }
+            sees[n] = 0xFFFFFFFFu;
+            if (masked) {
+                const int count = limit[n] - first + 1;
+                sees[n] = (now & (count >= kTokens ? 0xFFFFFFFFu : count <= 0 ? 0u : (1u << count) - 1u)) >> (4 * group);
+#pragma unroll
+                for (int i = 0; i < kScores; ++i) {
+                    const bool see = (sees[n] & (1u << token_of(i))) != 0;
+                    x[i] = see ? x[i] : -INFINITY;
+                    // What a row does not see may be NaN, or far above its own scales.
+                    if constexpr (kCodes) by[i] = see ? by[i] : 0.0f;
+                }
+            }
+            // Probabilities of codes are taken relative to a power of two 2^unit above all
+            // scales of values that the row met, sums too: times a scale they are at most
+            // 2^(kLift + kLag), as fp16 has to hold them.
+            int most = kLeastUnit;
+            if constexpr (kCodes) {
+                float above = fabsf(by[0]);
+#pragma unroll
+                for (int i = 1; i < kScores; ++i) above = fmaxf(above, fabsf(by[i]));
+                most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(above));
+            }
+            float top = x[0];
+#pragma unroll
+            for (int i = 1; i < kScores; ++i) top = fmaxf(top, x[i]);
+            const float m_new = fmaxf(m[n], groups_max<L::kRows>(top) * c[n]);
+            if (__builtin_amdgcn_ballot_w64(m_new > m[n] + L::kLag || (kCodes && most > unit[n])) != 0) {
+                float f = __builtin_amdgcn_exp2f(m[n] - (m_new == -INFINITY ? 0.0f : m_new));
+                m[n] = m_new;
+                if constexpr (kCodes) {
+                    const int old = unit[n];
+                    unit[n] = most > old ? most : old;
+                    f = __builtin_amdgcn_ldexpf(f, old - unit[n]);
+                }
+                l[n] *= f;
+#pragma unroll
+                for (int b = 0; b < L::kBlocks; ++b) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][b][i] *= f;
+                }
+                shift[n] = (m[n] == -INFINITY ? 0.0f : m[n]) + (kCodes ? static_cast<float>(unit[n]) : 0.0f) - L::kLift;
+            }
+#pragma unroll
+            for (int i = 0; i < kScores; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c[n], -shift[n]));
+                l[n] += x[i];
+                if constexpr (kCodes) x[i] *= by[i];
+                // One value for both fp16 parts: the product could be rounded to fp16 at once.
+                if constexpr (kSplit) {
+                    float y = x[i];
+                    asm volatile("" : "+v"(y));
+                    x[i] = y;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (std::is_same<T, bf16_t>::value) {
+                    weights[n][e] = f32x2_to_bf16x2_bits(x[2 * e], x[2 * e + 1]);
+                } else {
+                    typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+                    const f16x2_v high = {static_cast<_Float16>(x[2 * e]), static_cast<_Float16>(x[2 * e + 1])};
+                    weights[n][e] = __builtin_bit_cast(uint32_t, high);
+                    if constexpr (kSplit) {
+                        rest[n][e] = __builtin_bit_cast(
+                            uint32_t, f16x2_v{static_cast<_Float16>(x[2 * e] - static_cast<float>(high[0])),
+                                              static_cast<_Float16>(x[2 * e + 1] - static_cast<float>(high[1]))});
+                    }
+                }
+            }
+        }
+
+        // Values. A token that a row of the tile does not see may hold NaN or infinities,
+        // which times a weight of 0 would reach that row. In such tiles they are replaced
+        // by 0, and a row that sees one gets a sum of NaN.
+        if (kHeld != CF_CACHE_INT8 && masked) {
+            // Adding `one` to an exponent of ones, or to e4m3's NaN, carries into the sign.
+            constexpr uint32_t one = kCodes ? 0x01010101u : std::is_same<T, f16_t>::value ? 0x04000400u : 0x00800080u;
+            constexpr uint32_t sign = kCodes ? 0x80808080u : 0x80008000u;
+            uint32_t bad = 0;  // of the lane's tokens, like sees
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int p = 0; p < L::kPieces; ++p) {
+#pragma unroll
+                    for (int word = 0; word < L::kWords; ++word) {
+                        const uint32_t out = ((values[j][p][word] & (sign - one)) + one) & sign;
+                        any |= out;
+                        values[j][p][word] &= ~((out >> (kCodes ? 7 : 15)) * (kCodes ? 0xFFu : 0xFFFFu));
+                    }
+                }
+                bad |= any != 0 ? 1u << token_of(j) : 0u;
+            }
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) bad |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(bad), d));
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+                if ((bad & sees[n]) != 0) l[n] = __uint_as_float(0x7FC00000u);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < L::kPieces; ++p) {
+#pragma unroll
+            for (int word = 0; word < L::kWords; ++word) {
+#pragma unroll
+                for (int half = 0; half < 2 / L::kSize; ++half) {  // two dims at a time, for the registers
+                    __builtin_amdgcn_sched_barrier(0);
+                    u32x4_t part[2];  // of a dim each: the lane's 8 tokens
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t x0 = values[2 * e][p][word];
+                        const uint32_t x1 = values[2 * e + 1][p][word];
+                        if constexpr (kCodes) {
+                            const uint2 two = widen4<kHeld>(__builtin_amdgcn_perm(x1, x0, half == 0 ? 0x05010400u : 0x07030602u));
+                            part[0][e] = two.x;
+                            part[1][e] = two.y;
+                        } else {
+                            part[0][e] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
+                            part[1][e] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        const int b = p * L::kPiece + word * (4 / L::kSize) + 2 * half + d;
+#pragma unroll
+                        for (int n = 0; n < kTiles; ++n) {
+                            acc[n][b] = multiply(part[d], weights[n], acc[n][b]);
+                            if constexpr (kSplit) acc[n][b] = multiply(part[d], rest[n], acc[n][b]);
+                        }
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_values();
+    }
+
+    // The waves' outputs joined, 16 rows at a time.
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        if (group == 0) {
+            lds_m[wave][n * L::kRows + of16] = m[n] + (kCodes ? static_cast<float>(unit[n]) : 0.0f);
+            lds_l[wave][n * L::kRows + of16] = l[n];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+        if (w.first_row + n * L::kRows >= w.rows) break;
+        __syncthreads();
+        float* mine = reinterpret_cast<float*>(own) + of16 * L::kOutPitch;
+#pragma unroll
+        for (int b = 0; b < L::kBlocks; b += 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                *reinterpret_cast<f32x4_t*>(mine + L::value_dim(4 * group + i, b)) =
+                    f32x4_t{acc[n][b][i], acc[n][b + 1][i], acc[n][b + 2][i], acc[n][b + 3][i]};
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < L::kRows * (kD / 4); i += kTeam * kWaveSize) {
+            const int r = i / (kD / 4);
+            const int dim = i % (kD / 4) * 4;
+            const int out = w.first_row + n * L::kRows + r;
+            if (out >= w.rows || dim >= a.head_dim) continue;
+            const Joined j = join_waves<kTeam>(reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim,
+                                               L::kOwnBytes / 4, lds_m, lds_l, n * L::kRows + r);
+            put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
+        }
+    }
 }
 
 /// LDS of attend_rows: two tiles of 64 tokens of K and of V, and for codes their
@@ -842,7 +1150,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     const int limit = inside ? w.offset + token : -1;  // the last token the row sees
     typename L::Query q[L::kQueries];
     [[maybe_unused]] typename L::Query q_low[kSplit ? L::kQueries : 1];
-    const float c = load_query<T, kD, kCodes, kSplit>(a, w, inside, token, inside ? row % a.per : 0, lane, q, q_low);
+    const float c = load_query<L, T, kCodes, kSplit>(a, w, inside, token, inside ? row % a.per : 0, lane, q, q_low);
     // The smallest limit of the rows: tiles up to it need no mask.
     const int tile_least = w.offset + w.first_row / a.per;
     if (a.head_dim < kD) {  // the copies leave the end of every row as it is
@@ -863,8 +1171,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     uint32_t window = w.table[min(window_base + lane, last_block)];
     constexpr uint64_t kAll = ~uint64_t{0};
     struct Place {
-        uint32_t piece;  // of token `lane` of the tile: where its row begins in the cache, in 16 bytes;
-                         // 0 where it is not there
+        uint32_t row;    // of the cache: token `lane` of the tile, 0 where it is not there
+        uint32_t piece;  // where it begins, in 16 bytes
         uint64_t there;  // a bit per token
     };
     auto look_up = [&](int tile) {
@@ -880,7 +1188,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         const uint32_t page = static_cast<uint32_t>(__shfl(static_cast<int>(window), block - window_base));
         const bool there = page < a.pages && first + lane < w.hi;
         const uint32_t row = page * a.block_size + (static_cast<uint32_t>(t) - static_cast<uint32_t>(block) * a.block_size);
-        return Place{there ? row * a.token_pieces : 0u, __builtin_amdgcn_ballot_w64(there)};
+        return Place{there ? row : 0u, there ? row * a.token_pieces : 0u, __builtin_amdgcn_ballot_w64(there)};
     };
 
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
@@ -954,7 +1262,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         if (wave == (is_v ? 1 : 0)) {
             // A value's scale that is not finite makes its key's one NaN and is 0 itself:
             // rows that see the token are NaN, the others never meet it.
-            const int64_t at = static_cast<int64_t>(p.piece / a.token_pieces) * a.kv_heads + w.kv_head;
+            const int64_t at = static_cast<int64_t>(p.row) * a.kv_heads + w.kv_head;
             const bool there = ((p.there >> lane) & 1) != 0;
             const float of_v = there ? a.v_scales[at] : 0.0f;
             const bool finite = __builtin_isfinite(of_v);
@@ -996,7 +1304,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     float m = -INFINITY;  // the row's running maximum
     float l = 0.0f;       // this lane's share of the running sum
     float shift = -L::kLift;
-    [[maybe_unused]] int unit = kLeastUnit;  // see soften in attend
+    [[maybe_unused]] int unit = kLeastUnit;  // see attend_few
     Score acc[L::kAcc / L::kScores];
 #pragma unroll
     for (int b = 0; b < L::kAcc / L::kScores; ++b) {
@@ -1113,7 +1421,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         }
     };
     // Values of tokens that are not there, and in tiles that some row does not see
-    // whole those that are not finite (see guard in attend), to 0. Returns the latter
+    // whole those that are not finite (see attend_few), to 0. Returns the latter
     // tokens, a bit each.
     auto sanitise = [&](int slot, int first, uint64_t there) -> uint64_t {
         const bool hidden = min(first + kTokens, w.hi) - 1 > tile_least;
@@ -1144,7 +1452,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     };
 
     Place here = look_up(0);  // of tile i
-    Place next{0u, 0u};       // of tile i + 1
+    Place next{};       // of tile i + 1
     if (tiles > 1) next = look_up(1);
     Score s0, s1;
     if constexpr (kCodes) {
@@ -1169,7 +1477,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     for (int i = 0; i < tiles; ++i) {
         const int at = i & 1;
         const int first = w.lo + i * kTokens;
-        Place far{0u, 0u};
+        Place far{};
         [[maybe_unused]] Score n0, n1;
         // Codes: tile i is in LDS, tile i + 1 in registers, loaded an iteration ago.
         // Plain: K of tile i + 1 and V of tile i are in LDS. The places that the
@@ -1266,72 +1574,99 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
 
 /// Zeros for the rows first_row .. first_row + count - 1 of a KV head's heads,
 /// counted from token `first`.
-template <typename O>
+template <typename O, int kTeam>
 __device__ void zero_rows(const ChunkArgs& a, int first, int kv_head, int first_row, int end_row) {
-    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(end_row - first_row) * a.head_dim; i += kThreads) {
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(end_row - first_row) * a.head_dim; i += kTeam * kWaveSize) {
         const int r = first_row + static_cast<int>(i / a.head_dim);
         const int64_t out_row = static_cast<int64_t>(first + r / a.per) * a.heads + kv_head * a.per + r % a.per;
         static_cast<O*>(a.out)[out_row * a.head_dim + i % a.head_dim] = O{};
     }
 }
 
-template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
-constexpr int lds_of() {
-    constexpr int own = Kind<T, kD, kHeld, kSplit>::lds_bytes();
-    if constexpr (Tile<T, kD>::kWide) {
-        return own;
-    } else {
-        constexpr int rows = RowsKind<T, kD, kHeld>::lds_bytes();
-        return own > rows ? own : rows;
-    }
-}
-
-template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
-__global__ __launch_bounds__(kThreads)
-__attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_kernel(ChunkArgs a) {
-    using K = Kind<T, kD, kHeld, kSplit>;
-    using L = typename K::L;
-    using O = std::conditional_t<kSplit, float, T>;
-    constexpr int kLds = lds_of<T, kD, kHeld, kSplit>();
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-    __shared__ float lds_m[kWaves][32];
-    __shared__ float lds_l[kWaves][32];
-    __shared__ uint64_t lds_bad[kWaves];
-    constexpr int kRows = kWaves * L::kRows;
+/// What workgroup `id` does, or nothing (after writing zeros for rows that see no
+/// token, where it is the first of theirs). O: the type of the result.
+template <typename O, int kTeam>
+__device__ bool item_of(const ChunkArgs& a, int rows, Item& w, int& end_row) {
     // KV heads vary fastest: workgroup i runs on XCD i % 8, so with 8 of them an
     // XCD reads one head's keys and values.
     int id = static_cast<int>(blockIdx.x);
-    Item w{};
     w.kv_head = id % a.kv_heads;
     id /= a.kv_heads;
     w.split = id % a.splits;
-    const Segment s = segment_of(a, kRows, id / a.splits);
-    if (s.count == 0) return;
+    const Segment s = segment_of(a, rows, id / a.splits);
+    if (s.count == 0) return false;
     w.first = s.first;
     w.rows = s.count * a.per;
-    w.first_row = s.tile * kRows;
-    const int end_row = min(w.rows, w.first_row + kRows);
+    w.first_row = s.tile * rows;
+    end_row = min(w.rows, w.first_row + rows);
     Reach reach{};
-    if (s.sequence >= 0) reach = reach_of(a, s, kRows);
+    if (s.sequence >= 0) reach = reach_of(a, s, rows);
     const Range range = range_of(0, reach.hi, reach.each, w.split);
     if (range.lo >= range.hi) {
-        if (reach.hi == 0 && w.split == 0) zero_rows<O>(a, s.first, w.kv_head, w.first_row, end_row);
-        return;
+        if (reach.hi == 0 && w.split == 0) zero_rows<O, kTeam>(a, s.first, w.kv_head, w.first_row, end_row);
+        return false;
     }
     w.lo = range.lo;
     w.hi = range.hi;
     w.offset = reach.offset;
     w.table = a.tables + static_cast<int64_t>(s.sequence) * a.max_blocks;
     w.direct = reach.each >= reach.hi;
-    if (end_row - w.first_row > L::kRows) {
-        if constexpr (L::kWide) {
-            attend<T, kD, kHeld, kSplit, true>(a, w, lds, lds_m, lds_l, lds_bad);
-        } else {
-            attend_rows<T, kD, kHeld, kSplit>(a, w, lds, lds_m, lds_l, lds_bad);
-        }
+    return true;
+}
+
+/// fp32 caches.
+template <int kD>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(2, 4))) void chunk_attention_wide_kernel(ChunkArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[WideKind<kD>::lds_bytes()];
+    __shared__ float lds_m[kWaves][32];
+    __shared__ float lds_l[kWaves][32];
+    __shared__ uint64_t lds_bad[kWaves];
+    constexpr int kRows = Tile<float, kD>::kRows;
+    Item w{};
+    int end_row = 0;
+    if (!item_of<float, kWaves>(a, kWaves * kRows, w, end_row)) return;
+    if (end_row - w.first_row > kRows) {
+        attend<kD, true>(a, w, lds, lds_m, lds_l, lds_bad);
     } else {
-        attend<T, kD, kHeld, kSplit, false>(a, w, lds, lds_m, lds_l, lds_bad);
+        attend<kD, false>(a, w, lds, lds_m, lds_l, lds_bad);
     }
+}
+
+/// 16-bit and 8-bit caches, chunks and single tokens in one launch.
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_kernel(ChunkArgs a) {
+    constexpr int kFew = kWaves * FewTile<T, kD, kHeld != CF_CACHE_PLAIN>::kOwnBytes;
+    constexpr int kMany = RowsKind<T, kD, kHeld>::lds_bytes();
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kFew > kMany ? kFew : kMany];
+    __shared__ float lds_m[kWaves][32];
+    __shared__ float lds_l[kWaves][32];
+    __shared__ uint64_t lds_bad[kWaves];
+    constexpr int kRows = Tile<T, kD>::kRows;
+    Item w{};
+    int end_row = 0;
+    if (!item_of<std::conditional_t<kSplit, float, T>, kWaves>(a, kWaves * kRows, w, end_row)) return;
+    if (end_row - w.first_row > kRows) {
+        attend_rows<T, kD, kHeld, kSplit>(a, w, lds, lds_m, lds_l, lds_bad);
+    } else if (end_row - w.first_row > 16) {
+        attend_few<T, kD, kHeld, kSplit, 2, kWaves>(a, w, lds, lds_m, lds_l);
+    } else {
+        attend_few<T, kD, kHeld, kSplit, 1, kWaves>(a, w, lds, lds_m, lds_l);
+    }
+}
+
+/// The same caches where there are only single tokens, or few more.
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kTiles, int kTeam>
+__global__ __launch_bounds__(kTeam * kWaveSize)
+__attribute__((amdgpu_waves_per_eu(kTeam == 8 ? 4 : kD > 128 ? 1 : 2, 4))) void few_attention_kernel(ChunkArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kTeam * FewTile<T, kD, kHeld != CF_CACHE_PLAIN>::kOwnBytes];
+    __shared__ float lds_m[kTeam][32];
+    __shared__ float lds_l[kTeam][32];
+    Item w{};
+    int end_row = 0;
+    if (!item_of<std::conditional_t<kSplit, float, T>, kTeam>(a, 16 * kTiles, w, end_row)) return;
+    attend_few<T, kD, kHeld, kSplit, kTiles, kTeam>(a, w, lds, lds_m, lds_l);
 }
 
 /// The general kernel: any head size and alignment, a wave per (token, head,
@@ -1475,10 +1810,18 @@ __global__ __launch_bounds__(kThreads) void chunk_attention_join_kernel(ChunkArg
 struct Plan {
     int dim;   // head size of the matrix kernel, or 0: the general kernel
     int rows;  // of a tile
+    bool few;  // tiles of 16 or 32 rows only
     int splits;
     int step;
     int least;
 };
+
+/// Row tiles of `segments` segments, at most: one more than the rows fill for each,
+/// and no more than tokens where a tile has a token's rows.
+int64_t tiles_of(int64_t rows, int64_t tokens, int64_t segments, int64_t per) {
+    const int64_t n = tokens * per / rows + segments;
+    return per <= rows && n > tokens ? tokens : n;
+}
 
 Plan plan_of(cf_dtype dtype, cf_cache_format format, int64_t tokens, int64_t sequences, int64_t heads,
              int64_t kv_heads, int64_t head_dim, int64_t capacity) {
@@ -1502,10 +1845,15 @@ Plan plan_of(cf_dtype dtype, cf_cache_format format, int64_t tokens, int64_t seq
         p.splits = splits(tokens * heads, 4096, p.least);
         return p;
     }
-    p.step = static_cast<int>(kWaves * wave_rows);
     p.least = 256;
-    const int64_t tiles = tokens * per / p.rows + (sequences < tokens ? sequences : tokens);
-    p.splits = splits(tiles * kv_heads, 512, p.least);
+    // Where no more tokens than sequences are given they are single ones, or a few
+    // sequences have several: small tiles and their own kernel, of more waves than the
+    // one for chunks has room for. (64 sequences of up to 4096 tokens, 8-bit cache: @@ us
+    // against @@.)
+    p.few = !wide && tokens <= sequences && per <= 32;
+    if (p.few) p.rows = per <= 16 ? 16 : 32;
+    p.step = static_cast<int>(p.few ? p.least : kWaves * wave_rows);
+    p.splits = splits(tiles_of(p.rows, tokens, sequences < tokens ? sequences : tokens, per) * kv_heads, 512, p.least);
     return p;
 }
 
@@ -1525,19 +1873,28 @@ bool sizes_ok(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads
            block_size > 0 && max_blocks > 0 && heads % kv_heads == 0;
 }
 
-/// Row tiles of all segments, at most: one more than the rows fill for each.
-int64_t tiles_of(const Plan& p, int64_t tokens, int64_t sequences, int64_t per) {
-    return tokens * per / p.rows + sequences + 2;
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
+void run_size(const ChunkArgs& a, const Plan& p, dim3 grid, hipStream_t stream) {
+    if constexpr (Tile<T, kD>::kWide) {
+        launch(chunk_attention_wide_kernel<kD>, grid, dim3(kThreads), 0, stream, a);
+    } else if (!p.few) {
+        launch(chunk_attention_kernel<T, kD, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
+    } else if (p.rows == 16) {
+        constexpr int kTeam = kHeld != CF_CACHE_PLAIN && kD <= 128 ? 8 : 4;
+        launch(few_attention_kernel<T, kD, kHeld, kSplit, 1, kTeam>, grid, dim3(kTeam * kWaveSize), 0, stream, a);
+    } else {
+        launch(few_attention_kernel<T, kD, kHeld, kSplit, 2, 4>, grid, dim3(4 * kWaveSize), 0, stream, a);
+    }
 }
 
 template <typename T, cf_cache_format kHeld, bool kSplit>
 void run_matrix(const ChunkArgs& a, const Plan& p, dim3 grid, hipStream_t stream) {
     if (p.dim == 64) {
-        launch(chunk_attention_kernel<T, 64, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
+        run_size<T, 64, kHeld, kSplit>(a, p, grid, stream);
     } else if (p.dim == 128) {
-        launch(chunk_attention_kernel<T, 128, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
+        run_size<T, 128, kHeld, kSplit>(a, p, grid, stream);
     } else if constexpr (kHeld != CF_CACHE_PLAIN || sizeof(T) == 2) {
-        launch(chunk_attention_kernel<T, 256, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
+        run_size<T, 256, kHeld, kSplit>(a, p, grid, stream);
     }
 }
 
@@ -1642,9 +1999,18 @@ cf_status cf_paged_attention_chunk(const void* query, const void* k_cache, const
     if (p.dim != 0 && !(cf::host_aligned(query, 16) && cf::host_aligned(k_cache, 16) &&
                         cf::host_aligned(v_cache, 16) && cf::host_aligned(out, 16))) {
         p.dim = 0;  // within the same workspace: as many ranges at most
+        p.few = false;
         p.rows = static_cast<int>(num_heads / num_kv_heads);
         p.step = 32;
         p.least = 64;
+    }
+    // The kernel for chunks counts a cache's 16-byte pieces in 32 bits. In larger ones
+    // (64 GiB and more) chunks go through the small tiles, which count them in 64.
+    const bool wide = dtype == CF_F32 && format == CF_CACHE_PLAIN;
+    const int64_t token_pieces = num_kv_heads * head_dim * static_cast<int64_t>(held) / 16;
+    if (p.dim != 0 && !wide && !p.few && num_pages * block_size > (int64_t{1} << 32) / token_pieces) {
+        p.few = true;
+        p.rows = 32;
     }
     cf::ChunkArgs a{};
     a.query = query;
@@ -1668,12 +2034,12 @@ cf_status cf_paged_attention_chunk(const void* query, const void* k_cache, const
     a.pitch = (a.head_dim + 3) / 4 * 4;
     a.max_blocks = static_cast<int>(max_blocks_per_sequence);
     a.capacity = static_cast<int>(cf::capacity_of(max_blocks_per_sequence, block_size));
-    a.token_pieces = static_cast<uint32_t>(num_kv_heads * head_dim * static_cast<int64_t>(held) / 16);
+    a.token_pieces = static_cast<uint32_t>(token_pieces);
     a.splits = p.splits;
     a.step = p.step;
     a.least = p.least;
     a.query_bf16 = dtype == CF_BF16;
-    const int64_t tiles = cf::tiles_of(p, num_tokens, num_sequences, a.per);
+    const int64_t tiles = cf::tiles_of(p.rows, num_tokens, num_sequences + 2, a.per);
     const int64_t rows = num_tokens * num_heads;
     const int64_t workgroups = p.dim == 0 ? cf::ceil_div<int64_t>(rows * p.splits, cf::kWaves)
                                           : tiles * p.splits * num_kv_heads;
