@@ -1423,7 +1423,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     // Values of tokens that are not there, and in tiles that some row does not see
     // whole those that are not finite (see attend_few), to 0. Returns the latter
     // tokens, a bit each.
-    auto sanitise = [&](int slot, int first, uint64_t there) -> uint64_t {
+    [[maybe_unused]] auto sanitise = [&](int slot, int first, uint64_t there) -> uint64_t {
         const bool hidden = min(first + kTokens, w.hi) - 1 > tile_least;
         if (there == kAll && !hidden) return 0;
         constexpr uint32_t kExponent = std::is_same<T, f16_t>::value ? 0x7C00u : 0x7F80u;
@@ -1511,7 +1511,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         int most = 0;
         if constexpr (kCodes) most = reinterpret_cast<const int*>(scales_of(i))[2 * kTokens];
         const bool masked = here.there != kAll || first + kTokens - 1 > tile_least;
-        uint64_t sees = kAll;
+        [[maybe_unused]] uint64_t sees = kAll;
         if (masked) {
             const int count = limit - first + 1;
             sees = here.there & (count >= kTokens ? kAll : count <= 0 ? 0u : (uint64_t{1} << count) - 1u);
@@ -1533,9 +1533,11 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
             if constexpr (kCodes) most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(above));
         }
         rescale_to(largest(s0, s1), most);
-        if (masked) {
-            const uint64_t bad = sanitise(at, first, here.there);
-            if ((bad & sees) != 0) l = __uint_as_float(0x7FC00000u);
+        if constexpr (kHeld != CF_CACHE_INT8) {  // whose codes are all finite
+            if (masked) {
+                const uint64_t bad = sanitise(at, first, here.there);
+                if ((bad & sees) != 0) l = __uint_as_float(0x7FC00000u);
+            }
         }
         // Three stretches of products, each with the vector work of another part
         // among them; values are read a stretch ahead of their product.
