@@ -6,6 +6,19 @@
 //
 // x [m, k] and w [n, k] are int8, both dense along k (w is a torch Linear's
 // weight), sums exact in int32.
+//
+// Few rows are bound by w, which is read once: its rows go from memory straight to
+// the matrix cores, 16 of them a workgroup, whose waves split k (8 rows by 11008
+// columns of 4096: 13.2 us, 3.4 TB/s; sending the next loads ahead of the products
+// changed nothing). Middling batches are bound by the steps of the loop over k,
+// each a barrier, LDS reads and a short chain of products: tiles of 64 x 64 give
+// the GPU enough workgroups to hide them in (333 x 4096 x 4096: 18 us; a fifth
+// stage of LDS changed nothing). Large ones are bound by the matrix cores and the
+// power they draw: 8192 x 4096 x 4096 takes 124 us, 2.2 POP/s, with the matrix
+// cores 70% busy at 1.64 GHz.
+//
+// The quantiser is bound by memory: a row is read once and held in registers
+// (8192 rows of 4096 in bf16: 18.4 us, 5.5 TB/s).
 #include "cf_codes.hpp"
 #include "cf_common.hpp"
 #include "cf_lds_dma.hpp"
@@ -140,13 +153,12 @@ void launch_rows(const RowsArgs& a, hipStream_t stream) {
         launch(quantize_rows_any_kernel<T>, capped(a.rows), dim3(kRowThreads), 0, stream, a);
         return;
     }
-    // A wave per row where there are rows enough to fill the GPU with that.
-    if (vecs <= 64 * 8 && a.rows >= 2048) {
+    // A wave per row where rows are short and enough to fill the GPU with that (4096
+    // rows of 1024 in bf16 6.6 us, a workgroup per row 7.8; 2048 of them 6.4 either
+    // way; 4096 rows of 4096 would take 13.7 us against 12.3).
+    if (vecs <= 64 * 2 && a.rows >= 2048) {
         const dim3 grid = capped(ceil_div<int64_t>(a.rows, 4));
-        auto* kernel = vecs <= 64    ? quantize_rows_kernel<T, 64, 1>
-                       : vecs <= 128 ? quantize_rows_kernel<T, 64, 2>
-                       : vecs <= 256 ? quantize_rows_kernel<T, 64, 4>
-                                     : quantize_rows_kernel<T, 64, 8>;
+        auto* kernel = vecs <= 64 ? quantize_rows_kernel<T, 64, 1> : quantize_rows_kernel<T, 64, 2>;
         launch(kernel, grid, dim3(kRowThreads), 0, stream, a);
     } else if (vecs <= 256 * 8) {
         auto* kernel = vecs <= 256    ? quantize_rows_kernel<T, 256, 1>
@@ -684,10 +696,18 @@ enum class Way { kAny, kRows, kTile64, kTile128, kTile256 };
 
 Way way_of(const Int8Args& a) {
     if (a.k % 16 != 0 || !host_aligned(a.x, 16) || !host_aligned(a.w, 16) || !host_aligned(a.y, 16)) return Way::kAny;
-    if (a.m <= 64) return Way::kRows;
-    const int64_t big = ceil_div<int64_t>(a.m, 256) * ceil_div<int64_t>(a.n, 256);
+    // Up to 16 rows w streams by. Up to 64 it still may, where there are too few tiles of
+    // 64 columns to fill the GPU: 32 rows of 4096 by 4096 columns take 12 us against
+    // 14.5 in tiles (64 of them), 64 rows 16 against 15; but by 11008 columns (172
+    // tiles) 22 and 33 us against 15 and 16, and 17 rows 18 against 15.
+    if (a.m <= 16 || (a.m <= 64 && ceil_div<int64_t>(a.n, 64) < 128)) return Way::kRows;
+    // Tiles of 128 x 128 run two a CU, 512 at once. Fewer than 192 leave too many CUs
+    // idle (96 and 160 of them, k 4096: 30 and 32 us against 20 and 30 in tiles of 64;
+    // 192 and 256: 32 and 33 against 32 and 36). More than 512 take a second round, and
+    // tiles of 256 are faster (384 and 512: 40 and 45 us against 46 and 47; 516 and
+    // 640: 73 and 65 against 47 and 49).
     const int64_t mid = ceil_div<int64_t>(a.m, 128) * ceil_div<int64_t>(a.n, 128);
-    return big >= 192 ? Way::kTile256 : mid >= 192 ? Way::kTile128 : Way::kTile64;
+    return mid > 512 ? Way::kTile256 : mid >= 192 ? Way::kTile128 : Way::kTile64;
 }
 
 void tiles(Int8Args& a, int bm, int bn) {
