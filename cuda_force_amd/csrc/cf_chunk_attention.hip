@@ -63,6 +63,7 @@ struct ChunkArgs {
     int max_blocks;
     int capacity;  // tokens a table row reaches
     uint32_t token_pieces;  // 16 bytes of a token of the cache
+    int rows;  // of a tile
     int splits;
     int step;  // tokens of a range are a multiple of this
     int least;  // and at least about this
@@ -304,14 +305,13 @@ struct Joined {
     float m, l;
     f32x4_t sum;
 };
-template <int kTeam>
 __device__ __forceinline__ Joined join_waves(const float* sums, int pitch, const float (*lds_m)[32],
                                              const float (*lds_l)[32], int row) {
     Joined j{lds_m[0][row], 0.0f, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-    for (int t = 1; t < kTeam; ++t) j.m = fmaxf(j.m, lds_m[t][row]);
+    for (int t = 1; t < kWaves; ++t) j.m = fmaxf(j.m, lds_m[t][row]);
 #pragma unroll
-    for (int t = 0; t < kTeam; ++t) {
+    for (int t = 0; t < kWaves; ++t) {
         const float mt = lds_m[t][row];
         const float f = mt == -INFINITY ? 0.0f : exp2f(mt - j.m);
         // A wave without a finite score still passes its NaN on.
@@ -399,7 +399,7 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
             put<T, kCodes, kSplit>(a, w, out, dim, lds_m[r / L::kRows][r % L::kRows], lds_l[r / L::kRows][r % L::kRows],
                                    *reinterpret_cast<const f32x4_t*>(sums));
         } else {
-            const Joined j = join_waves<kWaves>(sums, L::kRows * L::kOutPitch, lds_m, lds_l, r);
+            const Joined j = join_waves(sums, L::kRows * L::kOutPitch, lds_m, lds_l, r);
             put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
         }
     }
@@ -696,23 +696,20 @@ struct FewTile {
         return kPiece * of16 + block % kPiece + 16 * kPiece * (block / kPiece);
     }
     static constexpr int kOutPitch = kD + 4;
-    /// LDS of a wave: a tile's places and scales, then the query of 16 rows where it is
-    /// kept there, in two parts at most; the outputs at the end.
-    static constexpr int kQueryAt = kTokens * 16;
-    static constexpr int kQueryBytes = kQueries * kWaveSize * 16;
-    static constexpr int kOwnBytes = kQueryAt + 2 * kQueryBytes > kRows * kOutPitch * 4 ? kQueryAt + 2 * kQueryBytes
-                                                                                        : kRows * kOutPitch * 4;
+    /// LDS of a wave: a tile's places and scales, at the end the outputs.
+    static constexpr int kOwnBytes = kRows * kOutPitch * 4;
+    static_assert(kOwnBytes >= kTokens * 16, "8 bytes a place, 4 a scale");
     static constexpr float kLag = Tile<T, kD>::kLag;
     static constexpr float kLift = Tile<T, kD>::kLift;
 };
 
-/// Up to 16 kTiles rows, the team's waves on different tokens. Keys go from memory
+/// Up to 16 kTiles rows, the waves on different tokens. Keys go from memory
 /// to the registers of the matrix products: a lane loads the dims that it
 /// multiplies. Values are transposed there, by byte permutations of the 8 tokens
 /// that a lane needs of each of its dims. So a wave keeps a tile of keys or values
 /// in flight while it works on the other, and LDS holds no more than the tile's
 /// places and scales.
-template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kTiles, int kTeam>
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kTiles>
 __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32]) {
     constexpr bool kCodes = kHeld != CF_CACHE_PLAIN;
     using L = FewTile<T, kD, kCodes>;
@@ -744,21 +741,9 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
     const int wave_least = __builtin_amdgcn_readfirstlane(least);
 
     uint8_t* const own = lds + wave * L::kOwnBytes;
-    // Teams of 8, four waves a SIMD, have registers for all but the query.
-    constexpr bool kParked = kTeam == 8;
-    static_assert(!kParked || kTiles == 1, "one tile's query");
-    u32x4_t* const parked = reinterpret_cast<u32x4_t*>(own + L::kQueryAt) + lane;
-    if constexpr (kParked) {
-#pragma unroll
-        for (int u = 0; u < L::kQueries; ++u) {
-            parked[u * kWaveSize] = q[0][u];
-            if constexpr (kSplit) parked[(L::kQueries + u) * kWaveSize] = q_low[0][u];
-        }
-    }
-
     // Tiles begin at multiples of kTokens (ranges do).
     const int begin = w.lo + wave * kTokens;
-    constexpr int kStride = kTeam * kTokens;
+    constexpr int kStride = kWaves * kTokens;
     const int tiles = begin < w.hi ? (w.hi - begin + kStride - 1) / kStride : 0;
     const int last_block = static_cast<int>(static_cast<uint32_t>(w.hi - 1) / a.block_size);
     auto block_of = [&](int t) {
@@ -896,10 +881,8 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
                     const int u = kCodes ? 2 * i + e : i;
 #pragma unroll
                     for (int n = 0; n < kTiles; ++n) {
-                        s[n][h] = multiply(part[e], kParked ? parked[u * kWaveSize] : q[n][u], s[n][h]);
-                        if constexpr (kSplit) {
-                            s[n][h] = multiply(part[e], kParked ? parked[(L::kQueries + u) * kWaveSize] : q_low[n][u], s[n][h]);
-                        }
+                        s[n][h] = multiply(part[e], q[n][u], s[n][h]);
+                        if constexpr (kSplit) s[n][h] = multiply(part[e], q_low[n][u], s[n][h]);
                     }
                 }
             }
@@ -1099,12 +1082,12 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
             }
         }
         __syncthreads();
-        for (int i = tid; i < L::kRows * (kD / 4); i += kTeam * kWaveSize) {
+        for (int i = tid; i < L::kRows * (kD / 4); i += kThreads) {
             const int r = i / (kD / 4);
             const int dim = i % (kD / 4) * 4;
             const int out = w.first_row + n * L::kRows + r;
             if (out >= w.rows || dim >= a.head_dim) continue;
-            const Joined j = join_waves<kTeam>(reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim,
+            const Joined j = join_waves(reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim,
                                                L::kOwnBytes / 4, lds_m, lds_l, n * L::kRows + r);
             put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
         }
@@ -1576,9 +1559,9 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
 
 /// Zeros for the rows first_row .. first_row + count - 1 of a KV head's heads,
 /// counted from token `first`.
-template <typename O, int kTeam>
+template <typename O>
 __device__ void zero_rows(const ChunkArgs& a, int first, int kv_head, int first_row, int end_row) {
-    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(end_row - first_row) * a.head_dim; i += kTeam * kWaveSize) {
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(end_row - first_row) * a.head_dim; i += kThreads) {
         const int r = first_row + static_cast<int>(i / a.head_dim);
         const int64_t out_row = static_cast<int64_t>(first + r / a.per) * a.heads + kv_head * a.per + r % a.per;
         static_cast<O*>(a.out)[out_row * a.head_dim + i % a.head_dim] = O{};
@@ -1587,25 +1570,25 @@ __device__ void zero_rows(const ChunkArgs& a, int first, int kv_head, int first_
 
 /// What workgroup `id` does, or nothing (after writing zeros for rows that see no
 /// token, where it is the first of theirs). O: the type of the result.
-template <typename O, int kTeam>
-__device__ bool item_of(const ChunkArgs& a, int rows, Item& w, int& end_row) {
+template <typename O>
+__device__ bool item_of(const ChunkArgs& a, Item& w, int& end_row) {
     // KV heads vary fastest: workgroup i runs on XCD i % 8, so with 8 of them an
     // XCD reads one head's keys and values.
     int id = static_cast<int>(blockIdx.x);
     w.kv_head = id % a.kv_heads;
     id /= a.kv_heads;
     w.split = id % a.splits;
-    const Segment s = segment_of(a, rows, id / a.splits);
+    const Segment s = segment_of(a, a.rows, id / a.splits);
     if (s.count == 0) return false;
     w.first = s.first;
     w.rows = s.count * a.per;
-    w.first_row = s.tile * rows;
-    end_row = min(w.rows, w.first_row + rows);
+    w.first_row = s.tile * a.rows;
+    end_row = min(w.rows, w.first_row + a.rows);
     Reach reach{};
-    if (s.sequence >= 0) reach = reach_of(a, s, rows);
+    if (s.sequence >= 0) reach = reach_of(a, s, a.rows);
     const Range range = range_of(0, reach.hi, reach.each, w.split);
     if (range.lo >= range.hi) {
-        if (reach.hi == 0 && w.split == 0) zero_rows<O, kTeam>(a, s.first, w.kv_head, w.first_row, end_row);
+        if (reach.hi == 0 && w.split == 0) zero_rows<O>(a, s.first, w.kv_head, w.first_row, end_row);
         return false;
     }
     w.lo = range.lo;
@@ -1627,7 +1610,7 @@ __attribute__((amdgpu_waves_per_eu(2, 4))) void chunk_attention_wide_kernel(Chun
     constexpr int kRows = Tile<float, kD>::kRows;
     Item w{};
     int end_row = 0;
-    if (!item_of<float, kWaves>(a, kWaves * kRows, w, end_row)) return;
+    if (!item_of<float>(a, w, end_row)) return;
     if (end_row - w.first_row > kRows) {
         attend<kD, true>(a, w, lds, lds_m, lds_l, lds_bad);
     } else {
@@ -1648,27 +1631,14 @@ __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_k
     constexpr int kRows = Tile<T, kD>::kRows;
     Item w{};
     int end_row = 0;
-    if (!item_of<std::conditional_t<kSplit, float, T>, kWaves>(a, kWaves * kRows, w, end_row)) return;
+    if (!item_of<std::conditional_t<kSplit, float, T>>(a, w, end_row)) return;
     if (end_row - w.first_row > kRows) {
         attend_rows<T, kD, kHeld, kSplit>(a, w, lds, lds_m, lds_l, lds_bad);
     } else if (end_row - w.first_row > 16) {
-        attend_few<T, kD, kHeld, kSplit, 2, kWaves>(a, w, lds, lds_m, lds_l);
+        attend_few<T, kD, kHeld, kSplit, 2>(a, w, lds, lds_m, lds_l);
     } else {
-        attend_few<T, kD, kHeld, kSplit, 1, kWaves>(a, w, lds, lds_m, lds_l);
+        attend_few<T, kD, kHeld, kSplit, 1>(a, w, lds, lds_m, lds_l);
     }
-}
-
-/// The same caches where there are only single tokens, or few more.
-template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kTiles, int kTeam>
-__global__ __launch_bounds__(kTeam * kWaveSize)
-__attribute__((amdgpu_waves_per_eu(kTeam == 8 ? 4 : kD > 128 ? 1 : 2, 4))) void few_attention_kernel(ChunkArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kTeam * FewTile<T, kD, kHeld != CF_CACHE_PLAIN>::kOwnBytes];
-    __shared__ float lds_m[kTeam][32];
-    __shared__ float lds_l[kTeam][32];
-    Item w{};
-    int end_row = 0;
-    if (!item_of<std::conditional_t<kSplit, float, T>, kTeam>(a, 16 * kTiles, w, end_row)) return;
-    attend_few<T, kD, kHeld, kSplit, kTiles, kTeam>(a, w, lds, lds_m, lds_l);
 }
 
 /// The general kernel: any head size and alignment, a wave per (token, head,
@@ -1812,7 +1782,6 @@ __global__ __launch_bounds__(kThreads) void chunk_attention_join_kernel(ChunkArg
 struct Plan {
     int dim;   // head size of the matrix kernel, or 0: the general kernel
     int rows;  // of a tile
-    bool few;  // tiles of 16 or 32 rows only
     int splits;
     int step;
     int least;
@@ -1848,13 +1817,7 @@ Plan plan_of(cf_dtype dtype, cf_cache_format format, int64_t tokens, int64_t seq
         return p;
     }
     p.least = 256;
-    // Where no more tokens than sequences are given they are single ones, or a few
-    // sequences have several: small tiles and their own kernel, of more waves than the
-    // one for chunks has room for. (64 sequences of up to 4096 tokens, 8-bit cache: @@ us
-    // against @@.)
-    p.few = !wide && tokens <= sequences && per <= 32;
-    if (p.few) p.rows = per <= 16 ? 16 : 32;
-    p.step = static_cast<int>(p.few ? p.least : kWaves * wave_rows);
+    p.step = static_cast<int>(kWaves * wave_rows);
     p.splits = splits(tiles_of(p.rows, tokens, sequences < tokens ? sequences : tokens, per) * kv_heads, 512, p.least);
     return p;
 }
@@ -1876,27 +1839,22 @@ bool sizes_ok(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads
 }
 
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
-void run_size(const ChunkArgs& a, const Plan& p, dim3 grid, hipStream_t stream) {
+void run_size(const ChunkArgs& a, dim3 grid, hipStream_t stream) {
     if constexpr (Tile<T, kD>::kWide) {
         launch(chunk_attention_wide_kernel<kD>, grid, dim3(kThreads), 0, stream, a);
-    } else if (!p.few) {
-        launch(chunk_attention_kernel<T, kD, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
-    } else if (p.rows == 16) {
-        constexpr int kTeam = kHeld != CF_CACHE_PLAIN && kD <= 128 ? 8 : 4;
-        launch(few_attention_kernel<T, kD, kHeld, kSplit, 1, kTeam>, grid, dim3(kTeam * kWaveSize), 0, stream, a);
     } else {
-        launch(few_attention_kernel<T, kD, kHeld, kSplit, 2, 4>, grid, dim3(4 * kWaveSize), 0, stream, a);
+        launch(chunk_attention_kernel<T, kD, kHeld, kSplit>, grid, dim3(kThreads), 0, stream, a);
     }
 }
 
 template <typename T, cf_cache_format kHeld, bool kSplit>
 void run_matrix(const ChunkArgs& a, const Plan& p, dim3 grid, hipStream_t stream) {
     if (p.dim == 64) {
-        run_size<T, 64, kHeld, kSplit>(a, p, grid, stream);
+        run_size<T, 64, kHeld, kSplit>(a, grid, stream);
     } else if (p.dim == 128) {
-        run_size<T, 128, kHeld, kSplit>(a, p, grid, stream);
+        run_size<T, 128, kHeld, kSplit>(a, grid, stream);
     } else if constexpr (kHeld != CF_CACHE_PLAIN || sizeof(T) == 2) {
-        run_size<T, 256, kHeld, kSplit>(a, p, grid, stream);
+        run_size<T, 256, kHeld, kSplit>(a, grid, stream);
     }
 }
 
@@ -2001,19 +1959,16 @@ cf_status cf_paged_attention_chunk(const void* query, const void* k_cache, const
     if (p.dim != 0 && !(cf::host_aligned(query, 16) && cf::host_aligned(k_cache, 16) &&
                         cf::host_aligned(v_cache, 16) && cf::host_aligned(out, 16))) {
         p.dim = 0;  // within the same workspace: as many ranges at most
-        p.few = false;
         p.rows = static_cast<int>(num_heads / num_kv_heads);
         p.step = 32;
         p.least = 64;
     }
-    // The kernel for chunks counts a cache's 16-byte pieces in 32 bits. In larger ones
-    // (64 GiB and more) chunks go through the small tiles, which count them in 64.
+    // The kernel for many rows counts a cache's 16-byte pieces in 32 bits. In larger
+    // ones (64 GiB and more) tiles have no more rows than the one for few, which
+    // counts them in 64, takes.
     const bool wide = dtype == CF_F32 && format == CF_CACHE_PLAIN;
     const int64_t token_pieces = num_kv_heads * head_dim * static_cast<int64_t>(held) / 16;
-    if (p.dim != 0 && !wide && !p.few && num_pages * block_size > (int64_t{1} << 32) / token_pieces) {
-        p.few = true;
-        p.rows = 32;
-    }
+    if (p.dim != 0 && !wide && num_pages * block_size > (int64_t{1} << 32) / token_pieces) p.rows = 32;
     cf::ChunkArgs a{};
     a.query = query;
     a.k_cache = static_cast<const uint8_t*>(k_cache);
@@ -2037,6 +1992,7 @@ cf_status cf_paged_attention_chunk(const void* query, const void* k_cache, const
     a.max_blocks = static_cast<int>(max_blocks_per_sequence);
     a.capacity = static_cast<int>(cf::capacity_of(max_blocks_per_sequence, block_size));
     a.token_pieces = static_cast<uint32_t>(token_pieces);
+    a.rows = p.rows;
     a.splits = p.splits;
     a.step = p.step;
     a.least = p.least;
