@@ -11,9 +11,11 @@
 // the matrix cores, 16 of them a workgroup, whose waves split k (8 rows by 11008
 // columns of 4096: 13.2 us, 3.4 TB/s; sending the next loads ahead of the products
 // changed nothing). Middling batches are bound by the steps of the loop over k,
-// each a barrier, LDS reads and a short chain of products: tiles of 64 x 64 give
-// the GPU enough workgroups to hide them in (333 x 4096 x 4096: 18 us; a fifth
-// stage of LDS changed nothing). Large ones are bound by the matrix cores and the
+// each a barrier, copies, LDS reads and a short chain of products: small tiles,
+// and two groups of waves on one, give the CUs enough to do beside them (333 x
+// 4096 x 4096: 15 us by kernel time, 11 TB/s from L2 to LDS at 15% of the matrix
+// cores' rate; neither a fifth stage of LDS nor steps in another order for every
+// tile changed anything). Large ones are bound by the matrix cores and the
 // power they draw: 8192 x 4096 x 4096 takes 124 us, 2.2 POP/s, with the matrix
 // cores 70% busy at 1.64 GHz.
 //
@@ -230,19 +232,25 @@ __device__ __forceinline__ void store4(const Int8Args& a, int i, int j, const in
 
 /// kBM x kBN results per workgroup, kWM x kWN per wave, kStages stages of 128
 /// bytes of k in LDS. The product is formed transposed (w the first operand), so
-/// a lane holds runs of four columns of one row.
-template <typename T, int kBM, int kBN, int kWM, int kWN, int kStages>
-__global__ __launch_bounds__(kBM / kWM * (kBN / kWN) * kWaveSize) void matmul_int8_kernel(Int8Args a) {
+/// a lane holds runs of four columns of one row. With two groups each of them has
+/// the whole tile, stages of its own and every other 128 bytes of k, and the
+/// second hands its sums over at the end: half as many barriers, whose steps are
+/// what a workgroup that is alone on its CU waits for.
+template <typename T, int kBM, int kBN, int kWM, int kWN, int kStages, int kGroups>
+__global__ __launch_bounds__(kGroups * (kBM / kWM) * (kBN / kWN) * kWaveSize) void matmul_int8_kernel(Int8Args a) {
     constexpr int kWavesM = kBM / kWM;
     constexpr int kWavesN = kBN / kWN;
     constexpr int kWaves = kWavesM * kWavesN;
-    constexpr int kCopies = (kBM + kBN) / 8 / kWaves;  // of 1 KiB, per wave and stage
+    // Copies of 1 KiB per wave and stage; the last waves may have none.
+    constexpr int kCopies = ((kBM + kBN) / 8 + kWaves - 1) / kWaves;
     constexpr int kStageBytes = (kBM + kBN) * kStep;
-    static_assert((kBM + kBN) / 8 % kWaves == 0 && kBM / 8 % kCopies == 0, "a wave copies rows of one operand");
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kStages * kStageBytes];
+    static_assert((kBM + kBN) / 8 % kCopies == 0 && kBM / 8 % kCopies == 0, "a wave copies rows of one operand");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kGroups * kStages * kStageBytes];
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int group = kGroups == 1 ? 0 : __builtin_amdgcn_readfirstlane((tid >> 6) / kWaves);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) - group * kWaves;
+    uint8_t* const own = lds + group * kStages * kStageBytes;
     int tm;
     int tn;
     tile_of(static_cast<int>(blockIdx.x), a.tiles_m, a.tiles_n, tm, tn);
@@ -265,10 +273,14 @@ __global__ __launch_bounds__(kBM / kWM * (kBN / kWN) * kWaveSize) void matmul_in
         offset[b] = static_cast<uint32_t>((lane >> 3) * a.k + piece * 16);
         tail[b] = of_x && (steps - 1) * kStep + piece * 16 >= a.k ? kOutOfRange : offset[b];
     }
-    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8_t*)lds)) +
+    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8_t*)own)) +
                               static_cast<uint32_t>(wave * kCopies) * 1024;
-    auto issue = [&](int step) {
-        const uint32_t dst = lds_base + static_cast<uint32_t>(step % kStages) * kStageBytes;
+    const int turns = (steps - group + kGroups - 1) / kGroups;  // this group's steps
+    const bool copies = (kBM + kBN) / 8 == kCopies * kWaves || wave * kCopies < (kBM + kBN) / 8;
+    auto issue = [&](int turn) {
+        if (!copies) return;
+        const int step = turn * kGroups + group;
+        const uint32_t dst = lds_base + static_cast<uint32_t>(turn % kStages) * kStageBytes;
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
             const uint32_t at = static_cast<uint32_t>((first_copy + c) * 8) * static_cast<uint32_t>(a.k) +
@@ -298,19 +310,21 @@ __global__ __launch_bounds__(kBM / kWM * (kBN / kWN) * kWaveSize) void matmul_in
 
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) {
-        if (s < steps) issue(s);
+        if (s < turns) issue(s);
     }
-    for (int step = 0; step < steps; ++step) {
-        // This wave's copies of the step have landed, then everyone's.
-        if (step + kStages - 2 < steps) {
+    // (The first group has as many turns as the other or one more.)
+    for (int turn = 0; turn < (steps + kGroups - 1) / kGroups; ++turn) {
+        // This wave's copies of the turn have landed, then everyone's.
+        if (turn + kStages - 2 < turns) {
             __builtin_amdgcn_s_waitcnt(vmcnt_imm((kStages - 2) * kCopies));
         } else {
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         }
         bare_barrier();
-        if (step + kStages - 1 < steps) issue(step + kStages - 1);
-        const uint8_t* xs = lds + step % kStages * kStageBytes + wm * kWM * kStep;
-        const uint8_t* ws = lds + step % kStages * kStageBytes + (kBM + wn * kWN) * kStep;
+        if (turn >= turns) break;  // the last barrier is passed
+        if (turn + kStages - 1 < turns) issue(turn + kStages - 1);
+        const uint8_t* xs = own + turn % kStages * kStageBytes + wm * kWM * kStep;
+        const uint8_t* ws = own + turn % kStages * kStageBytes + (kBM + wn * kWN) * kStep;
 #pragma unroll
         for (int u = 0; u < kStep / 32; ++u) {
             const int at = row * kStep + (((2 * u + h) ^ sw) << 4);
@@ -329,6 +343,40 @@ __global__ __launch_bounds__(kBM / kWM * (kBN / kWN) * kWaveSize) void matmul_in
             }
         }
         __builtin_amdgcn_s_waitcnt(0xF | (3 << 14) | (7 << 4));  // LDS reads are done before the next barrier
+    }
+
+    if constexpr (kGroups == 2) {
+        // 16 sums a lane and block; the first group's stages take the second one's.
+        __syncthreads();
+        i32x4v_t* sums = reinterpret_cast<i32x4v_t*>(lds) + wave * (kM * kN * 4 * kWaveSize) + lane;
+        static_assert(kWaves * kM * kN * 64 * kWaveSize <= kGroups * kStages * kStageBytes, "room for the sums");
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+#pragma unroll
+            for (int i = 0; i < kM; ++i) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    i32x4v_t& at = sums[((j * kM + i) * 4 + q) * kWaveSize];
+                    if (group == 1) {
+                        at = i32x4v_t{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (group == 1) return;
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+#pragma unroll
+            for (int i = 0; i < kM; ++i) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const i32x4v_t at = sums[((j * kM + i) * 4 + q) * kWaveSize];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[j][i][4 * q + e] += at[e];
+                }
+            }
+        }
     }
 
     const bool vectors = a.n % 4 == 0;
@@ -692,7 +740,7 @@ __global__ __launch_bounds__(256) void matmul_int8_any_kernel(Int8Args a) {
 
 // ---- host -----------------------------------------------------------------------
 
-enum class Way { kAny, kRows, kTile64, kTile128, kTile256 };
+enum class Way { kAny, kRows, kTile64, kSplit64, kSplit96, kTile128, kTile256 };
 
 Way way_of(const Int8Args& a) {
     if (a.k % 16 != 0 || !host_aligned(a.x, 16) || !host_aligned(a.w, 16) || !host_aligned(a.y, 16)) return Way::kAny;
@@ -707,7 +755,14 @@ Way way_of(const Int8Args& a) {
     // tiles of 256 are faster (384 and 512: 40 and 45 us against 46 and 47; 516 and
     // 640: 73 and 65 against 47 and 49).
     const int64_t mid = ceil_div<int64_t>(a.m, 128) * ceil_div<int64_t>(a.n, 128);
-    return mid > 512 ? Way::kTile256 : mid >= 192 ? Way::kTile128 : Way::kTile64;
+    if (mid >= 192) return mid > 512 ? Way::kTile256 : Way::kTile128;
+    auto small = [&](int bm) { return ceil_div<int64_t>(a.m, bm) * ceil_div<int64_t>(a.n, 64); };
+    // Where a CU has one tile of 64 x 64, or one of 96 x 64 instead of two, two groups of
+    // waves share its k: 128 rows by 4096 columns of 4096 13.0 us against 15.3; 333 rows
+    // 16.1 us against 19.4 in tiles of 64 and 18.0 with one group, of 11008 32 us against
+    // 49 and 37.
+    if (small(64) <= 256) return Way::kSplit64;
+    return small(96) <= 256 ? Way::kSplit96 : Way::kTile64;
 }
 
 void tiles(Int8Args& a, int bm, int bn) {
@@ -729,8 +784,18 @@ cf_status run(Int8Args a, hipStream_t stream) {
                      : a.m <= 32 ? matmul_int8_rows_kernel<T, 2>
                                  : matmul_int8_rows_kernel<T, 4>;
             break;
-        case Way::kTile64: tiles(a, 64, 64); kernel = matmul_int8_kernel<T, 64, 64, 32, 32, 4>; break;
-        case Way::kTile128: tiles(a, 128, 128); kernel = matmul_int8_kernel<T, 128, 128, 64, 64, 2>; break;
+        case Way::kTile64: tiles(a, 64, 64); kernel = matmul_int8_kernel<T, 64, 64, 32, 32, 4, 1>; break;
+        case Way::kSplit64:
+            tiles(a, 64, 64);
+            threads = 512;
+            kernel = matmul_int8_kernel<T, 64, 64, 32, 32, 4, 2>;
+            break;
+        case Way::kSplit96:
+            tiles(a, 96, 64);
+            threads = 768;
+            kernel = matmul_int8_kernel<T, 96, 64, 32, 32, 3, 2>;
+            break;
+        case Way::kTile128: tiles(a, 128, 128); kernel = matmul_int8_kernel<T, 128, 128, 64, 64, 2, 1>; break;
         case Way::kTile256: tiles(a, 256, 256); kernel = matmul_int8_big_kernel<T>; break;
     }
     const int64_t grid = static_cast<int64_t>(a.tiles_m) * a.tiles_n;

@@ -85,6 +85,15 @@ def test_large_tiles(dtype, m, n, k):
     product(m, n, k, dtype, bias=n % 2 == 1)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(17, 8200, 400), (64, 8200, 128), (40, 8250, 16), (200, 4000, 2064), (333, 4096, 144),
+                                   (333, 4100, 4112), (500, 2600, 1040), (640, 4096, 272), (128, 11008, 1152)])
+def test_middling_products(dtype, m, n, k):
+    """Tiles of 64 and 96 rows, one or two groups of waves on a tile's k (of as
+    many stages, of one more, of a single one)."""
+    product(m, n, k, dtype)
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 5, 1), (20, 30, 7), (65, 70, 100), (130, 40, 1001), (4, 4, 131071)])
 def test_any_depth(m, n, k):
     for dtype in DTYPES:
