@@ -9,19 +9,26 @@
 // keys are a matrix product; a row tile of a long chunk is bound by the matrix
 // and vector units, a single token's few rows by HBM.
 //   * A work item is (row tile, KV head, range of the context), a workgroup of
-//     four waves. Tiles with more rows than a wave takes are shared by the
-//     waves, a quarter of the rows each; with fewer, the waves take different
-//     tokens of the same rows. Ranges are cut only where there are few items;
-//     a second kernel joins their pieces.
-//   * 8-bit codes are exact in fp16, so they are widened to it on their way to
-//     LDS and the products run on fp16 tiles whatever the query's type: a bf16
-//     query is scaled by a power of two per row (it has fewer bits than fp16
-//     holds, and what falls below fp16's smallest number is 2^-39 of the row's
-//     largest), an fp32 query is taken as the sum of two fp16 numbers. Keys'
-//     scales multiply the scores, values' scales the probabilities, relative to
-//     a power of two above all scales met so far, all in fp32.
-//   * Tokens that are not there (behind the range, in no page) get no weight and
-//     their values are cleared in LDS.
+//     four waves. Of tiles with more than 32 rows each wave has 32 and they share
+//     the keys and values in LDS (attend_rows); with fewer, the waves take
+//     different tokens of the same rows and share nothing (attend_few); fp32
+//     caches have tiles of half the rows and tokens (attend). Ranges are cut only
+//     where there are few items; a second kernel joins their pieces.
+//   * 8-bit codes are exact in fp16, so they are widened to it on their way to the
+//     products, which run in fp16 whatever the query's type: a bf16 query is scaled
+//     by a power of two per row (it has fewer bits than fp16 holds, and what falls
+//     below fp16's smallest number is 2^-39 of the row's largest), an fp32 query is
+//     taken as the sum of two fp16 numbers. Keys' scales multiply the scores,
+//     values' scales the probabilities, in fp32.
+//   * Tokens that are not there (behind the range, in no page) get no weight, and
+//     what the cache holds in their place never reaches a row.
+// Measured, 32 heads over 8 of 128: a prompt of 2048 tokens in bf16 67 us (510
+// TFLOP/s: the chain product, probabilities, product, at two waves a SIMD, and
+// the causal tiles' different lengths); 2048 tokens behind 30720 1.13 to 1.24 ms
+// (860 to 940 TFLOP/s: matrix cores 44% and vector units 48% busy, and the clock
+// falls from 2.2 to 1.7 GHz under them); 64 sequences of 2051 to 4096 tokens in
+// int8, a token each, 102 us (4.1 TB/s; 4.8 TB/s at equal lengths: reads of single
+// 128-byte lines, where bf16's of 256 bytes reach 5.9).
 #include "cf_attention_tile.hpp"
 #include "cf_codes.hpp"
 #include "cf_common.hpp"
@@ -405,7 +412,9 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
     }
 }
 
-/// fp32 caches. kShared: the waves take different rows of the tile, else different
+/// fp32 caches, in fp32 products: the matrix cores' slowest, half busy where a CU
+/// has two workgroups (four chunks of up to 100 tokens behind 900, 86 us, and
+/// 12 us for the join). kShared: the waves take different rows of the tile, else different
 /// tokens of the same rows.
 template <int kD, bool kShared>
 __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
@@ -708,7 +717,9 @@ struct FewTile {
 /// multiplies. Values are transposed there, by byte permutations of the 8 tokens
 /// that a lane needs of each of its dims. So a wave keeps a tile of keys or values
 /// in flight while it works on the other, and LDS holds no more than the tile's
-/// places and scales.
+/// places and scales. (Widened into LDS instead, and with products of 32 rows, 64
+/// sequences of up to 4096 tokens in int8 took 126 us, not 102. Twice the waves a
+/// SIMD, in a kernel of their own, changed nothing.)
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kTiles>
 __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32]) {
     constexpr bool kCodes = kHeld != CF_CACHE_PLAIN;
@@ -1114,7 +1125,10 @@ struct RowsKind {
 /// The waves take different rows, of 16-bit tiles: 64 tokens a step. In plain
 /// caches the next step's scores are formed while this one's are made
 /// probabilities, so that a wave has work for the matrix cores beside its vector
-/// instructions; codes, which need more of those, leave no registers for it.
+/// instructions (a 2048-token prompt 68 us, without it and the reads ahead 75);
+/// codes, which need more of those, leave no registers for it: 512 tokens each of
+/// three sequences of 4000 in e4m3, next to 41 single ones, take 205 us with the
+/// vector units 45% and the matrix cores 19% busy.
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
 __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
                             uint64_t* lds_bad) {
@@ -1816,6 +1830,9 @@ Plan plan_of(cf_dtype dtype, cf_cache_format format, int64_t tokens, int64_t seq
         p.splits = splits(tokens * heads, 4096, p.least);
         return p;
     }
+    // Two workgroups a CU, in ranges of 256 tokens or more. (Four chunks of 100 in fp32
+    // behind 900 tokens: 110 us uncut, 98 in two ranges for 512 workgroups, 107 in four;
+    // seven chunks of 333 in int8 67 us uncut, 90 in two.)
     p.least = 256;
     p.step = static_cast<int>(kWaves * wave_rows);
     p.splits = splits(tiles_of(p.rows, tokens, sequences < tokens ? sequences : tokens, per) * kv_heads, 512, p.least);

@@ -16,8 +16,8 @@
 // 4096 x 4096: 15 us by kernel time, 11 TB/s from L2 to LDS at 15% of the matrix
 // cores' rate; neither a fifth stage of LDS nor steps in another order for every
 // tile changed anything). Large ones are bound by the matrix cores and the
-// power they draw: 8192 x 4096 x 4096 takes 124 us, 2.2 POP/s, with the matrix
-// cores 70% busy at 1.64 GHz.
+// power they draw: 8192 x 4096 x 4096 takes 119 to 124 us, 2.2 to 2.3 POP/s, with
+// the matrix cores 56% busy at 1.6 to 1.8 GHz.
 //
 // The quantiser is bound by memory: a row is read once and held in registers
 // (8192 rows of 4096 in bf16: 18.4 us, 5.5 TB/s).
