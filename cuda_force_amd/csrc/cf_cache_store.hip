@@ -439,6 +439,8 @@ cf_status cf_cache_write(const void* keys, const void* values, cf_dtype dtype, i
     const cf_status st = cf::check_store(who, dtype, format, tokens, num_kv_heads, head_dim, num_slots,
                                          {keys, values, k_cache, v_cache, slots}, k_scales, v_scales);
     if (st != CF_OK) return st;
+    CF_REQUIRE(k_cache != v_cache && (format == CF_CACHE_PLAIN || k_scales != v_scales),
+               "%s: keys and values have one place", who);
     cf::StoreArgs a{};
     a.x[0] = keys;
     a.x[1] = values;

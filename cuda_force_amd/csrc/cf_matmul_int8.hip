@@ -743,7 +743,7 @@ __global__ __launch_bounds__(256) void matmul_int8_any_kernel(Int8Args a) {
 enum class Way { kAny, kRows, kTile64, kSplit64, kSplit96, kTile128, kTile256 };
 
 Way way_of(const Int8Args& a) {
-    if (a.k % 16 != 0 || !host_aligned(a.x, 16) || !host_aligned(a.w, 16) || !host_aligned(a.y, 16)) return Way::kAny;
+    if (a.k == 0 || a.k % 16 != 0 || !host_aligned(a.x, 16) || !host_aligned(a.w, 16) || !host_aligned(a.y, 16)) return Way::kAny;
     // Up to 16 rows w streams by. Up to 64 it still may, where there are too few tiles of
     // 64 columns to fill the GPU: 32 rows of 4096 by 4096 columns take 12 us against
     // 14.5 in tiles (64 of them), 64 rows 16 against 15; but by 11008 columns (172

@@ -272,7 +272,8 @@ bool try_cache_write(py::handle keys_, py::handle values_, py::handle k_, py::ha
         slots->dim() != 1 || slots->scalar_type() != torch::kInt64 || keys->sizes() != values->sizes() ||
         keys->scalar_type() != values->scalar_type() || keys->size(0) != slots->size(0) ||
         keys->size(1) != k->size(2) || keys->size(2) != k->size(3) ||
-        (!k_scales && keys->scalar_type() != k->scalar_type()) || !same_device(*keys, {values, k, slots})) {
+        (!k_scales && keys->scalar_type() != k->scalar_type()) || !same_device(*keys, {values, k, slots}) ||
+        k_.ptr() == v_.ptr() || (k_scales && k_scales_.ptr() == v_scales_.ptr())) {
         return false;
     }
     py::gil_scoped_release no_gil;

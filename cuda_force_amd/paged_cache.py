@@ -298,8 +298,8 @@ def cache_write(
     scales are written in place. Not differentiable. Not in the reference's API.
 
     Raises:
-        ValueError: for shapes, devices or layouts that do not match, or tensors
-            that require gradients.
+        ValueError: for shapes, devices or layouts that do not match, one cache
+            for both, or tensors that require gradients.
         TypeError: for slots that are not int64, scales that are not fp32 or a
             cache of another type.
     """
@@ -307,6 +307,8 @@ def cache_write(
         if ops._DIRECT.try_cache_write(keys, values, k_cache, v_cache, slots, k_scales, v_scales):
             return
     codes = _check_held(k_cache, v_cache, k_scales, v_scales, keys)
+    if k_cache is v_cache or (codes and k_scales is v_scales):
+        raise ValueError("keys and values need caches and scales of their own")
     slots = _check_slots(slots, keys)
     shape = (slots.shape[0], *k_cache.shape[2:])
     for x, name in ((keys, "keys"), (values, "values")):

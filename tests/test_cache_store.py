@@ -86,6 +86,8 @@ def test_refusals():
     write(ValueError, k=plain, v=plain)
     write(ValueError, slots=slots.view(2, 2))
     write(ValueError, x=x.clone().requires_grad_(True))
+    write(ValueError, v=k)
+    write(ValueError, vs=ks)
     write(TypeError, slots=slots.int())
     write(TypeError, ks=ks.double())
     write(TypeError, values=x.double())
@@ -101,12 +103,12 @@ def test_refusals():
 
 def test_c_abi_refusals_before_any_launch():
     lib = _lib.load()
-    fake, null = ctypes.c_void_p(0x1000), ctypes.c_void_p(0)
+    fake, null, other = ctypes.c_void_p(0x1000), ctypes.c_void_p(0), ctypes.c_void_p(0x2000)
 
     def write(x=fake, dtype=_lib.CF_BF16, tokens=4, heads=2, dim=64, slots=fake, cache=fake, form=_lib.CF_CACHE_INT8,
               scales=fake, num_slots=100):
-        return lib.cf_cache_write(x, fake, dtype, tokens, heads, dim, 128, 64, 128, 64, slots, cache, fake, form,
-                                  scales, fake, num_slots, null)
+        return lib.cf_cache_write(x, fake, dtype, tokens, heads, dim, 128, 64, 128, 64, slots, cache, other, form,
+                                  scales, other, num_slots, null)
 
     def read(x=fake, dtype=_lib.CF_BF16, tokens=4, heads=2, dim=64, slots=fake, cache=fake, form=_lib.CF_CACHE_INT8,
              scales=fake, num_slots=100):
@@ -120,3 +122,5 @@ def test_c_abi_refusals_before_any_launch():
                      {"scales": ctypes.c_void_p(0x1002)}, {"slots": ctypes.c_void_p(0x1004)},
                      {"tokens": 2**40}):
             assert call(**case) == _lib.CF_ERR_INVALID_ARGUMENT, case
+    # One place for keys and values.
+    assert write(cache=other) == write(scales=other) == _lib.CF_ERR_INVALID_ARGUMENT

@@ -130,3 +130,18 @@ def test_graph_and_stream():
         _write_reference(x[:, 0].cpu(), x[:, 1].cpu(), *state[:2], slots.cpu(), *state[2:])
         for a, b in zip(got, _read_reference(*state[:2], slots.cpu(), *state[2:], torch.bfloat16)):
             assert torch.equal(bits(a), bits(b))
+
+
+def test_one_place_for_keys_and_values_is_refused():
+    x = torch.randn(4, 2, 64, device="cuda")
+    slots = torch.arange(4, device="cuda")
+    cache = torch.zeros(2, 4, 2, 64, device="cuda")
+    with pytest.raises(ValueError):
+        cf.cache_write(x, x, cache, cache, slots)
+    with pytest.raises(RuntimeError):
+        cf.cache_write(x, x, cache, cache.view(cache.shape), slots)
+    codes = [torch.zeros(2, 4, 2, 64, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = torch.zeros(2, 4, 2, device="cuda")
+    with pytest.raises(RuntimeError):
+        cf.cache_write(x, x, *codes, slots, scales, scales.view(scales.shape))
+    assert (cache == 0).all() and (scales == 0).all()

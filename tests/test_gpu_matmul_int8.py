@@ -100,6 +100,12 @@ def test_any_depth(m, n, k):
         product(m, n, k, dtype)
 
 
+def test_no_products():
+    for m, n in ((1, 5), (40, 300), (333, 4100), (2100, 4096)):
+        product(m, n, 0, torch.bfloat16, bias=False)
+        product(m, n, 0, torch.float32)
+
+
 def test_the_longest_sums():
     product(17, 40, 131056, torch.float32, bias=False)
     product(300, 260, 131056, torch.float32, bias=False)
