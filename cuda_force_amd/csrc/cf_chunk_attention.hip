@@ -9,9 +9,10 @@
 // keys are a matrix product; a row tile of a long chunk is bound by the matrix
 // and vector units, a single token's few rows by HBM.
 //   * A work item is (row tile, KV head, range of the context), a workgroup of
-//     four waves. Of tiles with more than 32 rows each wave has 32 and they share
-//     the keys and values in LDS (attend_rows); with fewer, the waves take
-//     different tokens of the same rows and share nothing (attend_few); fp32
+//     four waves. Of tiles with more than 32 rows each wave has 32 (of up to 64
+//     against half of the tokens) and they share the keys and values in LDS
+//     (attend_rows); with fewer, the waves take different tokens of the same rows
+//     and share nothing (attend_few); fp32
 //     caches have tiles of half the rows and tokens (attend). Ranges are cut only
 //     where there are few items; a second kernel joins their pieces.
 //   * 8-bit codes are exact in fp16, so they are widened to it on their way to the
@@ -306,19 +307,21 @@ __device__ __forceinline__ float load_query(const ChunkArgs& a, const Item& w, b
     return c;
 }
 
-/// Four neighbouring dims of a row from all of the waves that have some of its
-/// tokens: `sums` of the first, the others `pitch` floats apart.
+/// Four neighbouring dims of a row from the kCount waves that have some of its
+/// tokens, kApart waves apart: `sums`, lds_m and lds_l of the first, sums of
+/// neighbouring waves `pitch` floats apart.
 struct Joined {
     float m, l;
     f32x4_t sum;
 };
+template <int kCount, int kApart>
 __device__ __forceinline__ Joined join_waves(const float* sums, int pitch, const float (*lds_m)[32],
                                              const float (*lds_l)[32], int row) {
     Joined j{lds_m[0][row], 0.0f, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-    for (int t = 1; t < kWaves; ++t) j.m = fmaxf(j.m, lds_m[t][row]);
+    for (int t = kApart; t < kCount * kApart; t += kApart) j.m = fmaxf(j.m, lds_m[t][row]);
 #pragma unroll
-    for (int t = 0; t < kWaves; ++t) {
+    for (int t = 0; t < kCount * kApart; t += kApart) {
         const float mt = lds_m[t][row];
         const float f = mt == -INFINITY ? 0.0f : exp2f(mt - j.m);
         // A wave without a finite score still passes its NaN on.
@@ -363,8 +366,9 @@ __device__ __forceinline__ void put(const ChunkArgs& a, const Item& w, int row, 
     }
 }
 
-/// The waves' outputs, of different rows (kShared) or of different tokens.
-template <typename T, int kD, bool kCodes, bool kSplit, bool kShared>
+/// The waves' outputs, kRowWaves of them of different rows, the others behind them
+/// of different tokens of the same.
+template <typename T, int kD, bool kCodes, bool kSplit, int kRowWaves>
 __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32],
                                        float (*lds_l)[32], float m, float l,
                                        const typename Tile<T, kD>::Score (&acc)[Tile<T, kD>::kAcc / Tile<T, kD>::kScores]) {
@@ -390,7 +394,7 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
     }
     __syncthreads();
     // Rows x groups of four dims, over the workgroup.
-    constexpr int kOutRows = (kShared ? kWaves : 1) * L::kRows;
+    constexpr int kOutRows = kRowWaves * L::kRows;
     constexpr int kFours = kD / 4;
     constexpr int kRounds = (kOutRows * kFours + kThreads - 1) / kThreads;
 #pragma unroll 2
@@ -402,11 +406,13 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
         const int out = w.first_row + r;
         if (out >= w.rows || dim >= a.head_dim) continue;
         const float* sums = reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim;
-        if constexpr (kShared) {
-            put<T, kCodes, kSplit>(a, w, out, dim, lds_m[r / L::kRows][r % L::kRows], lds_l[r / L::kRows][r % L::kRows],
+        const int wave_of = r / L::kRows;
+        if constexpr (kRowWaves == kWaves) {
+            put<T, kCodes, kSplit>(a, w, out, dim, lds_m[wave_of][r % L::kRows], lds_l[wave_of][r % L::kRows],
                                    *reinterpret_cast<const f32x4_t*>(sums));
         } else {
-            const Joined j = join_waves(sums, L::kRows * L::kOutPitch, lds_m, lds_l, r);
+            const Joined j = join_waves<kWaves / kRowWaves, kRowWaves>(sums, L::kRows * L::kOutPitch, lds_m + wave_of,
+                                                                       lds_l + wave_of, r % L::kRows);
             put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
         }
     }
@@ -675,7 +681,7 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
         }
     }
 
-    finish<float, kD, false, false, kShared>(a, w, lds, lds_m, lds_l, m, l, acc);
+    finish<float, kD, false, false, kShared ? kWaves : 1>(a, w, lds, lds_m, lds_l, m, l, acc);
 }
 
 /// Where a lane's values lie when 16 rows meet 32 tokens in 16 x 16 products.
@@ -1098,7 +1104,7 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
             const int dim = i % (kD / 4) * 4;
             const int out = w.first_row + n * L::kRows + r;
             if (out >= w.rows || dim >= a.head_dim) continue;
-            const Joined j = join_waves(reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim,
+            const Joined j = join_waves<kWaves, 1>(reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim,
                                                L::kOwnBytes / 4, lds_m, lds_l, n * L::kRows + r);
             put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
         }
@@ -1122,14 +1128,16 @@ struct RowsKind {
     }
 };
 
-/// The waves take different rows, of 16-bit tiles: 64 tokens a step. In plain
+/// 16-bit tiles of more than 32 rows, 64 tokens a step. The waves take different
+/// rows, with kHalves = 2 (up to 64 rows) two of them the first half of the tokens
+/// and two the second. In plain
 /// caches the next step's scores are formed while this one's are made
 /// probabilities, so that a wave has work for the matrix cores beside its vector
 /// instructions (a 2048-token prompt 68 us, without it and the reads ahead 75);
 /// codes, which need more of those, leave no registers for it: 512 tokens each of
 /// three sequences of 4000 in e4m3, next to 41 single ones, take 205 us with the
 /// vector units 45% and the matrix cores 19% busy.
-template <typename T, int kD, cf_cache_format kHeld, bool kSplit>
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kHalves>
 __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
                             uint64_t* lds_bad) {
     using K = RowsKind<T, kD, kHeld>;
@@ -1141,7 +1149,9 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & (kWaveSize - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
-    const int row = w.first_row + wave * L::kRows + L::row_of(lane);
+    constexpr int kRowWaves = kWaves / kHalves;
+    const int mine = kHalves == 1 ? 0 : wave / kRowWaves;  // this wave's half of a tile, or the first of both
+    const int row = w.first_row + wave % kRowWaves * L::kRows + L::row_of(lane);
     const bool inside = row < w.rows;
     const int token = inside ? row / a.per : 0;
     const int limit = inside ? w.offset + token : -1;  // the last token the row sees
@@ -1467,8 +1477,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         if (tiles > 1) send(next, 1, false);
         wait_vm<0>();
         bare_barrier();
-        s0 = scores(0, 0);
-        s1 = scores(0, 1);
+        s0 = scores(0, mine);
+        if constexpr (kHalves == 1) s1 = scores(0, 1);
     }
 #pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
@@ -1492,8 +1502,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
                 load_codes(k_codes, far, false);
                 load_codes(v_codes, far, true);
             }
-            s0 = scores(at, 0);
-            s1 = scores(at, 1);
+            s0 = scores(at, mine);
+            if constexpr (kHalves == 1) s1 = scores(at, 1);
         } else {
             if (i + 2 < tiles) {
                 far = look_up(i + 2);
@@ -1502,9 +1512,9 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
             if (i + 1 < tiles) send(next, at ^ 1, true);
         }
         // (Behind the last tile these are scores of nothing, used by nobody.)
-        if constexpr (!kCodes) n0 = scores(at ^ 1, 0);
-        scale_scores(s0, i, 0);
-        scale_scores(s1, i, 1);
+        if constexpr (!kCodes) n0 = scores(at ^ 1, mine);
+        scale_scores(s0, i, mine);
+        if constexpr (kHalves == 1) scale_scores(s1, i, 1); else s1 = s0;  // (one place, for the maximum)
         int most = 0;
         if constexpr (kCodes) most = reinterpret_cast<const int*>(scales_of(i))[2 * kTokens];
         const bool masked = here.there != kAll || first + kTokens - 1 > tile_least;
@@ -1512,7 +1522,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         if (masked) {
             const int count = limit - first + 1;
             sees = here.there & (count >= kTokens ? kAll : count <= 0 ? 0u : (uint64_t{1} << count) - 1u);
-            const uint32_t sees0 = static_cast<uint32_t>(sees) >> (4 * L::part_of(lane));
+            const uint32_t sees0 = static_cast<uint32_t>(sees >> (32 * mine)) >> (4 * L::part_of(lane));
             const uint32_t sees1 = static_cast<uint32_t>(sees >> 32) >> (4 * L::part_of(lane));
             float above = 0.0f;
 #pragma unroll
@@ -1520,11 +1530,11 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
                 const bool see0 = (sees0 & (1u << L::token_of(e))) != 0;
                 const bool see1 = (sees1 & (1u << L::token_of(e))) != 0;
                 s0[e] = see0 ? s0[e] : -INFINITY;
-                s1[e] = see1 ? s1[e] : -INFINITY;
+                if constexpr (kHalves == 1) s1[e] = see1 ? s1[e] : -INFINITY; else s1[e] = s0[e];
                 if constexpr (kCodes) {
                     const float* by = scales_of(i) + kTokens + 4 * L::part_of(lane) + L::token_of(e);
-                    above = fmaxf(above, see0 ? fabsf(by[0]) : 0.0f);
-                    above = fmaxf(above, see1 ? fabsf(by[32]) : 0.0f);
+                    above = fmaxf(above, see0 ? fabsf(by[32 * mine]) : 0.0f);
+                    if constexpr (kHalves == 1) above = fmaxf(above, see1 ? fabsf(by[32]) : 0.0f);
                 }
             }
             if constexpr (kCodes) most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(above));
@@ -1538,37 +1548,44 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         }
         // Three stretches of products, each with the vector work of another part
         // among them; values are read a stretch ahead of their product.
-        if constexpr (!kCodes) n1 = scores(at ^ 1, 1);
-        weigh(s0, i, 0);
+        if constexpr (!kCodes && kHalves == 1) n1 = scores(at ^ 1, 1);
+        weigh(s0, i, mine);
         const Weights p0 = pack(s0);
         constexpr int kFar = 4;  // products that values are read ahead of theirs
         u32x4_t v[kFar];
 #pragma unroll
-        for (int n = 0; n < kFar; ++n) v[n] = read_values(at, 0, n);
+        for (int n = 0; n < kFar; ++n) v[n] = read_values(at, mine, n);
         __builtin_amdgcn_sched_barrier(0);
-        weigh(s1, i, 1);
-        const Weights p1 = pack(s1);
+        if constexpr (kHalves == 1) weigh(s1, i, 1);
+        [[maybe_unused]] Weights p1;
+        if constexpr (kHalves == 1) p1 = pack(s1);
 #pragma unroll
         for (int n = 0; n < kPieces; ++n) {
             multiply(v[n % kFar], p0.part[n & 1], acc[n >> 1]);
             if constexpr (kSplit) multiply(v[n % kFar], pack(rest_of(s0)).part[n & 1], acc[n >> 1]);
-            v[n % kFar] = n + kFar < kPieces ? read_values(at, 0, n + kFar) : read_values(at, 1, n + kFar - kPieces);
+            if (n + kFar < kPieces) {
+                v[n % kFar] = read_values(at, mine, n + kFar);
+            } else if constexpr (kHalves == 1) {
+                v[n % kFar] = read_values(at, 1, n + kFar - kPieces);
+            }
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kHalves == 1) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < kPieces; ++n) {
-            multiply(v[n % kFar], p1.part[n & 1], acc[n >> 1]);
-            if constexpr (kSplit) multiply(v[n % kFar], pack(rest_of(s1)).part[n & 1], acc[n >> 1]);
-            if (n + kFar < kPieces) v[n % kFar] = read_values(at, 1, n + kFar);
+            for (int n = 0; n < kPieces; ++n) {
+                multiply(v[n % kFar], p1.part[n & 1], acc[n >> 1]);
+                if constexpr (kSplit) multiply(v[n % kFar], pack(rest_of(s1)).part[n & 1], acc[n >> 1]);
+                if (n + kFar < kPieces) v[n % kFar] = read_values(at, 1, n + kFar);
+            }
         }
         if constexpr (!kCodes) {
             s0 = n0;
-            s1 = n1;
+            if constexpr (kHalves == 1) s1 = n1;
         }
         here = next;
         next = far;
     }
-    finish<T, kD, kCodes, kSplit, true>(a, w, lds, lds_m, lds_l, m + (kCodes ? static_cast<float>(unit) : 0.0f), l, acc);
+    finish<T, kD, kCodes, kSplit, kRowWaves>(a, w, lds, lds_m, lds_l, m + (kCodes ? static_cast<float>(unit) : 0.0f), l, acc);
 }
 
 /// Zeros for the rows first_row .. first_row + count - 1 of a KV head's heads,
@@ -1646,8 +1663,10 @@ __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_k
     Item w{};
     int end_row = 0;
     if (!item_of<std::conditional_t<kSplit, float, T>>(a, w, end_row)) return;
-    if (end_row - w.first_row > kRows) {
-        attend_rows<T, kD, kHeld, kSplit>(a, w, lds, lds_m, lds_l, lds_bad);
+    if (end_row - w.first_row > 2 * kRows) {
+        attend_rows<T, kD, kHeld, kSplit, 1>(a, w, lds, lds_m, lds_l, lds_bad);
+    } else if (end_row - w.first_row > kRows) {
+        attend_rows<T, kD, kHeld, kSplit, 2>(a, w, lds, lds_m, lds_l, lds_bad);
     } else if (end_row - w.first_row > 16) {
         attend_few<T, kD, kHeld, kSplit, 2>(a, w, lds, lds_m, lds_l);
     } else {
@@ -1835,7 +1854,19 @@ Plan plan_of(cf_dtype dtype, cf_cache_format format, int64_t tokens, int64_t seq
     // seven chunks of 333 in int8 67 us uncut, 90 in two.)
     p.least = 256;
     p.step = static_cast<int>(kWaves * wave_rows);
-    p.splits = splits(tiles_of(p.rows, tokens, sequences < tokens ? sequences : tokens, per) * kv_heads, 512, p.least);
+    auto ranges = [&](int64_t rows) {
+        return splits(tiles_of(rows, tokens, sequences < tokens ? sequences : tokens, per) * kv_heads, 512, p.least);
+    };
+    p.splits = ranges(p.rows);
+    // Tiles of 64 rows, uncut, instead of tiles of 128 in two or three ranges, where a
+    // table reaches 2048 tokens at most: two prompts of 400 tokens in bf16 24 us
+    // against 42, in int8 29 against 47; 700 tokens behind 1300 59 against 68, and 81
+    // against 83. In longer contexts each tile's own pass over them costs more than
+    // the join (three chunks of 256 behind 3744: 115 us against 110, 174 against 146).
+    if (!wide && p.splits > 1 && capacity <= 2048 && ranges(64) == 1) {
+        p.rows = 64;
+        p.splits = 1;
+    }
     return p;
 }
 

@@ -130,6 +130,36 @@ def test_row_tiles_of_a_context_split_and_not():
             run(build(sequences, 8, 1, 64, 16, torch.bfloat16, held))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("dim", [64, 128, 256, 96])
+def test_tiles_of_64_rows(dtype, held, dim):
+    """Taken for all rows where tables are short and tiles of 128 would be cut."""
+    run(build([(130, 300), (97, 300), (1, 200), (160, 160), (0, 9), (33, 290)], 32, 8, dim, 16, dtype, held, before=2, behind=9))
+    run(build([(150, 400)] * 2, 16, 16, dim, 16, dtype, held))
+    # A tile's second half without tokens, rows without any.
+    run(build([(90, 90), (60, 20), (160, 161)], 32, 8, dim, 16, dtype, held))
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_a_row_of_such_a_tile_does_not_see(held, bad):
+    for dtype in DTYPES:
+        c = build([(150, 170)] * 3, 32, 8, 64, 16, dtype, held)
+        clean = cf.paged_attention_chunk(*c.args()).cpu()
+        for row in (3, 40, 80):  # in either half of a step's tokens
+            page, at = int(c.tables[1, (20 + row) // 16]), (20 + row) % 16
+            if held is None:
+                c.k[page, at], c.v[page, at] = bad, bad
+            else:
+                c.k_scales[page, at], c.v_scales[page, at] = bad, bad
+                if held == torch.float8_e4m3fn:
+                    c.v.view(torch.uint8)[page, at] = 0x7F
+        got = cf.paged_attention_chunk(*c.args()).cpu()
+        assert torch.equal(got[:153], clean[:153]) and torch.equal(got[300:], clean[300:])
+        assert not torch.isfinite(got[153:300]).all(-1).any()
+
+
 def test_views_misaligned_and_other_streams():
     c = build(MIXED, 4, 2, 64, 16, torch.bfloat16)
     want = cf.paged_attention_chunk(*c.args())
