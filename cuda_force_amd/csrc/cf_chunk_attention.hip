@@ -1854,19 +1854,24 @@ Plan plan_of(cf_dtype dtype, cf_cache_format format, int64_t tokens, int64_t seq
     // seven chunks of 333 in int8 67 us uncut, 90 in two.)
     p.least = 256;
     p.step = static_cast<int>(kWaves * wave_rows);
-    auto ranges = [&](int64_t rows) {
-        return splits(tiles_of(rows, tokens, sequences < tokens ? sequences : tokens, per) * kv_heads, 512, p.least);
+    auto items = [&](int64_t rows) {
+        return tiles_of(rows, tokens, sequences < tokens ? sequences : tokens, per) * kv_heads;
     };
-    p.splits = ranges(p.rows);
+    p.splits = splits(items(p.rows), 512, p.least);
     // Tiles of 64 rows, uncut, instead of tiles of 128 in two or three ranges, where a
     // table reaches 2048 tokens at most: two prompts of 400 tokens in bf16 24 us
     // against 42, in int8 29 against 47; 700 tokens behind 1300 59 against 68, and 81
     // against 83. In longer contexts each tile's own pass over them costs more than
     // the join (three chunks of 256 behind 3744: 115 us against 110, 174 against 146).
-    if (!wide && p.splits > 1 && capacity <= 2048 && ranges(64) == 1) {
+    if (!wide && p.splits > 1 && capacity <= 2048 && splits(items(64), 512, p.least) == 1) {
         p.rows = 64;
         p.splits = 1;
     }
+    // And where codes in heads of 64, of which three workgroups fit a CU, do not fill the
+    // GPU in tiles of 128 (seven chunks of 333 in int8, 400 items, 67 us against 77;
+    // 448 items 47 against 54; 576 would take 76 against 58, and the query's type 400
+    // items 60 against 51).
+    if (format != CF_CACHE_PLAIN && p.dim == 64 && p.splits == 1 && p.rows == 128 && items(128) < 512) p.rows = 64;
     return p;
 }
 
