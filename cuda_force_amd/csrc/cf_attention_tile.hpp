@@ -46,16 +46,18 @@ __device__ __forceinline__ void copy16_to_lds(const uint8_t* base, uint32_t offs
                  : "memory");
 }
 
-/// Four copies like the first, to LDS bytes dst + 1024 n + 16 lane: the
-/// instruction's offset counts for both addresses, so the sources are given
-/// less 1024 n.
+/// Four copies like the first, to LDS bytes dst + kCopyBytes n + 16 lane: the
+/// instruction's offset counts for both addresses, so the sources are given less
+/// kCopyBytes n.
+constexpr int kCopyBytes = 16 * kWaveSize;
 __device__ __forceinline__ void copy16x4_to_lds(const uint8_t* from0, const uint8_t* from1, const uint8_t* from2,
                                                 const uint8_t* from3, uint32_t dst) {
     asm volatile(
-        "s_nop 4\n\tglobal_load_lds_dwordx4 %0, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024\n\t"
-        "global_load_lds_dwordx4 %2, off offset:2048\n\tglobal_load_lds_dwordx4 %3, off offset:3072"
+        "s_nop 4\n\tglobal_load_lds_dwordx4 %0, off\n\tglobal_load_lds_dwordx4 %1, off offset:%5\n\t"
+        "global_load_lds_dwordx4 %2, off offset:%6\n\tglobal_load_lds_dwordx4 %3, off offset:%7"
         :
-        : "v"(from0), "v"(from1), "v"(from2), "v"(from3), "{m0}"(__builtin_amdgcn_readfirstlane(dst))
+        : "v"(from0), "v"(from1), "v"(from2), "v"(from3), "{m0}"(__builtin_amdgcn_readfirstlane(dst)), "n"(kCopyBytes),
+          "n"(2 * kCopyBytes), "n"(3 * kCopyBytes)
         : "memory");
 }
 

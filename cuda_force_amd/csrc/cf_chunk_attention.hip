@@ -1232,7 +1232,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
             }
             if constexpr (kBatch == 4) {
                 if (whole) {
-                    copy16x4_to_lds(from[0], from[1] - 1024, from[2] - 2048, from[3] - 3072,
+                    copy16x4_to_lds(from[0], from[1] - kCopyBytes, from[2] - 2 * kCopyBytes, from[3] - 3 * kCopyBytes,
                                     dst + static_cast<uint32_t>(n0) * 16 * kWaveSize);
                     continue;
                 }
