@@ -156,3 +156,23 @@ def test_graph(m):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, step())
+
+
+def test_results_and_rows_past_2_to_the_31():
+    m, n, k = 70000, 40000, 16
+    x = torch.randint(-128, 128, (m, k), device="cuda", dtype=torch.int8)
+    w = torch.randint(-128, 128, (n, k), device="cuda", dtype=torch.int8)
+    ones = torch.ones(m, device="cuda")
+    y = cf.matmul_int8(x, w, ones, ones[:n])
+    for at in (0, 53687, 53688, m - 1):  # 2^31 / n lies between the middle two
+        want = (x[at].double() @ w.double().t()).to(torch.bfloat16)
+        assert torch.equal(y[at], want)
+    del y
+    rows = 2**31 // 8192 + 9
+    x = torch.randn(rows, 8192, device="cuda", dtype=torch.bfloat16)
+    codes, scales = cf.quantize_int8_rows(x)
+    for at in (0, rows - 10, rows - 9, rows - 1):
+        want, want_scales = _nearest_codes(x[at : at + 1].cpu(), torch.int8)
+        assert torch.equal(codes[at : at + 1].cpu(), want) and torch.equal(scales[at : at + 1].cpu(), want_scales)
+    del x, codes
+    torch.cuda.empty_cache()
