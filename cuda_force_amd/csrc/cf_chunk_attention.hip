@@ -82,6 +82,13 @@ struct ChunkArgs {
 
 __device__ __forceinline__ int clamp_to(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
 
+/// The exponent of the power of two above the largest of scales, kLeastUnit at
+/// least: what is taken where there is none of them, too (0's exponent is 0, far
+/// above those of small values).
+__device__ __forceinline__ int unit_above(float largest) {
+    return largest > 0.0f ? max(__builtin_amdgcn_frexp_expf(largest), kLeastUnit) : kLeastUnit;
+}
+
 // ---- items ----------------------------------------------------------------------
 
 /// Neighbouring rows (tokens) of one sequence, or of none.
@@ -958,7 +965,7 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
                 float above = fabsf(by[0]);
 #pragma unroll
                 for (int i = 1; i < kScores; ++i) above = fmaxf(above, fabsf(by[i]));
-                most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(above));
+                most = unit_above(groups_max<L::kRows>(above));
             }
             float top = x[0];
 #pragma unroll
@@ -1303,7 +1310,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
             scales[(is_v ? kTokens : 0) + lane] = raw_scale;
             if (is_v) {
                 const float top = wave_reduce_f32<MaxF32>(fabsf(raw_scale));
-                if (lane == 0) reinterpret_cast<int*>(scales)[2 * kTokens] = max(__builtin_amdgcn_frexp_expf(top), kLeastUnit);
+                if (lane == 0) reinterpret_cast<int*>(scales)[2 * kTokens] = unit_above(top);
             }
         }
     };
@@ -1537,7 +1544,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
                     if constexpr (kHalves == 1) above = fmaxf(above, see1 ? fabsf(by[32]) : 0.0f);
                 }
             }
-            if constexpr (kCodes) most = __builtin_amdgcn_frexp_expf(groups_max<L::kRows>(above));
+            if constexpr (kCodes) most = unit_above(groups_max<L::kRows>(above));
         }
         rescale_to(largest(s0, s1), most);
         if constexpr (kHeld != CF_CACHE_INT8) {  // whose codes are all finite
