@@ -204,6 +204,24 @@ struct Item {
     bool direct;    // the only piece: straight to the result
 };
 
+/// What counts as the scale of a row of values: a row of zeros, which is stored
+/// with the scale 1 whatever the others' are, must not stand for the largest of
+/// them, so its scale is taken as 0. `row`: its codes, read only if the scale is 1.
+template <cf_cache_format kHeld>
+__device__ __forceinline__ float value_scale(float scale, const uint8_t* row, int bytes) {
+    if (scale == 1.0f) {
+        uint32_t any = 0;
+#pragma unroll 1
+        for (int at = 0; at < bytes; at += 16) {
+            const u32x4_t codes = *reinterpret_cast<const u32x4_t*>(row + at);
+            any |= codes[0] | codes[1] | codes[2] | codes[3];
+        }
+        constexpr uint32_t kMagnitudes = kHeld == CF_CACHE_E4M3 ? 0x7F7F7F7Fu : 0xFFFFFFFFu;
+        if ((any & kMagnitudes) == 0) scale = 0.0f;
+    }
+    return scale;
+}
+
 /// LDS of attend: its tiles, a ring that the waves share or one for each of them.
 template <int kD>
 struct WideKind {
@@ -882,7 +900,10 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
         const int first = begin + i * kStride;
         const uint32_t now = there;
         const bool masked = now != 0xFFFFFFFFu || first + kTokens - 1 > wave_least;
-        if constexpr (kCodes) scales[lane] = scale;
+        if constexpr (kCodes) {
+            if (lane >= kTokens) scale = value_scale<kHeld>(scale, a.v_cache + places[lane - kTokens], row_bytes);
+            scales[lane] = scale;
+        }
         // The next tile; behind the last one its tokens are not there, and every lane reads
         // row 0 of the cache, for nobody: loads behind a branch would be waited for
         // wherever one of the others is.
@@ -1291,7 +1312,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     [[maybe_unused]] auto scales_of = [&](int tile) {
         return reinterpret_cast<float*>(lds + K::kScalesAt) + (tile & 1) * K::kScales;
     };
-    [[maybe_unused]] auto store_codes = [&](const Codes& from, int tile, bool is_v) {
+    [[maybe_unused]] auto store_codes = [&](const Codes& from, const Place& p, int tile, bool is_v) {
         uint8_t* to = lds + ((is_v ? 2 : 0) + (tile & 1)) * K::kOperand;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
@@ -1307,6 +1328,10 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         }
         if (wave == (is_v ? 1 : 0)) {
             float* scales = scales_of(tile);
+            if (is_v) {
+                raw_scale = value_scale<kHeld>(raw_scale, a.v_cache + head_bytes + (static_cast<uint64_t>(p.piece) << 4),
+                                               a.head_dim);
+            }
             scales[(is_v ? kTokens : 0) + lane] = raw_scale;
             if (is_v) {
                 const float top = wave_reduce_f32<MaxF32>(fabsf(raw_scale));
@@ -1472,8 +1497,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     if constexpr (kCodes) {
         load_codes(k_codes, here, false);
         load_codes(v_codes, here, true);
-        store_codes(k_codes, 0, false);
-        store_codes(v_codes, 0, true);
+        store_codes(k_codes, here, 0, false);
+        store_codes(v_codes, here, 0, true);
         if (tiles > 1) {
             load_codes(k_codes, next, false);
             load_codes(v_codes, next, true);
@@ -1501,8 +1526,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         bare_barrier();
         if constexpr (kCodes) {
             if (i + 1 < tiles) {
-                store_codes(k_codes, i + 1, false);
-                store_codes(v_codes, i + 1, true);
+                store_codes(k_codes, next, i + 1, false);
+                store_codes(v_codes, next, i + 1, true);
             }
             if (i + 2 < tiles) {
                 far = look_up(i + 2);

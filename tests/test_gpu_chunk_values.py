@@ -37,3 +37,39 @@ def test_small_values_behind_pages_left_out(dtype, held, sequences, dim):
     c = small(sequences, dtype, held, dim)
     c.tables[:, 4:12] = -1
     run(c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("held", CODES)
+@pytest.mark.parametrize("sequences", ROWS)
+@pytest.mark.parametrize("dim", [64, 128, 256, 80])
+def test_small_values_beside_rows_of_zeros(dtype, held, sequences, dim):
+    """Rows of zeros have the scale 1, far above the others': alone in the first
+    steps, among others in one, as tokens of both halves of a step, and (in e4m3)
+    with codes of -0."""
+    zeros = [range(0, 200), [3], [350, 351, 420, 470], range(500, 540)]
+    for places in zeros:
+        c = small(sequences, dtype, held, dim)
+        for s, length in enumerate(c.context.tolist()):
+            for t in places:
+                if t < length:
+                    page, at = int(c.tables[s, t // 16]), t % 16
+                    c.v[page, at] = 0
+                    if held == torch.float8_e4m3fn:
+                        c.v.view(torch.uint8)[page, at, :, ::3] = 0x80
+                    c.v_scales[page, at] = 1.0
+        run(c)
+
+
+@pytest.mark.parametrize("held", CODES)
+@pytest.mark.parametrize("sequences", ROWS)
+def test_a_scale_of_1_that_is_no_row_of_zeros(held, sequences):
+    """Small values next to tokens whose values are up to the largest code times 1."""
+    c = small(sequences, torch.float32, held)
+    for s, length in enumerate(c.context.tolist()):
+        for t in (2, 40, length - 1):
+            page, at = int(c.tables[s, t // 16]), t % 16
+            c.v[page, at] = 0
+            c.v[page, at, :, t % 128] = 1.0
+            c.v_scales[page, at] = 1.0
+    run(c)
