@@ -222,6 +222,65 @@ __device__ __forceinline__ float value_scale(float scale, const uint8_t* row, in
     return scale;
 }
 
+/// Values that are not finite, of tokens that some rows of a tile see and others do
+/// not: a product would take them, times 0, to all rows. They are set to 0 in it.
+/// Where that happened the range's values are looked through again at the end, and
+/// for each dim the first position that holds one is kept in LDS: the rows from there
+/// on see it, and their results are made what it makes them. (Changing the sums within
+/// the loop, or noting the positions there, cost heads of 256 20 to 35%.)
+template <int kD>
+struct BadValues {
+    static constexpr int kNone = 0x7FFFFFFF;
+    int plus[kD];  // positions of infinities, and of what is no number, which is in both
+    int minus[kD];
+    int from[kWaves];  // the first token of a wave's first tile with such a value
+
+    /// Whether there are any; then they are noted. Called by the whole workgroup, behind
+    /// a barrier after `from` was set.
+    template <typename T, cf_cache_format kHeld>
+    __device__ __forceinline__ bool find(const ChunkArgs& a, const Item& w) {
+        static_assert(kWaves == 4, "four of them");
+        const int first = min(min(from[0], from[1]), min(from[2], from[3]));
+        if (first >= w.hi) return false;
+        const int tid = static_cast<int>(threadIdx.x);
+        for (int i = tid; i < kD; i += kThreads) plus[i] = minus[i] = kNone;
+        __syncthreads();
+        constexpr int kSize = kHeld == CF_CACHE_PLAIN ? static_cast<int>(sizeof(T)) : 1;
+        constexpr uint32_t kSign = 1u << (8 * kSize - 1);
+        constexpr uint32_t kInfinity = kSize == 4 ? 0x7F800000u : std::is_same<T, f16_t>::value ? 0x7C00u : 0x7F80u;
+        for (int64_t i = static_cast<int64_t>(first) * a.head_dim + tid; i < static_cast<int64_t>(w.hi) * a.head_dim; i += kThreads) {
+            const int t = static_cast<int>(i / a.head_dim);
+            const int dim = static_cast<int>(i % a.head_dim);
+            const uint32_t block = static_cast<uint32_t>(t) / a.block_size;
+            const uint32_t page = w.table[block];
+            if (page >= a.pages) continue;
+            const uint64_t row = static_cast<uint64_t>(page) * a.block_size + (static_cast<uint32_t>(t) - block * a.block_size);
+            const uint64_t at = (row * static_cast<uint32_t>(a.kv_heads) + static_cast<uint32_t>(w.kv_head)) *
+                                    static_cast<uint32_t>(a.head_dim) + static_cast<uint32_t>(dim);
+            if constexpr (kHeld == CF_CACHE_PLAIN) {
+                uint32_t bits;
+                if constexpr (kSize == 4) bits = reinterpret_cast<const uint32_t*>(a.v_cache)[at];
+                else bits = reinterpret_cast<const uint16_t*>(a.v_cache)[at];
+                const uint32_t magnitude = bits & (kSign - 1);
+                if (magnitude > kInfinity || bits == kInfinity) atomicMin(&plus[dim], t);
+                if (magnitude > kInfinity || bits == (kInfinity | kSign)) atomicMin(&minus[dim], t);
+            } else if ((a.v_cache[at] & 0x7F) == 0x7F) {  // e4m3 has no infinities
+                atomicMin(&plus[dim], t);
+                atomicMin(&minus[dim], t);
+            }
+        }
+        __syncthreads();
+        return true;
+    }
+    /// Into four neighbouring dims of the row at `position`.
+    __device__ __forceinline__ void add_to(f32x4_t& sum, int dim, int position) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            sum[e] += (position >= plus[dim + e] ? INFINITY : 0.0f) - (position >= minus[dim + e] ? INFINITY : 0.0f);
+        }
+    }
+};
+
 /// LDS of attend: its tiles, a ring that the waves share or one for each of them.
 template <int kD>
 struct WideKind {
@@ -392,10 +451,10 @@ __device__ __forceinline__ void put(const ChunkArgs& a, const Item& w, int row, 
 }
 
 /// The waves' outputs, kRowWaves of them of different rows, the others behind them
-/// of different tokens of the same.
-template <typename T, int kD, bool kCodes, bool kSplit, int kRowWaves>
+/// of different tokens of the same. bad_from: see BadValues.
+template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kRowWaves>
 __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32],
-                                       float (*lds_l)[32], float m, float l,
+                                       float (*lds_l)[32], BadValues<kD>* bad, int bad_from, float m, float l,
                                        const typename Tile<T, kD>::Score (&acc)[Tile<T, kD>::kAcc / Tile<T, kD>::kScores]) {
     using L = Tile<T, kD>;
     const int tid = static_cast<int>(threadIdx.x);
@@ -417,7 +476,10 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
         lds_m[wave][L::row_of(lane)] = m;
         lds_l[wave][L::row_of(lane)] = l;
     }
+    if (kHeld != CF_CACHE_INT8 && lane == 0) bad->from[wave] = bad_from;
     __syncthreads();
+    bool any_bad = false;
+    if constexpr (kHeld != CF_CACHE_INT8) any_bad = bad->template find<T, kHeld>(a, w);
     // Rows x groups of four dims, over the workgroup.
     constexpr int kOutRows = kRowWaves * L::kRows;
     constexpr int kFours = kD / 4;
@@ -432,14 +494,15 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
         if (out >= w.rows || dim >= a.head_dim) continue;
         const float* sums = reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim;
         const int wave_of = r / L::kRows;
+        Joined j;
         if constexpr (kRowWaves == kWaves) {
-            put<T, kCodes, kSplit>(a, w, out, dim, lds_m[wave_of][r % L::kRows], lds_l[wave_of][r % L::kRows],
-                                   *reinterpret_cast<const f32x4_t*>(sums));
+            j = Joined{lds_m[wave_of][r % L::kRows], lds_l[wave_of][r % L::kRows], *reinterpret_cast<const f32x4_t*>(sums)};
         } else {
-            const Joined j = join_waves<kWaves / kRowWaves, kRowWaves>(sums, L::kRows * L::kOutPitch, lds_m + wave_of,
-                                                                       lds_l + wave_of, r % L::kRows);
-            put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
+            j = join_waves<kWaves / kRowWaves, kRowWaves>(sums, L::kRows * L::kOutPitch, lds_m + wave_of,
+                                                          lds_l + wave_of, r % L::kRows);
         }
+        if (any_bad) bad->add_to(j.sum, dim, w.offset + out / a.per);
+        put<T, kHeld != CF_CACHE_PLAIN, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
     }
 }
 
@@ -449,7 +512,7 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
 /// tokens of the same rows.
 template <int kD, bool kShared>
 __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
-                       uint64_t* lds_bad) {
+                       BadValues<kD>* bad) {
     using K = WideKind<kD>;
     using L = typename K::L;
     constexpr int kTokenWaves = kShared ? 1 : kWaves;
@@ -592,40 +655,30 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
             l += s[i];
         }
     };
-    // A token that a row of the tile does not see may hold NaN or infinities, which
-    // times a weight of 0 would reach that row. In such tiles they are replaced by 0,
-    // and a row that sees one gets a sum of NaN.
-    auto guard = [&](uint8_t* v, int first, uint32_t there) {
+    // Values that are not finite, in tiles that some row does not see whole (see
+    // BadValues).
+    int bad_from = BadValues<kD>::kNone;
+    auto guard = [&](uint8_t* v, int first) {
         if (min(first + L::kTokens, w.hi) - 1 <= w.offset + w.first_row / a.per) return;
-        uint32_t bad = 0;  // tokens
+        bool any = false;
 #pragma unroll 1
         for (int i = kShared ? tid : lane; i < L::kTokens * L::kChunks; i += kShared ? kThreads : kWaveSize) {
             u32x4_t four = reinterpret_cast<const u32x4_t*>(v)[i];
-            bool any = false;
+            bool here = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const bool out = (four[e] & 0x7F800000u) == 0x7F800000u;
-                any = any || out;
+                here = here || out;
                 four[e] = out ? 0u : four[e];
             }
-            if (any) {
-                reinterpret_cast<u32x4_t*>(v)[i] = four;
-                bad |= 1u << (i / L::kChunks);
-            }
+            if (here) reinterpret_cast<u32x4_t*>(v)[i] = four;
+            any = any || here;
         }
-#pragma unroll
-        for (int d = 1; d < kWaveSize; d <<= 1) bad |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(bad), d));
-        if constexpr (kShared) {
-            if (lane == 0) lds_bad[wave] = bad;
-            __syncthreads();
-            bad = static_cast<uint32_t>(lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3]);
-        } else {
-            wait_lds();
-        }
-        if ((bad & seen(first, there)) != 0) l = __uint_as_float(0x7FC00000u);
+        if (__builtin_amdgcn_ballot_w64(any) != 0) bad_from = min(bad_from, first);
+        if constexpr (kShared) __syncthreads(); else wait_lds();
     };
-    auto add_values = [&](uint8_t* v, typename L::Score& s, int first, uint32_t there) {
-        guard(v, first, there);
+    auto add_values = [&](uint8_t* v, typename L::Score& s, int first) {
+        guard(v, first);
         L::values(v, s, acc, lane);
     };
 
@@ -657,7 +710,7 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
                 clear(v, there, lane, kWaveSize);
                 wait_lds();
             }
-            add_values(v, s, first, there);
+            add_values(v, s, first);
             wait_lds();
             if (more) copy(v_dst, true);
         }
@@ -694,7 +747,7 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
                 clear(v, now, tid, kThreads);
                 __syncthreads();
             }
-            add_values(v, s, begin + i * kStride, now);
+            add_values(v, s, begin + i * kStride);
             wait_lds();  // before the barrier that lets the tile be overwritten
         };
         static_assert(kStages == 4, "four steps");
@@ -706,7 +759,7 @@ __device__ void attend(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*
         }
     }
 
-    finish<float, kD, false, false, kShared ? kWaves : 1>(a, w, lds, lds_m, lds_l, m, l, acc);
+    finish<float, kD, CF_CACHE_PLAIN, false, kShared ? kWaves : 1>(a, w, lds, lds_m, lds_l, bad, bad_from, m, l, acc);
 }
 
 /// Where a lane's values lie when 16 rows meet 32 tokens in 16 x 16 products.
@@ -752,7 +805,8 @@ struct FewTile {
 /// sequences of up to 4096 tokens in int8 took 126 us, not 102. Twice the waves a
 /// SIMD, in a kernel of their own, changed nothing.)
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kTiles>
-__device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32]) {
+__device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
+                           BadValues<kD>* bad) {
     constexpr bool kCodes = kHeld != CF_CACHE_PLAIN;
     using L = FewTile<T, kD, kCodes>;
     constexpr int kTokens = L::kTokens;
@@ -887,6 +941,7 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
     constexpr int kScores = 8;  // a lane's, tokens 4 group + (i & 3) + 16 (i >> 2)
     auto token_of = [](int i) { return (i & 3) + 16 * (i >> 2); };
 
+    [[maybe_unused]] int bad_from = BadValues<kD>::kNone;
     if (tiles > 0) {
         look_up(begin);
         load_keys();
@@ -953,7 +1008,6 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
                 }
             }
         }
-        uint32_t sees[kTiles];  // of the lane's tokens
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
             float x[kScores];
@@ -966,13 +1020,12 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
                     by[i] = of_value[i];
                 }
             }
-            sees[n] = 0xFFFFFFFFu;
             if (masked) {
                 const int count = limit[n] - first + 1;
-                sees[n] = (now & (count >= kTokens ? 0xFFFFFFFFu : count <= 0 ? 0u : (1u << count) - 1u)) >> (4 * group);
+                const uint32_t sees = (now & (count >= kTokens ? 0xFFFFFFFFu : count <= 0 ? 0u : (1u << count) - 1u)) >> (4 * group);
 #pragma unroll
                 for (int i = 0; i < kScores; ++i) {
-                    const bool see = (sees[n] & (1u << token_of(i))) != 0;
+                    const bool see = (sees & (1u << token_of(i))) != 0;
                     x[i] = see ? x[i] : -INFINITY;
                     // What a row does not see may be NaN, or far above its own scales.
                     if constexpr (kCodes) by[i] = see ? by[i] : 0.0f;
@@ -1037,17 +1090,15 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
             }
         }
 
-        // Values. A token that a row of the tile does not see may hold NaN or infinities,
-        // which times a weight of 0 would reach that row. In such tiles they are replaced
-        // by 0, and a row that sees one gets a sum of NaN.
+        // Values. Those that are not finite, in tiles that some row does not see whole (see
+        // BadValues).
         if (kHeld != CF_CACHE_INT8 && masked) {
             // Adding `one` to an exponent of ones, or to e4m3's NaN, carries into the sign.
             constexpr uint32_t one = kCodes ? 0x01010101u : std::is_same<T, f16_t>::value ? 0x04000400u : 0x00800080u;
             constexpr uint32_t sign = kCodes ? 0x80808080u : 0x80008000u;
-            uint32_t bad = 0;  // of the lane's tokens, like sees
+            uint32_t any = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                uint32_t any = 0;
 #pragma unroll
                 for (int p = 0; p < L::kPieces; ++p) {
 #pragma unroll
@@ -1057,14 +1108,8 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
                         values[j][p][word] &= ~((out >> (kCodes ? 7 : 15)) * (kCodes ? 0xFFu : 0xFFFFu));
                     }
                 }
-                bad |= any != 0 ? 1u << token_of(j) : 0u;
             }
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) bad |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(bad), d));
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n) {
-                if ((bad & sees[n]) != 0) l[n] = __uint_as_float(0x7FC00000u);
-            }
+            if (__builtin_amdgcn_ballot_w64(any != 0) != 0) bad_from = min(bad_from, first);
         }
 #pragma unroll
         for (int p = 0; p < L::kPieces; ++p) {
@@ -1113,6 +1158,8 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
             lds_l[wave][n * L::kRows + of16] = l[n];
         }
     }
+    if (kHeld != CF_CACHE_INT8 && lane == 0) bad->from[wave] = bad_from;
+    bool any_bad = false;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
         if (w.first_row + n * L::kRows >= w.rows) break;
@@ -1127,13 +1174,17 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
             }
         }
         __syncthreads();
+        if (n == 0) {
+            if constexpr (kHeld != CF_CACHE_INT8) any_bad = bad->template find<T, kHeld>(a, w);
+        }
         for (int i = tid; i < L::kRows * (kD / 4); i += kThreads) {
             const int r = i / (kD / 4);
             const int dim = i % (kD / 4) * 4;
             const int out = w.first_row + n * L::kRows + r;
             if (out >= w.rows || dim >= a.head_dim) continue;
-            const Joined j = join_waves<kWaves, 1>(reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim,
-                                               L::kOwnBytes / 4, lds_m, lds_l, n * L::kRows + r);
+            Joined j = join_waves<kWaves, 1>(reinterpret_cast<const float*>(lds) + r * L::kOutPitch + dim,
+                                             L::kOwnBytes / 4, lds_m, lds_l, n * L::kRows + r);
+            if (any_bad) bad->add_to(j.sum, dim, w.offset + out / a.per);
             put<T, kCodes, kSplit>(a, w, out, dim, j.m, j.l, j.sum);
         }
     }
@@ -1167,7 +1218,7 @@ struct RowsKind {
 /// vector units 45% and the matrix cores 19% busy.
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kHalves>
 __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
-                            uint64_t* lds_bad) {
+                            BadValues<kD>* bad) {
     using K = RowsKind<T, kD, kHeld>;
     using L = typename K::L;
     using Score = typename L::Score;
@@ -1460,34 +1511,31 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         }
     };
     // Values of tokens that are not there, and in tiles that some row does not see
-    // whole those that are not finite (see attend_few), to 0. Returns the latter
-    // tokens, a bit each.
-    [[maybe_unused]] auto sanitise = [&](int slot, int first, uint64_t there) -> uint64_t {
+    // whole those that are not finite (see BadValues), to 0.
+    [[maybe_unused]] int bad_from = BadValues<kD>::kNone;
+    [[maybe_unused]] auto sanitise = [&](int slot, int first, uint64_t there) {
         const bool hidden = min(first + kTokens, w.hi) - 1 > tile_least;
-        if (there == kAll && !hidden) return 0;
+        if (there == kAll && !hidden) return;
         constexpr uint32_t kExponent = std::is_same<T, f16_t>::value ? 0x7C00u : 0x7F80u;
         u32x4_t* v = reinterpret_cast<u32x4_t*>(lds + (2 + slot) * K::kOperand);
-        uint64_t bad = 0;
+        bool any = false;
 #pragma unroll 1
         for (int i = tid; i < kTokens * L::kChunks; i += kThreads) {
             u32x4_t four = v[i];
-            bool any = false;
+            bool here = false;
             const bool out = ((there >> (i / L::kChunks)) & 1) == 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const bool low = hidden && (four[e] & kExponent) == kExponent;
                 const bool high = hidden && (four[e] >> 16 & kExponent) == kExponent;
-                any = any || low || high;
+                here = here || low || high;
                 four[e] = out ? 0u : four[e] & (low ? 0xFFFF0000u : 0xFFFFFFFFu) & (high ? 0xFFFFu : 0xFFFFFFFFu);
             }
-            if (any || out) v[i] = four;
-            if (any && !out) bad |= uint64_t{1} << (i / L::kChunks);
+            if (here || out) v[i] = four;
+            any = any || (here && !out);
         }
-#pragma unroll
-        for (int d = 1; d < kWaveSize; d <<= 1) bad |= static_cast<uint64_t>(__shfl_xor(static_cast<long long>(bad), d));
-        if (lane == 0) lds_bad[wave] = bad;
+        if (__builtin_amdgcn_ballot_w64(any) != 0) bad_from = min(bad_from, first);
         __syncthreads();
-        return lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3];
     };
 
     Place here = look_up(0);  // of tile i
@@ -1573,10 +1621,7 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         }
         rescale_to(largest(s0, s1), most);
         if constexpr (kHeld != CF_CACHE_INT8) {  // whose codes are all finite
-            if (masked) {
-                const uint64_t bad = sanitise(at, first, here.there);
-                if ((bad & sees) != 0) l = __uint_as_float(0x7FC00000u);
-            }
+            if (masked) sanitise(at, first, here.there);
         }
         // Three stretches of products, each with the vector work of another part
         // among them; values are read a stretch ahead of their product.
@@ -1617,7 +1662,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         here = next;
         next = far;
     }
-    finish<T, kD, kCodes, kSplit, kRowWaves>(a, w, lds, lds_m, lds_l, m + (kCodes ? static_cast<float>(unit) : 0.0f), l, acc);
+    finish<T, kD, kHeld, kSplit, kRowWaves>(a, w, lds, lds_m, lds_l, bad, bad_from,
+                                            m + (kCodes ? static_cast<float>(unit) : 0.0f), l, acc);
 }
 
 /// Zeros for the rows first_row .. first_row + count - 1 of a KV head's heads,
@@ -1669,15 +1715,15 @@ __attribute__((amdgpu_waves_per_eu(2, 4))) void chunk_attention_wide_kernel(Chun
     __shared__ __attribute__((aligned(16))) uint8_t lds[WideKind<kD>::lds_bytes()];
     __shared__ float lds_m[kWaves][32];
     __shared__ float lds_l[kWaves][32];
-    __shared__ uint64_t lds_bad[kWaves];
+    __shared__ BadValues<kD> bad;
     constexpr int kRows = Tile<float, kD>::kRows;
     Item w{};
     int end_row = 0;
     if (!item_of<float>(a, w, end_row)) return;
     if (end_row - w.first_row > kRows) {
-        attend<kD, true>(a, w, lds, lds_m, lds_l, lds_bad);
+        attend<kD, true>(a, w, lds, lds_m, lds_l, &bad);
     } else {
-        attend<kD, false>(a, w, lds, lds_m, lds_l, lds_bad);
+        attend<kD, false>(a, w, lds, lds_m, lds_l, &bad);
     }
 }
 
@@ -1690,19 +1736,23 @@ __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_k
     __shared__ __attribute__((aligned(16))) uint8_t lds[kFew > kMany ? kFew : kMany];
     __shared__ float lds_m[kWaves][32];
     __shared__ float lds_l[kWaves][32];
-    __shared__ uint64_t lds_bad[kWaves];
+    BadValues<kD>* bad = nullptr;
+    if constexpr (kHeld != CF_CACHE_INT8) {  // whose codes are all finite
+        __shared__ BadValues<kD> values;
+        bad = &values;
+    }
     constexpr int kRows = Tile<T, kD>::kRows;
     Item w{};
     int end_row = 0;
     if (!item_of<std::conditional_t<kSplit, float, T>>(a, w, end_row)) return;
     if (end_row - w.first_row > 2 * kRows) {
-        attend_rows<T, kD, kHeld, kSplit, 1>(a, w, lds, lds_m, lds_l, lds_bad);
+        attend_rows<T, kD, kHeld, kSplit, 1>(a, w, lds, lds_m, lds_l, bad);
     } else if (end_row - w.first_row > kRows) {
-        attend_rows<T, kD, kHeld, kSplit, 2>(a, w, lds, lds_m, lds_l, lds_bad);
+        attend_rows<T, kD, kHeld, kSplit, 2>(a, w, lds, lds_m, lds_l, bad);
     } else if (end_row - w.first_row > 16) {
-        attend_few<T, kD, kHeld, kSplit, 2>(a, w, lds, lds_m, lds_l);
+        attend_few<T, kD, kHeld, kSplit, 2>(a, w, lds, lds_m, lds_l, bad);
     } else {
-        attend_few<T, kD, kHeld, kSplit, 1>(a, w, lds, lds_m, lds_l);
+        attend_few<T, kD, kHeld, kSplit, 1>(a, w, lds, lds_m, lds_l, bad);
     }
 }
 

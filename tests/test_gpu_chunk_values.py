@@ -1,5 +1,6 @@
-"""Attention of chunks over caches of codes whose values are small, against
-float64: a row's weights keep their bits whatever else it meets."""
+"""Attention of chunks over values of every kind, against float64: small ones in
+caches of codes, whose weights keep their bits whatever else a row meets, and
+ones that are not finite."""
 
 from __future__ import annotations
 
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 import cuda_force_amd as cf
-from tests.chunk_util import CODES, build, check
+from tests.chunk_util import CODES, build, check, reference
 
 pytestmark = pytest.mark.gpu
 # Few rows a tile, some more, and many (tiles of 32, 64 and 128 rows).
@@ -73,3 +74,41 @@ def test_a_scale_of_1_that_is_no_row_of_zeros(held, sequences):
             c.v[page, at, :, t % 128] = 1.0
             c.v_scales[page, at] = 1.0
     run(c)
+
+
+def not_finite(c, s, t, dims, bad):
+    """Values of token t of sequence s, of all its heads."""
+    page, at = int(c.tables[s, t // 16]), t % 16
+    if c.v_scales is None:
+        c.v[page, at][:, dims] = bad
+    else:
+        c.v.view(torch.uint8)[page, at][:, dims] = 0x7F if bad > 0 else 0xFF
+
+
+@pytest.mark.parametrize("dtype,held", [(torch.float32, None), (torch.bfloat16, None), (torch.float16, None),
+                                        (torch.float32, CODES[1]), (torch.bfloat16, CODES[1])])
+@pytest.mark.parametrize("sequences", [*ROWS, [(100, 100), (3, 100), (40, 300), (1, 17)]])
+@pytest.mark.parametrize("dim", [64, 128, 256, 80, 20])
+def test_values_that_are_not_finite_reach_their_own_dims_alone(dtype, held, sequences, dim):
+    """Of tokens that some rows of a step see and others do not, and of tokens
+    that all of them see: infinities keep their signs, two of them give NaN."""
+    c = build(sequences, 4, 1, dim, 16, dtype, held)
+    for s, (new, length) in enumerate(sequences):
+        for t in {0, length - new, length - new // 2 - 1, length - 1}:
+            not_finite(c, s, t, [1, dim - 1], float("inf"))
+        not_finite(c, s, length - new // 3 - 1, [dim - 1, dim - 2], -float("inf"))
+        if held is None:
+            not_finite(c, s, length - new // 4 - 1, [5], float("nan"))
+    got = cf.paged_attention_chunk(*c.args()).cpu()
+    want, _ = reference(c)
+    assert (~torch.isfinite(want)).any() and torch.isfinite(want).any()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isposinf(got), torch.isposinf(want))
+    assert torch.equal(torch.isneginf(got), torch.isneginf(want))
+    # The others as without them: dims do not meet.
+    bits = c.v if held is None else c.v.view(torch.uint8)
+    bits[~torch.isfinite(c.v.float())] = 0
+    clean = cf.paged_attention_chunk(*c.args()).cpu()
+    finite = torch.isfinite(want)
+    assert torch.equal(got[finite], clean[finite])
+    check(clean, c)
