@@ -702,39 +702,41 @@ __global__ __launch_bounds__(512) void matmul_int8_rows_kernel(Int8Args a) {
     }
 }
 
-/// Any k and alignment.
+/// Any k and alignment. Tiles beyond the grid's number go in turn.
 template <typename T>
 __global__ __launch_bounds__(256) void matmul_int8_any_kernel(Int8Args a) {
     constexpr int kTile = 16;
     constexpr int kDeep = 64;
-    __shared__ int8_t xs[kTile][kDeep + 4];
-    __shared__ int8_t ws[kTile][kDeep + 4];
+    __shared__ __attribute__((aligned(4))) int8_t xs[kTile][kDeep + 4];
+    __shared__ __attribute__((aligned(4))) int8_t ws[kTile][kDeep + 4];
     const int tid = static_cast<int>(threadIdx.x);
-    const int tm = static_cast<int>(blockIdx.x) / a.tiles_n;
-    const int tn = static_cast<int>(blockIdx.x) % a.tiles_n;
-    const int i = tm * kTile + tid / kTile;
-    const int j = tn * kTile + tid % kTile;
-    int sum = 0;
-    for (int k0 = 0; k0 < a.k; k0 += kDeep) {
-        for (int c = tid; c < kTile * kDeep; c += 256) {
-            const int r = c / kDeep;
-            const int k = k0 + c % kDeep;
-            const int xr = tm * kTile + r;
-            const int wr = tn * kTile + r;
-            xs[r][c % kDeep] = xr < a.m && k < a.k ? a.x[static_cast<int64_t>(xr) * a.k + k] : static_cast<int8_t>(0);
-            ws[r][c % kDeep] = wr < a.n && k < a.k ? a.w[static_cast<int64_t>(wr) * a.k + k] : static_cast<int8_t>(0);
-        }
-        __syncthreads();
+    for (int64_t tile = blockIdx.x; tile < static_cast<int64_t>(a.tiles_m) * a.tiles_n; tile += gridDim.x) {
+        const int tm = static_cast<int>(tile / a.tiles_n);
+        const int tn = static_cast<int>(tile % a.tiles_n);
+        const int i = tm * kTile + tid / kTile;
+        const int j = tn * kTile + tid % kTile;
+        int sum = 0;
+        for (int k0 = 0; k0 < a.k; k0 += kDeep) {
+            for (int c = tid; c < kTile * kDeep; c += 256) {
+                const int r = c / kDeep;
+                const int k = k0 + c % kDeep;
+                const int xr = tm * kTile + r;
+                const int wr = tn * kTile + r;
+                xs[r][c % kDeep] = xr < a.m && k < a.k ? a.x[static_cast<int64_t>(xr) * a.k + k] : static_cast<int8_t>(0);
+                ws[r][c % kDeep] = wr < a.n && k < a.k ? a.w[static_cast<int64_t>(wr) * a.k + k] : static_cast<int8_t>(0);
+            }
+            __syncthreads();
 #pragma unroll 4
-        for (int k = 0; k < kDeep; k += 4) {
-            sum = __builtin_amdgcn_sdot4(*reinterpret_cast<const int*>(&xs[tid / kTile][k]),
-                                         *reinterpret_cast<const int*>(&ws[tid % kTile][k]), sum, false);
+            for (int k = 0; k < kDeep; k += 4) {
+                sum = __builtin_amdgcn_sdot4(*reinterpret_cast<const int*>(&xs[tid / kTile][k]),
+                                             *reinterpret_cast<const int*>(&ws[tid % kTile][k]), sum, false);
+            }
+            __syncthreads();
         }
-        __syncthreads();
-    }
-    if (i < a.m && j < a.n) {
-        Storage<T>::store(static_cast<T*>(a.y) + static_cast<int64_t>(i) * a.n + j,
-                          result(sum, a.x_scales[i], a.w_scales[j], bias_at<T>(a, j)));
+        if (i < a.m && j < a.n) {
+            Storage<T>::store(static_cast<T*>(a.y) + static_cast<int64_t>(i) * a.n + j,
+                              result(sum, a.x_scales[i], a.w_scales[j], bias_at<T>(a, j)));
+        }
     }
 }
 
@@ -748,6 +750,8 @@ Way way_of(const Int8Args& a) {
     // 64 columns to fill the GPU: 32 rows of 4096 by 4096 columns take 12 us against
     // 14.5 in tiles (64 of them), 64 rows 16 against 15; but by 11008 columns (172
     // tiles) 22 and 33 us against 15 and 16, and 17 rows 18 against 15.
+    // (The general kernel takes columns past one launch.)
+    if (ceil_div<int64_t>(a.n, 16) > kMaxWorkgroups / 2 && a.m <= 16) return Way::kAny;
     if (a.m <= 16 || (a.m <= 64 && ceil_div<int64_t>(a.n, 64) < 128)) return Way::kRows;
     // Tiles of 128 x 128 run two a CU, 512 at once. Fewer than 192 leave too many CUs
     // idle (96 and 160 of them, k 4096: 30 and 32 us against 20 and 30 in tiles of 64;
@@ -798,8 +802,9 @@ cf_status run(Int8Args a, hipStream_t stream) {
         case Way::kTile128: tiles(a, 128, 128); kernel = matmul_int8_kernel<T, 128, 128, 64, 64, 2, 1>; break;
         case Way::kTile256: tiles(a, 256, 256); kernel = matmul_int8_big_kernel<T>; break;
     }
-    const int64_t grid = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
-    CF_REQUIRE(grid <= kMaxWorkgroups / 2, "cf_matmul_int8: %d x %d results are too many for a launch", a.m, a.n);
+    int64_t grid = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+    if (way == Way::kAny && grid > kMaxWorkgroups) grid = kMaxWorkgroups;
+    CF_REQUIRE(grid <= UINT32_MAX / threads, "cf_matmul_int8: %d x %d results are too many for a launch", a.m, a.n);
     launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, a);
     return check_launch("launching the int8 product", stream);
 }
