@@ -148,7 +148,11 @@ template <typename T>
 void launch_rows(const RowsArgs& a, hipStream_t stream) {
     constexpr int kPer = Storage<T>::kPerVec;
     const int64_t vecs = a.cols / kPer;
-    auto capped = [](int64_t n) { return dim3(static_cast<unsigned>(n < kMaxWorkgroups ? n : kMaxWorkgroups)); };
+    // (Rows beyond a launch's workgroups go in turn.)
+    auto capped = [](int64_t n, int threads = kRowThreads) {
+        const int64_t most = UINT32_MAX / threads;
+        return dim3(static_cast<unsigned>(n < most ? n : most));
+    };
     const bool vectors = a.cols % kPer == 0 && host_aligned(a.x, 16) && a.stride % kPer == 0 &&
                          host_aligned(a.codes, kPer) && vecs <= 1024 * 8;
     if (!vectors) {
@@ -169,7 +173,7 @@ void launch_rows(const RowsArgs& a, hipStream_t stream) {
                                       : quantize_rows_kernel<T, 256, 8>;
         launch(kernel, capped(a.rows), dim3(256), 0, stream, a);
     } else {
-        launch(quantize_rows_kernel<T, 1024, 8>, capped(a.rows), dim3(1024), 0, stream, a);
+        launch(quantize_rows_kernel<T, 1024, 8>, capped(a.rows, 1024), dim3(1024), 0, stream, a);
     }
 }
 

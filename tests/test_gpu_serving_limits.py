@@ -37,3 +37,18 @@ def test_one_row_by_columns_past_one_launch(k):
         assert torch.equal(y[0, a : a + 2**25], (w[a : a + 2**25].float() * x.float()).sum(1))
     del y, w, ones
     torch.cuda.empty_cache()
+
+
+def test_more_wide_rows_than_a_launch_of_large_workgroups_has():
+    """Rows of more than 8192 fp32 numbers have a workgroup of 1024 threads each."""
+    rows, cols = 2**22 + 3, 8200
+    if torch.cuda.mem_get_info()[0] < 190 << 30:
+        pytest.skip("needs 190 GiB of memory")
+    x = torch.empty(rows, cols, device="cuda")
+    at = [0, 1, 2**21, 2**22 - 2, 2**22 - 1, 2**22, rows - 1]
+    x[at] = torch.randn(len(at), cols, device="cuda")
+    codes, scales = cf.quantize_int8_rows(x)
+    want, want_scales = cf.quantize_int8_rows(x[at].cpu())
+    assert torch.equal(codes[at].cpu(), want) and torch.equal(scales[at].cpu(), want_scales)
+    del x, codes
+    torch.cuda.empty_cache()
