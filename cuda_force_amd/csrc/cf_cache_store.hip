@@ -411,6 +411,26 @@ cf_status check_store(const char* who, cf_dtype dtype, cf_cache_format format, i
     return CF_OK;
 }
 
+/// Bytes from `begin` to `end`, of rows a stride of elements apart.
+struct Bytes {
+    uintptr_t begin, end;
+
+    bool meet(const Bytes& o) const { return begin < end && o.begin < o.end && begin < o.end && o.begin < end; }
+};
+Bytes bytes_of(const void* p, size_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return Bytes{at, at + bytes};
+}
+Bytes bytes_of_rows(const void* p, int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim,
+                    size_t size) {
+    const int64_t reach[2] = {(tokens - 1) * token_stride, (heads - 1) * head_stride};
+    int64_t first = 0, last = dim;
+    for (const int64_t r : reach) (r < 0 ? first : last) += r;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return Bytes{at + static_cast<uintptr_t>(first * static_cast<int64_t>(size)),
+                 at + static_cast<uintptr_t>(last * static_cast<int64_t>(size))};
+}
+
 /// Whole vectors: of the given type, and as many codes of the cache.
 bool whole_vectors(const StoreArgs& a, cf_dtype dtype, cf_cache_format format, bool strided) {
     const int64_t per = dtype == CF_F32 ? 4 : 8;
@@ -439,8 +459,26 @@ cf_status cf_cache_write(const void* keys, const void* values, cf_dtype dtype, i
     const cf_status st = cf::check_store(who, dtype, format, tokens, num_kv_heads, head_dim, num_slots,
                                          {keys, values, k_cache, v_cache, slots}, k_scales, v_scales);
     if (st != CF_OK) return st;
-    CF_REQUIRE(k_cache != v_cache && (format == CF_CACHE_PLAIN || k_scales != v_scales),
-               "%s: keys and values have one place", who);
+    {
+        const size_t size = cf::dtype_size(dtype);
+        const size_t rows = static_cast<size_t>(num_slots) * static_cast<size_t>(num_kv_heads);
+        const size_t cache_bytes = rows * static_cast<size_t>(head_dim) * (format == CF_CACHE_PLAIN ? size : 1);
+        const size_t scale_bytes = format == CF_CACHE_PLAIN ? 0 : rows * 4;
+        const cf::Bytes written[4] = {cf::bytes_of(k_cache, cache_bytes), cf::bytes_of(v_cache, cache_bytes),
+                                      cf::bytes_of(k_scales, scale_bytes), cf::bytes_of(v_scales, scale_bytes)};
+        const cf::Bytes given[2] = {
+            cf::bytes_of_rows(keys, tokens, key_token_stride, num_kv_heads, key_head_stride, head_dim, size),
+            cf::bytes_of_rows(values, tokens, value_token_stride, num_kv_heads, value_head_stride, head_dim, size)};
+        const int many = format == CF_CACHE_PLAIN ? 2 : 4;
+        for (int i = 0; i < many; ++i) {
+            for (int j = 0; j < i; ++j) {
+                CF_REQUIRE(!written[i].meet(written[j]), "%s: caches or scales share memory", who);
+            }
+            for (const cf::Bytes& g : given) {
+                CF_REQUIRE(!written[i].meet(g), "%s: keys or values share memory with what is written", who);
+            }
+        }
+    }
     cf::StoreArgs a{};
     a.x[0] = keys;
     a.x[1] = values;

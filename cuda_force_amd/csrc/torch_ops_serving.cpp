@@ -62,6 +62,16 @@ void check_slots(const torch::Tensor& slots, const torch::Tensor& like) {
 
 // ---- storing into a paged cache ------------------------------------------------
 
+/// Whether a tensor of any strides has memory in common with a dense one.
+bool shares_memory(const torch::Tensor& x, const torch::Tensor& dense) {
+    if (!x.is_alias_of(dense) || x.numel() == 0 || dense.numel() == 0) return false;
+    int64_t last = 1;
+    for (int64_t d = 0; d < x.dim(); ++d) last += (x.size(d) - 1) * x.stride(d);
+    const char* from = static_cast<const char*>(x.data_ptr());
+    const char* to = static_cast<const char*>(dense.data_ptr());
+    return from < to + dense.nbytes() && to < from + last * x.element_size();
+}
+
 void cache_write_hip(const torch::Tensor& keys, const torch::Tensor& values, const torch::Tensor& k_cache,
                      const torch::Tensor& v_cache, const torch::Tensor& slots,
                      const std::optional<torch::Tensor>& k_scales, const std::optional<torch::Tensor>& v_scales) {
@@ -79,8 +89,15 @@ void cache_write_hip(const torch::Tensor& keys, const torch::Tensor& values, con
     }
     if (keys.numel() == 0 || k_cache.numel() == 0) return;
     const at::DeviceGuard guard(keys.device());
-    check_status(cf_cache_write(keys.data_ptr(), values.data_ptr(), to_cf(keys, "keys"), keys.size(0), kv_heads, dim,
-                                keys.stride(0), keys.stride(1), values.stride(0), values.stride(1),
+    // Rows of the caches themselves are read before any is written.
+    auto apart = [&](const torch::Tensor& x) {
+        const bool shares = shares_memory(x, k_cache) || shares_memory(x, v_cache) ||
+                            (k_scales && shares_memory(x, *k_scales)) || (v_scales && shares_memory(x, *v_scales));
+        return shares ? x.clone(at::MemoryFormat::Contiguous) : x;
+    };
+    const torch::Tensor k = apart(keys), v = apart(values);
+    check_status(cf_cache_write(k.data_ptr(), v.data_ptr(), to_cf(keys, "keys"), keys.size(0), kv_heads, dim,
+                                k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                 slots.data_ptr<int64_t>(), k_cache.data_ptr(), v_cache.data_ptr(), format,
                                 scales_of(k_scales), scales_of(v_scales), k_cache.size(0) * k_cache.size(1),
                                 stream_for(keys)));

@@ -207,11 +207,15 @@ def _write_reference(
     keys: torch.Tensor, values: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
     k_scales: torch.Tensor | None, v_scales: torch.Tensor | None,
 ) -> None:
+    written = [t for t in (k_cache, v_cache, k_scales, v_scales) if t is not None and t.numel()]
+    for i, t in enumerate(written):
+        if any(t.data_ptr() < o.data_ptr() + o.nbytes and o.data_ptr() < t.data_ptr() + t.nbytes for o in written[:i]):
+            raise RuntimeError("caches or scales share memory")
     last = {s: i for i, s in enumerate(slots.tolist()) if 0 <= s < k_cache.shape[0] * k_cache.shape[1]}
     at = torch.tensor(list(last), dtype=torch.int64, device=slots.device)
     rows = torch.tensor(list(last.values()), dtype=torch.int64, device=slots.device)
-    for x, cache, scales in ((keys, k_cache, k_scales), (values, v_cache, v_scales)):
-        given = x.detach()[rows]
+    taken = [x.detach()[rows] for x in (keys, values)]  # before anything is written: they may lie in the caches
+    for given, cache, scales in zip(taken, (k_cache, v_cache), (k_scales, v_scales)):
         if scales is not None:
             given, scale = ops._nearest_codes(given, cache.dtype)
             scales.view(-1, scales.shape[2])[at] = scale
@@ -295,13 +299,15 @@ def cache_write(
     kv_heads]``. A row's scale is its largest magnitude times fp32's 1 / 127 (1 /
     448), 1 for a row of zeros, and a code the one nearest to ``x / scale``, ties to even; a row
     that holds NaN or an infinity gets codes of 0 and the scale NaN. Caches and
-    scales are written in place. Not differentiable. Not in the reference's API.
+    scales are written in place; keys and values may be views of them, and are read
+    before anything is written. Not differentiable. Not in the reference's API.
 
     Raises:
         ValueError: for shapes, devices or layouts that do not match, one cache
             for both, or tensors that require gradients.
         TypeError: for slots that are not int64, scales that are not fp32 or a
             cache of another type.
+        RuntimeError: for caches or scales that share memory.
     """
     if ops._DIRECT is not None and not ops._compiling():
         if ops._DIRECT.try_cache_write(keys, values, k_cache, v_cache, slots, k_scales, v_scales):

@@ -679,8 +679,9 @@ cf_status cf_paged_attention_shared(const void* query, const void* k_cache, cons
  * v_scales [num_slots, num_kv_heads], is absmax times fp32's 1 / 127 or 1 / 448
  * (1 where that is 0; NaN, with codes of 0, for a row that is not finite), and
  * each code the one nearest to x / s: exactly, ties to even.
- * The caches, and the scales, are not the same memory. Rows of up to 4096 bytes of
- * whole 16-byte vectors, aligned, move fastest.
+ * The caches and the scales share no memory with one another, nor with keys and
+ * values: an invalid argument. Rows of up to 4096 bytes of whole 16-byte vectors,
+ * aligned, move fastest.
  * num_slots is at most 2^31 - 4096. It has no counterpart in the reference. */
 cf_status cf_cache_write(const void* keys, const void* values, cf_dtype dtype, int64_t tokens,
                          int64_t num_kv_heads, int64_t head_dim, int64_t key_token_stride,
