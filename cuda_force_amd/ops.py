@@ -767,9 +767,11 @@ def _nearest_codes(x: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, t
     q = (wide / scales.double().unsqueeze(-1)).clamp(-top, top)
     q = torch.where(torch.isnan(scales).unsqueeze(-1), torch.zeros_like(q), q)
     if dtype != torch.int8:
-        # Three bits behind the leading one, steps of 2^-9 at least.
-        steps = 4 - torch.frexp(q)[1].clamp(min=-5)
-        return torch.ldexp(torch.ldexp(q, steps).round(), -steps).float().to(dtype), scales
+        # Three bits behind the leading one, steps of 2^-9 at least. (By a table: torch's
+        # ldexp multiplies by a power that the GPU's fp64 may have a unit off.)
+        powers = torch.tensor([2.0**e for e in range(-9, 6)], dtype=torch.float64, device=q.device)
+        steps = powers[torch.frexp(q)[1].clamp(min=-5).long() + 5]
+        return ((q / steps).round() * steps).float().to(dtype), scales
     return q.round().to(dtype), scales
 
 
