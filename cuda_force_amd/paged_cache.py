@@ -198,7 +198,9 @@ def _rows_of(cache: torch.Tensor) -> torch.Tensor:
 
 def _values_at(cache: torch.Tensor, scales: torch.Tensor | None, at: torch.Tensor) -> torch.Tensor:
     """What the cache holds at slots, in fp32 (fp64 where the cache is)."""
-    rows = _rows_of(cache)[at].view(cache.dtype)
+    rows = _rows_of(cache)[at]
+    if rows.dtype != cache.dtype:  # (a view as another type, even as its own, has no gradient)
+        rows = rows.view(cache.dtype)
     wide = rows if rows.dtype == torch.float64 else rows.float()
     return wide if scales is None else wide * scales.view(-1, scales.shape[2])[at].unsqueeze(-1)
 
