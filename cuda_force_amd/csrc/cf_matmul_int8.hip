@@ -202,7 +202,7 @@ __device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ ((row >> 3)
 
 /// One result: as the header has it.
 __device__ __forceinline__ float result(int sum, float xs, float ws, float bias) {
-    return static_cast<float>(sum) * xs * ws + bias;
+    return fmaf(static_cast<float>(sum) * xs, ws, bias);
 }
 
 template <typename T>

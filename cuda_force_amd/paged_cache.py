@@ -344,9 +344,9 @@ def cache_read(
     """What a paged cache holds at ``slots`` (int64 ``[tokens]``): ``(keys,
     values)``, each ``[tokens, kv_heads, head_dim]``, zeros for a slot out of range.
 
-    Caches and scales are as in :func:`cache_write`. 8-bit caches give ``code *
-    scale`` in ``dtype`` (fp32, fp16 or bf16; default fp32), rounded once; others
-    their own type. Token t of sequence s lies at slot ``block_tables[s, t //
+    Caches and scales are as in :func:`cache_write`. 8-bit caches give the fp32
+    product ``code * scale``, rounded to ``dtype`` (fp32, fp16 or bf16; default
+    fp32); others their own type. Token t of sequence s lies at slot ``block_tables[s, t //
     block] * block + t % block``. Not differentiable on the kernels. Not in the
     reference's API.
 
@@ -392,7 +392,11 @@ def paged_attention_chunk(
 
     Returns ``[tokens, heads, head_dim]``; zeros for a row that no sequence holds
     (padding behind the last one), or whose position is below 0. A table entry
-    that names no page leaves its tokens out. fp32, fp16 and bf16; not
+    that names no page leaves its tokens out. Probabilities are rounded to 16 bits
+    before they meet the values, in bf16 or, for fp16 and codes, in fp16 (to 22 bits
+    for an fp32 query over codes; not at all in plain fp32). Over codes a token whose
+    value scale is less than about 2^-38 of the largest that its row sees adds
+    nothing; a row of zeros does not count. fp32, fp16 and bf16; not
     differentiable on the kernels (a call that needs a gradient runs the PyTorch
     composition). Not in the reference's API.
 

@@ -691,8 +691,8 @@ cf_status cf_cache_write(const void* keys, const void* values, cf_dtype dtype, i
                          int64_t num_slots, void* stream);
 
 /* Reads places back: row i of keys and values [tokens, num_kv_heads, head_dim]
- * (dense, of `dtype`) is what slot slots[i] holds, code * scale rounded once for
- * 8-bit caches, and zeros for a slot out of range. CF_CACHE_PLAIN caches are of
+ * (dense, of `dtype`) is what slot slots[i] holds, for 8-bit caches the fp32
+ * product code * scale rounded to `dtype`, and zeros for a slot out of range. CF_CACHE_PLAIN caches are of
  * `dtype`. It has no counterpart in the reference. */
 cf_status cf_cache_read(const void* k_cache, const void* v_cache, cf_cache_format format,
                         const float* k_scales, const float* v_scales, int64_t num_slots,
@@ -717,7 +717,15 @@ size_t cf_paged_attention_chunk_workspace_bytes(cf_dtype dtype, cf_cache_format 
  * the last one to all context_lens[s] of them. Caches, tables and context lengths
  * are as in cf_paged_attention_shared, or the caches hold 8-bit codes (`format`)
  * with k_scales and v_scales [num_pages, block_size, num_kv_heads]. Keys and
- * values are used as code * scale.
+ * values are used as code * scale, with two limits. Probabilities are rounded to 16
+ * bits for the product with the values: bf16 for bf16 caches, fp16 for fp16 ones and
+ * for codes, where they are times the value's scale (of fp32 queries, and of plain
+ * fp32 caches, they keep 22 bits and all). fp16 ones are kept relative to the row's
+ * largest probability, for codes times the largest value scale that it has met (rows
+ * of zeros do not count), and less than about 2^-38 of that is lost: a token whose
+ * scale is that much below the largest that its row sees adds nothing.
+ * Scales below 2^-90 count as 2^-90 there. A row that sees a scale that is not
+ * finite is not finite itself; an infinity or NaN in a value reaches its dim alone.
  * Rows whose position is below 0 (more rows than context), rows that no sequence
  * holds, rows all of whose tokens are left out or whose scores are all -inf get
  * zeros. Starts are taken in ascending order (one below an earlier one counts as
@@ -752,8 +760,9 @@ cf_status cf_quantize_int8_rows(const void* x, cf_dtype dtype, int64_t rows, int
 
 /* y[i, j] = x_scales[i] * w_scales[j] * sum_k x[i, k] * w[j, k] (+ bias[j]): x
  * [m, k] and w [n, k] dense int8, scales fp32, bias (may be NULL) and y [m, n] of
- * `dtype`. The sum is exact in 32 bits; it is converted to fp32, multiplied by
- * x's scale and then by w's, the bias is added, and the result rounded to `dtype`.
+ * `dtype`. The sum is exact in 32 bits; it is converted to fp32 and multiplied by
+ * x's scale; the product of that with w's scale plus the bias is one fma, and its
+ * result is rounded to `dtype`.
  * k at most 131071 (a sum of k products of -128 stays in 32 bits). k a multiple
  * of 16 and 16-byte aligned operands run on the matrix cores, others a general
  * kernel. It has no counterpart in the reference, whose 8-bit codes are
