@@ -23,11 +23,11 @@
 //     values' scales the probabilities, in fp32.
 //   * Tokens that are not there (behind the range, in no page) get no weight, and
 //     what the cache holds in their place never reaches a row.
-// Measured, 32 heads over 8 of 128: a prompt of 2048 tokens in bf16 67 us (510
+// Measured, 32 heads over 8 of 128: a prompt of 2048 tokens in bf16 61 us (560
 // TFLOP/s: the chain product, probabilities, product, at two waves a SIMD, and
-// the causal tiles' different lengths); 2048 tokens behind 30720 1.13 to 1.24 ms
-// (860 to 940 TFLOP/s: matrix cores 44% and vector units 48% busy, and the clock
-// falls from 2.2 to 1.7 GHz under them); 64 sequences of 2051 to 4096 tokens in
+// the causal tiles' different lengths); 2048 tokens behind 30720 1.10 to 1.22 ms by
+// the card (870 to 970 TFLOP/s: matrix cores 44% and vector units 48% busy, and the
+// clock falls from 2.2 to 1.7 GHz under them); 64 sequences of 2051 to 4096 tokens in
 // int8, a token each, 102 us (4.1 TB/s; 4.8 TB/s at equal lengths: reads of single
 // 128-byte lines, where bf16's of 256 bytes reach 5.9).
 #include "cf_attention_tile.hpp"
@@ -507,7 +507,7 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Item& w, uint8_
 }
 
 /// fp32 caches, in fp32 products: the matrix cores' slowest, half busy where a CU
-/// has two workgroups (four chunks of up to 100 tokens behind 900, 86 us, and
+/// has two workgroups (four chunks of up to 100 tokens behind 900, 84 us, and
 /// 12 us for the join). kShared: the waves take different rows of the tile, else different
 /// tokens of the same rows.
 template <int kD, bool kShared>
@@ -1214,8 +1214,8 @@ struct RowsKind {
 /// probabilities, so that a wave has work for the matrix cores beside its vector
 /// instructions (a 2048-token prompt 68 us, without it and the reads ahead 75);
 /// codes, which need more of those, leave no registers for it: 512 tokens each of
-/// three sequences of 4000 in e4m3, next to 41 single ones, take 205 us with the
-/// vector units 45% and the matrix cores 19% busy.
+/// three sequences of 4000 in e4m3, next to 41 single ones, take 203 us with the
+/// vector units 43% and the matrix cores 18% busy.
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kHalves>
 __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],
                             BadValues<kD>* bad) {
@@ -1757,7 +1757,9 @@ __attribute__((amdgpu_waves_per_eu(kD > 128 ? 1 : 2, 4))) void chunk_attention_k
 }
 
 /// The general kernel: any head size and alignment, a wave per (token, head,
-/// range), a token of the context at a time, dims over the lanes.
+/// range), a token of the context at a time, dims over the lanes. Slow: a prompt of
+/// 2048 tokens with 32 heads of 256 in fp32 takes 16 ms, 16 single tokens behind up
+/// to 2000 0.9 ms, more than PyTorch's batched products (2.3 and 0.8 ms).
 template <typename T, cf_cache_format kHeld, int kPer>
 __global__ __launch_bounds__(kThreads) void chunk_attention_any_kernel(ChunkArgs a) {
     const int lane = static_cast<int>(threadIdx.x) & (kWaveSize - 1);
