@@ -206,18 +206,21 @@ struct Item {
 
 /// What counts as the scale of a row of values: a row of zeros, which is stored
 /// with the scale 1 whatever the others' are, must not stand for the largest of
-/// them, so its scale is taken as 0. `row`: its codes, read only if the scale is 1.
-template <cf_cache_format kHeld>
-__device__ __forceinline__ float value_scale(float scale, const uint8_t* row, int bytes) {
-    if (scale == 1.0f) {
+/// them, so its scale is taken as 0. `row()`: its codes, read only if the scale is 1
+/// and, by `matters`, until a row has met a larger one or another of 1 (a cache of
+/// scales that are all 1 would be read twice).
+template <cf_cache_format kHeld, typename Row>
+__device__ __forceinline__ float value_scale(float scale, bool matters, Row row, int bytes) {
+    if (scale == 1.0f && matters) {
+        const uint8_t* from = row();
+        constexpr uint32_t kMagnitudes = kHeld == CF_CACHE_E4M3 ? 0x7F7F7F7Fu : 0xFFFFFFFFu;
         uint32_t any = 0;
 #pragma unroll 1
-        for (int at = 0; at < bytes; at += 16) {
-            const u32x4_t codes = *reinterpret_cast<const u32x4_t*>(row + at);
-            any |= codes[0] | codes[1] | codes[2] | codes[3];
+        for (int at = 0; at < bytes && any == 0; at += 16) {
+            const u32x4_t codes = *reinterpret_cast<const u32x4_t*>(from + at);
+            any = (codes[0] | codes[1] | codes[2] | codes[3]) & kMagnitudes;
         }
-        constexpr uint32_t kMagnitudes = kHeld == CF_CACHE_E4M3 ? 0x7F7F7F7Fu : 0xFFFFFFFFu;
-        if ((any & kMagnitudes) == 0) scale = 0.0f;
+        if (any == 0) scale = 0.0f;
     }
     return scale;
 }
@@ -956,7 +959,13 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
         const uint32_t now = there;
         const bool masked = now != 0xFFFFFFFFu || first + kTokens - 1 > wave_least;
         if constexpr (kCodes) {
-            if (lane >= kTokens) scale = value_scale<kHeld>(scale, a.v_cache + places[lane - kTokens], row_bytes);
+            // (A row that sees none of the tokens that another has met sees none of these.)
+            int met = unit[0];
+            if constexpr (kTiles > 1) met = max(met, unit[kTiles - 1]);
+            const bool matters = __builtin_amdgcn_ballot_w64(met > 0) == 0;
+            if (lane >= kTokens) {
+                scale = value_scale<kHeld>(scale, matters, [&]() { return a.v_cache + places[lane - kTokens]; }, row_bytes);
+            }
             scales[lane] = scale;
         }
         // The next tile; behind the last one its tokens are not there, and every lane reads
@@ -1104,7 +1113,8 @@ __device__ void attend_few(const ChunkArgs& a, const Item& w, uint8_t* lds, floa
 #pragma unroll
                     for (int word = 0; word < L::kWords; ++word) {
                         const uint32_t out = ((values[j][p][word] & (sign - one)) + one) & sign;
-                        any |= out;
+                        // (What is read in place of a token that is not there does not count.)
+                        any |= (now >> (4 * group + token_of(j)) & 1) != 0 ? out : 0;
                         values[j][p][word] &= ~((out >> (kCodes ? 7 : 15)) * (kCodes ? 0xFFu : 0xFFFFu));
                     }
                 }
@@ -1334,15 +1344,24 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     };
     [[maybe_unused]] Codes k_codes, v_codes;
     [[maybe_unused]] float raw_scale = 0.0f;
+    // Heads of 256 have no registers for places in rows and LDS that stay the same from
+    // step to step: kept, they are spilled (three chunks of 512 behind 3488 in e4m3
+    // 710 us, computed again 615). The lane that they come from is hidden.
+    [[maybe_unused]] auto step_lane = [&]() {
+        int l2 = lane;
+        if constexpr (kD > 128) asm volatile("" : "+v"(l2));
+        return l2;
+    };
     [[maybe_unused]] auto load_codes = [&](Codes& to, const Place& p, bool is_v) {
+        const int at_lane = step_lane();
         const uint8_t* base = (is_v ? a.v_cache : a.k_cache) + head_bytes;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int r = wave * kMine + n * kCodeTokens + lane / kCodeLanes;
+            const int r = wave * kMine + n * kCodeTokens + at_lane / kCodeLanes;
             const uint32_t at = static_cast<uint32_t>(__shfl(static_cast<int>(p.piece), r));
             // A row that is not there, or the end of a narrow one, is read from the cache's
             // or row's beginning instead and not used.
-            const int piece = lane % kCodeLanes < row_pieces ? lane % kCodeLanes : 0;
+            const int piece = at_lane % kCodeLanes < row_pieces ? at_lane % kCodeLanes : 0;
             to.raw[n] = *reinterpret_cast<const u32x4_t*>(base + (static_cast<uint64_t>(at + static_cast<uint32_t>(piece)) << 4));
         }
         if (wave == (is_v ? 1 : 0)) {
@@ -1363,13 +1382,15 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     [[maybe_unused]] auto scales_of = [&](int tile) {
         return reinterpret_cast<float*>(lds + K::kScalesAt) + (tile & 1) * K::kScales;
     };
-    [[maybe_unused]] auto store_codes = [&](const Codes& from, const Place& p, int tile, bool is_v) {
+    [[maybe_unused]] int unit = kLeastUnit;  // see attend_few
+    [[maybe_unused]] auto store_codes = [&](const Codes& from, int tile, bool is_v) {
+        const int at_lane = step_lane();
         uint8_t* to = lds + ((is_v ? 2 : 0) + (tile & 1)) * K::kOperand;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int r = wave * kMine + n * kCodeTokens + lane / kCodeLanes;
+            const int r = wave * kMine + n * kCodeTokens + at_lane / kCodeLanes;
             const int sw = is_v ? L::v_swizzle(r) : L::k_swizzle(r);
-            const int piece = lane % kCodeLanes;
+            const int piece = at_lane % kCodeLanes;
             u32x4_t lo, hi;
             widen16<kCodes ? kHeld : CF_CACHE_INT8>(from.raw[n], lo, hi);
             if (piece < row_pieces) {
@@ -1380,8 +1401,16 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         if (wave == (is_v ? 1 : 0)) {
             float* scales = scales_of(tile);
             if (is_v) {
-                raw_scale = value_scale<kHeld>(raw_scale, a.v_cache + head_bytes + (static_cast<uint64_t>(p.piece) << 4),
-                                               a.head_dim);
+                // (A row that sees none of the tokens that another has met sees none of these;
+                // the waves with later rows have met what this one has.)
+                const bool matters = __builtin_amdgcn_ballot_w64(unit > 0) == 0;
+                raw_scale = value_scale<kHeld>(raw_scale, matters, [&]() {
+                    // (Looked up again: a register less to keep.)
+                    const uint32_t t = static_cast<uint32_t>(w.lo + tile * kTokens + lane);
+                    const uint32_t block = t / a.block_size;
+                    const uint32_t row = w.table[block] * a.block_size + (t - block * a.block_size);
+                    return a.v_cache + head_bytes + (static_cast<uint64_t>(row * a.token_pieces) << 4);
+                }, a.head_dim);
             }
             scales[(is_v ? kTokens : 0) + lane] = raw_scale;
             if (is_v) {
@@ -1394,7 +1423,6 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     float m = -INFINITY;  // the row's running maximum
     float l = 0.0f;       // this lane's share of the running sum
     float shift = -L::kLift;
-    [[maybe_unused]] int unit = kLeastUnit;  // see attend_few
     Score acc[L::kAcc / L::kScores];
 #pragma unroll
     for (int b = 0; b < L::kAcc / L::kScores; ++b) {
@@ -1545,8 +1573,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
     if constexpr (kCodes) {
         load_codes(k_codes, here, false);
         load_codes(v_codes, here, true);
-        store_codes(k_codes, here, 0, false);
-        store_codes(v_codes, here, 0, true);
+        store_codes(k_codes, 0, false);
+        store_codes(v_codes, 0, true);
         if (tiles > 1) {
             load_codes(k_codes, next, false);
             load_codes(v_codes, next, true);
@@ -1574,8 +1602,8 @@ __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, flo
         bare_barrier();
         if constexpr (kCodes) {
             if (i + 1 < tiles) {
-                store_codes(k_codes, next, i + 1, false);
-                store_codes(v_codes, next, i + 1, true);
+                store_codes(k_codes, i + 1, false);
+                store_codes(v_codes, i + 1, true);
             }
             if (i + 2 < tiles) {
                 far = look_up(i + 2);

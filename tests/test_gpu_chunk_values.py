@@ -112,3 +112,18 @@ def test_values_that_are_not_finite_reach_their_own_dims_alone(dtype, held, sequ
     finite = torch.isfinite(want)
     assert torch.equal(got[finite], clean[finite])
     check(clean, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("held", CODES)
+@pytest.mark.parametrize("sequences", ROWS)
+def test_scales_of_1_throughout(dtype, held, sequences):
+    """A cache of codes without scales of their own, some rows of zeros at first and later."""
+    c = build(sequences, 4, 1, 64, 16, dtype, held)
+    c.k_scales[c.k_scales.isfinite()] = 1.0
+    c.v_scales[c.v_scales.isfinite()] = 1.0
+    c.scale = 1e-3
+    for s, length in enumerate(c.context.tolist()):
+        for t in [*range(70), *range(130, 135), length - 1]:
+            c.v[int(c.tables[s, t // 16]), t % 16] = 0
+    run(c)
