@@ -11,9 +11,9 @@
 //     after the other. A workgroup owns neighbouring tokens; it puts their slots
 //     into a hash table in LDS and looks up those of all later tokens in it,
 //     while its first rows are on their way.
-// 8192 tokens of 8 heads of 128, bf16 to e4m3: 17.3 us written (2.9 TB/s, behind
-// that search), 11.1 us read back (4.6 TB/s); to bf16 15.1 and 14.4 us.
-// 64 tokens, 4.4 and 2.7 us, are a launch and its chain of loads.
+// 8192 tokens of 8 heads of 128, bf16 to e4m3: 17.7 us written (2.9 TB/s, behind
+// that search), 11.3 us read back (4.5 TB/s); to bf16 15.2 and 14.4 us.
+// 64 tokens, 4.4 and 2.8 us, are a launch and its chain of loads.
 #include "cf_codes.hpp"
 #include "cf_common.hpp"
 #include "cf_ranges.hpp"

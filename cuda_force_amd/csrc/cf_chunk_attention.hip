@@ -1224,7 +1224,7 @@ struct RowsKind {
 /// probabilities, so that a wave has work for the matrix cores beside its vector
 /// instructions (a 2048-token prompt 68 us, without it and the reads ahead 75);
 /// codes, which need more of those, leave no registers for it: 512 tokens each of
-/// three sequences of 4000 in e4m3, next to 41 single ones, take 203 us with the
+/// three sequences of 4000 in e4m3, next to 41 single ones, take 202 us with the
 /// vector units 43% and the matrix cores 18% busy.
 template <typename T, int kD, cf_cache_format kHeld, bool kSplit, int kHalves>
 __device__ void attend_rows(const ChunkArgs& a, const Item& w, uint8_t* lds, float (*lds_m)[32], float (*lds_l)[32],

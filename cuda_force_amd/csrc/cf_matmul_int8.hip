@@ -9,18 +9,18 @@
 //
 // Few rows are bound by w, which is read once: its rows go from memory straight to
 // the matrix cores, 16 of them a workgroup, whose waves split k (8 rows by 11008
-// columns of 4096: 14.0 us, 3.2 TB/s; sending the next loads ahead of the products
+// columns of 4096: 14.1 us, 3.2 TB/s; sending the next loads ahead of the products
 // changed nothing). Middling batches are bound by the steps of the loop over k,
 // each a barrier, copies, LDS reads and a short chain of products: small tiles,
 // and two groups of waves on one, give the CUs enough to do beside them (333 x
 // 4096 x 4096: 15 us by kernel time, 11 TB/s from L2 to LDS at 15% of the matrix
 // cores' rate; neither a fifth stage of LDS nor steps in another order for every
 // tile changed anything). Large ones are bound by the matrix cores and the
-// power they draw: 8192 x 4096 x 4096 takes 119 to 124 us, 2.2 to 2.3 POP/s, with
+// power they draw: 8192 x 4096 x 4096 takes 115 to 128 us by the card, 2.1 to 2.4 POP/s, with
 // the matrix cores 56% busy at 1.6 to 1.8 GHz.
 //
 // The quantiser is bound by memory: a row is read once and held in registers
-// (8192 rows of 4096 in bf16: 17.6 us, 5.7 TB/s).
+// (8192 rows of 4096 in bf16: 17.8 us, 5.7 TB/s).
 #include "cf_codes.hpp"
 #include "cf_common.hpp"
 #include "cf_lds_dma.hpp"
